@@ -76,6 +76,17 @@ SIGNATURES = {
     "fsc_bucket_mix_transpose_y": [_i64] + [_i32] * 4 + [_p] * 4 + [_i32, _p, _p],
     "fsc_bucket_mix_transpose_w": [_i64] + [_i32] * 4 + [_p] * 4 + [_i32, _p, _p],
     "fsc_bucket_mix_transpose_g": [_i64] + [_i32] * 4 + [_p] * 4 + [_i32, _p],
+    "fsc_rms_norm_forward": [_i64, _i32, _i32, _i32, _i64, _i64, _p, _p, _p, _f32, _p, _p, _p, _p],
+    "fsc_rms_norm_q8": [_i64, _i32, _i32, _i32, _i64, _i64, _p, _p, _p, _f32, _p, _p, _p, _p],
+    "fsc_rms_norm_workspace": [_i64, _i32, _pi64],
+    "fsc_rms_norm_backward": [_i64, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _f32] + [_p] * 6,
+    "fsc_route_experts": [_i64, _i32, _i32, _i64, _p, _p] + [_i32] * 6 + [_f32, _p, _p, _p],
+    "fsc_route_experts_backward": [_i64, _i32, _i32, _i64, _p, _p, _p, _p, _i32, _i32, _i32, _f32, _p, _p],
+    "fsc_expert_sizes": [_p, _pi64, _pi64, _pi64, _pi64],
+    "fsc_expert_plan": [_p, _p, _p, _p],
+    "fsc_expert_mlp_forward": [_p, _i64] + [_p] * 9,
+    "fsc_expert_mlp_backward": [_p, _i64, _i64] + [_p] * 13,
+    "fsc_expert_mlp_q8": [_p, _i64] + [_p] * 11,
 }
 # the fp64 twins of the bucket functions take the same arguments (double arrays)
 SIGNATURES.update({n + "_f64": SIGNATURES[n] for n in (

@@ -518,6 +518,80 @@ int fsc_readout_mlp_forward(const FscMlpDims* dims, int64_t n_atoms, const float
 int fsc_readout_mlp_backward(const FscMlpDims* dims, int64_t n_atoms, const float* x, const float* weights,
                              const float* grad_energy, float* grad_x, hipStream_t stream);
 
+/* ------------------------------------------------------------------ expert readout
+ * A mixture of experts on the rows of per-atom invariants, between a trunk's readout features and its energy
+ * head: norm, router, gated products.  No counterpart in the reference (its head is one MainNet, models/mlp.py:8-66).
+ * Element types: */
+#define FSC_F32 0
+#define FSC_BF16 1
+#define FSC_I8 2
+
+/* Root-mean-square norm of `rows` rows of `width` values (last dimension contiguous, row strides in elements):
+ *   z = x + residual (rounded to the rows' type; residual null: z is x and is not written)
+ *   rstd = 1 / sqrt(mean z^2 + eps), y = (z rstd) weight
+ * dtype of x, residual, y, z: FSC_F32 or FSC_BF16; weight FSC_F32 or the rows' type.  y and z are contiguous.
+ * fsc_rms_norm_q8 gives y in codes and a scale for each row: scale = max |y| / 127, code = rint(y (127 / max |y|))
+ * (0 in a row of zeros; a row with a NaN has a NaN scale).  rstd is rounded from a 64-bit sum, so codes do not
+ * depend on the order of additions. */
+int fsc_rms_norm_forward(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int64_t x_stride,
+                         int64_t residual_stride, const void* x, const void* residual, const void* weight, float eps,
+                         void* y, void* z, float* rstd, hipStream_t stream);
+int fsc_rms_norm_q8(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int64_t x_stride,
+                    int64_t residual_stride, const void* x, const void* residual, const void* weight, float eps,
+                    int8_t* codes, float* scales, void* z, hipStream_t stream);
+/* Gradients: dx = rstd (g - zn mean(g zn)) + dz with g = dy weight, zn = z rstd (dz null: 0), the gradient of x and
+ * of the residual; dweight = sum over rows of dy zn.  dx or dweight null: not wanted; dweight needs the workspace. */
+int fsc_rms_norm_workspace(int64_t rows, int32_t width, int64_t* floats);
+int fsc_rms_norm_backward(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int64_t z_stride,
+                          int64_t dy_stride, int64_t dz_stride, const void* z, const void* weight, const float* rstd,
+                          float eps, const void* dy, const void* dz, void* dx, void* dweight, float* workspace,
+                          hipStream_t stream);
+
+/* Router: index and weight [rows][k] of the k experts with the largest biased score c = s + bias (bias null: 0),
+ * in falling order of c, ties to the lowest expert; s = softmax(logits) (score 0) or sigmoid(logits) (score 1).
+ * groups > 1: only experts of the groups_kept groups of largest rank, the sum of a group's group_best (1 or 2)
+ * largest c.  An expert with a logit or c of -inf is never chosen; slots left over have index -1 and weight 0.
+ * weight = scale s / (sum of the row's chosen s if renormalise, else 1).  A row with a NaN gets experts 0..k-1 and
+ * NaN weights.  At most 512 experts, 16 choices, 128 groups; logits FSC_F32 or FSC_BF16.
+ * Backward: dlogits [rows][n_experts] (contiguous, the logits' type) from dweight [rows][k]. */
+int fsc_route_experts(int64_t rows, int32_t n_experts, int32_t dtype, int64_t logits_stride, const void* logits,
+                      const float* bias, int32_t k, int32_t score, int32_t groups, int32_t groups_kept,
+                      int32_t group_best, int32_t renormalise, float scale, int32_t* index, float* weight,
+                      hipStream_t stream);
+int fsc_route_experts_backward(int64_t rows, int32_t n_experts, int32_t dtype, int64_t logits_stride,
+                               const void* logits, const int32_t* index, const float* weight, const float* dweight,
+                               int32_t k, int32_t score, int32_t renormalise, float scale, void* dlogits,
+                               hipStream_t stream);
+
+/* The experts' products: y_t = sum_j weight_tj W_out[e] (silu(W_in[e][:F] x_t) * (W_in[e][F:] x_t)), e = index_tj,
+ * with w_in [n_experts][2 hidden][width], w_out [n_experts][width][hidden] and index, weight [rows][k]; an index
+ * outside [0, n_experts) adds nothing.  dtype of x, w_in, w_out, y and the gradients: FSC_F32 (products as accurate
+ * as fp32 ones) or FSC_BF16 (32-bit sums); weight and dweight are fp32.
+ * fsc_expert_sizes: int32 of a plan, floats that the forward keeps for the backward, bytes of the two workspaces
+ * (64-byte aligned).  fsc_expert_plan sorts the slots by expert (stable); one plan serves forward and backward.
+ * saved null: the forward keeps nothing.  Backward outputs that are null are not computed. */
+typedef struct FscExpertDims {
+  int64_t rows;
+  int32_t width, hidden, n_experts, k, dtype;
+} FscExpertDims;
+int fsc_expert_sizes(const FscExpertDims* dims, int64_t* plan_ints, int64_t* saved_floats, int64_t* forward_bytes,
+                     int64_t* backward_bytes);
+int fsc_expert_plan(const FscExpertDims* dims, const int32_t* index, int32_t* plan, hipStream_t stream);
+int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const void* x, const int32_t* plan,
+                           const float* weight, const void* w_in, const void* w_out, float* saved, void* workspace,
+                           void* y, hipStream_t stream);
+int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t dy_stride, const void* dy,
+                            const void* x, const int32_t* plan, const float* weight, const void* w_in,
+                            const void* w_out, const float* saved, void* workspace, void* dx, float* dweight,
+                            void* dw_in, void* dw_out, hipStream_t stream);
+/* The same with dtype FSC_I8: codes x [rows][width] with a scale for each row, weights in codes with a scale for each
+ * of their rows (w_in_scale [n_experts][2 hidden], w_out_scale [n_experts][width]).  The hidden values are held in
+ * codes with a unit for each row and 128 columns (unit = max / 127, code = rint(h (127 / max))); products of
+ * codes are whole numbers, everything else is fp32; y is bf16. */
+int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t* x, const float* x_scale,
+                      const int32_t* plan, const float* weight, const int8_t* w_in, const float* w_in_scale,
+                      const int8_t* w_out, const float* w_out_scale, void* workspace, void* y, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
