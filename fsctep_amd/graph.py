@@ -131,6 +131,13 @@ def species_rows(graph: Graph, device) -> torch.Tensor:
     return torch.arange(graph.n_species, device=device)
 
 
+def atomic_numbers(graph: Graph) -> torch.Tensor:
+    """Atomic number of each node, as the graph was prepared from (ids out of range clamped)."""
+    if graph.species_z is None:
+        return graph.node_species.long()
+    return graph.species_z.index_select(0, graph.node_species.long())
+
+
 def poison_invalid(e: torch.Tensor, graph: Graph, pos: torch.Tensor | None = None,
                    edge_vec: torch.Tensor | None = None) -> torch.Tensor:
     """NaN energies when the graph preparation found an out-of-range edge or species id (the ids were

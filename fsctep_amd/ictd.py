@@ -22,7 +22,7 @@ import torch.nn.functional as F
 
 from . import ictd_ops
 from .readout_ops import ReadoutMaps, prepare_gram, readout_features
-from .graph import Graph, poison_invalid, prepare_species_graph, species_rows
+from .graph import Graph, atomic_numbers, poison_invalid, prepare_species_graph, species_rows
 from .ictd_basis import canonical, coupling, layout_full, layout_o3
 from .sparse import MainNet, RobustScalarWeightedSum, _radial_mlp, readout_energy
 
@@ -136,6 +136,8 @@ class _ICTDTrunk(nn.Module):
             self.physical_tensor_heads = nn.ModuleDict(
                 {"dipole": nn.ModuleDict({"1": nn.Linear(nC, 1, bias=False)})})
             self._dipole = True
+        # fsctep_amd.experts.ExpertReadout on the invariants before the energy head, or None (as the reference)
+        self.readout_experts = None
         self._cache = {}
 
     def _make_layout(self, preset, active, phys):
@@ -220,7 +222,7 @@ class _ICTDTrunk(nn.Module):
         for tp, fc2 in zip(self.tp2_layers, self.fc2_layers):
             feats.append(ictd_ops.ictd_conv_apply(feats[-1], Y, self._gates(fc2, r), tp.weight.detach(),
                                                   self._wt(tp), cg, g, self.layout_id))
-        e, dip = self.readout(feats, batch, cell.shape[0], factors, with_dipole)
+        e, dip = self.readout(feats, batch, cell.shape[0], factors, with_dipole, species=self._expert_species(g))
         return poison_invalid(e, g, pos, edge_vec), dip
 
     def _field_term(self, Y, external_tensor, src_batch, detach: bool):
@@ -268,7 +270,8 @@ class _ICTDTrunk(nn.Module):
             gates = T.radial_full(r, fc2, self.max_radius, self.function_type)
             feats.append(ictd_ops.ictd_conv_apply(feats[-1], Y, gates, tp.weight, self._wt(tp), cg, g,
                                                   self.layout_id))
-        e, dip = self.readout(feats, batch, cell.shape[0], factors, with_dipole, train=True)
+        e, dip = self.readout(feats, batch, cell.shape[0], factors, with_dipole, train=True,
+                              species=self._expert_species(g))
         return poison_invalid(e, g, pos, edge_vec), dip
 
     def _gates(self, fc, r):
@@ -281,7 +284,10 @@ class _ICTDTrunk(nn.Module):
     def _wread(self, i, k):
         return self.W_read[_key_str(k)] if self.o3 else self.W_read[i]
 
-    def readout(self, feats, batch, n_graphs, factors, with_dipole=True, train=False):
+    def _expert_species(self, g: Graph):
+        return None if self.readout_experts is None else atomic_numbers(g)
+
+    def readout(self, feats, batch, n_graphs, factors, with_dipole=True, train=False, species=None):
         """Gram bilinear + 0e products + MainNet (full :977-1033, o3 :987-1030), re-split included: the
         Gram inputs (the reference's channel-major flatten, layer concatenation and re-split by key)
         and the per-key squared norms of the layer concatenation come from one fused readout op
@@ -307,6 +313,8 @@ class _ICTDTrunk(nn.Module):
                 sq = torch.cat([sq, scalars * scalars], dim=-1)
             outs.append(sq * factors[i])
         f = torch.cat(outs, dim=-1)
+        if self.readout_experts is not None:
+            f = self.readout_experts(f, species, differentiable=train)
         e = self.weighted_sum(self.proj_total(f)) if train else readout_energy(self.proj_total, self.weighted_sum, f)
         dip = None
         if self._dipole and with_dipole:

@@ -27,7 +27,7 @@ import torch.nn.functional as F
 
 from . import ops
 from .readout_ops import ReadoutMaps, prepare_gram, readout_features
-from .graph import Graph, poison_invalid, prepare_species_graph, species_rows
+from .graph import Graph, atomic_numbers, poison_invalid, prepare_species_graph, species_rows
 
 _COMPS = ((0, 1), (1, 4), (4, 13))   # component ranges of ranks 0, 1, 2
 
@@ -231,6 +231,8 @@ class PureCartesianSparseTransformerLayer(nn.Module):
         # products of the conv2..n channel mix: "fp32" (fp32-accurate split products, the default) or "bf16"
         # (one bf16 MFMA per product with fp32 accumulation; an MI355X option, not in the reference)
         self.channel_mix_precision = "fp32"
+        # fsctep_amd.experts.ExpertReadout on the invariants before the energy head, or None (as the reference)
+        self.readout_experts = None
 
     # ------------------------------------------------------------------ graph handling
     def prepare(self, edge_src, edge_dst, edge_shifts, num_nodes, A, pos=None) -> Graph:
@@ -290,7 +292,7 @@ class PureCartesianSparseTransformerLayer(nn.Module):
             bk1, bk6 = conv.prepared_weights()
             h = ops.radial_hidden(r, conv.fc, self.max_radius, self.function_type)
             feats.append(ops.sparse_conv_apply(feats[-1], h, n, bk1, bk6, g, self._precision_code()))
-        return poison_invalid(self.readout(feats), g, pos)
+        return poison_invalid(self.readout(feats, species=self._expert_species(g)), g, pos)
 
     def _forward_train(self, pos, batch, cell, g: Graph):
         """The training step: geometry, radial MLPs, conv1 and readout as differentiable GPU torch
@@ -311,7 +313,7 @@ class PureCartesianSparseTransformerLayer(nn.Module):
             h = T.radial_hidden(r, conv.fc, self.max_radius, self.function_type)
             feats.append(ops.sparse_conv_apply(feats[-1], h, n, bk1, bk6, g, self._precision_code(),
                                                conv.fc[4].weight, conv.fc[4].bias))
-        return poison_invalid(self.readout(feats, train=True), g, pos)
+        return poison_invalid(self.readout(feats, train=True, species=self._expert_species(g)), g, pos)
 
     def _precision_code(self) -> int:
         prec = getattr(self, "channel_mix_precision", "fp32")
@@ -319,7 +321,10 @@ class PureCartesianSparseTransformerLayer(nn.Module):
             raise ValueError(f"channel_mix_precision must be 'fp32' or 'bf16', got {prec!r}")
         return 1 if prec == "bf16" else 0
 
-    def readout(self, feats, train: bool = False):
+    def _expert_species(self, g: Graph):
+        return None if self.readout_experts is None else atomic_numbers(g)
+
+    def readout(self, feats, train: bool = False, species=None):
         """pure_cartesian_sparse_layers.py:769-833 on x[N][13][C] features: the rank-L blocks of all
         layers (t_L = cat_l x_l[:, block L, :]) feed product_3 and their squared norms
         sum_m x^2 / 3^{L/2} the invariants, all assembled by one fused readout op (``train``: by its
@@ -343,6 +348,8 @@ class PureCartesianSparseTransformerLayer(nn.Module):
         # invariants in the reference order: layer-major, then rank L
         invs = (sq.view(-1, len(_COMPS), nL, self.channels) * self._readout_cache[skey]).transpose(1, 2)
         f5 = torch.cat([invs.flatten(1), f3 * f3], dim=-1)
+        if self.readout_experts is not None:
+            f5 = self.readout_experts(f5, species, differentiable=train)
         if train:
             return self.weighted_sum(self.proj_total(f5))
         return readout_energy(self.proj_total, self.weighted_sum, f5)

@@ -216,3 +216,36 @@ def readout_features(feats, Ws, scales, maps):
         sqs.append(torch.cat([(f[:, comp:comp + d, :] ** 2).sum(1) for f in feats], dim=1))
         comp += d
     return scalars, torch.stack(sqs, dim=1)
+
+
+# ------------------------------------------------------------------ expert readout (rms_norm.hip, expert_mlp.hip)
+def rms_norm(x, weight, residual=None, eps: float = 1e-6):
+    """(y, z) of ``expert_ops.rms_norm``, differentiable to any order."""
+    z = x if residual is None else x + residual
+    return z * torch.rsqrt((z * z).mean(-1, keepdim=True) + eps) * weight, z
+
+
+def route_weights(logits, index, score: str, renormalise: bool, scale: float):
+    """The routing weights of the experts already chosen (``expert_ops.route_experts``' index), differentiable
+    in the logits to any order; 0 where the index is -1."""
+    s = torch.softmax(logits, -1) if score == "softmax" else torch.sigmoid(logits)
+    there = index >= 0
+    picked = torch.where(there, s.gather(1, index.clamp(min=0).long()), torch.zeros((), device=s.device, dtype=s.dtype))
+    if renormalise:
+        total = picked.sum(-1, keepdim=True)
+        picked = picked / torch.where(total > 0, total, torch.ones_like(total))
+    return scale * picked
+
+
+def expert_mlp(x, index, weight, w_in, w_out):
+    """``expert_ops.expert_mlp``, differentiable to any order: every expert on every row (training
+    configurations are small; the sizes follow from the tensors, so nothing waits for the GPU)."""
+    E, H, f = w_out.shape
+    there = index >= 0
+    share = weight.new_zeros(x.shape[0], E).scatter_add(1, index.clamp(min=0).long(),
+                                                        torch.where(there, weight, torch.zeros_like(weight)))
+    y = torch.zeros_like(x)
+    for e in range(E):
+        a = x @ w_in[e].t()
+        y = y + share[:, e:e + 1] * ((F.silu(a[:, :f]) * a[:, f:]) @ w_out[e].t())
+    return y
