@@ -84,9 +84,9 @@ SIGNATURES = {
     "fsc_route_experts_backward": [_i64, _i32, _i32, _i64, _p, _p, _p, _p, _i32, _i32, _i32, _f32, _p, _p],
     "fsc_expert_sizes": [_p, _pi64, _pi64, _pi64, _pi64],
     "fsc_expert_plan": [_p, _p, _p, _p],
-    "fsc_expert_mlp_forward": [_p, _i64] + [_p] * 9,
-    "fsc_expert_mlp_backward": [_p, _i64, _i64] + [_p] * 13,
-    "fsc_expert_mlp_q8": [_p, _i64] + [_p] * 11,
+    "fsc_expert_mlp_forward": [_p, _i64] + [_p] * 10,
+    "fsc_expert_mlp_backward": [_p, _i64, _i64] + [_p] * 14,
+    "fsc_expert_mlp_q8": [_p, _i64] + [_p] * 12,
 }
 # the fp64 twins of the bucket functions take the same arguments (double arrays)
 SIGNATURES.update({n + "_f64": SIGNATURES[n] for n in (

@@ -17,8 +17,9 @@
 #include <type_traits>
 
 #include "common.h"
-#include "expert_plan.h"
 #include "expert_types.h"
+#include "expert_args.h"
+#include "expert_plan.h"
 #include "fsctep.h"
 
 namespace fsc {
@@ -27,36 +28,14 @@ namespace experts {
 typedef int i4v __attribute__((ext_vector_type(4)));
 
 enum Kind { F32 = 0, BF16 = 1, I8 = 2 };
-enum Mode { UP = 0, DOWN = 1, DH = 2, DX = 3, DWIN = 4, DWOUT = 5 };
 
 constexpr int NT = 256;          // four waves, two by two
 constexpr int BN = 128;          // rows of the tile's weight operand
-constexpr int QG = 128;          // hidden columns that share a scale in 8 bits
 
 template <int KIND> struct El;
 template <> struct El<F32> { using T = float; static constexpr int BK = 32, CE = 8, PL = 3; };
 template <> struct El<BF16> { using T = __bf16; static constexpr int BK = 64, CE = 8, PL = 1; };
 template <> struct El<I8> { using T = int8_t; static constexpr int BK = 128, CE = 16, PL = 1; };
-
-struct Args {
-  // sizes: rows T, slots M = T k, width H, hidden F (row length ldf in the arrays between), experts E
-  int64_t T, M;
-  int H, F, ldf, ldo, E, k, n_tiles;
-  int64_t xs, ds;                   // row strides of x and dy, in elements
-  const int32_t *offsets, *slot_of, *tiles;
-  const void *x, *w_in, *w_out, *dy;
-  const float* weight;              // [M]
-  float* a;                         // [M][2 ldf] gate and up before the activation (null: not kept)
-  void* h;                          // [M][ldf]
-  float* o;                         // [M][ldo] products by slot, before they are combined
-  void* da;                         // [M][2 ldf]
-  void* hw;                         // [M][ldf] weight h, for dw_out (null: not wanted)
-  float* dwpart;                    // [n column tiles of dh][M] partial dweight by sorted position
-  void *dw_in, *dw_out;
-  // 8 bits: scales of x's rows, of the weights' rows and of h's groups [M][ldf / QG]
-  const float *xscale, *in_scale, *out_scale;
-  float* hscale;
-};
 
 // ---------------------------------------------------------------- tiles of the operands
 // A chunk is 16 bytes of an LDS plane: 8 values (16 in 8 bits) along the row.  Straight operands (rows of the tile
@@ -177,24 +156,6 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
       }
     }
   }
-}
-
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
-
-__device__ __forceinline__ void store4(float* p, const f4& v, int n) {
-  if (n >= 4 && (uintptr_t)p % 16 == 0) st4(p, v);
-  else
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) p[j] = v[j];
-}
-__device__ __forceinline__ void store4(__bf16* p, const f4& v, int n) {
-  typedef __bf16 bf4 __attribute__((ext_vector_type(4)));
-  if (n >= 4 && (uintptr_t)p % 8 == 0) *reinterpret_cast<bf4*>(p) = bf4{(__bf16)v.x, (__bf16)v.y, (__bf16)v.z, (__bf16)v.w};
-  else
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (j < n) p[j] = (__bf16)v[j];
 }
 
 // Workgroup -> (row tile, column tile).  Workgroup w runs on XCD w % 8: each XCD takes a contiguous run of row
@@ -468,7 +429,8 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
 // ---------------------------------------------------------------- weight gradients
 // dw_in[e][m][n] = sum over expert e's positions of da[.][m] x[.][n]; dw_out[e][m][n] = that of dy[.][m] hw[.][n].
 // The matrix of the contiguous output index n is the MFMA's A operand; both are turned.
-template <int KIND, typename S, int MODE, bool VEC>
+// FEW: h's arrays lie by slot and the block finds the expert's slots itself.
+template <int KIND, typename S, int MODE, bool VEC, bool FEW>
 __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
   using E = El<KIND>;
   using T = typename E::T;
@@ -484,7 +446,15 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
   int e, c;
   if (!tile_of(g.E, ta * tb, e, c)) return;
   const int b0 = (c / ta) * BN, a0 = (c % ta) * BN;
-  const int64_t p0 = g.offsets[e], cnt = g.offsets[e + 1] - p0;
+  __shared__ int16_t list[FEW ? FEW_SLOTS : 1];
+  int64_t p0 = 0, cnt;
+  if constexpr (FEW) {
+    cnt = few_slots(g, e, list);
+    __syncthreads();
+  } else {
+    p0 = g.offsets[e];
+    cnt = g.offsets[e + 1] - p0;
+  }
   TT A;
   TB B;
   auto fetch = [&](int64_t k0) {
@@ -496,12 +466,13 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
       const RA* pa = nullptr;
       const RB* pb = nullptr;
       if (k < cnt) {
-        const int64_t tok = g.slot_of[p0 + k] / g.k;
+        const int64_t pos = FEW ? list[k] : p0 + k;
+        const int64_t tok = (FEW ? list[k] : g.slot_of[pos]) / g.k;
         if (MODE == DWIN) {
           pa = (const RA*)g.x + tok * g.xs + a0 + n;
-          pb = (const RB*)g.da + (p0 + k) * 2 * g.ldf + b0 + n;
+          pb = (const RB*)g.da + pos * 2 * g.ldf + b0 + n;
         } else {
-          pa = (const RA*)g.hw + (p0 + k) * g.ldf + a0 + n;
+          pa = (const RA*)g.hw + pos * g.ldf + a0 + n;
           pb = (const RB*)g.dy + tok * g.ds + b0 + n;
         }
       }
@@ -547,9 +518,17 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
 }
 
 // ---------------------------------------------------------------- rows from their experts, in slot order
+// The row of a slot in the arrays between the kernels, -1 for a slot with no expert.
+__device__ __forceinline__ int place_of(const int32_t* place, const int32_t* index, int E, int64_t s) {
+  if (place) return place[s];
+  const int e = index[s];
+  return e >= 0 && e < E ? (int)s : -1;
+}
+
 template <typename T>
 __global__ __launch_bounds__(NT) void combine_kernel(int64_t rows, int H, int ldo, int k,
                                                      const int32_t* __restrict__ place,
+                                                     const int32_t* __restrict__ index, int E,
                                                      const float* __restrict__ weight, const float* __restrict__ o,
                                                      T* __restrict__ y) {
   const int nv = (H + 3) / 4;
@@ -559,7 +538,7 @@ __global__ __launch_bounds__(NT) void combine_kernel(int64_t rows, int H, int ld
     const int c = (int)(i - t * nv) * 4;
     f4 s = {0.f, 0.f, 0.f, 0.f};
     for (int j = 0; j < k; ++j) {
-      const int p = place[t * k + j];
+      const int p = place_of(place, index, E, t * k + j);
       if (p < 0) continue;
       const float w = weight ? weight[t * k + j] : 1.f;
       s += w * ld4(o + (int64_t)p * ldo + c);
@@ -570,10 +549,10 @@ __global__ __launch_bounds__(NT) void combine_kernel(int64_t rows, int H, int ld
 
 // dweight by slot: the partial sums over the column tiles, in order; 0 for a slot with no expert.
 __global__ __launch_bounds__(NT) void dweight_kernel(int64_t M, int parts, const int32_t* __restrict__ place,
-                                                     const float* __restrict__ part, float* __restrict__ dweight) {
+                                                     const int32_t* __restrict__ index, int E, const float* __restrict__ part, float* __restrict__ dweight) {
   const int64_t s = (int64_t)blockIdx.x * NT + threadIdx.x;
   if (s >= M) return;
-  const int p = place[s];
+  const int p = place_of(place, index, E, s);
   float t = 0.f;
   if (p >= 0)
     for (int i = 0; i < parts; ++i) t += part[(int64_t)i * M + p];
@@ -606,6 +585,10 @@ __global__ __launch_bounds__(NT) void quant_kernel(Args g) {
 inline int up8(int v) { return (v + 7) / 8 * 8; }
 inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 
+// Few rows: at most 16 for each expert on average, and few enough slots for a block to look through.  The few-rows
+// kernels read an expert's weights once for 16 rows, the tiles once for up to 128.
+inline bool few(int64_t M, int E) { return M <= FEW_SLOTS && M <= 16 * (int64_t)E; }
+
 // Rows of a tile by the rows that an expert has on average: the weights are read once for each tile of an expert,
 // and rows that a tile lacks are still computed.
 inline int tile_rows(int64_t M, int E) {
@@ -632,19 +615,19 @@ void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
   else go(std::integral_constant<int, 1>{});
 }
 
-template <int KIND, typename S, int MODE>
+template <int KIND, typename S, int MODE, bool FEW = false>
 void launch_weights(const Args& g, bool vec, hipStream_t st) {
   const int64_t na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;
   const unsigned grid = tile_grid(g.E, ((na + BN - 1) / BN) * ((nb + BN - 1) / BN));
-  if (vec) weights_kernel<KIND, S, MODE, true><<<grid, NT, 0, st>>>(g);
-  else weights_kernel<KIND, S, MODE, false><<<grid, NT, 0, st>>>(g);
+  if (vec) weights_kernel<KIND, S, MODE, true, FEW><<<grid, NT, 0, st>>>(g);
+  else weights_kernel<KIND, S, MODE, false, FEW><<<grid, NT, 0, st>>>(g);
 }
 
 template <typename T>
-void launch_combine(const Args& g, const int32_t* place, const float* weight, T* y, hipStream_t st) {
+void launch_combine(const Args& g, const float* weight, T* y, hipStream_t st) {
   const int64_t n = g.T * ((g.H + 3) / 4);
   const unsigned grid = (unsigned)std::min<int64_t>((n + NT - 1) / NT, 1 << 20);
-  combine_kernel<T><<<grid, NT, 0, st>>>(g.T, g.H, g.ldo, g.k, place, weight, g.o, y);
+  combine_kernel<T><<<grid, NT, 0, st>>>(g.T, g.H, g.ldo, g.k, g.place, g.index, g.E, weight, g.o, y);
 }
 
 int check_dims(const FscExpertDims* d, bool q8) {
@@ -667,7 +650,8 @@ inline int ldo_of(const FscExpertDims& d) { return (d.width + 3) / 4 * 4; }
 // bf16 rows, few for each expert: the products wait for the weights from memory, so what is held between the
 // kernels stays in fp32 and the products run as those of fp32 rows do.
 inline bool fine(const FscExpertDims& d) {
-  return d.dtype == FSC_BF16 && tile_rows(d.rows * d.k, d.n_experts) == 32;
+  const int64_t M = d.rows * d.k;
+  return d.dtype == FSC_BF16 && (few(M, d.n_experts) || tile_rows(M, d.n_experts) == 32);
 }
 // bytes of a value of the arrays between the kernels
 inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 : d.dtype == FSC_F32 || fine(d) ? 4 : 2; }
@@ -696,7 +680,7 @@ inline Space backward_space(const FscExpertDims& d) {
   s.o = at; at += align64(M * ldo_of(d) * 4);
   s.da = at; at += align64(M * 2 * ldf * size);
   s.hw = at; at += align64(M * ldf * size);
-  s.part = at; at += align64(M * ((d.hidden + BN - 1) / BN) * 4);
+  s.part = at; at += align64(M * ((d.hidden + 63) / 64) * 4);
   s.total = at;
   return s;
 }
@@ -711,37 +695,60 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
   g.ldo = ldo_of(d);
   g.E = d.n_experts;
   g.k = d.k;
-  g.n_tiles = p.n_tiles;
-  g.offsets = p.offsets;
-  g.slot_of = p.slot_of;
-  g.tiles = p.tiles;
+  if (!few(g.M, g.E)) {
+    g.n_tiles = p.n_tiles;
+    g.offsets = p.offsets;
+    g.slot_of = p.slot_of;
+    g.tiles = p.tiles;
+    g.place = p.place;
+  }
   return g;
 }
 
 template <int KIND, typename S>
-void forward(Args g, const Plan& p, int tile, void* y, hipStream_t st) {
+void forward(Args g, int tile, void* y, hipStream_t st) {
   const bool vin = vec_ok(g.x, g.xs, sizeof(S), g.H) && vec_ok(g.w_in, g.H, sizeof(S), g.H);
   const bool vout = vec_ok(g.w_out, g.F, sizeof(S), g.F);
-  launch_rows<KIND, S, UP>(g, tile, vin, st);
-  if constexpr (KIND == I8) quant_kernel<<<(unsigned)((g.M * (g.ldf / QG) + 3) / 4), NT, 0, st>>>(g);
-  launch_rows<KIND, S, DOWN>(g, tile, vout, st);
+  if (!g.place) {
+    if constexpr (KIND == I8) {
+      few_launch_q8(g, vin, vout, st);
+    } else {
+      few_launch<S>(UP, g, vin, st);
+      few_launch<S>(DOWN, g, vout, st);
+    }
+  } else {
+    launch_rows<KIND, S, UP>(g, tile, vin, st);
+    if constexpr (KIND == I8) quant_kernel<<<(unsigned)((g.M * (g.ldf / QG) + 3) / 4), NT, 0, st>>>(g);
+    launch_rows<KIND, S, DOWN>(g, tile, vout, st);
+  }
   using Y = std::conditional_t<KIND == I8, __bf16, S>;
-  launch_combine<Y>(g, p.place, g.weight, (Y*)y, st);
+  launch_combine<Y>(g, g.weight, (Y*)y, st);
 }
 
 template <int KIND, typename S>
-void backward(Args g, const Plan& p, int tile, void* dx, float* dweight, hipStream_t st) {
+void backward(Args g, int tile, void* dx, float* dweight, hipStream_t st) {
   const bool vdy = vec_ok(g.dy, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.xs, sizeof(S), g.H);
   const bool vin = vec_ok(g.w_in, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.F, sizeof(S), g.F);
-  launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
+  const bool by_slot = !g.place;
+  if (by_slot) few_launch<S>(DH, g, vout, st);
+  else launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
   if (dweight)
-    dweight_kernel<<<(unsigned)((g.M + NT - 1) / NT), NT, 0, st>>>(g.M, (g.F + BN - 1) / BN, p.place, g.dwpart, dweight);
+    dweight_kernel<<<(unsigned)((g.M + NT - 1) / NT), NT, 0, st>>>(
+        g.M, by_slot ? few_parts(g.F, sizeof(S)) : (g.F + BN - 1) / BN, g.place, g.index, g.E, g.dwpart, dweight);
   if (dx) {
-    launch_rows<KIND, S, DX>(g, tile, vin, st);
-    launch_combine<S>(g, p.place, nullptr, (S*)dx, st);
+    if (by_slot) few_launch<S>(DX, g, vin, st);
+    else launch_rows<KIND, S, DX>(g, tile, vin, st);
+    launch_combine<S>(g, nullptr, (S*)dx, st);
   }
-  if (g.dw_in) launch_weights<KIND, S, DWIN>(g, vx, st);
-  if (g.dw_out) launch_weights<KIND, S, DWOUT>(g, vdy, st);
+  if (by_slot) {
+    if constexpr (KIND == F32) {
+      if (g.dw_in) launch_weights<F32, S, DWIN, true>(g, vx, st);
+      if (g.dw_out) launch_weights<F32, S, DWOUT, true>(g, vdy, st);
+    }
+  } else {
+    if (g.dw_in) launch_weights<KIND, S, DWIN>(g, vx, st);
+    if (g.dw_out) launch_weights<KIND, S, DWOUT>(g, vdy, st);
+  }
 }
 
 }  // namespace experts
@@ -755,7 +762,7 @@ int fsc_expert_sizes(const FscExpertDims* dims, int64_t* plan_ints, int64_t* sav
   if (int rc = check_dims(dims, dims && dims->dtype == FSC_I8)) return rc;
   FSC_CHECK_ARG(plan_ints && saved_floats && forward_bytes && backward_bytes, "expert_sizes: null output");
   const int64_t M = dims->rows * dims->k;
-  *plan_ints = fsc::experts::plan_ints(M, dims->n_experts, tile_rows(M, dims->n_experts));
+  *plan_ints = few(M, dims->n_experts) ? 0 : fsc::experts::plan_ints(M, dims->n_experts, tile_rows(M, dims->n_experts));
   *saved_floats = dims->dtype == FSC_I8 ? 0 : M * 2 * ldf_of(*dims);
   *forward_bytes = forward_space(*dims).total;
   *backward_bytes = dims->dtype == FSC_I8 ? 0 : backward_space(*dims).total;
@@ -766,50 +773,54 @@ int fsc_expert_plan(const FscExpertDims* dims, const int32_t* index, int32_t* pl
   using namespace fsc::experts;
   if (int rc = check_dims(dims, dims && dims->dtype == FSC_I8)) return rc;
   const int64_t M = dims->rows * dims->k;
-  FSC_CHECK_ARG(plan && (M == 0 || index), "expert_plan: null array");
+  if (few(M, dims->n_experts)) return 0;       // the products find their rows themselves
+  FSC_CHECK_ARG(plan && index, "expert_plan: null array");
   const int tile = tile_rows(M, dims->n_experts);
   launch_plan(plan_of(plan, M, dims->n_experts, tile), M, dims->n_experts, tile, index, stream);
   return fsc::check_launch("expert_plan") ? 2 : 0;
 }
 
-int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const void* x, const int32_t* plan,
-                           const float* weight, const void* w_in, const void* w_out, float* saved, void* workspace,
-                           void* y, hipStream_t stream) {
+int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const void* x, const int32_t* index,
+                           const int32_t* plan, const float* weight, const void* w_in, const void* w_out, float* saved,
+                           void* workspace, void* y, hipStream_t stream) {
   using namespace fsc::experts;
   if (int rc = check_dims(dims, false)) return rc;
   if (dims->rows == 0) return 0;
-  FSC_CHECK_ARG(x && plan && weight && w_in && w_out && workspace && y, "expert_mlp_forward: null array");
-  FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_forward: negative row stride");
   const int64_t M = dims->rows * dims->k;
+  FSC_CHECK_ARG(x && index && (plan || few(M, dims->n_experts)) && weight && w_in && w_out && workspace && y,
+                "expert_mlp_forward: null array");
+  FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_forward: negative row stride");
   const int tile = tile_rows(M, dims->n_experts);
   const Plan p = plan_of(const_cast<int32_t*>(plan), M, dims->n_experts, tile);
   Args g = args_of(*dims, p);
   const Space s = forward_space(*dims);
   char* ws = (char*)workspace;
+  g.index = index;
   g.x = x; g.xs = x_stride; g.weight = weight; g.w_in = w_in; g.w_out = w_out; g.a = saved;
   g.h = ws + s.h;
   g.o = (float*)(ws + s.o);
-  if (dims->dtype == FSC_F32) forward<F32, float>(g, p, tile, y, stream);
-  else if (fine(*dims)) forward<F32, __bf16>(g, p, tile, y, stream);
-  else forward<BF16, __bf16>(g, p, tile, y, stream);
+  if (dims->dtype == FSC_F32) forward<F32, float>(g, tile, y, stream);
+  else if (fine(*dims)) forward<F32, __bf16>(g, tile, y, stream);
+  else forward<BF16, __bf16>(g, tile, y, stream);
   return fsc::check_launch("expert_mlp_forward") ? 2 : 0;
 }
 
 int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t dy_stride, const void* dy,
-                            const void* x, const int32_t* plan, const float* weight, const void* w_in,
-                            const void* w_out, const float* saved, void* workspace, void* dx, float* dweight,
+                            const void* x, const int32_t* index, const int32_t* plan, const float* weight,
+                            const void* w_in, const void* w_out, const float* saved, void* workspace, void* dx, float* dweight,
                             void* dw_in, void* dw_out, hipStream_t stream) {
   using namespace fsc::experts;
   if (int rc = check_dims(dims, false)) return rc;
   const int64_t M = dims->rows * dims->k;
-  FSC_CHECK_ARG(plan && w_in && w_out, "expert_mlp_backward: null array");
-  FSC_CHECK_ARG(M == 0 || (dy && x && weight && saved && workspace), "expert_mlp_backward: null array");
+  FSC_CHECK_ARG((plan || few(M, dims->n_experts)) && w_in && w_out, "expert_mlp_backward: null array");
+  FSC_CHECK_ARG(M == 0 || (dy && x && index && weight && saved && workspace), "expert_mlp_backward: null array");
   FSC_CHECK_ARG(x_stride >= 0 && dy_stride >= 0, "expert_mlp_backward: negative row stride");
   const int tile = tile_rows(M, dims->n_experts);
   const Plan p = plan_of(const_cast<int32_t*>(plan), M, dims->n_experts, tile);
   Args g = args_of(*dims, p);
   const Space s = backward_space(*dims);
   char* ws = (char*)workspace;
+  g.index = index;
   g.x = x; g.xs = x_stride; g.dy = dy; g.ds = dy_stride; g.weight = weight; g.w_in = w_in; g.w_out = w_out;
   g.a = const_cast<float*>(saved);
   g.o = (float*)(ws + s.o);
@@ -820,44 +831,45 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
   g.dw_out = dw_out;
   if (M == 0) {              // no rows: zero weight gradients, written by the products' empty sums
     if (dims->dtype == FSC_F32) {
-      if (dw_in) launch_weights<F32, float, DWIN>(g, false, stream);
-      if (dw_out) launch_weights<F32, float, DWOUT>(g, false, stream);
+      if (dw_in) launch_weights<F32, float, DWIN, true>(g, false, stream);
+      if (dw_out) launch_weights<F32, float, DWOUT, true>(g, false, stream);
     } else {
-      if (dw_in) launch_weights<BF16, __bf16, DWIN>(g, false, stream);
-      if (dw_out) launch_weights<BF16, __bf16, DWOUT>(g, false, stream);
+      if (dw_in) launch_weights<F32, __bf16, DWIN, true>(g, false, stream);
+      if (dw_out) launch_weights<F32, __bf16, DWOUT, true>(g, false, stream);
     }
   } else if (dims->dtype == FSC_F32) {
-    backward<F32, float>(g, p, tile, dx, dweight, stream);
+    backward<F32, float>(g, tile, dx, dweight, stream);
   } else if (fine(*dims)) {
-    backward<F32, __bf16>(g, p, tile, dx, dweight, stream);
+    backward<F32, __bf16>(g, tile, dx, dweight, stream);
   } else {
-    backward<BF16, __bf16>(g, p, tile, dx, dweight, stream);
+    backward<BF16, __bf16>(g, tile, dx, dweight, stream);
   }
   return fsc::check_launch("expert_mlp_backward") ? 2 : 0;
 }
 
 int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t* x, const float* x_scale,
-                      const int32_t* plan, const float* weight, const int8_t* w_in, const float* w_in_scale,
+                      const int32_t* index, const int32_t* plan, const float* weight, const int8_t* w_in, const float* w_in_scale,
                       const int8_t* w_out, const float* w_out_scale, void* workspace, void* y, hipStream_t stream) {
   using namespace fsc::experts;
   if (int rc = check_dims(dims, true)) return rc;
   if (dims->rows == 0) return 0;
-  FSC_CHECK_ARG(x && x_scale && plan && weight && w_in && w_in_scale && w_out && w_out_scale && workspace && y,
+  const int64_t M = dims->rows * dims->k;
+  FSC_CHECK_ARG(x && x_scale && index && (plan || few(M, dims->n_experts)) && weight && w_in && w_in_scale && w_out && w_out_scale && workspace && y,
                 "expert_mlp_q8: null array");
   FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_q8: negative row stride");
-  const int64_t M = dims->rows * dims->k;
   const int tile = tile_rows(M, dims->n_experts);
   const Plan p = plan_of(const_cast<int32_t*>(plan), M, dims->n_experts, tile);
   Args g = args_of(*dims, p);
   const Space s = forward_space(*dims);
   char* ws = (char*)workspace;
+  g.index = index;
   g.x = x; g.xs = x_stride; g.weight = weight; g.w_in = w_in; g.w_out = w_out;
   g.xscale = x_scale; g.in_scale = w_in_scale; g.out_scale = w_out_scale;
   g.h = ws + s.h;
   g.o = (float*)(ws + s.o);
   g.a = (float*)(ws + s.da);
   g.hscale = (float*)(ws + s.hs);
-  forward<I8, int8_t>(g, p, tile, y, stream);
+  forward<I8, int8_t>(g, tile, y, stream);
   return fsc::check_launch("expert_mlp_q8") ? 2 : 0;
 }
 

@@ -261,6 +261,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     ctx->saved_data["score"] = score;
     ctx->saved_data["renormalise"] = renormalise;
     ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({index});
     return {index, weight};
   }
@@ -330,8 +331,8 @@ std::tuple<Tensor, Tensor, Tensor> expert_mlp_forward(const Tensor& x_, const Te
   Tensor saved = at::empty({keep ? s.saved : 0}, weight.options());
   Tensor ws = at::empty({s.fwd}, x.options().dtype(at::kByte));
   check(fsc_expert_plan(&d, (const int32_t*)ptr(index), (int32_t*)mptr(plan), stream_of(x)), "fsc_expert_plan");
-  check(fsc_expert_mlp_forward(&d, stride_of(x), ptr(x), (const int32_t*)ptr(plan), (const float*)ptr(weight), ptr(w_in),
-                               ptr(w_out), (float*)mptr(saved), mptr(ws), mptr(y), stream_of(x)),
+  check(fsc_expert_mlp_forward(&d, stride_of(x), ptr(x), (const int32_t*)ptr(index), (const int32_t*)ptr(plan),
+                               (const float*)ptr(weight), ptr(w_in), ptr(w_out), (float*)mptr(saved), mptr(ws), mptr(y), stream_of(x)),
         "fsc_expert_mlp_forward");
   return {y, plan, saved};
 }
@@ -345,16 +346,16 @@ std::tuple<Tensor, Tensor, Tensor> expert_mlp_forward_meta(const Tensor& x, cons
 }
 
 // (dx, dweight, dw_in, dw_out), empty where not wanted
-std::tuple<Tensor, Tensor, Tensor, Tensor> expert_mlp_backward(const Tensor& dy_, const Tensor& x_, const Tensor& index,
+std::tuple<Tensor, Tensor, Tensor, Tensor> expert_mlp_backward(const Tensor& dy_, const Tensor& x_, const Tensor& index_,
                                                                const Tensor& weight_, const Tensor& w_in_,
                                                                const Tensor& w_out_, const Tensor& plan,
                                                                const Tensor& saved, bool want_x, bool want_weight,
                                                                bool want_in, bool want_out) {
-  require_gpu({x_, dy_, index, weight_, w_in_, w_out_, plan, saved}, "expert_mlp_backward");
-  const FscExpertDims d = expert_dims(x_, index, weight_, w_in_, w_out_, "expert_mlp_backward");
+  require_gpu({x_, dy_, index_, weight_, w_in_, w_out_, plan, saved}, "expert_mlp_backward");
+  const FscExpertDims d = expert_dims(x_, index_, weight_, w_in_, w_out_, "expert_mlp_backward");
   TORCH_CHECK(dy_.sizes() == x_.sizes() && dy_.scalar_type() == x_.scalar_type(),
               "expert_mlp_backward: dy must have x's shape and type");
-  const Tensor x = rows2d(x_, "x"), dy = rows2d(dy_, "dy"), weight = weight_.contiguous();
+  const Tensor x = rows2d(x_, "x"), dy = rows2d(dy_, "dy"), index = index_.contiguous(), weight = weight_.contiguous();
   const Tensor w_in = w_in_.contiguous(), w_out = w_out_.contiguous();
   const Sizes s = sizes_of(d);
   TORCH_CHECK(plan.scalar_type() == at::kInt && plan.is_contiguous() && plan.numel() == s.plan &&
@@ -365,7 +366,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> expert_mlp_backward(const Tensor& dy_
   };
   Tensor dx = out(want_x, x), dweight = out(want_weight, weight), dw_in = out(want_in, w_in), dw_out = out(want_out, w_out);
   Tensor ws = at::empty({s.bwd}, x.options().dtype(at::kByte));
-  check(fsc_expert_mlp_backward(&d, stride_of(x), stride_of(dy), ptr(dy), ptr(x), (const int32_t*)ptr(plan),
+  check(fsc_expert_mlp_backward(&d, stride_of(x), stride_of(dy), ptr(dy), ptr(x), (const int32_t*)ptr(index), (const int32_t*)ptr(plan),
                                 (const float*)ptr(weight), ptr(w_in), ptr(w_out), (const float*)ptr(saved), mptr(ws),
                                 mptr(dx), (float*)mptr(dweight), mptr(dw_in), mptr(dw_out), stream_of(x)),
         "fsc_expert_mlp_backward");
@@ -448,7 +449,7 @@ Tensor expert_mlp_q8(const Tensor& x_, const Tensor& x_scale_, const Tensor& ind
   Tensor plan = at::empty({s.plan}, index.options());
   Tensor ws = at::empty({s.fwd}, x.options().dtype(at::kByte));
   check(fsc_expert_plan(&d, (const int32_t*)ptr(index), (int32_t*)mptr(plan), stream_of(x)), "fsc_expert_plan");
-  check(fsc_expert_mlp_q8(&d, stride_of(x), (const int8_t*)ptr(x), (const float*)ptr(xs), (const int32_t*)ptr(plan),
+  check(fsc_expert_mlp_q8(&d, stride_of(x), (const int8_t*)ptr(x), (const float*)ptr(xs), (const int32_t*)ptr(index), (const int32_t*)ptr(plan),
                           (const float*)ptr(weight), (const int8_t*)ptr(w_in), (const float*)ptr(is),
                           (const int8_t*)ptr(w_out), (const float*)ptr(os), mptr(ws), mptr(y), stream_of(x)),
         "fsc_expert_mlp_q8");

@@ -568,7 +568,8 @@ int fsc_route_experts_backward(int64_t rows, int32_t n_experts, int32_t dtype, i
  * outside [0, n_experts) adds nothing.  dtype of x, w_in, w_out, y and the gradients: FSC_F32 (products as accurate
  * as fp32 ones) or FSC_BF16 (32-bit sums); weight and dweight are fp32.
  * fsc_expert_sizes: int32 of a plan, floats that the forward keeps for the backward, bytes of the two workspaces
- * (64-byte aligned).  fsc_expert_plan sorts the slots by expert (stable); one plan serves forward and backward.
+ * (64-byte aligned).  fsc_expert_plan sorts the slots by expert (stable); one plan serves forward and backward
+ * (with few rows its size is 0 and it may be null).
  * saved null: the forward keeps nothing.  Backward outputs that are null are not computed. */
 typedef struct FscExpertDims {
   int64_t rows;
@@ -577,19 +578,19 @@ typedef struct FscExpertDims {
 int fsc_expert_sizes(const FscExpertDims* dims, int64_t* plan_ints, int64_t* saved_floats, int64_t* forward_bytes,
                      int64_t* backward_bytes);
 int fsc_expert_plan(const FscExpertDims* dims, const int32_t* index, int32_t* plan, hipStream_t stream);
-int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const void* x, const int32_t* plan,
-                           const float* weight, const void* w_in, const void* w_out, float* saved, void* workspace,
-                           void* y, hipStream_t stream);
+int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const void* x, const int32_t* index,
+                           const int32_t* plan, const float* weight, const void* w_in, const void* w_out, float* saved,
+                           void* workspace, void* y, hipStream_t stream);
 int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t dy_stride, const void* dy,
-                            const void* x, const int32_t* plan, const float* weight, const void* w_in,
-                            const void* w_out, const float* saved, void* workspace, void* dx, float* dweight,
+                            const void* x, const int32_t* index, const int32_t* plan, const float* weight,
+                            const void* w_in, const void* w_out, const float* saved, void* workspace, void* dx, float* dweight,
                             void* dw_in, void* dw_out, hipStream_t stream);
 /* The same with dtype FSC_I8: codes x [rows][width] with a scale for each row, weights in codes with a scale for each
  * of their rows (w_in_scale [n_experts][2 hidden], w_out_scale [n_experts][width]).  The hidden values are held in
  * codes with a unit for each row and 128 columns (unit = max / 127, code = rint(h (127 / max))); products of
  * codes are whole numbers, everything else is fp32; y is bf16. */
 int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t* x, const float* x_scale,
-                      const int32_t* plan, const float* weight, const int8_t* w_in, const float* w_in_scale,
+                      const int32_t* index, const int32_t* plan, const float* weight, const int8_t* w_in, const float* w_in_scale,
                       const int8_t* w_out, const float* w_out_scale, void* workspace, void* y, hipStream_t stream);
 
 #ifdef __cplusplus
