@@ -18,7 +18,8 @@ struct Args {
   int H, F, ldf, ldo, E, k, n_tiles;
   int64_t xs, ds;                   // row strides of x and dy, in elements
   const int32_t *index;             // [M]
-  const int32_t *offsets, *slot_of, *tiles, *place;   // the rows by expert; null where there are few rows
+  uint32_t k_inv;                   // ceil(2^20 / k): slot / k = slot k_inv / 2^20 for the few-rows slots (below 1,024)
+  const int32_t *offsets, *slot_of, *row_of, *tiles, *place;   // the rows by expert; null where there are few rows
   const void *x, *w_in, *w_out, *dy;
   const float* weight;              // [M]
   // arrays between the kernels, a row for each sorted position, or for each slot where there are few rows
@@ -42,7 +43,11 @@ int few_parts(int F, int size);
 // Few rows in 8 bits: up (codes of h) and down.
 void few_launch_q8(const Args& g, bool vin, bool vout, hipStream_t st);
 
-__device__ __forceinline__ float sigmoid(float v) { return 1.f / (1.f + expf(-v)); }
+// 1 / (1 + 2^(-v log2 e)) by the hardware's exponential and reciprocal: within 1e-7 |v| of the value where it is
+// small, within 1e-7 elsewhere; four instructions where expf and a division take about forty.
+__device__ __forceinline__ float sigmoid(float v) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(v * -1.44269504f));
+}
 
 // n of four values to p, by one access where they are four and aligned
 __device__ __forceinline__ void store4(float* p, const f4& v, int n) {
@@ -73,15 +78,23 @@ __device__ __forceinline__ int few_expert(const Args& g, int b) {
   return __ballot(earlier) ? -1 : e;
 }
 inline int few_blocks(const Args& g) { return (int)(g.M < g.E ? g.M : g.E); }
+__device__ __forceinline__ int64_t few_row(const Args& g, int slot) { return (uint32_t)slot * g.k_inv >> 20; }
 
-// The slots of expert e in order into list (FEW_SLOTS entries); returns their number.  Every wave of the block does
-// the same work and writes the same values; the caller synchronises before it reads what other waves wrote.
-__device__ __forceinline__ int few_slots(const Args& g, int e, int16_t* list) {
+// The lane's expert among the first 64 slots (-1 past the last).  Loaded before the weights: loads return in order.
+__device__ __forceinline__ int few_first(const Args& g) {
+  const int lane = threadIdx.x & 63;
+  return lane < g.M ? g.index[lane] : -1;
+}
+
+// The slots of expert e in order into list (FEW_SLOTS entries), `first` from few_first; returns their number.  Every
+// wave of the block does the same work and writes the same values; the caller synchronises before it reads them.
+__device__ __forceinline__ int few_slots(const Args& g, int e, int first, int16_t* list) {
   const int lane = threadIdx.x & 63;
   int n = 0;
   for (int s0 = 0; s0 < g.M; s0 += 64) {
     const int s = s0 + lane;
-    const bool mine = s < g.M && g.index[s] == e;
+    if (s0) first = s < g.M ? g.index[s] : -1;
+    const bool mine = first == e;
     const uint64_t m = __ballot(mine);
     if (mine) list[n + __popcll(m & ((1ull << lane) - 1))] = (int16_t)s;
     n += __popcll(m);

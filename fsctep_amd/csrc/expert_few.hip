@@ -8,8 +8,8 @@
 // weights: more than memory gives).
 //   up, down (weights contiguous along the reduction): lane (r, q) holds column r, four (bf16: eight) neighbouring
 //     k from 4 q (8 q); a strip is 16 columns (up: their gate and up rows).
-//   dh, dx (weights contiguous along the output): lane (r, q) holds four (eight) neighbouring columns of one k; a
-//     strip is 64 (128) columns, product c of a load covering the columns 4 m + c (8 m + c).
+//   dh, dx (weights contiguous along the output): lane (r, q) holds two (four) neighbouring columns of one k; a
+//     strip is 32 (64) columns, 128 bytes of a weight row, product c of a load covering the columns 2 m + c (4 m + c).
 #include <type_traits>
 
 #include "common.h"
@@ -22,149 +22,249 @@ namespace experts {
 constexpr int FT = 512;             // eight waves
 constexpr int FW = FT / 64;
 
-// N values from p (all of them if n > 0 with VEC, the first n otherwise), widened
-template <int N, bool VEC, typename T>
-__device__ __forceinline__ void get(const T* p, int n, float (&v)[N]) {
-  if (VEC) {
-    if (n > 0) load_vec<N>(p, v);
-    else
+// B bytes from p, by 16- or 8-byte loads where ALIGNED
+template <int B, bool ALIGNED>
+struct Raw {
+  uint32_t v[B / 4];
+  template <typename T>
+  __device__ __forceinline__ void load(const T* p) {
+    if constexpr (ALIGNED && B % 16 == 0) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = 0.f;
-  } else {
+      for (int i = 0; i < B / 16; ++i) {
+        const u4v t = *(reinterpret_cast<const u4v*>(p) + i);
+        v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
+      }
+    } else if constexpr (ALIGNED) {
+      const u2v t = *reinterpret_cast<const u2v*>(p);
+      v[0] = t.x; v[1] = t.y;
+    } else {
+      T t[B / sizeof(T)];
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = i < n ? to_f(p[i]) : 0.f;
+      for (int i = 0; i < (int)(B / sizeof(T)); ++i) t[i] = p[i];
+      __builtin_memcpy(v, t, B);
+    }
   }
-}
+  // the first n values of p, zeros after them
+  template <typename T>
+  __device__ __forceinline__ void load(const T* p, int n) {
+    T t[B / sizeof(T)];
+#pragma unroll
+    for (int i = 0; i < (int)(B / sizeof(T)); ++i) t[i] = i < n ? p[i] : (T)0;
+    __builtin_memcpy(v, t, B);
+  }
+  // value i as a float
+  template <typename T>
+  __device__ __forceinline__ float at(int i) const {
+    if constexpr (sizeof(T) == 4) return __uint_as_float(v[i]);
+    else return __uint_as_float(i & 1 ? v[i >> 1] & 0xffff0000u : v[i >> 1] << 16);
+  }
+};
 
+// Whole steps of the reduction run without conditions: a lane past the last column or row reads the last one's
+// values, and what it computes is not stored.  The weights of a wave's first U steps are on their way before the
+// expert's slots are known.  Only the last, partial step looks at the bounds.
 template <typename S, int MODE, bool VEC>
-__global__ __launch_bounds__(FT) void few_kernel(Args g) {
-  constexpr int CE = 16 / sizeof(S);                   // weights of a load
+__global__ __launch_bounds__(FT, MODE == UP || MODE == DOWN ? 4 : 2) void few_kernel(Args g) {
   constexpr bool ALONG = MODE == UP || MODE == DOWN;   // weights contiguous along the reduction
+  constexpr int NW = FW;                               // waves
+  constexpr int WB = ALONG ? 16 : 8;                   // bytes of a load of weights
+  constexpr int CE = WB / sizeof(S);                   // its weights
+  constexpr int NL = ALONG ? (MODE == UP ? 2 : 1) : 4; // loads of weights in a step
   constexpr int NA = MODE == UP ? 2 : MODE == DOWN ? 1 : CE;   // accumulators of 16 rows
   constexpr int NC = ALONG ? 16 : 16 * CE;             // output columns of a strip
+  constexpr int STEP = ALONG ? 4 * CE : 16;            // reduction entries of a step
+  constexpr int U = 5;                                 // steps in flight
   using R = std::conditional_t<MODE == DOWN || MODE == DX, float, S>;
-  __shared__ f4 red[FW][NA][64];
+  constexpr int XE = ALONG ? CE : 4;                   // values of x of a step
+  __shared__ f4 red[NW][NA][64];
   __shared__ int16_t list[FEW_SLOTS];
   __shared__ float dred[NA][16];
   const int cols = MODE == UP || MODE == DH ? g.F : g.H;
-  const int strips = (cols + NC - 1) / NC;
-  const int e = few_expert(g, blockIdx.x / strips);
+  const int e = few_expert(g, blockIdx.y);
   if (e < 0) return;
-  const int n0 = (blockIdx.x % strips) * NC;
-  const int cnt = few_slots(g, e, list);
-  if (cnt == 0) return;
-  __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int K = MODE == UP || MODE == DH ? g.H : MODE == DOWN ? g.F : 2 * g.ldf;
+  const int first = few_first(g);
+  const int n0 = blockIdx.x * NC;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
 
-  for (int t0 = 0; t0 < cnt; t0 += 16) {
-    const int slot = t0 + r < cnt ? list[t0 + r] : -1;
-    const R* x = nullptr;
-    if (slot >= 0) {
-      if (MODE == UP) x = (const R*)g.x + (int64_t)(slot / g.k) * g.xs;
-      if (MODE == DH) x = (const R*)g.dy + (int64_t)(slot / g.k) * g.ds;
-      if (MODE == DOWN) x = (const R*)g.h + (int64_t)slot * g.ldf;
-      if (MODE == DX) x = (const R*)g.da + (int64_t)slot * 2 * g.ldf;
+  // The reduction: PARTS runs of K entries (dx: the gate and the up half of da), each of `whole` whole steps.
+  constexpr int PARTS = MODE == DX ? 2 : 1;
+  const int K = MODE == UP || MODE == DH ? g.H : g.F;
+  const int whole = K / STEP, steps = PARTS * whole;
+  const int n = n0 + (ALONG ? r : CE * r);
+  const int nc = ALONG ? min(n, cols - 1) : VEC ? min(n, cols - CE) : n;
+  const S* wbase = MODE == UP ? (const S*)g.w_in + ((int64_t)e * 2 * g.F + nc) * g.H
+                   : MODE == DOWN ? (const S*)g.w_out + ((int64_t)e * g.H + nc) * g.F
+                   : MODE == DH ? (const S*)g.w_out + (int64_t)e * g.H * g.F
+                                : (const S*)g.w_in + (int64_t)e * 2 * g.F * g.H;
+  const int64_t up = (int64_t)g.F * g.H;               // from a column's gate row to its up row
+  // A whole step's weights: the matrix of an expert (below 2^31 bytes) through a buffer descriptor, whose scalar
+  // offset carries the step, so that a load takes no address arithmetic.
+  const int64_t msize = (MODE == UP || MODE == DX ? 2 : 1) * up;
+  const S* const mbase = (MODE == UP || MODE == DX ? (const S*)g.w_in : (const S*)g.w_out) + e * msize;
+  const __amdgpu_buffer_rsrc_t rsrc = buffer_rsrc_bytes(const_cast<S*>(mbase), (uint32_t)(msize * sizeof(S)));
+  const int voff = (ALONG ? nc * K + CE * q : 4 * q * cols + nc) * (int)sizeof(S);
+  auto load_step = [&](Raw<WB, VEC> (&w)[NL], int part, int k) {
+    const int soff = (ALONG ? k : (part * K + k) * cols) * (int)sizeof(S);
+#pragma unroll
+    for (int c = 0; c < NL; ++c) {
+      const int so = soff + c * (int)(ALONG ? up : (int64_t)cols) * (int)sizeof(S);
+      if constexpr (WB == 16) {
+        const u4v t = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, voff, so, 0));
+        w[c].v[0] = t.x; w[c].v[1] = t.y; w[c].v[2] = t.z; w[c].v[3] = t.w;
+      } else {
+        const u2v t = __builtin_bit_cast(u2v, __builtin_amdgcn_raw_buffer_load_b64(rsrc, voff, so, 0));
+        w[c].v[0] = t.x; w[c].v[1] = t.y;
+      }
     }
-    f4 acc[NA];
-#pragma unroll
-    for (int c = 0; c < NA; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
+  };
+  // a step's weights from entry k of a part on, `left` of them
+  auto load_w = [&](Raw<WB, VEC> (&w)[NL], int part, int k, int left) {
     if constexpr (ALONG) {
-      const int n = n0 + r;
-      const S* w = nullptr;
-      if (n < cols)
-        w = MODE == UP ? (const S*)g.w_in + ((int64_t)e * 2 * g.F + n) * g.H : (const S*)g.w_out + ((int64_t)e * g.H + n) * g.F;
-      const int64_t up = (int64_t)g.F * g.H;           // from a column's gate row to its up row
-      constexpr int STEP = 4 * CE;
-#pragma unroll 5
-      for (int k0 = wave * STEP; k0 < K; k0 += FW * STEP) {
-        const int k = k0 + CE * q;
-        float wv[NA][CE], xv[CE];
 #pragma unroll
-        for (int c = 0; c < NA; ++c) get<CE, VEC>(w + c * up + k, w ? K - k : 0, wv[c]);
-        get<CE, VEC>(x + k, x ? K - k : 0, xv);
-#pragma unroll
-        for (int i = 0; i < CE; ++i)
-#pragma unroll
-          for (int c = 0; c < NA; ++c) acc[c] = mfma16x16x4(wv[c][i], xv[i], acc[c]);
+      for (int c = 0; c < NL; ++c) {
+        const S* p = wbase + c * up + k + CE * q;
+        if (left >= STEP) w[c].load(p);
+        else w[c].load(p, left - CE * q);
       }
     } else {
-      const int n = n0 + CE * r;
-#pragma unroll 2
-      for (int k0 = wave * 16; k0 < K; k0 += FW * 16) {
-        const int k = k0 + 4 * q;
-        float wv[4][CE], xv[4];
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-          const S* w = nullptr;
-          if (MODE == DH) {
-            if (k + s < g.H) w = (const S*)g.w_out + ((int64_t)e * g.H + k + s) * g.F + n;
-          } else {
-            const int half = k + s >= g.ldf, f = k + s - half * g.ldf;
-            if (k + s < K && f < g.F) w = (const S*)g.w_in + ((int64_t)e * 2 * g.F + half * g.F + f) * g.H + n;
-          }
-          get<CE, VEC>(w, w ? cols - n : 0, wv[s]);
-        }
-        if constexpr (MODE == DX) {
-          get<4, true>(x + k, x ? K - k : 0, xv);      // K is a multiple of 16, da's rows are aligned
-        } else {
-          get<4, false>(x + k, x ? K - k : 0, xv);
-        }
-#pragma unroll
-        for (int s = 0; s < 4; ++s)
-#pragma unroll
-          for (int c = 0; c < NA; ++c) acc[c] = mfma16x16x4(wv[s][c], xv[s], acc[c]);
+      for (int c = 0; c < NL; ++c) {
+        const int kk = 4 * q + c;
+        const int row = part * K + k + (kk < left ? kk : left - 1);
+        const S* p = wbase + (int64_t)row * cols + nc;
+        if (VEC) w[c].load(p);
+        else w[c].load(p, cols - nc);
       }
+    }
+  };
+  auto load_x = [&](Raw<XE * sizeof(R), VEC>& v, const R* x, int part, int k, int left) {
+    const R* p = x + (MODE == DX ? part * g.ldf : 0) + k + XE * q;
+    if (left >= STEP) v.load(p);
+    else v.load(p, left - XE * q);
+  };
+  f4 acc[NA];
+  auto mul = [&](const Raw<WB, VEC> (&w)[NL], const Raw<XE * sizeof(R), VEC>& v) {
+    if constexpr (ALONG) {
+#pragma unroll
+      for (int i = 0; i < CE; ++i)
+#pragma unroll
+        for (int c = 0; c < NA; ++c) acc[c] = mfma16x16x4(w[c].template at<S>(i), v.template at<R>(i), acc[c]);
+    } else {
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int c = 0; c < NA; ++c) acc[c] = mfma16x16x4(w[s].template at<S>(c), v.template at<R>(s), acc[c]);
+    }
+  };
+
+  Raw<WB, VEC> w[U][NL];
+  auto load_chunk = [&](int i0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = wave + (i0 + u) * NW;              // the same for the whole wave
+      if (s >= steps) continue;
+      const int part = PARTS == 2 && s >= whole, k = (s - part * whole) * STEP;
+      if constexpr (VEC) load_step(w[u], part, k);
+      else load_w(w[u], part, k, STEP);
+    }
+  };
+  load_chunk(0);
+  const int cnt = few_slots(g, e, first, list);
+  if (cnt == 0) return;
+  __syncthreads();
+
+  for (int t0 = 0; t0 < cnt; t0 += 16) {
+    const bool live = t0 + r < cnt;
+    const int slot = list[live ? t0 + r : 0];
+    const R* x = MODE == UP     ? (const R*)g.x + few_row(g, slot) * g.xs
+                 : MODE == DH   ? (const R*)g.dy + few_row(g, slot) * g.ds
+                 : MODE == DOWN ? (const R*)g.h + (int64_t)slot * g.ldf
+                                : (const R*)g.da + (int64_t)slot * 2 * g.ldf;
+#pragma unroll
+    for (int c = 0; c < NA; ++c) acc[c] = f4{0.f, 0.f, 0.f, 0.f};
+    // dh: what the epilogue needs of the forward, on its way during the products (columns past the padding: the last)
+    float av[2][4], wt = 0.f;
+    if (MODE == DH && wave < NA) {
+      wt = g.weight[slot];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float* a = g.a + (int64_t)slot * 2 * g.ldf + min(n0 + CE * (4 * q + j) + wave, g.ldf - 1);
+        av[0][j] = a[0];
+        av[1][j] = a[g.ldf];
+      }
+    }
+    for (int i0 = 0; wave + i0 * NW < steps; i0 += U) {
+      Raw<XE * sizeof(R), VEC> xv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        const int s = wave + (i0 + u) * NW;
+        const int part = PARTS == 2 && s >= whole;
+        if (s < steps) load_x(xv[u], x, part, (s - part * whole) * STEP, STEP);
+      }
+      if (i0 > 0 || (t0 > 0 && wave + U * NW < steps)) load_chunk(i0);   // else the first chunk is still there
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (wave + (i0 + u) * NW < steps) mul(w[u], xv[u]);
+    }
+    if (K % STEP != 0 && wave < PARTS) {               // the partial step of part `wave`
+      Raw<WB, VEC> wt[NL];
+      Raw<XE * sizeof(R), VEC> xt;
+      load_w(wt, wave, whole * STEP, K - whole * STEP);
+      load_x(xt, x, wave, whole * STEP, K - whole * STEP);
+      mul(wt, xt);
     }
     __syncthreads();                                   // the last tile's sums have been read
 #pragma unroll
     for (int c = 0; c < NA; ++c) red[wave][c][lane] = acc[c];
     __syncthreads();
-    // thread (c, lane) of the first NA waves: the eight waves' sums of one accumulator, in order
+    // thread (c, lane) of the first NA waves: the waves' sums of one accumulator, in order
     if (wave < (MODE == UP ? 1 : NA)) {
       f4 v[MODE == UP ? 2 : 1];
 #pragma unroll
       for (int c = 0; c < (MODE == UP ? 2 : 1); ++c) {
-        v[c] = red[0][MODE == UP ? c : wave][lane];
+        f4 t[NW];
 #pragma unroll
-        for (int u = 1; u < FW; ++u) v[c] += red[u][MODE == UP ? c : wave][lane];
+        for (int u = 0; u < NW; ++u) t[u] = red[u][MODE == UP ? c : wave][lane];
+        v[c] = ((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]));
       }
       if constexpr (MODE == UP) {
-        const int n = n0 + 4 * q;
-        if (slot >= 0 && n < g.ldf) {
+        const int m = n0 + 4 * q;
+        if (live && m < g.ldf) {
           f4 h;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) h[j] = v[0][j] * sigmoid(v[0][j]) * v[1][j];
+          for (int j = 0; j < 4; ++j) {
+            if (m + j >= g.F) v[0][j] = v[1][j] = 0.f;   // the padding
+            h[j] = v[0][j] * sigmoid(v[0][j]) * v[1][j];
+          }
           if (g.a) {
-            float* a = g.a + (int64_t)slot * 2 * g.ldf + n;
+            float* a = g.a + (int64_t)slot * 2 * g.ldf + m;
             st4(a, v[0]);
             st4(a + g.ldf, v[1]);
           }
-          st4((float*)g.h + (int64_t)slot * g.ldf + n, h);
+          st4((float*)g.h + (int64_t)slot * g.ldf + m, h);
         }
       } else if constexpr (MODE == DOWN) {
-        const int n = n0 + 4 * q;
-        if (slot >= 0) store4(g.o + (int64_t)slot * g.ldo + n, v[0], g.H - n);
+        const int m = n0 + 4 * q;
+        if (live) store4(g.o + (int64_t)slot * g.ldo + m, v[0], g.H - m);
       } else if constexpr (MODE == DX) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int n = n0 + CE * (4 * q + j) + wave;
-          if (slot >= 0 && n < g.H) g.o[(int64_t)slot * g.ldo + n] = v[0][j];
+          const int m = n0 + CE * (4 * q + j) + wave;
+          if (live && m < g.H) g.o[(int64_t)slot * g.ldo + m] = v[0][j];
         }
       } else {
         float part = 0.f;
-        const float wt = slot >= 0 ? g.weight[slot] : 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const int n = n0 + CE * (4 * q + j) + wave;
-          if (slot < 0 || n >= g.ldf) continue;
-          const float* a = g.a + (int64_t)slot * 2 * g.ldf + n;
-          const float ga = a[0], up = a[g.ldf], s = sigmoid(ga), act = ga * s, h = act * up, p = v[0][j], dh = p * wt;
+          const int m = n0 + CE * (4 * q + j) + wave;
+          if (!live || m >= g.ldf) continue;
+          const float ga = av[0][j], ua = av[1][j], s = sigmoid(ga), act = ga * s, h = act * ua;
+          const float p = m < g.F ? v[0][j] : 0.f, dh = p * wt;
           part += h * p;
-          float* d = (float*)g.da + (int64_t)slot * 2 * g.ldf + n;
-          d[0] = dh * up * (s * (1.f + ga * (1.f - s)));
+          float* d = (float*)g.da + (int64_t)slot * 2 * g.ldf + m;
+          d[0] = dh * ua * (s * (1.f + ga * (1.f - s)));
           d[g.ldf] = dh * act;
-          if (g.hw) ((float*)g.hw)[(int64_t)slot * g.ldf + n] = h * wt;
+          if (g.hw) ((float*)g.hw)[(int64_t)slot * g.ldf + m] = h * wt;
         }
         part += __shfl_xor(part, 16, 64);
         part += __shfl_xor(part, 32, 64);
@@ -173,21 +273,23 @@ __global__ __launch_bounds__(FT) void few_kernel(Args g) {
     }
     if constexpr (MODE == DH) {
       __syncthreads();
-      if (g.dwpart && threadIdx.x < 16 && slot >= 0) {
+      if (g.dwpart && threadIdx.x < 16 && live) {
         float t = dred[0][r];
 #pragma unroll
         for (int c = 1; c < NA; ++c) t += dred[c][r];
-        g.dwpart[(int64_t)(blockIdx.x % strips) * g.M + slot] = t;
+        g.dwpart[(int64_t)blockIdx.x * g.M + slot] = t;
       }
     }
   }
 }
 
+constexpr int strip_cols(int mode, int size) { return mode == UP || mode == DOWN ? 16 : 16 * (8 / size); }
+
 template <typename S, int MODE>
 void launch_mode(const Args& g, bool vec, hipStream_t st) {
-  constexpr int NC = MODE == UP || MODE == DOWN ? 16 : 16 * (16 / sizeof(S));
+  constexpr int NC = strip_cols(MODE, sizeof(S));
   const int cols = MODE == UP || MODE == DH ? g.F : g.H;
-  const unsigned grid = (unsigned)few_blocks(g) * ((cols + NC - 1) / NC);
+  const dim3 grid((cols + NC - 1) / NC, few_blocks(g));
   if (vec) few_kernel<S, MODE, true><<<grid, FT, 0, st>>>(g);
   else few_kernel<S, MODE, false><<<grid, FT, 0, st>>>(g);
 }
@@ -202,7 +304,7 @@ void few_launch(int mode, const Args& g, bool vec, hipStream_t st) {
 template void few_launch<float>(int, const Args&, bool, hipStream_t);
 template void few_launch<__bf16>(int, const Args&, bool, hipStream_t);
 
-int few_parts(int F, int size) { return (F + 16 * (16 / size) - 1) / (16 * (16 / size)); }
+int few_parts(int F, int size) { return (F + strip_cols(DH, size) - 1) / strip_cols(DH, size); }
 
 // ---------------------------------------------------------------- 8 bits
 typedef int i4v __attribute__((ext_vector_type(4)));
@@ -224,36 +326,63 @@ template <bool VEC>
 __global__ __launch_bounds__(FT) void few_up_q8_kernel(Args g) {
   __shared__ int16_t list[FEW_SLOTS];
   __shared__ float tops[FW][16];
-  const int ng = g.ldf / QG, grp = blockIdx.x % ng;
-  const int e = few_expert(g, blockIdx.x / ng);
+  const int ng = g.ldf / QG, grp = blockIdx.x;
+  const int e = few_expert(g, blockIdx.y);
   if (e < 0) return;
-  const int cnt = few_slots(g, e, list);
-  if (cnt == 0) return;
-  __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int first = few_first(g);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int nr = grp * QG + wave * 16 + r, n = grp * QG + wave * 16 + 4 * q;
-  const int8_t* wg = nr < g.F ? (const int8_t*)g.w_in + ((int64_t)e * 2 * g.F + nr) * g.H : nullptr;
+  const int8_t* wg = (const int8_t*)g.w_in + ((int64_t)e * 2 * g.F + min(nr, g.F - 1)) * g.H;
   const int64_t up = (int64_t)g.F * g.H;
+  // the first U steps' weights and the columns' scales (a column past the last: the last one's), before the slots
+  // are known
+  constexpr int U = VEC ? 10 : 1;
+  const int whole = g.H / 64;
+  Raw<16, VEC> a[U], b[U];
+  auto load_chunk = [&](int s0) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (s0 + u < whole) {
+        const int k = (s0 + u) * 64 + 16 * q;
+        a[u].load(wg + k);
+        b[u].load(wg + up + k);
+      }
+  };
+  load_chunk(0);
   f4 sg, su;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float* s = g.in_scale + (int64_t)e * 2 * g.F + n + j;
-    sg[j] = n + j < g.F ? s[0] : 0.f;
-    su[j] = n + j < g.F ? s[g.F] : 0.f;
+    const float* s = g.in_scale + (int64_t)e * 2 * g.F + min(n + j, g.F - 1);
+    sg[j] = s[0];
+    su[j] = s[g.F];
   }
+  const int cnt = few_slots(g, e, first, list);
+  if (cnt == 0) return;
+  __syncthreads();
   for (int t0 = 0; t0 < cnt; t0 += 16) {
-    const int slot = t0 + r < cnt ? list[t0 + r] : -1;
-    const int8_t* x = slot >= 0 ? (const int8_t*)g.x + (int64_t)(slot / g.k) * g.xs : nullptr;
+    const bool live = t0 + r < cnt;
+    const int slot = list[live ? t0 + r : 0];
+    const int8_t* x = (const int8_t*)g.x + few_row(g, slot) * g.xs;
+    const float xs = g.xscale[few_row(g, slot)];
     i4v ag = {0, 0, 0, 0}, au = {0, 0, 0, 0};
-#pragma unroll 5
-    for (int k0 = 0; k0 < g.H; k0 += 64) {
-      const int k = k0 + 16 * q;
-      const i4v a = get16<VEC>(wg + k, wg ? g.H - k : 0), b = get16<VEC>(wg + up + k, wg ? g.H - k : 0);
-      const i4v xv = get16<VEC>(x + k, x ? g.H - k : 0);
+    auto mul = [&](const i4v& a, const i4v& b, const i4v& xv) {
       ag = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, xv, ag, 0, 0, 0);
       au = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, xv, au, 0, 0, 0);
+    };
+    for (int s0 = 0; s0 < whole; s0 += U) {
+      Raw<16, VEC> xv[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s0 + u < whole) xv[u].load(x + (s0 + u) * 64 + 16 * q);
+      if (s0 > 0 || (t0 > 0 && U < whole)) load_chunk(s0);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (s0 + u < whole) mul(__builtin_bit_cast(i4v, a[u]), __builtin_bit_cast(i4v, b[u]), __builtin_bit_cast(i4v, xv[u]));
     }
-    const float xs = slot >= 0 ? g.xscale[slot / g.k] : 0.f;
+    if (whole * 64 < g.H) {
+      const int k = whole * 64 + 16 * q, n16 = g.H - k;
+      mul(get16<VEC>(wg + k, n16), get16<VEC>(wg + up + k, n16), get16<VEC>(x + k, n16));
+    }
     float h[4], top = 0.f;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -270,7 +399,7 @@ __global__ __launch_bounds__(FT) void few_up_q8_kernel(Args g) {
 #pragma unroll
     for (int w = 0; w < FW; ++w) top = max_nan(top, tops[w][r]);
     const float inv = top > 0.f ? 127.f / top : 0.f;
-    if (slot >= 0) {
+    if (live) {
       int8_t b[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -288,18 +417,19 @@ template <bool VEC>
 __global__ __launch_bounds__(256) void few_down_q8_kernel(Args g) {
   __shared__ int16_t list[FEW_SLOTS];
   __shared__ f4 red[4][64];
-  const int strips = (g.H + 15) / 16, n0 = (blockIdx.x % strips) * 16, ng = g.ldf / QG;
-  const int e = few_expert(g, blockIdx.x / strips);
+  const int n0 = blockIdx.x * 16, ng = g.ldf / QG;
+  const int e = few_expert(g, blockIdx.y);
   if (e < 0) return;
-  const int cnt = few_slots(g, e, list);
+  const int cnt = few_slots(g, e, few_first(g), list);
   if (cnt == 0) return;
   __syncthreads();
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int8_t* w = n0 + r < g.H ? (const int8_t*)g.w_out + ((int64_t)e * g.H + n0 + r) * g.F : nullptr;
+  const int8_t* w = (const int8_t*)g.w_out + ((int64_t)e * g.H + min(n0 + r, g.H - 1)) * g.F;
   const int n = n0 + 4 * q;
   for (int t0 = 0; t0 < cnt; t0 += 16) {
-    const int slot = t0 + r < cnt ? list[t0 + r] : -1;
-    const int8_t* h = slot >= 0 ? (const int8_t*)g.h + (int64_t)slot * g.ldf : nullptr;
+    const bool live = t0 + r < cnt;
+    const int slot = list[live ? t0 + r : 0];
+    const int8_t* h = (const int8_t*)g.h + (int64_t)slot * g.ldf;
     f4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
     for (int grp = wave; grp < ng; grp += 4) {
@@ -307,28 +437,27 @@ __global__ __launch_bounds__(256) void few_down_q8_kernel(Args g) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int k = grp * QG + 64 * s + 16 * q;
-        const i4v a = get16<VEC>(w + k, w ? g.F - k : 0), b = get16<true>(h + k, h ? 16 : 0);
+        const i4v a = get16<VEC>(w + k, g.F - k), b = get16<true>(h + k, 16);
         acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0);
       }
-      const float u = slot >= 0 ? g.hscale[(int64_t)slot * ng + grp] : 0.f;
+      const float u = g.hscale[(int64_t)slot * ng + grp];
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] += (float)acc[j] * u;
     }
     __syncthreads();
     red[wave][lane] = sum;
     __syncthreads();
-    if (wave == 0 && slot >= 0) {
+    if (wave == 0 && live) {
       sum = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (n + j < g.H) sum[j] *= g.out_scale[(int64_t)e * g.H + n + j];
+      for (int j = 0; j < 4; ++j) sum[j] *= g.out_scale[(int64_t)e * g.H + min(n + j, g.H - 1)];
       store4(g.o + (int64_t)slot * g.ldo + n, sum, g.H - n);
     }
   }
 }
 
 void few_launch_q8(const Args& g, bool vin, bool vout, hipStream_t st) {
-  const unsigned up = (unsigned)few_blocks(g) * (g.ldf / QG), down = (unsigned)few_blocks(g) * ((g.H + 15) / 16);
+  const dim3 up(g.ldf / QG, few_blocks(g)), down((g.H + 15) / 16, few_blocks(g));
   if (vin) few_up_q8_kernel<true><<<up, FT, 0, st>>>(g);
   else few_up_q8_kernel<false><<<up, FT, 0, st>>>(g);
   if (vout) few_down_q8_kernel<true><<<down, 256, 0, st>>>(g);

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
   using TW = Tile<KIND, BN, TR, S>;
   using TX = Tile<KIND, BM, false, R>;
   __shared__ __align__(16) char lds[TW::BYTES + TX::BYTES];
-  __shared__ int32_t slots[BM];
+  __shared__ int32_t slots[BM], rws[BM];
   char* lw = lds;
   char* lx = lds + TW::BYTES;
 
@@ -197,7 +197,10 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
   const int64_t left = g.offsets[e + 1] - p0;
   const int rows = left < BM ? (int)left : BM;
   const int n0 = ci * NC;
-  for (int i = threadIdx.x; i < BM; i += NT) slots[i] = i < rows ? g.slot_of[p0 + i] : -1;
+  for (int i = threadIdx.x; i < BM; i += NT) {
+    slots[i] = i < rows ? g.slot_of[p0 + i] : -1;
+    rws[i] = i < rows ? g.row_of[p0 + i] : 0;
+  }
   __syncthreads();
 
   // row pointers of this thread's chunks (straight operands); null where there is none
@@ -207,8 +210,8 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
     const int c = threadIdx.x + i * NT, row = TX::row_of(c);
     xp[i] = nullptr;
     if (c < TX::NCH && row < rows) {
-      if (MODE == UP) xp[i] = (const R*)g.x + (int64_t)(slots[row] / g.k) * g.xs;
-      if (MODE == DH) xp[i] = (const R*)g.dy + (int64_t)(slots[row] / g.k) * g.ds;
+      if (MODE == UP) xp[i] = (const R*)g.x + (int64_t)rws[row] * g.xs;
+      if (MODE == DH) xp[i] = (const R*)g.dy + (int64_t)rws[row] * g.ds;
       if (MODE == DOWN) xp[i] = (const R*)g.h + (p0 + row) * g.ldf;
       if (MODE == DX) xp[i] = (const R*)g.da + (p0 + row) * 2 * g.ldf;
     }
@@ -344,7 +347,7 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
         const int row = 16 * (x0 + j) + r;
         f4 ga, up;
         if constexpr (KIND == I8) {
-          const float xs = row < rows ? g.xscale[slots[row] / g.k] : 0.f;
+          const float xs = row < rows ? g.xscale[rws[row]] : 0.f;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             const float* s = g.in_scale + (int64_t)e * 2 * g.F + n + v;
@@ -449,7 +452,7 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
   __shared__ int16_t list[FEW ? FEW_SLOTS : 1];
   int64_t p0 = 0, cnt;
   if constexpr (FEW) {
-    cnt = few_slots(g, e, list);
+    cnt = few_slots(g, e, few_first(g), list);
     __syncthreads();
   } else {
     p0 = g.offsets[e];
@@ -457,6 +460,16 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
   }
   TT A;
   TB B;
+  // rows of x or dy of a step's positions, loaded a step ahead of the rows themselves
+  int tok[TT::PER];
+  auto find = [&](int64_t k0) {
+#pragma unroll
+    for (int i = 0; i < TT::PER; ++i) {
+      const int64_t k = k0 + TT::row_of(threadIdx.x + i * NT);
+      if constexpr (FEW) tok[i] = k < cnt ? (int)few_row(g, list[k]) : 0;
+      else tok[i] = g.row_of[p0 + (k < cnt ? k : cnt - 1)];
+    }
+  };
   auto fetch = [&](int64_t k0) {
 #pragma unroll
     for (int i = 0; i < TT::PER; ++i) {
@@ -467,13 +480,12 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
       const RB* pb = nullptr;
       if (k < cnt) {
         const int64_t pos = FEW ? list[k] : p0 + k;
-        const int64_t tok = (FEW ? list[k] : g.slot_of[pos]) / g.k;
         if (MODE == DWIN) {
-          pa = (const RA*)g.x + tok * g.xs + a0 + n;
+          pa = (const RA*)g.x + (int64_t)tok[i] * g.xs + a0 + n;
           pb = (const RB*)g.da + pos * 2 * g.ldf + b0 + n;
         } else {
           pa = (const RA*)g.hw + pos * g.ldf + a0 + n;
-          pb = (const RB*)g.dy + tok * g.ds + b0 + n;
+          pb = (const RB*)g.dy + (int64_t)tok[i] * g.ds + b0 + n;
         }
       }
       A.template fetch<VEC>(i, pa, pa ? na - a0 - n : 0);
@@ -487,13 +499,20 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
     for (int j = 0; j < 4; ++j) acc[i][j] = f4{0.f, 0.f, 0.f, 0.f};
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int w0 = (wave & 1) * 4, x0 = (wave >> 1) * 4;
-  if (cnt > 0) fetch(0);
+  if (cnt > 0) {
+    find(0);
+    fetch(0);
+    find(E::BK);
+  }
   for (int64_t k0 = 0; k0 < cnt; k0 += E::BK) {
     __syncthreads();
     A.put(la);
     B.put(lb);
     __syncthreads();
-    if (k0 + E::BK < cnt) fetch(k0 + E::BK);
+    if (k0 + E::BK < cnt) {
+      fetch(k0 + E::BK);
+      find(k0 + 2 * E::BK);
+    }
     step<KIND, 4, 4, TT, TB>(la, lb, w0, x0, acc);
   }
 #pragma unroll
@@ -680,7 +699,7 @@ inline Space backward_space(const FscExpertDims& d) {
   s.o = at; at += align64(M * ldo_of(d) * 4);
   s.da = at; at += align64(M * 2 * ldf * size);
   s.hw = at; at += align64(M * ldf * size);
-  s.part = at; at += align64(M * ((d.hidden + 63) / 64) * 4);
+  s.part = at; at += align64(M * ((d.hidden + 31) / 32) * 4);
   s.total = at;
   return s;
 }
@@ -695,10 +714,12 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
   g.ldo = ldo_of(d);
   g.E = d.n_experts;
   g.k = d.k;
+  g.k_inv = ((1u << 20) + d.k - 1) / d.k;
   if (!few(g.M, g.E)) {
     g.n_tiles = p.n_tiles;
     g.offsets = p.offsets;
     g.slot_of = p.slot_of;
+    g.row_of = p.row_of;
     g.tiles = p.tiles;
     g.place = p.place;
   }
@@ -730,7 +751,7 @@ void backward(Args g, int tile, void* dx, float* dweight, hipStream_t st) {
   const bool vdy = vec_ok(g.dy, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.xs, sizeof(S), g.H);
   const bool vin = vec_ok(g.w_in, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.F, sizeof(S), g.F);
   const bool by_slot = !g.place;
-  if (by_slot) few_launch<S>(DH, g, vout, st);
+  if (by_slot) few_launch<S>(DH, g, vdy && vout, st);
   else launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
   if (dweight)
     dweight_kernel<<<(unsigned)((g.M + NT - 1) / NT), NT, 0, st>>>(
@@ -776,7 +797,7 @@ int fsc_expert_plan(const FscExpertDims* dims, const int32_t* index, int32_t* pl
   if (few(M, dims->n_experts)) return 0;       // the products find their rows themselves
   FSC_CHECK_ARG(plan && index, "expert_plan: null array");
   const int tile = tile_rows(M, dims->n_experts);
-  launch_plan(plan_of(plan, M, dims->n_experts, tile), M, dims->n_experts, tile, index, stream);
+  launch_plan(plan_of(plan, M, dims->n_experts, tile), M, dims->n_experts, dims->k, tile, index, stream);
   return fsc::check_launch("expert_plan") ? 2 : 0;
 }
 

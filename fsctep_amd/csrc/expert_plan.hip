@@ -3,6 +3,7 @@
 //
 //   offsets [E + 1]   first sorted position of each expert
 //   slot_of [M]       slot at each sorted position          (M = T k)
+//   row_of  [M]       its row, slot / k
 //   place   [M]       sorted position of each slot, -1 for a slot with no expert
 //   tiles   [2 n]     (expert, first sorted position) of each tile of `tile` rows, expert -1 past the last one
 //                     (n = ceil(M / tile) + min(E, M) bounds their number)
@@ -31,9 +32,10 @@ __device__ __forceinline__ uint64_t peers(int e, bool ok) {
 
 // One block: wave w takes the w-th sixteenth of the slots, counts them by expert, and after a scan over (expert,
 // wave) ranks them in order.
-__global__ __launch_bounds__(PT) void plan_kernel(int64_t M, int E, int tile, int n_tiles,
+__global__ __launch_bounds__(PT) void plan_kernel(int64_t M, int E, int k, int tile, int n_tiles,
                                                   const int32_t* __restrict__ index, int32_t* __restrict__ offsets,
-                                                  int32_t* __restrict__ slot_of, int32_t* __restrict__ place,
+                                                  int32_t* __restrict__ slot_of, int32_t* __restrict__ row_of,
+                                                  int32_t* __restrict__ place,
                                                   int32_t* __restrict__ tiles) {
   __shared__ int cnt[PW][MAX_EXPERTS];
   __shared__ int total[MAX_EXPERTS + 1], first[MAX_EXPERTS + 1];
@@ -102,7 +104,10 @@ __global__ __launch_bounds__(PT) void plan_kernel(int64_t M, int E, int tile, in
     // the last lane of each expert moves its counter on (one wave: the reads above come first)
     if (ok && (m >> lane) == 1ull) cnt[wave][e] += __popcll(m);
     if (s < s1) place[s] = at;
-    if (ok) slot_of[at] = (int32_t)s;
+    if (ok) {
+      slot_of[at] = (int32_t)s;
+      row_of[at] = (int32_t)s / k;
+    }
   }
 }
 
@@ -110,18 +115,19 @@ Plan plan_of(int32_t* buf, int64_t M, int E, int tile) {
   Plan p;
   p.offsets = buf;
   p.slot_of = p.offsets + E + 1;
-  p.place = p.slot_of + M;
+  p.row_of = p.slot_of + M;
+  p.place = p.row_of + M;
   p.tiles = p.place + M;
   p.n_tiles = (int)((M + tile - 1) / tile + std::min<int64_t>(E, M));
   return p;
 }
 
 int64_t plan_ints(int64_t M, int E, int tile) {
-  return (E + 1) + 2 * M + 2 * ((M + tile - 1) / tile + std::min<int64_t>(E, M));
+  return (E + 1) + 3 * M + 2 * ((M + tile - 1) / tile + std::min<int64_t>(E, M));
 }
 
-void launch_plan(const Plan& p, int64_t M, int E, int tile, const int32_t* index, hipStream_t st) {
-  plan_kernel<<<1, PT, 0, st>>>(M, E, tile, p.n_tiles, index, p.offsets, p.slot_of, p.place, p.tiles);
+void launch_plan(const Plan& p, int64_t M, int E, int k, int tile, const int32_t* index, hipStream_t st) {
+  plan_kernel<<<1, PT, 0, st>>>(M, E, k, tile, p.n_tiles, index, p.offsets, p.slot_of, p.row_of, p.place, p.tiles);
 }
 
 }  // namespace experts

@@ -150,12 +150,16 @@ std::tuple<Tensor, Tensor> rms_norm_backward_meta(const Tensor&, const optional<
           want_dw ? at::empty_symint(weight.sym_sizes(), weight.options()) : at::empty({0}, weight.options())};
 }
 
+auto& rms_norm_op() {
+  static auto op = op_handle<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const optional<Tensor>&,
+                                                                double)>("fsctep::rms_norm");
+  return op;
+}
+
 struct RmsNormFn : public torch::autograd::Function<RmsNormFn> {
   static variable_list forward(AutogradContext* ctx, Tensor x, Tensor weight, optional<Tensor> residual, double eps) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = op_handle<std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const optional<Tensor>&,
-                                                                  double)>("fsctep::rms_norm");
-    auto [y, z, rstd] = op.call(x, weight, residual, eps);
+    auto [y, z, rstd] = rms_norm_op().call(x, weight, residual, eps);
     ctx->save_for_backward({residual.has_value() ? z : x, weight, rstd});
     ctx->saved_data["residual"] = residual.has_value();
     ctx->saved_data["eps"] = eps;
@@ -190,8 +194,12 @@ struct RmsNormFn : public torch::autograd::Function<RmsNormFn> {
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_autograd(const Tensor& x, const Tensor& weight,
                                                      const optional<Tensor>& residual, double eps) {
-  auto r = RmsNormFn::apply(x, weight, residual, eps);
-  return {r[0], r[1], r[2]};
+  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || some(residual).requires_grad())) {
+    auto r = RmsNormFn::apply(x, weight, residual, eps);
+    return {r[0], r[1], r[2]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return rms_norm_op().call(x, weight, residual, eps);
 }
 
 // ============================================================== router
@@ -249,14 +257,17 @@ Tensor route_experts_backward_meta(const Tensor&, const Tensor& l, const Tensor&
   return at::empty_symint(l.sym_sizes(), l.options());
 }
 
+auto& route_op() {
+  static auto op = op_handle<std::tuple<Tensor, Tensor>(const Tensor&, const optional<Tensor>&, int64_t, int64_t, int64_t,
+                                                        int64_t, int64_t, bool, double)>("fsctep::route_experts");
+  return op;
+}
+
 struct RouteFn : public torch::autograd::Function<RouteFn> {
   static variable_list forward(AutogradContext* ctx, Tensor logits, optional<Tensor> bias, int64_t k, int64_t score,
                                int64_t groups, int64_t kept, int64_t best, bool renormalise, double scale) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    static auto op = op_handle<std::tuple<Tensor, Tensor>(const Tensor&, const optional<Tensor>&, int64_t, int64_t,
-                                                          int64_t, int64_t, int64_t, bool, double)>(
-        "fsctep::route_experts");
-    auto [index, weight] = op.call(logits, bias, k, score, groups, kept, best, renormalise, scale);
+    auto [index, weight] = route_op().call(logits, bias, k, score, groups, kept, best, renormalise, scale);
     ctx->save_for_backward({logits, index, weight});
     ctx->saved_data["score"] = score;
     ctx->saved_data["renormalise"] = renormalise;
@@ -281,8 +292,12 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 std::tuple<Tensor, Tensor> route_experts_autograd(const Tensor& logits, const optional<Tensor>& bias, int64_t k,
                                                   int64_t score, int64_t groups, int64_t kept, int64_t best,
                                                   bool renormalise, double scale) {
-  auto r = RouteFn::apply(logits, bias, k, score, groups, kept, best, renormalise, scale);
-  return {r[0], r[1]};
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    auto r = RouteFn::apply(logits, bias, k, score, groups, kept, best, renormalise, scale);
+    return {r[0], r[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView guard;
+  return route_op().call(logits, bias, k, score, groups, kept, best, renormalise, scale);
 }
 
 // ============================================================== the experts' products
