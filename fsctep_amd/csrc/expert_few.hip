@@ -13,8 +13,7 @@
 #include <type_traits>
 
 #include "common.h"
-#include "expert_types.h"
-#include "expert_args.h"
+#include "expert_tiles.h"
 
 namespace fsc {
 namespace experts {
@@ -307,8 +306,6 @@ template void few_launch<__bf16>(int, const Args&, bool, hipStream_t);
 int few_parts(int F, int size) { return (F + strip_cols(DH, size) - 1) / strip_cols(DH, size); }
 
 // ---------------------------------------------------------------- 8 bits
-typedef int i4v __attribute__((ext_vector_type(4)));
-
 template <bool VEC>
 __device__ __forceinline__ i4v get16(const int8_t* p, int n) {
   if (VEC) return n > 0 ? *reinterpret_cast<const i4v*>(p) : i4v{0, 0, 0, 0};

@@ -17,34 +17,24 @@
 #include <type_traits>
 
 #include "common.h"
-#include "expert_types.h"
-#include "expert_args.h"
 #include "expert_plan.h"
+#include "expert_tiles.h"
 #include "fsctep.h"
 
 namespace fsc {
 namespace experts {
 
-typedef int i4v __attribute__((ext_vector_type(4)));
-
-enum Kind { F32 = 0, BF16 = 1, I8 = 2 };
-
 constexpr int NT = 256;          // four waves, two by two
 constexpr int BN = 128;          // rows of the tile's weight operand
-
-template <int KIND> struct El;
-template <> struct El<F32> { using T = float; static constexpr int BK = 32, CE = 8, PL = 3; };
-template <> struct El<BF16> { using T = __bf16; static constexpr int BK = 64, CE = 8, PL = 1; };
-template <> struct El<I8> { using T = int8_t; static constexpr int BK = 128, CE = 16, PL = 1; };
 
 // ---------------------------------------------------------------- tiles of the operands
 // A chunk is 16 bytes of an LDS plane: 8 values (16 in 8 bits) along the row.  Straight operands (rows of the tile
 // = rows of memory) lie as [row][chunk], the chunk's place XORed with the row so that 16 lanes reading one chunk
 // column of 16 rows meet no bank twice; turned operands (rows of memory along K) lie as [k][column] with 16
 // columns of padding and are read by ds_read_b64_tr_b16.
-constexpr int TRP = BN + 16;
+constexpr int TRP = 128 + 16;
 
-template <int KIND, int ROWS, bool TR, typename T>
+template <int KIND, int ROWS, bool TR, typename T, int NT>
 struct Tile {                                                        // T: the type in memory
   using E = El<KIND>;
   static constexpr int CPR = E::BK / E::CE;                          // chunks of a straight row
@@ -62,21 +52,18 @@ struct Tile {                                                        // T: the t
   __device__ static constexpr int chunk_of(int c) { return TR ? c % (ROWS / 8) : c % CPR; }
   __device__ static constexpr int swz(int row) { return CPR == 4 ? (row >> 1) & 3 : row & 7; }
 
-  // chunk c of the thread from p (n values of it exist, the rest are zeros; VEC: all or none, aligned)
-  template <bool VEC>
+  // chunk c of the thread at byte `off` of a buffer, zeros outside it
+  __device__ __forceinline__ void fetch(int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off) {
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+      reg[c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(off + 16 * i), 0, 0));
+  }
+  // chunk c of the thread from p (n values of it exist, the rest are zeros), of any alignment
   __device__ __forceinline__ void fetch(int c, const T* p, int n) {
-    Reg& g = reg[c];
-    if (VEC) {
-      const bool in = n > 0;
-      const u4v* q = reinterpret_cast<const u4v*>(p);
+    alignas(16) T t[E::CE];
 #pragma unroll
-      for (int i = 0; i < NV; ++i) g.v[i] = in ? q[i] : u4v{0, 0, 0, 0};
-    } else {
-      alignas(16) T t[E::CE];
-#pragma unroll
-      for (int i = 0; i < E::CE; ++i) t[i] = i < n ? p[i] : (T)0;
-      __builtin_memcpy(&g, t, sizeof(t));
-    }
+    for (int i = 0; i < E::CE; ++i) t[i] = i < n ? p[i] : (T)0;
+    __builtin_memcpy(&reg[c], t, sizeof(t));
   }
   // the thread's chunks into LDS
   __device__ __forceinline__ void put(char* lds) const {
@@ -121,9 +108,6 @@ struct Tile {                                                        // T: the t
   }
 };
 
-template <int KIND> struct Acc { using V = f4; };
-template <> struct Acc<I8> { using V = i4v; };
-
 // acc[i][j] += (weight tiles w0 + i) (row tiles x0 + j) over one K step in LDS.
 template <int KIND, int NI, int NJ, typename TW, typename TX>
 __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int x0,
@@ -158,34 +142,28 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
   }
 }
 
-// Workgroup -> (row tile, column tile).  Workgroup w runs on XCD w % 8: each XCD takes a contiguous run of row
-// tiles with all their column tiles, so that a tile's rows and an expert's weights meet in one L2.
-__device__ __forceinline__ bool tile_of(int n_tiles, int n_cols, int& t, int& c) {
-  const int per = (n_tiles * n_cols + 7) / 8;
-  const int i = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
-  t = i / n_cols;
-  c = i - t * n_cols;
-  return t < n_tiles && (int)(blockIdx.x >> 3) < per;
-}
-inline unsigned tile_grid(int64_t n_tiles, int64_t n_cols) { return (unsigned)((n_tiles * n_cols + 7) / 8 * 8); }
-
 // ---------------------------------------------------------------- the products by row tiles
 // up: 64 hidden columns a tile, their gate and up rows in turn by 16, so that a wave holds both of a column.
+// WW waves side by side along the weight operand, four (8-bit up: so many that 128 hidden columns make a tile)
+// 16-row tiles each, two along the rows.
+template <int KIND, int MODE>
+constexpr int waves_w() { return KIND == I8 && MODE == UP ? 4 : 2; }
+
 template <int KIND, typename S, int MODE, int NJ, bool VEC>
-__global__ __launch_bounds__(NT) void rows_kernel(Args g) {
+__global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(Args g) {
   using E = El<KIND>;
   using T = typename E::T;                                   // of the arrays between the kernels; S: the caller's
   using R = std::conditional_t<MODE == DOWN || MODE == DX, T, S>;
-  constexpr int BM = 32 * NJ;
+  constexpr int BM = 32 * NJ, NI = 4, WW = waves_w<KIND, MODE>(), BN = 64 * WW, NT = 128 * WW;
   constexpr bool TR = MODE == DH || MODE == DX;
-  using TW = Tile<KIND, BN, TR, S>;
-  using TX = Tile<KIND, BM, false, R>;
+  using TW = Tile<KIND, BN, TR, S, NT>;
+  using TX = Tile<KIND, BM, false, R, NT>;
   __shared__ __align__(16) char lds[TW::BYTES + TX::BYTES];
   __shared__ int32_t slots[BM], rws[BM];
   char* lw = lds;
   char* lx = lds + TW::BYTES;
 
-  const int NC = MODE == UP ? 64 : BN;                       // output columns of a tile
+  const int NC = MODE == UP ? BN / 2 : BN;                   // output columns of a tile
   // output columns (8 bits: the last group of h is whole)
   const int cols = KIND == I8 && MODE == UP ? g.ldf : MODE == UP || MODE == DH ? g.F : g.H;
   const int K = MODE == UP || MODE == DH ? g.H : MODE == DOWN ? g.F : 2 * g.ldf;
@@ -203,70 +181,85 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
   }
   __syncthreads();
 
-  // row pointers of this thread's chunks (straight operands); null where there is none
-  const R* xp[TX::PER];
+  // Where a chunk of the thread lies: VEC, byte offsets into a buffer over the expert's weights, over the tile's rows
+  // of an array between the kernels, or over the whole of x or dy (kDropOffset where there is nothing: loads without
+  // branches); else pointers and counts.  The arrays between the kernels are padded with zeros to ldf.
+  const int KX = MODE == DOWN ? g.ldf : K;
+  constexpr bool GATHER = MODE == UP || MODE == DH;
+  const int64_t xld = MODE == UP ? g.xs : MODE == DH ? g.ds : MODE == DOWN ? g.ldf : 2 * (int64_t)g.ldf;
+  const R* const xbase = MODE == UP     ? (const R*)g.x
+                         : MODE == DH   ? (const R*)g.dy
+                         : MODE == DOWN ? (const R*)g.h + p0 * g.ldf
+                                        : (const R*)g.da + p0 * 2 * g.ldf;
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc_bytes(
+      const_cast<R*>(xbase), (uint32_t)(((GATHER ? g.T : rows) - 1) * xld + (GATHER ? g.H : xld)) * sizeof(R));
+  const int64_t wsize = (MODE == UP || MODE == DX ? 2 : 1) * (int64_t)g.F * g.H;
+  const S* const wbase = (MODE == UP || MODE == DX ? (const S*)g.w_in : (const S*)g.w_out) + e * wsize;
+  const __amdgpu_buffer_rsrc_t wr = buffer_rsrc_bytes(const_cast<S*>(wbase), (uint32_t)(wsize * sizeof(S)));
+  int64_t xrow[TX::PER];                                     // first entry of the chunk's row, -1: none
 #pragma unroll
   for (int i = 0; i < TX::PER; ++i) {
     const int c = threadIdx.x + i * NT, row = TX::row_of(c);
-    xp[i] = nullptr;
-    if (c < TX::NCH && row < rows) {
-      if (MODE == UP) xp[i] = (const R*)g.x + (int64_t)rws[row] * g.xs;
-      if (MODE == DH) xp[i] = (const R*)g.dy + (int64_t)rws[row] * g.ds;
-      if (MODE == DOWN) xp[i] = (const R*)g.h + (p0 + row) * g.ldf;
-      if (MODE == DX) xp[i] = (const R*)g.da + (p0 + row) * 2 * g.ldf;
-    }
+    xrow[i] = c < TX::NCH && row < rows ? (GATHER ? rws[row] : row) * xld : -1;
   }
-  const S* wp[TW::PER];
-  if (!TR) {
+  int64_t wrow[TW::PER];
 #pragma unroll
-    for (int i = 0; i < TW::PER; ++i) {
-      const int row = TW::row_of(threadIdx.x + i * NT);
-      if (MODE == UP) {
-        const int n = n0 + (row >> 5) * 16 + (row & 15);
-        wp[i] = n < g.F ? (const S*)g.w_in + ((int64_t)e * 2 * g.F + (row & 16 ? g.F : 0) + n) * g.H : nullptr;
-      } else {
-        const int n = n0 + row;
-        wp[i] = n < g.H ? (const S*)g.w_out + ((int64_t)e * g.H + n) * g.F : nullptr;
-      }
+  for (int i = 0; i < TW::PER; ++i) {
+    const int row = TW::row_of(threadIdx.x + i * NT);
+    if (TR) {
+      const int n = n0 + TW::chunk_of(threadIdx.x + i * NT) * 8;
+      wrow[i] = n < cols ? n : -1;                           // the chunk's column
+    } else if (MODE == UP) {
+      const int n = n0 + (row >> 5) * 16 + (row & 15);
+      wrow[i] = n < g.F ? (int64_t)((row & 16 ? g.F : 0) + n) * g.H : -1;
+    } else {
+      wrow[i] = n0 + row < g.H ? (int64_t)(n0 + row) * g.F : -1;
     }
   }
   TW tw;
   TX tx;
-  // the arrays between the kernels are padded with zeros to ldf, a multiple of a chunk
-  const int KX = MODE == DOWN ? g.ldf : K;
   auto fetch = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < TX::PER; ++i) {
       const int k = k0 + TX::chunk_of(threadIdx.x + i * NT) * E::CE;
-      tx.template fetch<VEC>(i, xp[i] + k, xp[i] ? KX - k : 0);
+      const bool in = xrow[i] >= 0 && k < KX;
+      if constexpr (VEC) tx.fetch(i, xr, in ? (uint32_t)(xrow[i] + k) * (uint32_t)sizeof(R) : kDropOffset);
+      else tx.fetch(i, xbase + xrow[i] + k, in ? KX - k : 0);
     }
 #pragma unroll
     for (int i = 0; i < TW::PER; ++i) {
       const int c = threadIdx.x + i * NT;
+      int64_t at;
+      bool in;
+      int n;
       if (!TR) {
         const int k = k0 + TW::chunk_of(c) * E::CE;
-        tw.template fetch<VEC>(i, wp[i] + k, wp[i] ? K - k : 0);
+        in = wrow[i] >= 0 && k < K;
+        at = wrow[i] + k;
+        n = K - k;
       } else {
-        const int k = k0 + TW::row_of(c), n = n0 + TW::chunk_of(c) * 8;
-        const S* p = nullptr;
-        if (MODE == DH) {
-          if (k < g.H) p = (const S*)g.w_out + ((int64_t)e * g.H + k) * g.F + n;
-        } else {
+        int k = k0 + TW::row_of(c);
+        in = wrow[i] >= 0 && k < K;
+        n = cols - (int)wrow[i];
+        if (MODE == DX) {                                    // rows of the gate half, padding, rows of the up half
           const int half = k >= g.ldf, f = k - half * g.ldf;
-          if (k < K && f < g.F) p = (const S*)g.w_in + ((int64_t)e * 2 * g.F + half * g.F + f) * g.H + n;
+          in = in && f < g.F;
+          k = half * g.F + f;
         }
-        tw.template fetch<VEC>(i, p, p ? cols - n : 0);
+        at = (int64_t)k * cols + wrow[i];
       }
+      if constexpr (VEC) tw.fetch(i, wr, in ? (uint32_t)at * (uint32_t)sizeof(S) : kDropOffset);
+      else tw.fetch(i, wbase + at, in ? n : 0);
     }
   };
 
-  typename Acc<KIND>::V acc[4][NJ];
+  typename Acc<KIND>::V acc[NI][NJ];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[i][j] = {0, 0, 0, 0};
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int w0 = (wave & 1) * 4, x0 = (wave >> 1) * NJ;      // first tiles of the wave
+  const int w0 = wave % WW * NI, x0 = wave / WW * NJ;        // first tiles of the wave
 
   if constexpr (KIND == I8 && MODE == DOWN) {
     // a K step is one group of h: its sums are whole numbers, scaled by the group's unit into 32-bit floats
@@ -326,107 +319,9 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
     }
   }
 
-  if constexpr (MODE == DOWN || MODE == DX) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + (w0 + i) * 16 + 4 * q;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        if constexpr (KIND != I8)
-          if (row < rows) store4(g.o + (p0 + row) * g.ldo + n, acc[i][j], g.H - n);
-      }
-    }
-  } else if constexpr (MODE == UP) {
-    f4 hv[2][NJ];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int n = n0 + ((wave & 1) * 2 + i) * 16 + 4 * q;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        f4 ga, up;
-        if constexpr (KIND == I8) {
-          const float xs = row < rows ? g.xscale[rws[row]] : 0.f;
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const float* s = g.in_scale + (int64_t)e * 2 * g.F + n + v;
-            ga[v] = n + v < g.F ? (float)acc[2 * i][j][v] * (xs * s[0]) : 0.f;
-            up[v] = n + v < g.F ? (float)acc[2 * i + 1][j][v] * (xs * s[g.F]) : 0.f;
-          }
-        } else {
-          ga = acc[2 * i][j];
-          up = acc[2 * i + 1][j];
-        }
-#pragma unroll
-        for (int v = 0; v < 4; ++v) hv[i][j][v] = ga[v] * sigmoid(ga[v]) * up[v];
-        if constexpr (KIND != I8) {
-          if (row < rows && n < g.ldf) {
-            if (g.a) {
-              float* a = g.a + (p0 + row) * 2 * g.ldf + n;
-              st4(a, ga);
-              st4(a + g.ldf, up);
-            }
-            store4((T*)g.h + (p0 + row) * g.ldf + n, hv[i][j], 4);
-          }
-        }
-      }
-    }
-    if constexpr (KIND == I8) {
-      // the block holds half a group of 128 columns: h goes out in 32 bits, quant_kernel makes the codes
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int n = n0 + ((wave & 1) * 2 + i) * 16 + 4 * q;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          const int row = 16 * (x0 + j) + r;
-          if (row < rows && n < g.ldf) st4(g.a + (p0 + row) * g.ldf + n, hv[i][j]);
-        }
-      }
-    }
-  } else if constexpr (MODE == DH) {
-    float part[NJ];
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) part[j] = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int n = n0 + (w0 + i) * 16 + 4 * q;
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        if (row >= rows || n >= g.ldf) continue;
-        const float w = g.weight[slots[row]];
-        const float* a = g.a + (p0 + row) * 2 * g.ldf + n;
-        const f4 ga = ld4(a), up = ld4(a + g.ldf);
-        f4 dg, du, hw;
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float s = sigmoid(ga[v]), act = ga[v] * s, h = act * up[v], p = acc[i][j][v], dh = p * w;
-          part[j] += h * p;
-          hw[v] = h * w;
-          du[v] = dh * act;
-          dg[v] = dh * up[v] * (s * (1.f + ga[v] * (1.f - s)));
-        }
-        T* d = (T*)g.da + (p0 + row) * 2 * g.ldf + n;
-        store4(d, dg, 4);
-        store4(d + g.ldf, du, 4);
-        if (g.hw) store4((T*)g.hw + (p0 + row) * g.ldf + n, hw, 4);
-      }
-    }
-    if (g.dwpart) {
-      // rows' sums over this tile's columns: the four lanes of a row, then the two waves of the columns
-      __syncthreads();
-      float* red = reinterpret_cast<float*>(lds);
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        part[j] += __shfl_xor(part[j], 16, 64);
-        part[j] += __shfl_xor(part[j], 32, 64);
-        if (q == 0) red[(wave & 1) * BM + 16 * (x0 + j) + r] = part[j];
-      }
-      __syncthreads();
-      for (int i = threadIdx.x; i < rows; i += NT) g.dwpart[(int64_t)ci * g.M + p0 + i] = red[i] + red[BM + i];
-    }
-  }
+  __syncthreads();                                           // the operands in LDS have been read
+  finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, acc,
+                                     reinterpret_cast<float*>(lds));
 }
 
 // ---------------------------------------------------------------- weight gradients
@@ -434,20 +329,23 @@ __global__ __launch_bounds__(NT) void rows_kernel(Args g) {
 // The matrix of the contiguous output index n is the MFMA's A operand; both are turned.
 // FEW: h's arrays lie by slot and the block finds the expert's slots itself.
 template <int KIND, typename S, int MODE, bool VEC, bool FEW>
-__global__ __launch_bounds__(NT) void weights_kernel(Args g) {
+__global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   using E = El<KIND>;
   using T = typename E::T;
   using RA = std::conditional_t<MODE == DWIN, S, T>;
   using RB = std::conditional_t<MODE == DWIN, T, S>;
-  using TT = Tile<KIND, BN, true, RA>;
-  using TB = Tile<KIND, BN, true, RB>;
+  using TT = Tile<KIND, BN, true, RA, NT>;
+  using TB = Tile<KIND, BN, true, RB, NT>;
   __shared__ __align__(16) char lds[2 * TT::BYTES];
   char* la = lds;
   char* lb = lds + TT::BYTES;
   const int na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;   // columns of the operands
   const int ta = (na + BN - 1) / BN, tb = (nb + BN - 1) / BN;
-  int e, c;
-  if (!tile_of(g.E, ta * tb, e, c)) return;
+  // Workgroup w runs on XCD w % 8: every XCD takes a run of each expert's tiles, so that experts with many rows
+  // weigh on all of them
+  const int per = (ta * tb + 7) / 8, e = (int)(blockIdx.x >> 3) / per;
+  const int c = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3) % per;
+  if (c >= ta * tb) return;
   const int b0 = (c / ta) * BN, a0 = (c % ta) * BN;
   __shared__ int16_t list[FEW ? FEW_SLOTS : 1];
   int64_t p0 = 0, cnt;
@@ -470,26 +368,36 @@ __global__ __launch_bounds__(NT) void weights_kernel(Args g) {
       else tok[i] = g.row_of[p0 + (k < cnt ? k : cnt - 1)];
     }
   };
+  // DWIN: A the gathered rows of x, B da's; DWOUT: A hw's rows, B the gathered rows of dy.  VEC as in rows_kernel,
+  // the arrays between the kernels through a buffer over the step's rows.
+  const int64_t gs = MODE == DWIN ? g.xs : g.ds, ps = MODE == DWIN ? 2 * (int64_t)g.ldf : g.ldf;
+  const S* const gbase = MODE == DWIN ? (const S*)g.x : (const S*)g.dy;
+  const T* const pbase = (MODE == DWIN ? (const T*)g.da : (const T*)g.hw) + p0 * ps;
+  const __amdgpu_buffer_rsrc_t gr =
+      buffer_rsrc_bytes(const_cast<S*>(gbase), (uint32_t)((g.T - 1) * gs + g.H) * sizeof(S));
   auto fetch = [&](int64_t k0) {
+    const int left = cnt - k0 < E::BK ? (int)(cnt - k0) : E::BK;
+    const T* const prow = pbase + (FEW ? 0 : k0 * ps);
+    const __amdgpu_buffer_rsrc_t pr =
+        buffer_rsrc_bytes(const_cast<T*>(prow), (uint32_t)((FEW ? g.M : left) * ps) * sizeof(T));
 #pragma unroll
     for (int i = 0; i < TT::PER; ++i) {
-      const int cc = threadIdx.x + i * NT;
-      const int64_t k = k0 + TT::row_of(cc);
-      const int n = TT::chunk_of(cc) * 8;
-      const RA* pa = nullptr;
-      const RB* pb = nullptr;
-      if (k < cnt) {
-        const int64_t pos = FEW ? list[k] : p0 + k;
-        if (MODE == DWIN) {
-          pa = (const RA*)g.x + (int64_t)tok[i] * g.xs + a0 + n;
-          pb = (const RB*)g.da + pos * 2 * g.ldf + b0 + n;
+      const int cc = threadIdx.x + i * NT, kr = TT::row_of(cc), n = TT::chunk_of(cc) * 8;
+      const int ng = (MODE == DWIN ? a0 : b0) + n, np = (MODE == DWIN ? b0 : a0) + n;   // columns of the two
+      const int npc = MODE == DWIN ? nb : na;
+      const int64_t gat = (int64_t)tok[i] * gs + ng, pat = (FEW ? (kr < left ? list[k0 + kr] : 0) : kr) * ps + np;
+      const bool gin = kr < left && ng < g.H, pin = kr < left && np < npc;
+      auto load = [&](auto& gt, auto& pt) {
+        if constexpr (VEC) {
+          gt.fetch(i, gr, gin ? (uint32_t)gat * (uint32_t)sizeof(S) : kDropOffset);
+          pt.fetch(i, pr, pin ? (uint32_t)pat * (uint32_t)sizeof(T) : kDropOffset);
         } else {
-          pa = (const RA*)g.hw + pos * g.ldf + a0 + n;
-          pb = (const RB*)g.dy + (int64_t)tok[i] * g.ds + b0 + n;
+          gt.fetch(i, gbase + gat, gin ? g.H - ng : 0);
+          pt.fetch(i, prow + pat, pin ? npc - np : 0);
         }
-      }
-      A.template fetch<VEC>(i, pa, pa ? na - a0 - n : 0);
-      B.template fetch<VEC>(i, pb, pb ? nb - b0 - n : 0);
+      };
+      if constexpr (MODE == DWIN) load(A, B);
+      else load(B, A);
     }
   };
   f4 acc[4][4];
@@ -578,28 +486,6 @@ __global__ __launch_bounds__(NT) void dweight_kernel(int64_t M, int parts, const
   dweight[s] = t;
 }
 
-// 8 bits: codes and units of h by groups of 128 columns; a wave a group, two columns a lane.
-__global__ __launch_bounds__(NT) void quant_kernel(Args g) {
-  const int ng = g.ldf / QG;
-  const int64_t i = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
-  if (i >= (int64_t)g.offsets[g.E] * ng) return;
-  const int64_t p = i / ng;
-  const int grp = (int)(i - p * ng), lane = threadIdx.x & 63;
-  const float* h = g.a + p * g.ldf + grp * QG + 2 * lane;
-  const float v0 = h[0], v1 = h[1];
-  float top = max_nan(fabsf(v0), fabsf(v1));
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) top = max_nan(top, __shfl_xor(top, off, 64));
-  const float inv = top > 0.f ? 127.f / top : 0.f;
-  auto code = [&](float v) {
-    const float c = rintf(v * inv);
-    return c >= -127.f && c <= 127.f ? (int)c : 0;
-  };
-  *(uint16_t*)((int8_t*)g.h + p * g.ldf + grp * QG + 2 * lane) =
-      (uint16_t)((code(v0) & 0xff) | (code(v1) & 0xff) << 8);
-  if (lane == 0) g.hscale[i] = top / 127.f;
-}
-
 // ---------------------------------------------------------------- host
 inline int up8(int v) { return (v + 7) / 8 * 8; }
 inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
@@ -615,19 +501,21 @@ inline int tile_rows(int64_t M, int E) {
   return avg > 64 ? 128 : avg > 32 ? 64 : 32;
 }
 
-inline bool vec_ok(const void* p, int64_t stride, int size, int n) {
-  return !p || ((uintptr_t)p % 16 == 0 && (stride * size) % 16 == 0 && n % (size == 1 ? 16 : 8) == 0);
+// Whether rows at p can be read 16 bytes at a time through one buffer (all of them below kDropOffset bytes).
+inline bool vec_ok(const void* p, int64_t rows, int64_t stride, int size, int n) {
+  return !p || ((uintptr_t)p % 16 == 0 && (stride * size) % 16 == 0 && n % (size == 1 ? 16 : 8) == 0 &&
+                ((rows - 1) * stride + n) * size < (int64_t)kDropOffset);
 }
 
 template <int KIND, typename S, int MODE>
 void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
-  const int NC = MODE == UP ? 64 : BN;
+  constexpr int WW = waves_w<KIND, MODE>(), NC = MODE == UP ? 32 * WW : 64 * WW;
   const int cols = KIND == I8 && MODE == UP ? g.ldf : MODE == UP || MODE == DH ? g.F : g.H;
   const unsigned grid = tile_grid(g.n_tiles, (cols + NC - 1) / NC);
   auto go = [&](auto NJ) {
     constexpr int nj = decltype(NJ)::value;
-    if (vec) rows_kernel<KIND, S, MODE, nj, true><<<grid, NT, 0, st>>>(g);
-    else rows_kernel<KIND, S, MODE, nj, false><<<grid, NT, 0, st>>>(g);
+    if (vec) rows_kernel<KIND, S, MODE, nj, true><<<grid, 128 * WW, 0, st>>>(g);
+    else rows_kernel<KIND, S, MODE, nj, false><<<grid, 128 * WW, 0, st>>>(g);
   };
   if (tile == 128) go(std::integral_constant<int, 4>{});
   else if (tile == 64) go(std::integral_constant<int, 2>{});
@@ -637,7 +525,8 @@ void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
 template <int KIND, typename S, int MODE, bool FEW = false>
 void launch_weights(const Args& g, bool vec, hipStream_t st) {
   const int64_t na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;
-  const unsigned grid = tile_grid(g.E, ((na + BN - 1) / BN) * ((nb + BN - 1) / BN));
+  const int64_t tiles = ((na + BN - 1) / BN) * ((nb + BN - 1) / BN);
+  const unsigned grid = (unsigned)(8 * g.E * ((tiles + 7) / 8));
   if (vec) weights_kernel<KIND, S, MODE, true, FEW><<<grid, NT, 0, st>>>(g);
   else weights_kernel<KIND, S, MODE, false, FEW><<<grid, NT, 0, st>>>(g);
 }
@@ -686,7 +575,6 @@ inline Space forward_space(const FscExpertDims& d) {
   s.h = at; at += align64(M * ldf * size);
   s.o = at; at += align64(M * ldo_of(d) * 4);
   if (d.dtype == FSC_I8) {
-    s.da = at; at += align64(M * ldf * 4);          // h in 32 bits
     s.hs = at; at += align64(M * (ldf / QG) * 4);
   }
   s.total = at;
@@ -728,8 +616,8 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
 
 template <int KIND, typename S>
 void forward(Args g, int tile, void* y, hipStream_t st) {
-  const bool vin = vec_ok(g.x, g.xs, sizeof(S), g.H) && vec_ok(g.w_in, g.H, sizeof(S), g.H);
-  const bool vout = vec_ok(g.w_out, g.F, sizeof(S), g.F);
+  const bool vin = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H) && vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H);
+  const bool vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
   if (!g.place) {
     if constexpr (KIND == I8) {
       few_launch_q8(g, vin, vout, st);
@@ -739,7 +627,6 @@ void forward(Args g, int tile, void* y, hipStream_t st) {
     }
   } else {
     launch_rows<KIND, S, UP>(g, tile, vin, st);
-    if constexpr (KIND == I8) quant_kernel<<<(unsigned)((g.M * (g.ldf / QG) + 3) / 4), NT, 0, st>>>(g);
     launch_rows<KIND, S, DOWN>(g, tile, vout, st);
   }
   using Y = std::conditional_t<KIND == I8, __bf16, S>;
@@ -748,8 +635,8 @@ void forward(Args g, int tile, void* y, hipStream_t st) {
 
 template <int KIND, typename S>
 void backward(Args g, int tile, void* dx, float* dweight, hipStream_t st) {
-  const bool vdy = vec_ok(g.dy, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.xs, sizeof(S), g.H);
-  const bool vin = vec_ok(g.w_in, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.F, sizeof(S), g.F);
+  const bool vdy = vec_ok(g.dy, g.T, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H);
+  const bool vin = vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
   const bool by_slot = !g.place;
   if (by_slot) few_launch<S>(DH, g, vdy && vout, st);
   else launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
@@ -888,7 +775,6 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
   g.xscale = x_scale; g.in_scale = w_in_scale; g.out_scale = w_out_scale;
   g.h = ws + s.h;
   g.o = (float*)(ws + s.o);
-  g.a = (float*)(ws + s.da);
   g.hscale = (float*)(ws + s.hs);
   forward<I8, int8_t>(g, tile, y, stream);
   return fsc::check_launch("expert_mlp_q8") ? 2 : 0;
