@@ -158,7 +158,9 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
   constexpr bool TR = MODE == DH || MODE == DX;
   using TW = Tile<KIND, BN, TR, S, NT>;
   using TX = Tile<KIND, BM, false, R, NT>;
-  __shared__ __align__(16) char lds[TW::BYTES + TX::BYTES];
+  // the operands; after the products the waves' rows and the sums across waves
+  constexpr int OPERANDS = TW::BYTES + TX::BYTES, AFTER = (2 * WW * TURN + WW * BM) * 4;
+  __shared__ __align__(16) char lds[OPERANDS > AFTER ? OPERANDS : AFTER];
   __shared__ int32_t slots[BM], rws[BM];
   char* lw = lds;
   char* lx = lds + TW::BYTES;
@@ -295,18 +297,17 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
           for (int v = 0; v < 4; ++v) sum[i][j][v] += (float)acc[i][j][v] * u[j];
     }
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < NI; ++i) {
       const int n = n0 + (w0 + i) * 16 + 4 * q;
       f4 sc;
 #pragma unroll
-      for (int v = 0; v < 4; ++v) sc[v] = n + v < g.H ? g.out_scale[(int64_t)e * g.H + n + v] : 0.f;
+      for (int v = 0; v < 4; ++v) sc[v] = g.out_scale[(int64_t)e * g.H + min(n + v, g.H - 1)];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        if (row < rows) store4(g.o + (p0 + row) * g.ldo + n, sum[i][j] * sc, g.H - n);
-      }
+      for (int j = 0; j < NJ; ++j) sum[i][j] *= sc;
     }
-    return;
+    __syncthreads();
+    finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, sum,
+                                       reinterpret_cast<float*>(lds));
   } else {
     fetch(0);
     for (int k0 = 0; k0 < K; k0 += E::BK) {
@@ -317,11 +318,10 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
       if (k0 + E::BK < K) fetch(k0 + E::BK);
       step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
     }
+    __syncthreads();                                         // the operands in LDS have been read
+    finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, acc,
+                                       reinterpret_cast<float*>(lds));
   }
-
-  __syncthreads();                                           // the operands in LDS have been read
-  finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, acc,
-                                     reinterpret_cast<float*>(lds));
 }
 
 // ---------------------------------------------------------------- weight gradients

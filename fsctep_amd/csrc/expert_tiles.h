@@ -39,24 +39,47 @@ struct RowTile {
   const int32_t *slots, *rws;
 };
 
+// Sixteen rows of a wave's sums, NI weight tiles wide, through LDS (TURN floats a wave) into rows: lane l holds the
+// columns 4 (l % L) .. + 3 of the rows l / L + s (64 / L), L = 4 NI lanes a row, so that stores and loads of a row
+// cover whole 128-byte lines where lane (r, q) of the products would touch 64 bytes of sixteen rows.  The wave reads
+// only what it wrote itself.
+template <int NI> struct Turned {
+  static constexpr int L = 4 * NI, R = 64 / L, S = 16 / R, LD = 16 * NI + 4;
+  f4 v[S];
+};
+template <int NI, typename F>
+__device__ __forceinline__ void turn_rows(F&& sums, float* buf, Turned<NI>& t) {
+  const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  using U = Turned<NI>;
+#pragma unroll
+  for (int i = 0; i < NI; ++i) st4(buf + r * U::LD + 16 * i + 4 * q, sums(i));
+#pragma unroll
+  for (int s = 0; s < U::S; ++s) t.v[s] = ld4(buf + (s * U::R + lane / U::L) * U::LD + 4 * (lane % U::L));
+}
+constexpr int TURN = 16 * 68;
+
 // What becomes of a tile's sums.  acc[i][j]: weight tile w0 + i (16 rows of the weight operand), row tile x0 + j; lane
 // (r, q) holds the weight rows 4 q .. 4 q + 3 of row r.  n0: the tile's first output column (up: a weight tile pair
-// is 16 hidden columns, gate then up).  red: WW * BM floats of LDS that nobody reads any more (dh, 8-bit up), WW waves
-// side by side along the weights, this one the wn-th.
-template <int KIND, int MODE, int NI, int NJ, int WW, int BM>
+// is 16 hidden columns, gate then up).  buf: LDS that nobody reads any more, TURN floats for each wave, then WW * BM
+// floats (dh, 8-bit up); WW waves side by side along the weights, this one the wn-th.
+template <int KIND, int MODE, int NI, int NJ, int WW, int BM, typename V>
 __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, int ci, int wn, int w0, int x0,
-                                       typename Acc<KIND>::V (&acc)[NI][NJ], float* red) {
+                                       V (&acc)[NI][NJ], float* buf) {
   using T = typename El<KIND>::T;
   const int lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  float* const mine = buf + (threadIdx.x >> 6) * TURN;
+  float* const red = buf + (blockDim.x >> 6) * TURN;
   if constexpr (MODE == DOWN || MODE == DX) {
+    using U = Turned<NI>;
+    const int n = n0 + w0 * 16 + 4 * (lane % U::L);
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int n = n0 + (w0 + i) * 16 + 4 * q;
+    for (int j = 0; j < NJ; ++j) {
+      U u;
+      turn_rows<NI>([&](int i) { return acc[i][j]; }, mine, u);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        if constexpr (KIND != I8)
-          if (row < t.rows) store4(g.o + (t.p0 + row) * g.ldo + n, acc[i][j], g.H - n);
+      for (int s = 0; s < U::S; ++s) {
+        const int row = 16 * (x0 + j) + s * U::R + lane / U::L;
+        if (row < t.rows) store4(g.o + (t.p0 + row) * g.ldo + n, u.v[s], g.H - n);
       }
     }
   } else if constexpr (MODE == UP && KIND == I8) {
@@ -106,62 +129,72 @@ __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, 
       if (wn == 0 && q == 0) g.hscale[(t.p0 + row) * (g.ldf / QG) + n0 / QG] = top[j] / 127.f;
     }
   } else if constexpr (MODE == UP) {
+    using U = Turned<NI / 2>;
+    const int n = n0 + w0 / 2 * 16 + 4 * (lane % U::L);
 #pragma unroll
-    for (int i = 0; i < NI / 2; ++i) {
-      const int n = n0 + (w0 / 2 + i) * 16 + 4 * q;
+    for (int j = 0; j < NJ; ++j) {
+      U ga, up;
+      turn_rows<NI / 2>([&](int i) { return acc[2 * i][j]; }, mine, ga);
+      turn_rows<NI / 2>([&](int i) { return acc[2 * i + 1][j]; }, mine, up);
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
+      for (int s = 0; s < U::S; ++s) {
+        const int row = 16 * (x0 + j) + s * U::R + lane / U::L;
         if (row >= t.rows || n >= g.ldf) continue;
-        const f4 ga = acc[2 * i][j], up = acc[2 * i + 1][j];
         f4 h;
 #pragma unroll
-        for (int v = 0; v < 4; ++v) h[v] = ga[v] * sigmoid(ga[v]) * up[v];
+        for (int v = 0; v < 4; ++v) h[v] = ga.v[s][v] * sigmoid(ga.v[s][v]) * up.v[s][v];
         if (g.a) {
           float* a = g.a + (t.p0 + row) * 2 * g.ldf + n;
-          st4(a, ga);
-          st4(a + g.ldf, up);
+          st4(a, ga.v[s]);
+          st4(a + g.ldf, up.v[s]);
         }
         store4((T*)g.h + (t.p0 + row) * g.ldf + n, h, 4);
       }
     }
   } else if constexpr (MODE == DH) {
-    float part[NJ];
+    using U = Turned<NI>;
+    const int n = n0 + w0 * 16 + 4 * (lane % U::L);
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) part[j] = 0.f;
+    for (int j = 0; j < NJ; ++j) {
+      U p;
+      turn_rows<NI>([&](int i) { return acc[i][j]; }, mine, p);
+      f4 ga[U::S], up[U::S];
+      float w[U::S];
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int n = n0 + (w0 + i) * 16 + 4 * q;
+      for (int s = 0; s < U::S; ++s) {                     // rows and columns past the tile: the last ones, not stored
+        const int row = min(16 * (x0 + j) + s * U::R + lane / U::L, t.rows - 1);
+        const float* a = g.a + (t.p0 + row) * 2 * g.ldf + min(n, g.ldf - 4);
+        ga[s] = ld4(a);
+        up[s] = ld4(a + g.ldf);
+        w[s] = g.weight[t.slots[row]];
+      }
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        if (row >= t.rows || n >= g.ldf) continue;
-        const float w = g.weight[t.slots[row]];
-        const float* a = g.a + (t.p0 + row) * 2 * g.ldf + n;
-        const f4 ga = ld4(a), up = ld4(a + g.ldf);
+      for (int s = 0; s < U::S; ++s) {
+        const int row = 16 * (x0 + j) + s * U::R + lane / U::L;
+        const bool in = row < t.rows && n < g.ldf;
         f4 dg, du, hw;
+        float part = 0.f;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float s = sigmoid(ga[v]), act = ga[v] * s, h = act * up[v], p = acc[i][j][v], dh = p * w;
-          part[j] += h * p;
-          hw[v] = h * w;
+          const float sg = sigmoid(ga[s][v]), act = ga[s][v] * sg, h = act * up[s][v], pv = p.v[s][v], dh = pv * w[s];
+          part += h * pv;
+          hw[v] = h * w[s];
           du[v] = dh * act;
-          dg[v] = dh * up[v] * (s * (1.f + ga[v] * (1.f - s)));
+          dg[v] = dh * up[s][v] * (sg * (1.f + ga[s][v] * (1.f - sg)));
         }
-        T* d = (T*)g.da + (t.p0 + row) * 2 * g.ldf + n;
-        store4(d, dg, 4);
-        store4(d + g.ldf, du, 4);
-        if (g.hw) store4((T*)g.hw + (t.p0 + row) * g.ldf + n, hw, 4);
+        if (in) {
+          T* d = (T*)g.da + (t.p0 + row) * 2 * g.ldf + n;
+          store4(d, dg, 4);
+          store4(d + g.ldf, du, 4);
+          if (g.hw) store4((T*)g.hw + (t.p0 + row) * g.ldf + n, hw, 4);
+        }
+        if (g.dwpart) {                                    // the row's sum over the wave's columns
+          part = group_sum(in ? part : 0.f, U::L);
+          if (lane % U::L == 0) red[wn * BM + row] = part;
+        }
       }
     }
     if (g.dwpart) {
-      // rows' sums over this tile's columns: the four lanes of a row, then the waves along the columns
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        part[j] += __shfl_xor(part[j], 16, 64);
-        part[j] += __shfl_xor(part[j], 32, 64);
-        if (q == 0) red[wn * BM + 16 * (x0 + j) + r] = part[j];
-      }
       __syncthreads();
       for (int i = threadIdx.x; i < t.rows; i += blockDim.x) {
         float s = red[i];
