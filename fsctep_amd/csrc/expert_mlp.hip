@@ -52,11 +52,12 @@ struct Tile {                                                        // T: the t
   __device__ static constexpr int chunk_of(int c) { return TR ? c % (ROWS / 8) : c % CPR; }
   __device__ static constexpr int swz(int row) { return CPR == 4 ? (row >> 1) & 3 : row & 7; }
 
-  // chunk c of the thread at byte `off` of a buffer, zeros outside it
-  __device__ __forceinline__ void fetch(int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off) {
+  // chunk c of the thread at byte off + more of a buffer (more the same for the wave), zeros outside it or with drop
+  __device__ __forceinline__ void fetch(int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off, int more = 0, bool drop = false) {
+    const int o = (int)(drop ? kDropOffset : off);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      reg[c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, (int)(off + 16 * i), 0, 0));
+      reg[c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, o + 16 * i, more, 0));
   }
   // chunk c of the thread from p (n values of it exist, the rest are zeros), of any alignment
   __device__ __forceinline__ void fetch(int c, const T* p, int n) {
@@ -168,7 +169,6 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
   const int NC = MODE == UP ? BN / 2 : BN;                   // output columns of a tile
   // output columns (8 bits: the last group of h is whole)
   const int cols = KIND == I8 && MODE == UP ? g.ldf : MODE == UP || MODE == DH ? g.F : g.H;
-  const int K = MODE == UP || MODE == DH ? g.H : MODE == DOWN ? g.F : 2 * g.ldf;
   int ti, ci;
   if (!tile_of(g.n_tiles, (cols + NC - 1) / NC, ti, ci)) return;
   const int e = g.tiles[2 * ti];
@@ -183,75 +183,77 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
   }
   __syncthreads();
 
-  // Where a chunk of the thread lies: VEC, byte offsets into a buffer over the expert's weights, over the tile's rows
-  // of an array between the kernels, or over the whole of x or dy (kDropOffset where there is nothing: loads without
-  // branches); else pointers and counts.  The arrays between the kernels are padded with zeros to ldf.
-  const int KX = MODE == DOWN ? g.ldf : K;
+  // The reduction: SEG segments of K entries (dx: the gate half of da and W_in, then the up half).  h and da are padded
+  // with zeros to ldf.
   constexpr bool GATHER = MODE == UP || MODE == DH;
+  constexpr int SEG = MODE == DX ? 2 : 1;
+  const int K = GATHER ? g.H : g.F, KX = GATHER ? g.H : g.ldf;
   const int64_t xld = MODE == UP ? g.xs : MODE == DH ? g.ds : MODE == DOWN ? g.ldf : 2 * (int64_t)g.ldf;
   const R* const xbase = MODE == UP     ? (const R*)g.x
                          : MODE == DH   ? (const R*)g.dy
                          : MODE == DOWN ? (const R*)g.h + p0 * g.ldf
                                         : (const R*)g.da + p0 * 2 * g.ldf;
-  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc_bytes(
-      const_cast<R*>(xbase), (uint32_t)(((GATHER ? g.T : rows) - 1) * xld + (GATHER ? g.H : xld)) * sizeof(R));
-  const int64_t wsize = (MODE == UP || MODE == DX ? 2 : 1) * (int64_t)g.F * g.H;
-  const S* const wbase = (MODE == UP || MODE == DX ? (const S*)g.w_in : (const S*)g.w_out) + e * wsize;
-  const __amdgpu_buffer_rsrc_t wr = buffer_rsrc_bytes(const_cast<S*>(wbase), (uint32_t)(wsize * sizeof(S)));
-  int64_t xrow[TX::PER];                                     // first entry of the chunk's row, -1: none
+  const int64_t wseg = (int64_t)(MODE == UP ? 2 : 1) * g.F * g.H;   // entries of the weights that a segment reads
+  const S* const wbase = (MODE == UP || MODE == DX ? (const S*)g.w_in : (const S*)g.w_out) + e * wseg * SEG;
+  // Where the thread's chunks lie in the first step, in entries (OFF: a 32-bit byte offset for VEC, where buffers over
+  // x or dy, the tile's rows and a segment's weights give zeros outside: loads without branches); kNoChunk: nowhere.
+  using Off = std::conditional_t<VEC, uint32_t, int64_t>;
+  constexpr Off kNoChunk = VEC ? (Off)kDropOffset : (Off)-1;
+  Off xo[TX::PER], wo[TW::PER];
 #pragma unroll
   for (int i = 0; i < TX::PER; ++i) {
     const int c = threadIdx.x + i * NT, row = TX::row_of(c);
-    xrow[i] = c < TX::NCH && row < rows ? (GATHER ? rws[row] : row) * xld : -1;
+    xo[i] = c < TX::NCH && row < rows
+                ? (Off)(((GATHER ? rws[row] : row) * xld + TX::chunk_of(c) * E::CE) * (VEC ? sizeof(R) : 1))
+                : kNoChunk;
   }
-  int64_t wrow[TW::PER];
 #pragma unroll
   for (int i = 0; i < TW::PER; ++i) {
-    const int row = TW::row_of(threadIdx.x + i * NT);
+    const int c = threadIdx.x + i * NT, row = TW::row_of(c);
+    int64_t at = -1;
     if (TR) {
-      const int n = n0 + TW::chunk_of(threadIdx.x + i * NT) * 8;
-      wrow[i] = n < cols ? n : -1;                           // the chunk's column
+      const int n = n0 + TW::chunk_of(c) * 8;
+      if (n < cols) at = (int64_t)row * cols + n;
     } else if (MODE == UP) {
       const int n = n0 + (row >> 5) * 16 + (row & 15);
-      wrow[i] = n < g.F ? (int64_t)((row & 16 ? g.F : 0) + n) * g.H : -1;
-    } else {
-      wrow[i] = n0 + row < g.H ? (int64_t)(n0 + row) * g.F : -1;
+      if (n < g.F) at = (int64_t)((row & 16 ? g.F : 0) + n) * g.H + TW::chunk_of(c) * E::CE;
+    } else if (n0 + row < g.H) {
+      at = (int64_t)(n0 + row) * g.F + TW::chunk_of(c) * E::CE;
     }
+    wo[i] = at >= 0 ? (Off)(at * (VEC ? sizeof(S) : 1)) : kNoChunk;
   }
+  const __amdgpu_buffer_rsrc_t xr = buffer_rsrc_bytes(
+      const_cast<R*>(xbase), (uint32_t)((((GATHER ? g.T : rows) - 1) * xld + (GATHER ? (int64_t)g.H : xld)) * sizeof(R)));
   TW tw;
   TX tx;
-  auto fetch = [&](int k0) {
+  const int per_seg = (K + E::BK - 1) / E::BK, steps = SEG * per_seg;
+  auto fetch = [&](int s) {
+    const int seg = SEG == 2 && s >= per_seg, k0 = (s - seg * per_seg) * E::BK;
+    const bool last = k0 + E::BK > K;                        // the same for the whole block
+    const int64_t xat = seg * g.ldf + k0;
 #pragma unroll
     for (int i = 0; i < TX::PER; ++i) {
-      const int k = k0 + TX::chunk_of(threadIdx.x + i * NT) * E::CE;
-      const bool in = xrow[i] >= 0 && k < KX;
-      if constexpr (VEC) tx.fetch(i, xr, in ? (uint32_t)(xrow[i] + k) * (uint32_t)sizeof(R) : kDropOffset);
-      else tx.fetch(i, xbase + xrow[i] + k, in ? KX - k : 0);
+      const int left = KX - k0 - TX::chunk_of(threadIdx.x + i * NT) * E::CE;
+      if constexpr (VEC) {
+        tx.fetch(i, xr, xo[i], (int)(xat * sizeof(R)), last && left <= 0);
+      } else {
+        tx.fetch(i, xbase + xo[i] + xat, xo[i] < 0 ? 0 : left);
+      }
     }
+    // turned: the buffer begins at row k0 of the segment and ends with it, rows past K are outside
+    const int64_t wat = TR ? (int64_t)k0 * cols : k0;
+    const __amdgpu_buffer_rsrc_t wr = buffer_rsrc_bytes(const_cast<S*>(wbase + seg * wseg + (TR ? wat : 0)),
+                                                        (uint32_t)((wseg - (TR ? wat : 0)) * sizeof(S)));
 #pragma unroll
     for (int i = 0; i < TW::PER; ++i) {
       const int c = threadIdx.x + i * NT;
-      int64_t at;
-      bool in;
-      int n;
-      if (!TR) {
-        const int k = k0 + TW::chunk_of(c) * E::CE;
-        in = wrow[i] >= 0 && k < K;
-        at = wrow[i] + k;
-        n = K - k;
+      const int left = TR ? K - k0 - TW::row_of(c) : K - k0 - TW::chunk_of(c) * E::CE;
+      if constexpr (VEC) {
+        tw.fetch(i, wr, wo[i], TR ? 0 : (int)(wat * sizeof(S)), !TR && last && left <= 0);
       } else {
-        int k = k0 + TW::row_of(c);
-        in = wrow[i] >= 0 && k < K;
-        n = cols - (int)wrow[i];
-        if (MODE == DX) {                                    // rows of the gate half, padding, rows of the up half
-          const int half = k >= g.ldf, f = k - half * g.ldf;
-          in = in && f < g.F;
-          k = half * g.F + f;
-        }
-        at = (int64_t)k * cols + wrow[i];
+        const int n = TR ? cols - n0 - TW::chunk_of(c) * 8 : left;
+        tw.fetch(i, wbase + seg * wseg + wo[i] + wat, wo[i] < 0 || left <= 0 ? 0 : n);
       }
-      if constexpr (VEC) tw.fetch(i, wr, in ? (uint32_t)at * (uint32_t)sizeof(S) : kDropOffset);
-      else tw.fetch(i, wbase + at, in ? n : 0);
     }
   };
 
@@ -272,17 +274,17 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
       for (int j = 0; j < NJ; ++j) sum[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     const int ng = g.ldf / QG;
     fetch(0);
-    for (int k0 = 0; k0 < K; k0 += E::BK) {
+    for (int s = 0; s < steps; ++s) {
       __syncthreads();
       tw.put(lw);
       tx.put(lx);
       __syncthreads();
-      if (k0 + E::BK < K) fetch(k0 + E::BK);
+      if (s + 1 < steps) fetch(s + 1);
       float u[NJ];
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int row = 16 * (x0 + j) + r;
-        u[j] = row < rows ? g.hscale[(p0 + row) * ng + k0 / QG] : 0.f;
+        u[j] = row < rows ? g.hscale[(p0 + row) * ng + s] : 0.f;
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -310,12 +312,12 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
                                        reinterpret_cast<float*>(lds));
   } else {
     fetch(0);
-    for (int k0 = 0; k0 < K; k0 += E::BK) {
+    for (int s = 0; s < steps; ++s) {
       __syncthreads();
       tw.put(lw);
       tx.put(lx);
       __syncthreads();
-      if (k0 + E::BK < K) fetch(k0 + E::BK);
+      if (s + 1 < steps) fetch(s + 1);
       step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
     }
     __syncthreads();                                         // the operands in LDS have been read
