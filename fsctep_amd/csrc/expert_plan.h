@@ -10,7 +10,7 @@ namespace experts {
 constexpr int MAX_EXPERTS = 512;
 
 struct Plan {
-  int32_t *offsets, *slot_of, *row_of, *place, *tiles;
+  int32_t *offsets, *slot_of, *row_of, *place, *tiles, *counts;
   int n_tiles;
 };
 

@@ -225,7 +225,8 @@ def problem(rows, width, hidden, experts, k, dt, seed, empty=True):
 # rows, width, hidden, experts, k: single rows, sizes around every tile, primes, many experts, all rows on one expert
 MLP = [(1, 640, 640, 8, 2), (1, 7, 5, 3, 1), (2, 64, 64, 2, 2), (15, 33, 17, 4, 3), (16, 128, 64, 1, 1), (17, 96, 130, 3, 2),
        (33, 640, 320, 8, 2), (100, 331, 203, 5, 2), (129, 130, 66, 2, 1), (300, 72, 136, 3, 2), (700, 264, 128, 4, 2),
-       (64, 48, 40, 64, 4), (1000, 40, 24, 1, 1), (513, 36, 1, 2, 1), (40, 1, 9, 2, 1)]
+       (64, 48, 40, 64, 4), (1000, 40, 24, 1, 1), (2500, 24, 16, 7, 4),
+       (4100, 16, 8, 300, 3), (513, 36, 1, 2, 1), (40, 1, 9, 2, 1)]
 
 
 @pytest.mark.parametrize("rows,width,hidden,experts,k", MLP)
@@ -337,7 +338,7 @@ def test_products_empty():
 
 
 Q8 = [(1, 640, 640, 8, 2), (33, 640, 320, 8, 2), (5, 17, 40, 2, 1), (100, 331, 203, 5, 2), (300, 128, 256, 3, 2),
-      (700, 64, 130, 4, 1), (40, 16, 128, 64, 4)]
+      (700, 64, 130, 4, 1), (40, 16, 128, 64, 4), (3000, 32, 48, 5, 3)]
 
 
 @pytest.mark.parametrize("rows,width,hidden,experts,k", Q8)
