@@ -5,8 +5,13 @@
 //   dx      W_in[e]^T da, summed over a row's experts                          (combine_kernel)
 //   dw_in   sum over rows of da x^T;  dw_out  sum over rows of dy (weight h)^T
 // All are products over tiles of 128 x (32, 64 or 128) entries on the matrix cores, 32-bit accumulators:
-//   bf16 rows: v_mfma_f32_16x16x32_bf16;  fp32 rows: three bf16 parts an operand and six such products (split3,
-//   mfma_x6: as accurate as fp32 at any scale);  8-bit rows: v_mfma_i32_16x16x64_i8.
+//   bf16 rows: v_mfma_f32_16x16x32_bf16;  8-bit rows: v_mfma_i32_16x16x64_i8;
+//   fp32 rows: two fp16 parts an operand and three products (split2h_pk, mfma_x3), each row of the rows' operand and
+//     each output column's weights brought below 2^14 by a power of two of their own (from their largest magnitude,
+//     one pass before the products; h's and da's come from the products that make them) and the sums brought back
+//     exactly: 22 bits of every value down to 2^-17 of its row's largest, 2^-39 of that below;
+//   fp32 weight gradients: three bf16 parts and six products (split3, mfma_x6), 24 bits at any scale, since there the
+//     sum runs over rows of different scales.
 // The weights are the MFMA's A operand, the rows its B operand: a lane's four results are four neighbouring
 // columns of one row, stored by one access.
 //
@@ -47,6 +52,9 @@ struct Tile {                                                        // T: the t
 
   struct Reg { u4v v[NV]; };
   Reg reg[PER];
+  // F32: what the values are multiplied by, for each chunk (straight) or column of the thread's chunks (turned)
+  static constexpr int NSC = KIND == F32 ? (TR ? 8 : PER) : 1;
+  float scale[NSC];
 
   __device__ static constexpr int row_of(int c) { return TR ? c / (ROWS / 8) : c / CPR; }
   __device__ static constexpr int chunk_of(int c) { return TR ? c % (ROWS / 8) : c % CPR; }
@@ -74,19 +82,29 @@ struct Tile {                                                        // T: the t
       if (NCH % NT && c >= NCH) break;
       const int row = row_of(c), kc = chunk_of(c);
       const int at = TR ? row * TRP * 2 + kc * 16 : (row * CPR + (kc ^ swz(row))) * 16;
-      if constexpr (KIND == F32) {
-        bf8 h, m, l;
+      if constexpr (KIND == F32 || KIND == X6) {
+        float v[8];
         if constexpr (sizeof(T) == 4) {
-          float v[8];
           __builtin_memcpy(v, &reg[i], 32);
-          split3(v, h, m, l);
-        } else {                                                     // a bf16 value is its own first part
-          h = __builtin_bit_cast(bf8, reg[i].v[0]);
-          m = l = __builtin_bit_cast(bf8, u4v{0, 0, 0, 0});
+        } else {
+          const bf8 b = __builtin_bit_cast(bf8, reg[i].v[0]);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = (float)b[j];
         }
-        *reinterpret_cast<bf8*>(lds + at) = h;
-        *reinterpret_cast<bf8*>(lds + PLANE + at) = m;
-        *reinterpret_cast<bf8*>(lds + 2 * PLANE + at) = l;
+        if constexpr (KIND == F32) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] *= scale[TR ? j : i];
+          h8 h, l;
+          split2h_pk(v, h, l);
+          *reinterpret_cast<h8*>(lds + at) = h;
+          *reinterpret_cast<h8*>(lds + PLANE + at) = l;
+        } else {
+          bf8 h, m, l;
+          split3(v, h, m, l);
+          *reinterpret_cast<bf8*>(lds + at) = h;
+          *reinterpret_cast<bf8*>(lds + PLANE + at) = m;
+          *reinterpret_cast<bf8*>(lds + 2 * PLANE + at) = l;
+        }
       } else {
         *reinterpret_cast<u4v*>(lds + at) = reg[i].v[0];
       }
@@ -130,6 +148,9 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         if constexpr (KIND == F32)
+          acc[i][j] = mfma_x3(__builtin_bit_cast(h8, w[0]), __builtin_bit_cast(h8, w[1]),
+                              __builtin_bit_cast(h8, x[j][0]), __builtin_bit_cast(h8, x[j][1]), acc[i][j]);
+        else if constexpr (KIND == X6)
           acc[i][j] = mfma_x6(__builtin_bit_cast(bf8, w[0]), __builtin_bit_cast(bf8, w[1]),
                               __builtin_bit_cast(bf8, w[2]), __builtin_bit_cast(bf8, x[j][0]),
                               __builtin_bit_cast(bf8, x[j][1]), __builtin_bit_cast(bf8, x[j][2]), acc[i][j]);
@@ -226,6 +247,25 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
       const_cast<R*>(xbase), (uint32_t)((((GATHER ? g.T : rows) - 1) * xld + (GATHER ? (int64_t)g.H : xld)) * sizeof(R)));
   TW tw;
   TX tx;
+  // fp32: the powers of two of this tile's rows and of the output columns' weights
+  const uint32_t* const xm = MODE == UP ? g.xmost : MODE == DH ? g.dymost : MODE == DOWN ? g.hmost + p0 : g.damost + p0;
+  const uint32_t* const wm = MODE == UP     ? g.in_row + (int64_t)e * 2 * g.F
+                             : MODE == DOWN ? g.out_row + (int64_t)e * g.H
+                             : MODE == DH   ? g.out_col + (int64_t)e * g.F
+                                            : g.in_col + (int64_t)e * g.H;
+  auto row_exp = [&](int row) { return part_exp(xm[GATHER ? rws[row < rows ? row : 0] : row < rows ? row : 0]); };
+  // weight row (straight) or column (turned) i of the tile; past the last: any
+  auto weight_exp = [&](int i) {
+    const int n = MODE == UP ? (i & 16 ? g.F : 0) + min(n0 + (i >> 5) * 16 + (i & 15), g.F - 1) : min(n0 + i, cols - 1);
+    return part_exp(wm[n]);
+  };
+  if constexpr (KIND == F32) {
+#pragma unroll
+    for (int i = 0; i < TX::PER; ++i) tx.scale[i] = ldexpf(1.f, row_exp(TX::row_of(threadIdx.x + i * NT) % BM));
+#pragma unroll
+    for (int i = 0; i < TW::NSC; ++i)
+      tw.scale[i] = ldexpf(1.f, weight_exp(TR ? TW::chunk_of(threadIdx.x) * 8 + i : TW::row_of(threadIdx.x + i * NT)));
+  }
   const int per_seg = (K + E::BK - 1) / E::BK, steps = SEG * per_seg;
   auto fetch = [&](int s) {
     const int seg = SEG == 2 && s >= per_seg, k0 = (s - seg * per_seg) * E::BK;
@@ -319,6 +359,20 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
       __syncthreads();
       if (s + 1 < steps) fetch(s + 1);
       step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
+    }
+    if constexpr (KIND == F32) {
+      const int r = lane & 15, q = lane >> 4;
+      int xe[NJ];
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) xe[j] = row_exp(16 * (x0 + j) + r);
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const int we = weight_exp(16 * (w0 + i) + 4 * q + v);
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[i][j][v] = __builtin_amdgcn_ldexpf(acc[i][j][v], -(xe[j] + we));
+        }
     }
     __syncthreads();                                         // the operands in LDS have been read
     finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, acc,
@@ -446,6 +500,62 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   }
 }
 
+// ---------------------------------------------------------------- largest magnitudes, for the fp32 products' parts
+// Rows of up to three arrays (a wave a row) and zeros for what later kernels raise.
+struct Maxima {
+  const void* p[3];
+  int64_t rows[3], ld[3];
+  int n[3];
+  uint32_t* out[3];
+  uint32_t* zero;
+  int64_t zeros;
+};
+
+template <typename S>
+__global__ __launch_bounds__(NT) void row_most_kernel(Maxima a) {
+  const int lane = threadIdx.x & 63;
+  int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
+  const int64_t z = (int64_t)blockIdx.x * NT + threadIdx.x, zn = (int64_t)gridDim.x * NT;
+  for (int64_t i = z; i < a.zeros; i += zn) a.zero[i] = 0;
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    if (row >= 0 && row < a.rows[k]) {
+      const S* p = (const S*)a.p[k] + row * a.ld[k];
+      constexpr int V = 16 / sizeof(S);
+      uint32_t m = 0;
+      if ((uintptr_t)p % 16 == 0 && a.n[k] % V == 0) {
+        for (int i = lane * V; i < a.n[k]; i += 64 * V) {
+          float v[V];
+          load_vec<V>(p + i, v);
+#pragma unroll
+          for (int j = 0; j < V; ++j) m = max(m, abs_bits(v[j]));
+        }
+      } else {
+        for (int i = lane; i < a.n[k]; i += 64) m = max(m, abs_bits(to_f(p[i])));
+      }
+#pragma unroll
+      for (int off = 32; off > 0; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
+      if (lane == 0) a.out[k][row] = m;
+    }
+    row -= a.rows[k];
+  }
+}
+
+// Columns of an expert's matrix (R x n): 64 columns and 64 rows a block, raised in `out` [E][n], zeros before.
+template <typename S>
+__global__ __launch_bounds__(NT) void col_most_kernel(const S* __restrict__ w, int R, int n, uint32_t* __restrict__ out) {
+  const int c = blockIdx.x * 64 + (threadIdx.x & 63), r0 = blockIdx.y * 64 + (threadIdx.x >> 6);
+  if (c >= n) return;
+  const S* p = w + (int64_t)blockIdx.z * R * n + c;
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const int r = r0 + 4 * i;
+    m = max(m, abs_bits(to_f(p[(int64_t)(r < R ? r : r0 < R ? r0 : 0) * n])));
+  }
+  atomicMax(out + (int64_t)blockIdx.z * n + c, m);
+}
+
 // ---------------------------------------------------------------- rows from their experts, in slot order
 // The row of a slot in the arrays between the kernels, -1 for a slot with no expert.
 __device__ __forceinline__ int place_of(const int32_t* place, const int32_t* index, int E, int64_t s) {
@@ -533,6 +643,12 @@ void launch_weights(const Args& g, bool vec, hipStream_t st) {
   else weights_kernel<KIND, S, MODE, false, FEW><<<grid, NT, 0, st>>>(g);
 }
 
+template <typename S>
+void launch_row_most(const Maxima& a, hipStream_t st) {
+  const int64_t rows = a.rows[0] + a.rows[1] + a.rows[2];
+  row_most_kernel<S><<<(unsigned)std::max<int64_t>(1, (rows + 3) / 4), NT, 0, st>>>(a);
+}
+
 template <typename T>
 void launch_combine(const Args& g, const float* weight, T* y, hipStream_t st) {
   const int64_t n = g.T * ((g.H + 3) / 4);
@@ -568,14 +684,21 @@ inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 
 
 // Parts of a workspace, in bytes.
 struct Space {
-  int64_t h, o, da, hw, part, hs, total;
+  int64_t h, o, da, hw, part, hs, most, total;
 };
+// whether the products are fp32 ones by tiles
+inline bool parts(const FscExpertDims& d) {
+  return !few(d.rows * d.k, d.n_experts) && (d.dtype == FSC_F32 || fine(d));
+}
 inline Space forward_space(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, ldf = ldf_of(d), size = held_size(d);
   Space s{};
   int64_t at = 0;
   s.h = at; at += align64(M * ldf * size);
   s.o = at; at += align64(M * ldo_of(d) * 4);
+  if (parts(d)) {
+    s.most = at; at += align64((d.rows + M + (int64_t)d.n_experts * (2 * d.hidden + d.width)) * 4);
+  }
   if (d.dtype == FSC_I8) {
     s.hs = at; at += align64(M * (ldf / QG) * 4);
   }
@@ -590,6 +713,9 @@ inline Space backward_space(const FscExpertDims& d) {
   s.da = at; at += align64(M * 2 * ldf * size);
   s.hw = at; at += align64(M * ldf * size);
   s.part = at; at += align64(M * ((d.hidden + 31) / 32) * 4);
+  if (parts(d)) {
+    s.most = at; at += align64((d.rows + M + (int64_t)d.n_experts * (d.hidden + d.width)) * 4);
+  }
   s.total = at;
   return s;
 }
@@ -628,6 +754,11 @@ void forward(Args g, int tile, void* y, hipStream_t st) {
       few_launch<S>(DOWN, g, vout, st);
     }
   } else {
+    if constexpr (KIND == F32) {
+      const int64_t in = (int64_t)g.E * 2 * g.F, out = (int64_t)g.E * g.H;
+      launch_row_most<S>(Maxima{{g.x, g.w_in, g.w_out}, {g.T, in, out}, {g.xs, g.H, g.F}, {g.H, g.H, g.F},
+                                {g.xmost, g.in_row, g.out_row}, g.hmost, g.M}, st);
+    }
     launch_rows<KIND, S, UP>(g, tile, vin, st);
     launch_rows<KIND, S, DOWN>(g, tile, vout, st);
   }
@@ -640,6 +771,13 @@ void backward(Args g, int tile, void* dx, float* dweight, hipStream_t st) {
   const bool vdy = vec_ok(g.dy, g.T, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H);
   const bool vin = vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
   const bool by_slot = !g.place;
+  if constexpr (KIND == F32)
+    if (!by_slot) {        // out_col, in_col and damost lie one after the other
+      launch_row_most<S>(Maxima{{g.dy, nullptr, nullptr}, {g.T, 0, 0}, {g.ds, 0, 0}, {g.H, 0, 0},
+                                {g.dymost, nullptr, nullptr}, g.out_col, (int64_t)g.E * (g.F + g.H) + g.M}, st);
+      col_most_kernel<S><<<dim3((g.F + 63) / 64, (g.H + 63) / 64, g.E), NT, 0, st>>>((const S*)g.w_out, g.H, g.F, g.out_col);
+      if (dx) col_most_kernel<S><<<dim3((g.H + 63) / 64, (2 * g.F + 63) / 64, g.E), NT, 0, st>>>((const S*)g.w_in, 2 * g.F, g.H, g.in_col);
+    }
   if (by_slot) few_launch<S>(DH, g, vdy && vout, st);
   else launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
   if (dweight)
@@ -652,12 +790,13 @@ void backward(Args g, int tile, void* dx, float* dweight, hipStream_t st) {
   }
   if (by_slot) {
     if constexpr (KIND == F32) {
-      if (g.dw_in) launch_weights<F32, S, DWIN, true>(g, vx, st);
-      if (g.dw_out) launch_weights<F32, S, DWOUT, true>(g, vdy, st);
+      if (g.dw_in) launch_weights<X6, S, DWIN, true>(g, vx, st);
+      if (g.dw_out) launch_weights<X6, S, DWOUT, true>(g, vdy, st);
     }
   } else {
-    if (g.dw_in) launch_weights<KIND, S, DWIN>(g, vx, st);
-    if (g.dw_out) launch_weights<KIND, S, DWOUT>(g, vdy, st);
+    constexpr int WK = KIND == F32 ? X6 : KIND;
+    if (g.dw_in) launch_weights<WK, S, DWIN>(g, vx, st);
+    if (g.dw_out) launch_weights<WK, S, DWOUT>(g, vdy, st);
   }
 }
 
@@ -709,6 +848,12 @@ int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const vo
   g.x = x; g.xs = x_stride; g.weight = weight; g.w_in = w_in; g.w_out = w_out; g.a = saved;
   g.h = ws + s.h;
   g.o = (float*)(ws + s.o);
+  if (parts(*dims)) {
+    g.xmost = (uint32_t*)(ws + s.most);
+    g.hmost = g.xmost + g.T;
+    g.in_row = g.hmost + g.M;
+    g.out_row = g.in_row + (int64_t)g.E * 2 * g.F;
+  }
   if (dims->dtype == FSC_F32) forward<F32, float>(g, tile, y, stream);
   else if (fine(*dims)) forward<F32, __bf16>(g, tile, y, stream);
   else forward<BF16, __bf16>(g, tile, y, stream);
@@ -735,17 +880,23 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
   g.a = const_cast<float*>(saved);
   g.o = (float*)(ws + s.o);
   g.da = ws + s.da;
+  if (parts(*dims)) {
+    g.dymost = (uint32_t*)(ws + s.most);
+    g.out_col = g.dymost + g.T;
+    g.in_col = g.out_col + (int64_t)g.E * g.F;
+    g.damost = g.in_col + (int64_t)g.E * g.H;
+  }
   g.hw = dw_out ? ws + s.hw : nullptr;
   g.dwpart = dweight ? (float*)(ws + s.part) : nullptr;
   g.dw_in = dw_in;
   g.dw_out = dw_out;
   if (M == 0) {              // no rows: zero weight gradients, written by the products' empty sums
     if (dims->dtype == FSC_F32) {
-      if (dw_in) launch_weights<F32, float, DWIN, true>(g, false, stream);
-      if (dw_out) launch_weights<F32, float, DWOUT, true>(g, false, stream);
+      if (dw_in) launch_weights<X6, float, DWIN, true>(g, false, stream);
+      if (dw_out) launch_weights<X6, float, DWOUT, true>(g, false, stream);
     } else {
-      if (dw_in) launch_weights<F32, __bf16, DWIN, true>(g, false, stream);
-      if (dw_out) launch_weights<F32, __bf16, DWOUT, true>(g, false, stream);
+      if (dw_in) launch_weights<X6, __bf16, DWIN, true>(g, false, stream);
+      if (dw_out) launch_weights<X6, __bf16, DWOUT, true>(g, false, stream);
     }
   } else if (dims->dtype == FSC_F32) {
     backward<F32, float>(g, tile, dx, dweight, stream);

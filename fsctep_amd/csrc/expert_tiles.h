@@ -10,16 +10,26 @@ namespace experts {
 
 typedef int i4v __attribute__((ext_vector_type(4)));
 
-enum Kind { F32 = 0, BF16 = 1, I8 = 2 };
+// F32: fp32 products from two scaled fp16 parts an operand (mfma_x3); X6: from three bf16 parts (mfma_x6)
+enum Kind { F32 = 0, BF16 = 1, I8 = 2, X6 = 3 };
 
 // T: the type between the kernels; BK: reduction entries of a step; CE: those of a 16-byte LDS chunk; PL: LDS planes
 template <int KIND> struct El;
-template <> struct El<F32> { using T = float; static constexpr int BK = 32, CE = 8, PL = 3; };
+template <> struct El<F32> { using T = float; static constexpr int BK = 32, CE = 8, PL = 2; };
+template <> struct El<X6> { using T = float; static constexpr int BK = 32, CE = 8, PL = 3; };
 template <> struct El<BF16> { using T = __bf16; static constexpr int BK = 64, CE = 8, PL = 1; };
 template <> struct El<I8> { using T = int8_t; static constexpr int BK = 128, CE = 16, PL = 1; };
 
 template <int KIND> struct Acc { using V = f4; };
 template <> struct Acc<I8> { using V = i4v; };
+
+// The power of two k that brings values up to `most` (bits of a non-negative float) below 2^14, for their two fp16
+// parts: 0 where there is nothing to bring (zero, infinity, NaN); within the exponents of normal floats.
+__device__ __forceinline__ int part_exp(uint32_t most) {
+  if (most == 0 || most >= 0x7f800000u) return 0;
+  return min(max(14 - __builtin_amdgcn_frexp_expf(__uint_as_float(most)), -126), 126);
+}
+__device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 // Workgroup -> (row tile, column tile).  Workgroup w runs on XCD w % 8: each XCD takes a contiguous run of row
 // tiles with all their column tiles, so that a tile's rows and an expert's weights meet in one L2.
@@ -57,6 +67,17 @@ __device__ __forceinline__ void turn_rows(F&& sums, float* buf, Turned<NI>& t) {
   for (int s = 0; s < U::S; ++s) t.v[s] = ld4(buf + (s * U::R + lane / U::L) * U::LD + 4 * (lane % U::L));
 }
 constexpr int TURN = 16 * 68;
+
+// Raises a row's largest magnitude so far (bits; a NaN is above all numbers) by the values of `width` neighbouring
+// lanes, all of which call it with the same row.  Maxima do not depend on their order.
+__device__ __forceinline__ uint32_t most4(const f4& v) {
+  return max(max(abs_bits(v.x), abs_bits(v.y)), max(abs_bits(v.z), abs_bits(v.w)));
+}
+__device__ __forceinline__ void raise(uint32_t* most, uint32_t m, int width, bool in) {
+#pragma unroll
+  for (int off = width >> 1; off > 0; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
+  if (in && (threadIdx.x & (width - 1)) == 0) atomicMax(most, m);
+}
 
 // What becomes of a tile's sums.  acc[i][j]: weight tile w0 + i (16 rows of the weight operand), row tile x0 + j; lane
 // (r, q) holds the weight rows 4 q .. 4 q + 3 of row r.  n0: the tile's first output column (up: a weight tile pair
@@ -139,10 +160,12 @@ __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, 
 #pragma unroll
       for (int s = 0; s < U::S; ++s) {
         const int row = 16 * (x0 + j) + s * U::R + lane / U::L;
-        if (row >= t.rows || n >= g.ldf) continue;
         f4 h;
 #pragma unroll
         for (int v = 0; v < 4; ++v) h[v] = ga.v[s][v] * sigmoid(ga.v[s][v]) * up.v[s][v];
+        // columns past the last have sums of zero
+        if constexpr (KIND == F32) raise(g.hmost + t.p0 + row, most4(h), U::L, row < t.rows);
+        if (row >= t.rows || n >= g.ldf) continue;
         if (g.a) {
           float* a = g.a + (t.p0 + row) * 2 * g.ldf + n;
           st4(a, ga.v[s]);
@@ -188,6 +211,7 @@ __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, 
           store4(d + g.ldf, du, 4);
           if (g.hw) store4((T*)g.hw + (t.p0 + row) * g.ldf + n, hw, 4);
         }
+        if constexpr (KIND == F32) raise(g.damost + t.p0 + row, in ? max(most4(dg), most4(du)) : 0, U::L, row < t.rows);
         if (g.dwpart) {                                    // the row's sum over the wave's columns
           part = group_sum(in ? part : 0.f, U::L);
           if (lane % U::L == 0) red[wn * BM + row] = part;
