@@ -17,6 +17,7 @@ struct Args {
   int64_t T, M;
   int H, F, ldf, ldo, E, k, n_tiles;
   int64_t xs, ds;                   // row strides of x and dy, in elements
+  int64_t li, lo;                   // row lengths of w_in and w_out (H and F, or padded to whole chunks)
   const int32_t *index;             // [M]
   uint32_t k_inv;                   // ceil(2^20 / k): slot / k = slot k_inv / 2^20 for the few-rows slots (below 1,024)
   const int32_t *offsets, *slot_of, *row_of, *tiles, *place;   // the rows by expert; null where there are few rows
@@ -30,6 +31,8 @@ struct Args {
   void* hw;                         // [M][ldf] weight h, for dw_out (null: not wanted)
   float* dwpart;                    // [column tiles of dh][M] partial dweight
   void *dw_in, *dw_out;
+  float* dwsplit;                   // [splits] partial weight gradients, where the positions are split
+  int splits;
   // fp32 products: largest magnitudes (bits) of the rows of x and dy [T], of h and da [M], of the weights along each
   // output: rows of w_in [E][2 F] and w_out [E][H] (up, down), columns of w_out [E][F] and w_in [E][H] (dh, dx)
   uint32_t *xmost, *dymost, *hmost, *damost, *in_row, *out_row, *out_col, *in_col;

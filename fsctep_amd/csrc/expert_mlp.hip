@@ -164,6 +164,8 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
   }
 }
 
+inline __host__ __device__ int64_t whole_chunks(int64_t n, int ce) { return (n + ce - 1) / ce * ce; }
+
 // ---------------------------------------------------------------- the products by row tiles
 // up: 64 hidden columns a tile, their gate and up rows in turn by 16, so that a wave holds both of a column.
 // WW waves side by side along the weight operand, four (8-bit up: so many that 128 hidden columns make a tile)
@@ -214,7 +216,8 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
                          : MODE == DH   ? (const R*)g.dy
                          : MODE == DOWN ? (const R*)g.h + p0 * g.ldf
                                         : (const R*)g.da + p0 * 2 * g.ldf;
-  const int64_t wseg = (int64_t)(MODE == UP ? 2 : 1) * g.F * g.H;   // entries of the weights that a segment reads
+  const int64_t wld = MODE == UP || MODE == DX ? g.li : g.lo;
+  const int64_t wseg = (MODE == UP ? 2 * g.F : MODE == DX ? g.F : g.H) * wld;   // entries of the weights of a segment
   const S* const wbase = (MODE == UP || MODE == DX ? (const S*)g.w_in : (const S*)g.w_out) + e * wseg * SEG;
   // Where the thread's chunks lie in the first step, in entries (OFF: a 32-bit byte offset for VEC, where buffers over
   // x or dy, the tile's rows and a segment's weights give zeros outside: loads without branches); kNoChunk: nowhere.
@@ -234,17 +237,17 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
     int64_t at = -1;
     if (TR) {
       const int n = n0 + TW::chunk_of(c) * 8;
-      if (n < cols) at = (int64_t)row * cols + n;
+      if (n < cols) at = row * wld + n;
     } else if (MODE == UP) {
       const int n = n0 + (row >> 5) * 16 + (row & 15);
-      if (n < g.F) at = (int64_t)((row & 16 ? g.F : 0) + n) * g.H + TW::chunk_of(c) * E::CE;
+      if (n < g.F) at = ((row & 16 ? g.F : 0) + n) * wld + TW::chunk_of(c) * E::CE;
     } else if (n0 + row < g.H) {
-      at = (int64_t)(n0 + row) * g.F + TW::chunk_of(c) * E::CE;
+      at = (n0 + row) * wld + TW::chunk_of(c) * E::CE;
     }
     wo[i] = at >= 0 ? (Off)(at * (VEC ? sizeof(S) : 1)) : kNoChunk;
   }
   const __amdgpu_buffer_rsrc_t xr = buffer_rsrc_bytes(
-      const_cast<R*>(xbase), (uint32_t)((((GATHER ? g.T : rows) - 1) * xld + (GATHER ? (int64_t)g.H : xld)) * sizeof(R)));
+      const_cast<R*>(xbase), (uint32_t)((((GATHER ? g.T : rows) - 1) * xld + (GATHER ? whole_chunks(g.H, E::CE) : xld)) * sizeof(R)));
   TW tw;
   TX tx;
   // fp32: the powers of two of this tile's rows and of the output columns' weights
@@ -281,7 +284,7 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
       }
     }
     // turned: the buffer begins at row k0 of the segment and ends with it, rows past K are outside
-    const int64_t wat = TR ? (int64_t)k0 * cols : k0;
+    const int64_t wat = TR ? k0 * wld : k0;
     const __amdgpu_buffer_rsrc_t wr = buffer_rsrc_bytes(const_cast<S*>(wbase + seg * wseg + (TR ? wat : 0)),
                                                         (uint32_t)((wseg - (TR ? wat : 0)) * sizeof(S)));
 #pragma unroll
@@ -409,8 +412,10 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
     cnt = few_slots(g, e, few_first(g), list);
     __syncthreads();
   } else {
-    p0 = g.offsets[e];
-    cnt = g.offsets[e + 1] - p0;
+    // the split's share of the expert's positions, in whole steps
+    const int64_t all = g.offsets[e + 1] - g.offsets[e], share = (all + g.splits * E::BK - 1) / (g.splits * E::BK) * E::BK;
+    p0 = g.offsets[e] + std::min<int64_t>(all, blockIdx.y * share);
+    cnt = std::min<int64_t>(share, g.offsets[e + 1] - p0);
   }
   TT A;
   TB B;
@@ -430,7 +435,7 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   const S* const gbase = MODE == DWIN ? (const S*)g.x : (const S*)g.dy;
   const T* const pbase = (MODE == DWIN ? (const T*)g.da : (const T*)g.hw) + p0 * ps;
   const __amdgpu_buffer_rsrc_t gr =
-      buffer_rsrc_bytes(const_cast<S*>(gbase), (uint32_t)((g.T - 1) * gs + g.H) * sizeof(S));
+      buffer_rsrc_bytes(const_cast<S*>(gbase), (uint32_t)(((g.T - 1) * gs + whole_chunks(g.H, E::CE)) * sizeof(S)));
   auto fetch = [&](int64_t k0) {
     const int left = cnt - k0 < E::BK ? (int)(cnt - k0) : E::BK;
     const T* const prow = pbase + (FEW ? 0 : k0 * ps);
@@ -492,52 +497,85 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
     if (out < 0) continue;
     const int len = MODE == DWIN ? g.H : g.F;
     S* dw = (S*)(MODE == DWIN ? g.dw_in : g.dw_out) + out;
+    float* part = g.dwsplit + blockIdx.y * ((int64_t)g.E * (MODE == DWIN ? 2 : 1) * g.F * g.H) + out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = a0 + (w0 + i) * 16 + 4 * q;
-      if (n < len) store4(dw + n, acc[i][j], len - n);
+      if (n >= len) continue;
+      if (!FEW && g.splits > 1) store4(part + n, acc[i][j], len - n);
+      else store4(dw + n, acc[i][j], len - n);
     }
   }
 }
 
-// ---------------------------------------------------------------- largest magnitudes, for the fp32 products' parts
-// Rows of up to three arrays (a wave a row) and zeros for what later kernels raise.
-struct Maxima {
-  const void* p[3];
-  int64_t rows[3], ld[3];
-  int n[3];
-  uint32_t* out[3];
+// A weight gradient from its splits, in their order.
+template <typename S>
+__global__ __launch_bounds__(NT) void sum_splits_kernel(int64_t n, int splits, const float* __restrict__ part, S* __restrict__ dw) {
+  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
+    float t = part[i];
+    for (int s = 1; s < splits; ++s) t += part[s * n + i];
+    dw[i] = from_f<S>(t);
+  }
+}
+
+// ---------------------------------------------------------------- one pass over the rows of the caller's arrays
+// A wave a row of up to four arrays: its largest magnitude (`most`, for the fp32 products' parts) and a copy padded with
+// zeros to whole chunks (`copy`, where the array's rows cannot be read 16 bytes at a time); and zeros for what later
+// kernels raise.
+struct Pass {
+  struct Array {
+    const void* p;
+    int64_t rows, ld;
+    int n;
+    uint32_t* most;
+    void* copy;
+    int cld;
+  } a[4];
+  int arrays;
   uint32_t* zero;
   int64_t zeros;
 };
 
 template <typename S>
-__global__ __launch_bounds__(NT) void row_most_kernel(Maxima a) {
+__global__ __launch_bounds__(NT) void pass_kernel(Pass a) {
   const int lane = threadIdx.x & 63;
   int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
   const int64_t z = (int64_t)blockIdx.x * NT + threadIdx.x, zn = (int64_t)gridDim.x * NT;
   for (int64_t i = z; i < a.zeros; i += zn) a.zero[i] = 0;
 #pragma unroll
-  for (int k = 0; k < 3; ++k) {
-    if (row >= 0 && row < a.rows[k]) {
-      const S* p = (const S*)a.p[k] + row * a.ld[k];
+  for (int k = 0; k < 4; ++k) {
+    if (k >= a.arrays) break;
+    const Pass::Array& v = a.a[k];
+    if (row >= 0 && row < v.rows) {
+      const S* p = (const S*)v.p + row * v.ld;
       constexpr int V = 16 / sizeof(S);
       uint32_t m = 0;
-      if ((uintptr_t)p % 16 == 0 && a.n[k] % V == 0) {
-        for (int i = lane * V; i < a.n[k]; i += 64 * V) {
-          float v[V];
-          load_vec<V>(p + i, v);
-#pragma unroll
-          for (int j = 0; j < V; ++j) m = max(m, abs_bits(v[j]));
+      if (v.copy) {
+        S* c = (S*)v.copy + row * v.cld;
+        for (int i = lane; i < v.cld; i += 64) {
+          const S x = i < v.n ? p[i] : (S)0;
+          c[i] = x;
+          if constexpr (sizeof(S) > 1) m = max(m, abs_bits(to_f(x)));
         }
-      } else {
-        for (int i = lane; i < a.n[k]; i += 64) m = max(m, abs_bits(to_f(p[i])));
-      }
+      } else if constexpr (sizeof(S) > 1) {
+        if ((uintptr_t)p % 16 == 0 && v.n % V == 0) {
+          for (int i = lane * V; i < v.n; i += 64 * V) {
+            float x[V];
+            load_vec<V>(p + i, x);
 #pragma unroll
-      for (int off = 32; off > 0; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
-      if (lane == 0) a.out[k][row] = m;
+            for (int j = 0; j < V; ++j) m = max(m, abs_bits(x[j]));
+          }
+        } else {
+          for (int i = lane; i < v.n; i += 64) m = max(m, abs_bits(to_f(p[i])));
+        }
+      }
+      if constexpr (sizeof(S) > 1) {
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, off, 64));
+        if (lane == 0 && v.most) v.most[row] = m;
+      }
     }
-    row -= a.rows[k];
+    row -= v.rows;
   }
 }
 
@@ -634,19 +672,53 @@ void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
   else go(std::integral_constant<int, 1>{});
 }
 
+// Tiles of a weight gradient, and how many parts its positions are split into: so many that about 512 blocks run, of
+// at least 256 positions each on average.
+inline int64_t weight_tiles(int64_t na, int64_t nb) { return ((na + BN - 1) / BN) * ((nb + BN - 1) / BN); }
+inline int weight_splits(int64_t M, int E, int64_t tiles) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, 512 / (E * tiles)), M / E / 256));
+}
+
 template <int KIND, typename S, int MODE, bool FEW = false>
-void launch_weights(const Args& g, bool vec, hipStream_t st) {
+void launch_weights(Args g, bool vec, hipStream_t st) {
   const int64_t na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;
-  const int64_t tiles = ((na + BN - 1) / BN) * ((nb + BN - 1) / BN);
-  const unsigned grid = (unsigned)(8 * g.E * ((tiles + 7) / 8));
+  const int64_t tiles = weight_tiles(na, nb);
+  g.splits = FEW ? 1 : weight_splits(g.M, g.E, tiles);
+  const dim3 grid((unsigned)(8 * g.E * ((tiles + 7) / 8)), g.splits);
   if (vec) weights_kernel<KIND, S, MODE, true, FEW><<<grid, NT, 0, st>>>(g);
   else weights_kernel<KIND, S, MODE, false, FEW><<<grid, NT, 0, st>>>(g);
+  if (g.splits > 1) {
+    const int64_t n = (int64_t)g.E * (MODE == DWIN ? 2 : 1) * g.F * g.H;
+    sum_splits_kernel<S><<<(unsigned)std::min<int64_t>((n + NT - 1) / NT, 1 << 16), NT, 0, st>>>(
+        n, g.splits, g.dwsplit, (S*)(MODE == DWIN ? g.dw_in : g.dw_out));
+  }
 }
 
 template <typename S>
-void launch_row_most(const Maxima& a, hipStream_t st) {
-  const int64_t rows = a.rows[0] + a.rows[1] + a.rows[2];
-  row_most_kernel<S><<<(unsigned)std::max<int64_t>(1, (rows + 3) / 4), NT, 0, st>>>(a);
+void launch_pass(const Pass& a, hipStream_t st) {
+  int64_t rows = 0;
+  for (int k = 0; k < a.arrays; ++k) rows += a.a[k].rows;
+  if (rows == 0 && a.zeros == 0) return;
+  pass_kernel<S><<<(unsigned)std::max<int64_t>(1, (rows + 3) / 4), NT, 0, st>>>(a);
+}
+
+// Adds an array to a pass if it has to be looked at: its largest magnitudes are wanted or its rows cannot be read in
+// whole chunks.  p and ld are then those of the padded copy at `room` (unless that were too large for one buffer:
+// returns false, and the products read single values).
+template <typename S>
+bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int64_t outer, int n, uint32_t* most, char*& room) {
+  constexpr int CE = sizeof(S) == 1 ? 16 : 8;
+  const int cld = (int)whole_chunks(n, CE);
+  const bool ok = vec_ok(p, rows, ld, sizeof(S), n), copy = !ok && rows * cld * (int64_t)sizeof(S) < (int64_t)kDropOffset;
+  if (copy || most) {
+    a.a[a.arrays++] = Pass::Array{p, rows * outer, ld, n, most, copy ? room : nullptr, cld};
+    if (copy) {
+      p = room;
+      ld = cld;
+      room += align64(rows * outer * cld * (int64_t)sizeof(S));
+    }
+  }
+  return ok || copy;
 }
 
 template <typename T>
@@ -684,11 +756,18 @@ inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 
 
 // Parts of a workspace, in bytes.
 struct Space {
-  int64_t h, o, da, hw, part, hs, most, total;
+  int64_t h, o, da, hw, part, hs, most, split, pad, total;
 };
 // whether the products are fp32 ones by tiles
 inline bool parts(const FscExpertDims& d) {
   return !few(d.rows * d.k, d.n_experts) && (d.dtype == FSC_F32 || fine(d));
+}
+// room for padded copies of x (or x and dy) and of weights whose rows are no whole chunks
+inline int64_t pad_bytes(const FscExpertDims& d, int rows_arrays) {
+  const int size = d.dtype == FSC_F32 ? 4 : d.dtype == FSC_BF16 ? 2 : 1, ce = size == 1 ? 16 : 8;
+  const int64_t hp = whole_chunks(d.width, ce), fp = whole_chunks(d.hidden, ce), E = d.n_experts;
+  return rows_arrays * align64(d.rows * hp * size) + (hp != d.width ? align64(E * 2 * d.hidden * hp * size) : 0) +
+         (fp != d.hidden ? align64(E * d.width * fp * size) : 0);
 }
 inline Space forward_space(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, ldf = ldf_of(d), size = held_size(d);
@@ -701,6 +780,9 @@ inline Space forward_space(const FscExpertDims& d) {
   }
   if (d.dtype == FSC_I8) {
     s.hs = at; at += align64(M * (ldf / QG) * 4);
+  }
+  if (!few(M, d.n_experts)) {
+    s.pad = at; at += pad_bytes(d, 1);
   }
   s.total = at;
   return s;
@@ -716,6 +798,14 @@ inline Space backward_space(const FscExpertDims& d) {
   if (parts(d)) {
     s.most = at; at += align64((d.rows + M + (int64_t)d.n_experts * (d.hidden + d.width)) * 4);
   }
+  if (!few(M, d.n_experts)) {
+    s.pad = at; at += pad_bytes(d, 2);
+    // the two weight gradients use the same room, one after the other
+    const int64_t si = weight_splits(M, d.n_experts, weight_tiles(d.width, 2 * ldf));
+    const int64_t so = weight_splits(M, d.n_experts, weight_tiles(ldf, d.width));
+    const int64_t n = (int64_t)d.n_experts * d.hidden * d.width;
+    s.split = at; at += align64(std::max(si > 1 ? si * 2 * n : 0, so > 1 ? so * n : 0) * 4);
+  }
   s.total = at;
   return s;
 }
@@ -730,6 +820,9 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
   g.ldo = ldo_of(d);
   g.E = d.n_experts;
   g.k = d.k;
+  g.li = d.width;
+  g.lo = d.hidden;
+  g.splits = 1;
   g.k_inv = ((1u << 20) + d.k - 1) / d.k;
   if (!few(g.M, g.E)) {
     g.n_tiles = p.n_tiles;
@@ -743,10 +836,10 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
 }
 
 template <int KIND, typename S>
-void forward(Args g, int tile, void* y, hipStream_t st) {
-  const bool vin = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H) && vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H);
-  const bool vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
+void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
   if (!g.place) {
+    const bool vin = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H) && vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H);
+    const bool vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
     if constexpr (KIND == I8) {
       few_launch_q8(g, vin, vout, st);
     } else {
@@ -754,11 +847,13 @@ void forward(Args g, int tile, void* y, hipStream_t st) {
       few_launch<S>(DOWN, g, vout, st);
     }
   } else {
-    if constexpr (KIND == F32) {
-      const int64_t in = (int64_t)g.E * 2 * g.F, out = (int64_t)g.E * g.H;
-      launch_row_most<S>(Maxima{{g.x, g.w_in, g.w_out}, {g.T, in, out}, {g.xs, g.H, g.F}, {g.H, g.H, g.F},
-                                {g.xmost, g.in_row, g.out_row}, g.hmost, g.M}, st);
-    }
+    Pass a{};
+    const bool vx = through<S>(a, g.x, g.xs, g.T, 1, g.H, g.xmost, room);
+    const bool vin = through<S>(a, g.w_in, g.li, 2 * g.F, g.E, g.H, g.in_row, room) && vx;
+    const bool vout = through<S>(a, g.w_out, g.lo, g.H, g.E, g.F, g.out_row, room);
+    a.zero = g.hmost;
+    a.zeros = g.hmost ? g.M : 0;
+    launch_pass<S>(a, st);
     launch_rows<KIND, S, UP>(g, tile, vin, st);
     launch_rows<KIND, S, DOWN>(g, tile, vout, st);
   }
@@ -767,19 +862,31 @@ void forward(Args g, int tile, void* y, hipStream_t st) {
 }
 
 template <int KIND, typename S>
-void backward(Args g, int tile, void* dx, float* dweight, hipStream_t st) {
-  const bool vdy = vec_ok(g.dy, g.T, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H);
-  const bool vin = vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
+void backward(Args g, int tile, char* room, void* dx, float* dweight, hipStream_t st) {
   const bool by_slot = !g.place;
-  if constexpr (KIND == F32)
-    if (!by_slot) {        // out_col, in_col and damost lie one after the other
-      launch_row_most<S>(Maxima{{g.dy, nullptr, nullptr}, {g.T, 0, 0}, {g.ds, 0, 0}, {g.H, 0, 0},
-                                {g.dymost, nullptr, nullptr}, g.out_col, (int64_t)g.E * (g.F + g.H) + g.M}, st);
-      col_most_kernel<S><<<dim3((g.F + 63) / 64, (g.H + 63) / 64, g.E), NT, 0, st>>>((const S*)g.w_out, g.H, g.F, g.out_col);
-      if (dx) col_most_kernel<S><<<dim3((g.H + 63) / 64, (2 * g.F + 63) / 64, g.E), NT, 0, st>>>((const S*)g.w_in, 2 * g.F, g.H, g.in_col);
+  bool vdy = vec_ok(g.dy, g.T, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H);
+  bool vin = vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
+  if (by_slot) {
+    few_launch<S>(DH, g, vdy && vout, st);
+  } else {
+    Pass a{};
+    if (g.out_col) {        // out_col, in_col and damost lie one after the other
+      a.zero = g.out_col;
+      a.zeros = (int64_t)g.E * (g.F + g.H) + g.M;
     }
-  if (by_slot) few_launch<S>(DH, g, vdy && vout, st);
-  else launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
+    const void *w_in = g.w_in, *w_out = g.w_out;
+    vdy = through<S>(a, g.dy, g.ds, g.T, 1, g.H, g.dymost, room);
+    vout = through<S>(a, g.w_out, g.lo, g.H, g.E, g.F, nullptr, room);
+    if (dx) vin = through<S>(a, g.w_in, g.li, 2 * g.F, g.E, g.H, nullptr, room);
+    if (g.dw_in) vx = through<S>(a, g.x, g.xs, g.T, 1, g.H, nullptr, room);
+    launch_pass<S>(a, st);
+    if (g.out_col) {
+      col_most_kernel<S><<<dim3((g.F + 63) / 64, (g.H + 63) / 64, g.E), NT, 0, st>>>((const S*)w_out, g.H, g.F, g.out_col);
+      if (dx)
+        col_most_kernel<S><<<dim3((g.H + 63) / 64, (2 * g.F + 63) / 64, g.E), NT, 0, st>>>((const S*)w_in, 2 * g.F, g.H, g.in_col);
+    }
+    launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
+  }
   if (dweight)
     dweight_kernel<<<(unsigned)((g.M + NT - 1) / NT), NT, 0, st>>>(
         g.M, by_slot ? few_parts(g.F, sizeof(S)) : (g.F + BN - 1) / BN, g.place, g.index, g.E, g.dwpart, dweight);
@@ -854,9 +961,9 @@ int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const vo
     g.in_row = g.hmost + g.M;
     g.out_row = g.in_row + (int64_t)g.E * 2 * g.F;
   }
-  if (dims->dtype == FSC_F32) forward<F32, float>(g, tile, y, stream);
-  else if (fine(*dims)) forward<F32, __bf16>(g, tile, y, stream);
-  else forward<BF16, __bf16>(g, tile, y, stream);
+  if (dims->dtype == FSC_F32) forward<F32, float>(g, tile, ws + s.pad, y, stream);
+  else if (fine(*dims)) forward<F32, __bf16>(g, tile, ws + s.pad, y, stream);
+  else forward<BF16, __bf16>(g, tile, ws + s.pad, y, stream);
   return fsc::check_launch("expert_mlp_forward") ? 2 : 0;
 }
 
@@ -890,6 +997,7 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
   g.dwpart = dweight ? (float*)(ws + s.part) : nullptr;
   g.dw_in = dw_in;
   g.dw_out = dw_out;
+  g.dwsplit = (float*)(ws + s.split);
   if (M == 0) {              // no rows: zero weight gradients, written by the products' empty sums
     if (dims->dtype == FSC_F32) {
       if (dw_in) launch_weights<X6, float, DWIN, true>(g, false, stream);
@@ -899,11 +1007,11 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
       if (dw_out) launch_weights<X6, __bf16, DWOUT, true>(g, false, stream);
     }
   } else if (dims->dtype == FSC_F32) {
-    backward<F32, float>(g, tile, dx, dweight, stream);
+    backward<F32, float>(g, tile, ws + s.pad, dx, dweight, stream);
   } else if (fine(*dims)) {
-    backward<F32, __bf16>(g, tile, dx, dweight, stream);
+    backward<F32, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
   } else {
-    backward<BF16, __bf16>(g, tile, dx, dweight, stream);
+    backward<BF16, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
   }
   return fsc::check_launch("expert_mlp_backward") ? 2 : 0;
 }
@@ -929,7 +1037,7 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
   g.h = ws + s.h;
   g.o = (float*)(ws + s.o);
   g.hscale = (float*)(ws + s.hs);
-  forward<I8, int8_t>(g, tile, y, stream);
+  forward<I8, int8_t>(g, tile, ws + s.pad, y, stream);
   return fsc::check_launch("expert_mlp_q8") ? 2 : 0;
 }
 
