@@ -11,6 +11,7 @@
 #include <algorithm>
 
 #include "common.h"
+#include "expert_types.h"
 #include "expert_plan.h"
 #include "fsctep.h"
 
@@ -60,8 +61,10 @@ __device__ __forceinline__ void place_slots(const int32_t* __restrict__ index, i
     const uint64_t m = peers(e, ok);
     int at = -1;
     if (ok) at = base[e] + cnt[e] + __popcll(m & ((1ull << lane) - 1));
-    // the last lane of each expert moves its counter on (one wave: the reads above come first)
+    wave_sync();
+    // the last lane of each expert moves its counter on
     if (ok && (m >> lane) == 1ull) cnt[e] += __popcll(m);
+    wave_sync();
     if (s < s1) p.place[s] = at;
     if (ok) {
       p.slot_of[at] = (int32_t)s;

@@ -86,73 +86,140 @@ __device__ __forceinline__ void load_row(const T* l, int e0, int experts, bool v
   }
 }
 
-// Scores of the row's logits (in place), 0 where the logit is -inf.
+// 1 / y for y >= 1: the hardware's reciprocal and one Newton step in fused operations, the correctly rounded quotient
+// unless y's fraction is all ones (a division takes three times the instructions).  Above 2^100 a division.
+__device__ __forceinline__ float over(float y) {
+  const float r = __builtin_amdgcn_rcpf(y);
+  return fmaf(r, fmaf(-y, r, 1.f), r);
+}
+
+// Largest logit and sum of the row's softmax; ex becomes exp(l - m).
 template <int V>
-__device__ __forceinline__ void scores(float (&v)[V], bool softmax) {
-  if (!softmax) {
+__device__ __forceinline__ void softmax_sum(float (&ex)[V], float& m, float& total) {
+  m = ex[0];
 #pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = 1.f / (1.f + expf(-v[i]));
-    return;
-  }
-  float m = v[0];
-#pragma unroll
-  for (int i = 1; i < V; ++i) m = fmaxf(m, v[i]);
+  for (int i = 1; i < V; ++i) m = fmaxf(m, ex[i]);
   m = row_max(m);
   if (m == kNone) m = 0.f;
   double z = 0.0;
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    v[i] = expf(v[i] - m);
-    z += (double)v[i];
+    ex[i] = expf(ex[i] - m);
+    z += (double)ex[i];
   }
-  const float total = (float)row_sum64(z);
-  if (total > 0.f || total != total)
-#pragma unroll
-    for (int i = 0; i < V; ++i) v[i] = v[i] / total;
+  total = (float)row_sum64(z);
+  if (total == 0.f) total = 1.f;               // nothing to choose: scores of 0
 }
 
+// Scores of a lane's logits, 0 where the logit is -inf.  m, total: the softmax's, for the scores of single experts.
+template <int V, bool SOFTMAX>
+__device__ __forceinline__ void scores(float (&v)[V], float& m, float& total) {
+  if constexpr (SOFTMAX) {
+    softmax_sum<V>(v, m, total);
+#pragma unroll
+    for (int i = 0; i < V; ++i) v[i] = v[i] / total;
+  } else {
+    bool far = false;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      v[i] = 1.f + expf(-v[i]);
+      far |= !(v[i] < 0x1p100f) && v[i] != INFINITY;
+    }
+    if (__ballot(far)) {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = 1.f / v[i];
+    } else {
+#pragma unroll
+      for (int i = 0; i < V; ++i) v[i] = v[i] == INFINITY ? 0.f : over(v[i]);
+    }
+  }
+}
+template <bool SOFTMAX>
+__device__ __forceinline__ float score_of(float l, float m, float total) {
+  return SOFTMAX ? expf(l - m) / total : 1.f / (1.f + expf(-l));
+}
+
+// The value of the lane s places further round in the row (s the same for all): a step of a loop.
+__device__ __forceinline__ float next_lane(float v) { return ror<1>(v); }
+
+// group_lanes: lanes of a group where groups lie in whole lanes that part the row's 16, so that ranks stay in registers;
+// 0: through LDS.
 template <typename T, int V, bool SOFTMAX>
-__global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec) {
-  __shared__ float cs[NT / RL][MAXE];          // biased scores and group ranks, used with groups > 1 only
-  __shared__ float gs[NT / RL][MAXE / 4];
+__global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec, int group_lanes) {
+  // biased scores and group ranks, where a group does not lie in whole lanes; the choices in order
+  extern __shared__ float extra[];
+  __shared__ int pick[NT / RL][RL];
   const int lane = threadIdx.x & (RL - 1), slot = threadIdx.x / RL;
   const int64_t row = (int64_t)blockIdx.x * (NT / RL) + slot;
   const bool live = row < a.rows;              // the lanes of a row past the end take part with no expert
   const int e0 = lane * V;
-  float s[V], c[V];
-  load_row<T, V>((const T*)a.logits + (live ? row : 0) * a.ls, e0, live ? a.experts : 0, vec, s);
+  const T* const lrow = (const T*)a.logits + (live ? row : 0) * a.ls;
+  float c[V];
+  load_row<T, V>(lrow, e0, live ? a.experts : 0, vec, c);
   bool bad = false;
-  unsigned open = 0;                           // bit i: expert e0 + i can be chosen
+  unsigned open = 0;                           // bit i: the logit is above -inf
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    bad |= s[i] != s[i];
-    if (s[i] > kNone) open |= 1u << i;
+    bad |= c[i] != c[i];
+    open |= (c[i] > kNone ? 1u : 0u) << i;
   }
-  scores<V>(s, SOFTMAX);
+  float m = 0.f, total = 1.f;
+  scores<V, SOFTMAX>(c, m, total);
+  if (a.bias) {
+    float b[V];
+    load_row<float, V>(a.bias, e0, a.experts, V >= 4 && a.experts % 4 == 0 && (uintptr_t)a.bias % 16 == 0, b);
+#pragma unroll
+    for (int i = 0; i < V; ++i) c[i] += b[i];
+  }
 #pragma unroll
   for (int i = 0; i < V; ++i) {
-    c[i] = kNone;
-    if (open >> i & 1) {
-      c[i] = a.bias ? s[i] + a.bias[e0 + i] : s[i];
-      bad |= c[i] != c[i];
-    }
+    c[i] = open >> i & 1 ? c[i] : kNone;
+    bad |= c[i] != c[i];
   }
   bad = row_ballot(bad) != 0;
 
-  if (a.groups > 1) {
+  if (a.groups > 1 && group_lanes) {
+    float t0 = kNone, t1 = kNone;              // the two largest of the lane, then of the group
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+      t1 = fmaxf(t1, fminf(t0, c[i]));
+      t0 = fmaxf(t0, c[i]);
+    }
+    for (int off = 1; off < group_lanes; off <<= 1) {
+      const float o0 = __shfl_xor(t0, off, RL), o1 = __shfl_xor(t1, off, RL);
+      t1 = fmaxf(fminf(t0, o0), fmaxf(t1, o1));
+      t0 = fmaxf(t0, o0);
+    }
+    const float mine = a.best == 2 && t1 > kNone ? t0 + t1 : t0;
+    // groups ahead: a larger rank, or the same and a lower place; every group is met group_lanes times
+    int ahead = 0;
+    float v = mine;
+    const int g = lane / group_lanes;
+#pragma unroll
+    for (int s = 1; s < RL; ++s) {
+      v = next_lane(v);                        // now of lane - s, round the row
+      const int o = ((lane - s) & (RL - 1)) / group_lanes;
+      ahead += v > mine || (v == mine && o < g);
+    }
+    if (ahead >= a.kept * group_lanes)
+#pragma unroll
+      for (int i = 0; i < V; ++i) c[i] = kNone;
+  } else if (a.groups > 1) {
+    float* const cs = extra + slot * (a.experts + a.groups);
+    float* const gs = cs + a.experts;
     const int per = a.experts / a.groups;
 #pragma unroll
     for (int i = 0; i < V; ++i)
-      if (e0 + i < a.experts) cs[slot][e0 + i] = c[i];
+      if (e0 + i < a.experts) cs[e0 + i] = c[i];
     __syncthreads();
     for (int g = lane; g < a.groups; g += RL) {
       float t0 = kNone, t1 = kNone;            // the two largest
       for (int i = 0; i < per; ++i) {
-        const float v = cs[slot][g * per + i];
+        const float v = cs[g * per + i];
         t1 = fmaxf(t1, fminf(t0, v));
         t0 = fmaxf(t0, v);
       }
-      gs[slot][g] = a.best == 2 && t1 > kNone ? t0 + t1 : t0;
+      gs[g] = a.best == 2 && t1 > kNone ? t0 + t1 : t0;
     }
     __syncthreads();
     const int g0 = e0 / per;                   // e0 < 2^13
@@ -163,9 +230,9 @@ __global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec) {
     for (int i = 0; i < V; ++i) {
       if (e0 + i < a.experts && last != g) {   // groups ahead: a larger rank, or the same and a lower place
         int ahead = 0;
-        const float mine = gs[slot][g];
+        const float mine = gs[g];
         for (int o = 0; o < a.groups; ++o) {
-          const float v = gs[slot][o];
+          const float v = gs[o];
           ahead += v > mine || (v == mine && o < g);
         }
         keep = ahead < a.kept;
@@ -176,31 +243,31 @@ __global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec) {
     }
   }
 
-  int my = -1;                                 // lane j keeps the j-th choice
-  float mys = 0.f;
+  // k rounds: the row's largest, the lowest lane that has it, its lowest expert; that lane writes the choice down
+  pick[slot][lane] = -1;
+  wave_sync();
   for (int j = 0; j < a.k; ++j) {
-    float m = c[0];
+    float most = c[0];
 #pragma unroll
-    for (int i = 1; i < V; ++i) m = fmaxf(m, c[i]);
-    const float top = row_max(m);
-    const unsigned who = row_ballot(m == top && top > kNone);
+    for (int i = 1; i < V; ++i) most = fmaxf(most, c[i]);
+    const float top = row_max(most);
+    const unsigned who = row_ballot(most == top && top > kNone);
     if (__ballot(who != 0) == 0) break;        // none of the wave's rows has one left
     const bool win = who != 0 && lane == __ffs(who) - 1;
-    int at = 0;
-    float sv = 0.f;
+    int at = V;
 #pragma unroll
-    for (int i = V - 1; i >= 0; --i)
-      if (c[i] == top) { at = i; sv = s[i]; }
+    for (int i = V - 1; i >= 0; --i) at = c[i] == top ? i : at;
+    if (!win) at = V;
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (win && i == at) c[i] = kNone;
-    const int from = who ? __ffs(who) - 1 : 0;
-    const int idx = __shfl(e0 + at, from, RL);
-    const float sc = __shfl(sv, from, RL);
-    if (who && lane == j) { my = idx; mys = sc; }
+    for (int i = 0; i < V; ++i) c[i] = i == at ? kNone : c[i];
+    if (win) pick[slot][j] = e0 + at;
   }
-  const float total = a.renorm ? row_sum(mys) : 1.f;
-  float w = total > 0.f || total != total ? a.scale * (mys / total) : 0.f;
+  // lane j takes the j-th choice
+  wave_sync();
+  int my = lane < a.k ? pick[slot][lane] : -1;
+  const float sc = my >= 0 ? score_of<SOFTMAX>(to_f(lrow[my]), m, total) : 0.f;
+  const float sum = a.renorm ? row_sum(sc) : 1.f;
+  float w = sum > 0.f || sum != sum ? a.scale * (sc / sum) : 0.f;
   if (bad) { my = lane; w = NAN; }
   if (live && lane < a.k) {
     a.index[row * a.k + lane] = my;
@@ -212,7 +279,7 @@ __global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec) {
 //   renormalised: ds_j s_j = w_j (u_j - sum u w / scale); else ds_j s_j = scale s_j u_j = w_j u_j
 //   sigmoid: dl_j = (ds_j s_j)(1 - s_j);  softmax: dl_i = (ds_i s_i) - s_i sum_j ds_j s_j
 // The last sum is zero for renormalised weights, so only sigmoid (the chosen logits) and softmax without
-// renormalisation (all) read the logits again.
+// renormalisation (all) read the logits again.  The chosen experts' gradients meet the rest of the row in LDS.
 struct BackArgs {
   int64_t rows, ls;
   int experts, k, renorm;
@@ -225,8 +292,10 @@ struct BackArgs {
 
 template <typename T, int V, bool SOFTMAX>
 __global__ __launch_bounds__(NT) void route_back_kernel(BackArgs a, bool vec) {
-  const int lane = threadIdx.x & (RL - 1);
-  const int64_t row = (int64_t)blockIdx.x * (NT / RL) + threadIdx.x / RL;
+  constexpr int LD = RL * V + (V % 4 == 0 ? 4 : 0);
+  __shared__ __align__(16) float buf[NT / RL][LD];
+  const int lane = threadIdx.x & (RL - 1), slot = threadIdx.x / RL;
+  const int64_t row = (int64_t)blockIdx.x * (NT / RL) + slot;
   const bool live = row < a.rows;
   const int e0 = lane * V;
   const T* l = (const T*)a.logits + (live ? row : 0) * a.ls;
@@ -248,21 +317,23 @@ __global__ __launch_bounds__(NT) void route_back_kernel(BackArgs a, bool vec) {
   if (SOFTMAX) {
     if (!a.renorm) {
       const float sum = row_sum(d);
+      float m, total;
       load_row<T, V>(l, e0, live ? a.experts : 0, vec, o);
-      scores<V>(o, true);
+      scores<V, true>(o, m, total);
 #pragma unroll
       for (int i = 0; i < V; ++i) o[i] *= -sum;
     }
   } else if (idx >= 0) {
-    d *= 1.f - 1.f / (1.f + expf(-to_f(l[idx])));
+    d *= 1.f - score_of<false>(to_f(l[idx]), 0.f, 1.f);
   }
-  for (int j = 0; j < a.k; ++j) {
-    const int at = __shfl(idx, j, RL) - e0;
-    const float v = __shfl(d, j, RL);
+  // one wave writes and reads its four rows
 #pragma unroll
-    for (int i = 0; i < V; ++i)
-      if (at == i) o[i] += v;
-  }
+  for (int i = 0; i < V; ++i) buf[slot][e0 + i] = o[i];
+  wave_sync();
+  if (idx >= 0) atomicAdd(&buf[slot][idx], d);   // a row's experts differ: one addition to a place
+  wave_sync();
+#pragma unroll
+  for (int i = 0; i < V; ++i) o[i] = buf[slot][e0 + i];
   if (!live) return;
   T* dl = (T*)a.dlogits + row * a.experts;
   if (V >= 4 && a.experts % 4 == 0) {
@@ -333,12 +404,15 @@ int fsc_route_experts(int64_t rows, int32_t n_experts, int32_t dtype, int64_t lo
   const bool vec = n_experts % 4 == 0 && logits_stride % 4 == 0 && (uintptr_t)logits % (4 * size) == 0;
   by_experts(n_experts, [&](auto V) {
     constexpr int v = decltype(V)::value;
+    // lanes of a group, 0 where groups do not lie in whole lanes, so many that they part the row's 16
+    const int per = n_experts / groups, gl = per % v == 0 && RL % (per / v) == 0 ? per / v : 0;
+    const size_t lds = groups > 1 && !gl ? NT / RL * (size_t)(n_experts + groups) * 4 : 0;
     if (dtype == FSC_F32) {
-      if (score == 0) route_kernel<float, v, true><<<grid, NT, 0, stream>>>(a, vec);
-      else route_kernel<float, v, false><<<grid, NT, 0, stream>>>(a, vec);
+      if (score == 0) route_kernel<float, v, true><<<grid, NT, lds, stream>>>(a, vec, gl);
+      else route_kernel<float, v, false><<<grid, NT, lds, stream>>>(a, vec, gl);
     } else {
-      if (score == 0) route_kernel<__bf16, v, true><<<grid, NT, 0, stream>>>(a, vec);
-      else route_kernel<__bf16, v, false><<<grid, NT, 0, stream>>>(a, vec);
+      if (score == 0) route_kernel<__bf16, v, true><<<grid, NT, lds, stream>>>(a, vec, gl);
+      else route_kernel<__bf16, v, false><<<grid, NT, lds, stream>>>(a, vec, gl);
     }
   });
   return check_launch("route_experts") ? 2 : 0;

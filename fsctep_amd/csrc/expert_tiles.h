@@ -63,8 +63,10 @@ __device__ __forceinline__ void turn_rows(F&& sums, float* buf, Turned<NI>& t) {
   using U = Turned<NI>;
 #pragma unroll
   for (int i = 0; i < NI; ++i) st4(buf + r * U::LD + 16 * i + 4 * q, sums(i));
+  wave_sync();
 #pragma unroll
   for (int s = 0; s < U::S; ++s) t.v[s] = ld4(buf + (s * U::R + lane / U::L) * U::LD + 4 * (lane % U::L));
+  wave_sync();
 }
 constexpr int TURN = 16 * 68;
 

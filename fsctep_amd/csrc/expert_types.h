@@ -18,6 +18,13 @@ __device__ __forceinline__ T from_f(float v) { return (T)v; }
 template <typename T>
 __device__ __forceinline__ float held(float v) { return to_f(from_f<T>(v)); }
 
+// LDS that one wave writes and reads: what its lanes wrote before is what they read after.
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 // Larger of two values, NaN if either is one (a row with a NaN shows it).
 __device__ __forceinline__ float max_nan(float a, float b) { return (a > b || a != a) ? a : b; }
 

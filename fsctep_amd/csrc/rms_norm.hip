@@ -185,7 +185,8 @@ struct BackArgs {
   float* part;                   // [gridDim.x][width] partial dw, or null
 };
 
-template <typename T, typename W, int V, int CH>
+// NARROW: at most 64 columns.
+template <typename T, typename W, int V, int CH, bool NARROW>
 __global__ __launch_bounds__(NT) void row_back_kernel(BackArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   __shared__ float buf[64 * V * CH];
@@ -227,8 +228,7 @@ __global__ __launch_bounds__(NT) void row_back_kernel(BackArgs a) {
     // In a narrow row g can lie along zn, and dx is what is left of their difference (nearly nothing at width 1):
     // there the difference is formed in 64 bits, from z and a 64-bit root.
     double zr = 1.0, fine = 0.0;
-    const bool narrow = CH <= 2 && a.width <= 64;
-    if (narrow) {
+    if constexpr (NARROW) {
       double ss = 0.0, gz = 0.0;
 #pragma unroll
       for (int c = 0; c < CH; ++c)
@@ -251,7 +251,7 @@ __global__ __launch_bounds__(NT) void row_back_kernel(BackArgs a) {
         else
 #pragma unroll
           for (int j = 0; j < V; ++j) o[j] = 0.f;
-        if (narrow) {
+        if constexpr (NARROW) {
 #pragma unroll
           for (int j = 0; j < V; ++j) {
             const double zn = (double)to_f(((const T*)a.z)[row * a.zs + at + j]) * zr;
@@ -319,27 +319,24 @@ __global__ __launch_bounds__(NT) void wide_back_kernel(BackArgs a) {
     for (int i = threadIdx.x; i < a.width; i += NT) part[i] = 0.f;
 }
 
-// dw[c] = sum over the blocks' partial rows: 64 columns a block, 16 threads a column, then a fixed tree.
+// dw[c] = sum over the blocks' partial rows: 32 columns a block, 32 threads a column, then a fixed tree.
 template <typename W>
 __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ part, int n, int width, W* __restrict__ dw) {
-  __shared__ float red[16][64];
-  const int col = blockIdx.x * 64 + (threadIdx.x & 63), k = threadIdx.x >> 6;
+  __shared__ float red[32][33];
+  const int c = threadIdx.x & 31, k = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
   float s = 0.f;
   if (col < width)
-    for (int i = k; i < n; i += 16) s += part[(int64_t)i * width + col];
-  red[k][threadIdx.x & 63] = s;
+#pragma unroll 8
+    for (int i = k; i < n; i += 32) s += part[(int64_t)i * width + col];
+  red[k][c] = s;
   __syncthreads();
-  if (k == 0 && col < width) {
-    float t = 0.f;
-#pragma unroll
-    for (int i = 0; i < 16; ++i) t += red[i][threadIdx.x];
-    dw[col] = from_f<W>(t);
-  }
+  s = group_sum(red[c][k], 32);          // column k of the block in lanes c = 0..31
+  if (c == 0 && blockIdx.x * 32 + k < width) dw[blockIdx.x * 32 + k] = from_f<W>(s);
 }
 
 // Blocks of the backward: enough waves to fill the chip, few enough that the partial rows stay small beside the
 // rows themselves.
-inline int back_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1024)); }
+inline int back_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 2048)); }
 
 inline bool aligned(const void* p, int64_t stride, int size, int vec) {
   return !p || ((uintptr_t)p % (size * vec) == 0 && stride % vec == 0);
@@ -383,10 +380,16 @@ void launch_backward(const BackArgs& a, bool vec, W* dw, hipStream_t st) {
   const int blocks = back_blocks(a.rows);
   const bool done = by_width<T, W>(a.width, vec, [&](auto V, auto CH) {
     constexpr int v = decltype(V)::value, ch = decltype(CH)::value;
-    row_back_kernel<T, W, v, ch><<<blocks, NT, 0, st>>>(a);
+    if constexpr (v * ch <= 8) {
+      if (a.width <= 64) {
+        row_back_kernel<T, W, v, ch, true><<<blocks, NT, 0, st>>>(a);
+        return;
+      }
+    }
+    row_back_kernel<T, W, v, ch, false><<<blocks, NT, 0, st>>>(a);
   });
   if (!done) wide_back_kernel<T, W><<<blocks, NT, 0, st>>>(a);
-  if (dw) sum_kernel<W><<<(a.width + 63) / 64, 1024, 0, st>>>(a.part, blocks, a.width, dw);
+  if (dw) sum_kernel<W><<<(a.width + 31) / 32, 1024, 0, st>>>(a.part, blocks, a.width, dw);
 }
 
 // runs the statements with (T, W) the element types of rows and weight

@@ -57,6 +57,14 @@ auto op_handle(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
 }
 
+// A backward op's call: below autograd unless a gradient of the gradient may be asked for, which then raises.
+struct BackwardGuard {
+  optional<at::AutoDispatchBelowADInplaceOrView> below;
+  BackwardGuard() {
+    if (!at::GradMode::is_enabled()) below.emplace();
+  }
+};
+
 // ============================================================== norm
 struct NormDims {
   int64_t rows, width;
@@ -182,6 +190,7 @@ struct RmsNormFn : public torch::autograd::Function<RmsNormFn> {
                                                           const Tensor&, const Tensor&, double, bool, bool)>(
         "fsctep::rms_norm_backward");
     const optional<Tensor> dz = res && grads[1].defined() ? optional<Tensor>(grads[1]) : std::nullopt;
+    BackwardGuard guard;
     auto [dx, dw] = op.call(grads[0], dz, s[0], s[1], s[2], ctx->saved_data["eps"].toDouble(), want_x, want_w);
     if (want_x) {
       out[0] = dx;
@@ -283,6 +292,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
     auto s = ctx->get_saved_variables();
     static auto op = op_handle<Tensor(const Tensor&, const Tensor&, const Tensor&, const Tensor&, int64_t, bool, double)>(
         "fsctep::route_experts_backward");
+    BackwardGuard guard;
     out[0] = op.call(grads[1], s[0], s[1], s[2], ctx->saved_data["score"].toInt(),
                      ctx->saved_data["renormalise"].toBool(), ctx->saved_data["scale"].toDouble());
     return out;
@@ -419,6 +429,7 @@ struct ExpertMlpFn : public torch::autograd::Function<ExpertMlpFn> {
         const Tensor&, bool, bool, bool, bool)>("fsctep::expert_mlp_backward");
     const bool want[4] = {ctx->needs_input_grad(0), ctx->needs_input_grad(2), ctx->needs_input_grad(3),
                           ctx->needs_input_grad(4)};
+    BackwardGuard guard;
     auto [dx, dweight, dw_in, dw_out] =
         op.call(grads[0], s[0], s[1], s[2], s[3], s[4], s[5], s[6], want[0], want[1], want[2], want[3]);
     if (want[0]) out[0] = dx;
