@@ -39,19 +39,20 @@ constexpr int BN = 128;          // rows of the tile's weight operand
 // columns of padding and are read by ds_read_b64_tr_b16.
 constexpr int TRP = 128 + 16;
 
-template <int KIND, int ROWS, bool TR, typename T, int NT>
+template <int KIND, int ROWS, bool TR, typename T, int NT, int AHEAD = 1>
 struct Tile {                                                        // T: the type in memory
   using E = El<KIND>;
   static constexpr int CPR = E::BK / E::CE;                          // chunks of a straight row
   static constexpr int NCH = TR ? E::BK * ROWS / 8 : ROWS * CPR;     // chunks of the tile
   static constexpr int PER = (NCH + NT - 1) / NT;                    // chunks of a thread
   static constexpr int PLANE = TR ? E::BK * TRP * 2 : ROWS * CPR * 16;   // bytes
-  static constexpr int BYTES = PLANE * E::PL;
+  static constexpr int PL = E::template planes<T>;
+  static constexpr int BYTES = PLANE * PL;
 
   static constexpr int NV = E::CE * sizeof(T) / 16;                  // 16-byte parts of a chunk in memory
 
   struct Reg { u4v v[NV]; };
-  Reg reg[PER];
+  Reg reg[AHEAD][PER];                                               // AHEAD: steps on their way at once
   // F32: what the values are multiplied by, for each chunk (straight) or column of the thread's chunks (turned)
   static constexpr int NSC = KIND == F32 ? (TR ? 8 : PER) : 1;
   float scale[NSC];
@@ -61,33 +62,45 @@ struct Tile {                                                        // T: the t
   __device__ static constexpr int swz(int row) { return CPR == 4 ? (row >> 1) & 3 : row & 7; }
 
   // chunk c of the thread at byte off + more of a buffer (more the same for the wave), zeros outside it or with drop
-  __device__ __forceinline__ void fetch(int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off, int more = 0, bool drop = false) {
+  __device__ __forceinline__ void fetch(int d, int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off, int more = 0, bool drop = false) {
     const int o = (int)(drop ? kDropOffset : off);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      reg[c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, o + 16 * i, more, 0));
+      reg[d][c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, o + 16 * i, more, 0));
   }
   // chunk c of the thread from p (n values of it exist, the rest are zeros), of any alignment
-  __device__ __forceinline__ void fetch(int c, const T* p, int n) {
+  __device__ __forceinline__ void fetch(int d, int c, const T* p, int n) {
     alignas(16) T t[E::CE];
 #pragma unroll
     for (int i = 0; i < E::CE; ++i) t[i] = i < n ? p[i] : (T)0;
-    __builtin_memcpy(&reg[c], t, sizeof(t));
+    __builtin_memcpy(&reg[d][c], t, sizeof(t));
+  }
+  // of step d's chunks, entries from `left` of the step's on become zeros (straight: along the reduction, where a row
+  // ends inside a chunk and the loads have gone on into the next one)
+  __device__ __forceinline__ void cut(int d, int left) {
+    static_assert(!TR);
+    constexpr int EW = 4 / sizeof(T);                                // entries of a 32-bit word
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int l = left - chunk_of(threadIdx.x + i * NT) * E::CE;
+#pragma unroll
+      for (int w = 0; w < 4 * NV; ++w) reg[d][i].v[w / 4][w % 4] = w * EW < l ? reg[d][i].v[w / 4][w % 4] : 0;
+    }
   }
   // the thread's chunks into LDS
-  __device__ __forceinline__ void put(char* lds) const {
+  __device__ __forceinline__ void put(int d, char* lds) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * NT;
       if (NCH % NT && c >= NCH) break;
       const int row = row_of(c), kc = chunk_of(c);
       const int at = TR ? row * TRP * 2 + kc * 16 : (row * CPR + (kc ^ swz(row))) * 16;
-      if constexpr (KIND == F32 || KIND == X6) {
+      if constexpr (KIND == F32 || KIND == X6 || PL == 3) {
         float v[8];
         if constexpr (sizeof(T) == 4) {
-          __builtin_memcpy(v, &reg[i], 32);
+          __builtin_memcpy(v, &reg[d][i], 32);
         } else {
-          const bf8 b = __builtin_bit_cast(bf8, reg[i].v[0]);
+          const bf8 b = __builtin_bit_cast(bf8, reg[d][i].v[0]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = (float)b[j];
         }
@@ -106,7 +119,7 @@ struct Tile {                                                        // T: the t
           *reinterpret_cast<bf8*>(lds + 2 * PLANE + at) = l;
         }
       } else {
-        *reinterpret_cast<u4v*>(lds + at) = reg[i].v[0];
+        *reinterpret_cast<u4v*>(lds + at) = reg[d][i].v[0];
       }
     }
   }
@@ -135,16 +148,16 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
   constexpr int KS = E::BK / (4 * E::CE);
 #pragma unroll
   for (int ks = 0; ks < KS; ++ks) {
-    u4v x[NJ][E::PL];
+    u4v x[NJ][TX::PL];
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int p = 0; p < E::PL; ++p) x[j][p] = TX::frag(lx, p, x0 + j, ks);
+      for (int p = 0; p < TX::PL; ++p) x[j][p] = TX::frag(lx, p, x0 + j, ks);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      u4v w[E::PL];
+      u4v w[TW::PL];
 #pragma unroll
-      for (int p = 0; p < E::PL; ++p) w[p] = TW::frag(lw, p, w0 + i, ks);
+      for (int p = 0; p < TW::PL; ++p) w[p] = TW::frag(lw, p, w0 + i, ks);
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         if constexpr (KIND == F32)
@@ -154,8 +167,10 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
           acc[i][j] = mfma_x6(__builtin_bit_cast(bf8, w[0]), __builtin_bit_cast(bf8, w[1]),
                               __builtin_bit_cast(bf8, w[2]), __builtin_bit_cast(bf8, x[j][0]),
                               __builtin_bit_cast(bf8, x[j][1]), __builtin_bit_cast(bf8, x[j][2]), acc[i][j]);
-        else if constexpr (KIND == BF16)
-          acc[i][j] = mfma_bf16(__builtin_bit_cast(bf8, w[0]), __builtin_bit_cast(bf8, x[j][0]), acc[i][j]);
+        else if constexpr (KIND == BF16 || KIND == FINE)
+#pragma unroll
+          for (int p = TW::PL * TX::PL - 1; p >= 0; --p)     // small terms first
+            acc[i][j] = mfma_bf16(__builtin_bit_cast(bf8, w[p % TW::PL]), __builtin_bit_cast(bf8, x[j][p / TW::PL]), acc[i][j]);
         else
           acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i4v, w[0]),
                                                             __builtin_bit_cast(i4v, x[j][0]), acc[i][j], 0, 0, 0);
@@ -164,7 +179,10 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
   }
 }
 
-inline __host__ __device__ int64_t whole_chunks(int64_t n, int ce) { return (n + ce - 1) / ce * ce; }
+// n entries in whole 32-bit words (rows that end inside one are read from padded copies)
+template <typename T>
+__device__ __forceinline__ int64_t whole_words(int n) { constexpr int w = 4 / sizeof(T); return (n + w - 1) / w * w; }
+inline int64_t whole_chunks(int64_t n, int ce) { return (n + ce - 1) / ce * ce; }
 
 // ---------------------------------------------------------------- the products by row tiles
 // up: 64 hidden columns a tile, their gate and up rows in turn by 16, so that a wave holds both of a column.
@@ -180,8 +198,11 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
   using R = std::conditional_t<MODE == DOWN || MODE == DX, T, S>;
   constexpr int BM = 32 * NJ, NI = 4, WW = waves_w<KIND, MODE>(), BN = 64 * WW, NT = 128 * WW;
   constexpr bool TR = MODE == DH || MODE == DX;
-  using TW = Tile<KIND, BN, TR, S, NT>;
-  using TX = Tile<KIND, BM, false, R, NT>;
+  // one step of 128 rows is on its way during the products of another; with fewer rows a step's products are shorter
+  // than memory's answer, and more steps are
+  constexpr int AHEAD = !VEC || NJ == 4 ? 1 : NJ == 2 ? 2 : 3;
+  using TW = Tile<KIND, BN, TR, S, NT, AHEAD>;
+  using TX = Tile<KIND, BM, false, R, NT, AHEAD>;
   // the operands; after the products the waves' rows and the sums across waves
   constexpr int OPERANDS = TW::BYTES + TX::BYTES, AFTER = (2 * WW * TURN + WW * BM) * 4;
   __shared__ __align__(16) char lds[OPERANDS > AFTER ? OPERANDS : AFTER];
@@ -220,7 +241,9 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
   const int64_t wseg = (MODE == UP ? 2 * g.F : MODE == DX ? g.F : g.H) * wld;   // entries of the weights of a segment
   const S* const wbase = (MODE == UP || MODE == DX ? (const S*)g.w_in : (const S*)g.w_out) + e * wseg * SEG;
   // Where the thread's chunks lie in the first step, in entries (OFF: a 32-bit byte offset for VEC, where buffers over
-  // x or dy, the tile's rows and a segment's weights give zeros outside: loads without branches); kNoChunk: nowhere.
+  // x or dy, the tile's rows and a segment's weights give zeros outside: loads without branches, at any multiple of
+  // four bytes; a chunk that goes on past its row's end is cut along the reduction, and past an output's last column
+  // it is not stored); kNoChunk: nowhere.
   using Off = std::conditional_t<VEC, uint32_t, int64_t>;
   constexpr Off kNoChunk = VEC ? (Off)kDropOffset : (Off)-1;
   Off xo[TX::PER], wo[TW::PER];
@@ -247,7 +270,7 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
     wo[i] = at >= 0 ? (Off)(at * (VEC ? sizeof(S) : 1)) : kNoChunk;
   }
   const __amdgpu_buffer_rsrc_t xr = buffer_rsrc_bytes(
-      const_cast<R*>(xbase), (uint32_t)((((GATHER ? g.T : rows) - 1) * xld + (GATHER ? whole_chunks(g.H, E::CE) : xld)) * sizeof(R)));
+      const_cast<R*>(xbase), (uint32_t)((((GATHER ? g.T : rows) - 1) * xld + (GATHER ? whole_words<R>(g.H) : xld)) * sizeof(R)));
   TW tw;
   TX tx;
   // fp32: the powers of two of this tile's rows and of the output columns' weights
@@ -270,7 +293,7 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
       tw.scale[i] = ldexpf(1.f, weight_exp(TR ? TW::chunk_of(threadIdx.x) * 8 + i : TW::row_of(threadIdx.x + i * NT)));
   }
   const int per_seg = (K + E::BK - 1) / E::BK, steps = SEG * per_seg;
-  auto fetch = [&](int s) {
+  auto fetch = [&](int d, int s) {
     const int seg = SEG == 2 && s >= per_seg, k0 = (s - seg * per_seg) * E::BK;
     const bool last = k0 + E::BK > K;                        // the same for the whole block
     const int64_t xat = seg * g.ldf + k0;
@@ -278,25 +301,34 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
     for (int i = 0; i < TX::PER; ++i) {
       const int left = KX - k0 - TX::chunk_of(threadIdx.x + i * NT) * E::CE;
       if constexpr (VEC) {
-        tx.fetch(i, xr, xo[i], (int)(xat * sizeof(R)), last && left <= 0);
+        tx.fetch(d, i, xr, xo[i], (int)(xat * sizeof(R)), last && left <= 0);
       } else {
-        tx.fetch(i, xbase + xo[i] + xat, xo[i] < 0 ? 0 : left);
+        tx.fetch(d, i, xbase + xo[i] + xat, xo[i] < 0 ? 0 : left);
       }
     }
     // turned: the buffer begins at row k0 of the segment and ends with it, rows past K are outside
     const int64_t wat = TR ? k0 * wld : k0;
     const __amdgpu_buffer_rsrc_t wr = buffer_rsrc_bytes(const_cast<S*>(wbase + seg * wseg + (TR ? wat : 0)),
-                                                        (uint32_t)((wseg - (TR ? wat : 0)) * sizeof(S)));
+                                                        (uint32_t)(std::max<int64_t>(0, wseg - (TR ? wat : 0)) * sizeof(S)));
 #pragma unroll
     for (int i = 0; i < TW::PER; ++i) {
       const int c = threadIdx.x + i * NT;
       const int left = TR ? K - k0 - TW::row_of(c) : K - k0 - TW::chunk_of(c) * E::CE;
       if constexpr (VEC) {
-        tw.fetch(i, wr, wo[i], TR ? 0 : (int)(wat * sizeof(S)), !TR && last && left <= 0);
+        tw.fetch(d, i, wr, wo[i], TR ? 0 : (int)(wat * sizeof(S)), !TR && last && left <= 0);
       } else {
         const int n = TR ? cols - n0 - TW::chunk_of(c) * 8 : left;
-        tw.fetch(i, wbase + seg * wseg + wo[i] + wat, wo[i] < 0 || left <= 0 ? 0 : n);
+        tw.fetch(d, i, wbase + seg * wseg + wo[i] + wat, wo[i] < 0 || left <= 0 ? 0 : n);
       }
+    }
+  };
+
+  // (dx: da is padded and its reduction runs over W_in's rows)
+  auto trim = [&](int d, int s) {
+    if constexpr (VEC && MODE != DX) {
+      if (K % E::CE == 0 || s + 1 < steps) return;
+      if constexpr (!TR) tw.cut(d, K - s * E::BK);
+      if constexpr (GATHER) tx.cut(d, K - s * E::BK);
     }
   };
 
@@ -316,18 +348,25 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
 #pragma unroll
       for (int j = 0; j < NJ; ++j) sum[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     const int ng = g.ldf / QG;
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
+    // the units, loaded before the operands of their step, since loads return in order; rows past the tile: the last's
+    float next[AHEAD][NJ];
+    auto units = [&](int d, int s) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j)
+        next[d][j] = g.hscale[(p0 + min(16 * (x0 + j) + r, rows - 1)) * ng + min(s, ng - 1)];
+    };
+    auto one = [&](int d, int s) {
+      trim(d, s);
       __syncthreads();
-      tw.put(lw);
-      tx.put(lx);
+      tw.put(d, lw);
+      tx.put(d, lx);
       __syncthreads();
-      if (s + 1 < steps) fetch(s + 1);
       float u[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const int row = 16 * (x0 + j) + r;
-        u[j] = row < rows ? g.hscale[(p0 + row) * ng + s] : 0.f;
+      for (int j = 0; j < NJ; ++j) u[j] = next[d][j];
+      if (AHEAD > 1 || s + AHEAD < steps) {
+        units(d, s + AHEAD);
+        fetch(d, s + AHEAD);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -340,7 +379,16 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int v = 0; v < 4; ++v) sum[i][j][v] += (float)acc[i][j][v] * u[j];
+    };
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) {
+      units(d, d);
+      fetch(d, d);
     }
+    for (int s = 0; s < steps; s += AHEAD)
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d)
+        if (s + d < steps) one(d, s + d);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int n = n0 + (w0 + i) * 16 + 4 * q;
@@ -354,15 +402,21 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(
     finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, sum,
                                        reinterpret_cast<float*>(lds));
   } else {
-    fetch(0);
-    for (int s = 0; s < steps; ++s) {
-      __syncthreads();
-      tw.put(lw);
-      tx.put(lx);
-      __syncthreads();
-      if (s + 1 < steps) fetch(s + 1);
-      step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
-    }
+#pragma unroll
+    for (int d = 0; d < AHEAD; ++d) fetch(d, d);
+    for (int s = 0; s < steps; s += AHEAD)
+#pragma unroll
+      for (int d = 0; d < AHEAD; ++d) {
+        if (s + d >= steps) break;
+        trim(d, s + d);
+        __syncthreads();
+        tw.put(d, lw);
+        tx.put(d, lx);
+        __syncthreads();
+        // (past the last step: zeros; without a branch the wait for a step leaves the later ones on their way)
+        if (AHEAD > 1 || s + 1 < steps) fetch(d, s + d + AHEAD);
+        step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
+      }
     if constexpr (KIND == F32) {
       const int r = lane & 15, q = lane >> 4;
       int xe[NJ];
@@ -395,7 +449,7 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   using RB = std::conditional_t<MODE == DWIN, T, S>;
   using TT = Tile<KIND, BN, true, RA, NT>;
   using TB = Tile<KIND, BN, true, RB, NT>;
-  __shared__ __align__(16) char lds[2 * TT::BYTES];
+  __shared__ __align__(16) char lds[TT::BYTES + TB::BYTES];
   char* la = lds;
   char* lb = lds + TT::BYTES;
   const int na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;   // columns of the operands
@@ -435,7 +489,7 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   const S* const gbase = MODE == DWIN ? (const S*)g.x : (const S*)g.dy;
   const T* const pbase = (MODE == DWIN ? (const T*)g.da : (const T*)g.hw) + p0 * ps;
   const __amdgpu_buffer_rsrc_t gr =
-      buffer_rsrc_bytes(const_cast<S*>(gbase), (uint32_t)(((g.T - 1) * gs + whole_chunks(g.H, E::CE)) * sizeof(S)));
+      buffer_rsrc_bytes(const_cast<S*>(gbase), (uint32_t)(((g.T - 1) * gs + whole_words<S>(g.H)) * sizeof(S)));
   auto fetch = [&](int64_t k0) {
     const int left = cnt - k0 < E::BK ? (int)(cnt - k0) : E::BK;
     const T* const prow = pbase + (FEW ? 0 : k0 * ps);
@@ -450,11 +504,11 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
       const bool gin = kr < left && ng < g.H, pin = kr < left && np < npc;
       auto load = [&](auto& gt, auto& pt) {
         if constexpr (VEC) {
-          gt.fetch(i, gr, gin ? (uint32_t)gat * (uint32_t)sizeof(S) : kDropOffset);
-          pt.fetch(i, pr, pin ? (uint32_t)pat * (uint32_t)sizeof(T) : kDropOffset);
+          gt.fetch(0, i, gr, gin ? (uint32_t)gat * (uint32_t)sizeof(S) : kDropOffset);
+          pt.fetch(0, i, pr, pin ? (uint32_t)pat * (uint32_t)sizeof(T) : kDropOffset);
         } else {
-          gt.fetch(i, gbase + gat, gin ? g.H - ng : 0);
-          pt.fetch(i, prow + pat, pin ? npc - np : 0);
+          gt.fetch(0, i, gbase + gat, gin ? g.H - ng : 0);
+          pt.fetch(0, i, prow + pat, pin ? npc - np : 0);
         }
       };
       if constexpr (MODE == DWIN) load(A, B);
@@ -475,8 +529,8 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   }
   for (int64_t k0 = 0; k0 < cnt; k0 += E::BK) {
     __syncthreads();
-    A.put(la);
-    B.put(lb);
+    A.put(0, la);
+    B.put(0, lb);
     __syncthreads();
     if (k0 + E::BK < cnt) {
       fetch(k0 + E::BK);
@@ -539,9 +593,12 @@ struct Pass {
 template <typename S>
 __global__ __launch_bounds__(NT) void pass_kernel(Pass a) {
   const int lane = threadIdx.x & 63;
-  int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
   const int64_t z = (int64_t)blockIdx.x * NT + threadIdx.x, zn = (int64_t)gridDim.x * NT;
   for (int64_t i = z; i < a.zeros; i += zn) a.zero[i] = 0;
+  int64_t total = 0;
+  for (int k = 0; k < a.arrays; ++k) total += a.a[k].rows;
+  for (int64_t all = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6); all < total; all += (int64_t)gridDim.x * (NT / 64)) {
+  int64_t row = all;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     if (k >= a.arrays) break;
@@ -577,6 +634,7 @@ __global__ __launch_bounds__(NT) void pass_kernel(Pass a) {
     }
     row -= v.rows;
   }
+  }
 }
 
 // Columns of an expert's matrix (R x n): 64 columns and 64 rows a block, raised in `out` [E][n], zeros before.
@@ -602,38 +660,61 @@ __device__ __forceinline__ int place_of(const int32_t* place, const int32_t* ind
   return e >= 0 && e < E ? (int)s : -1;
 }
 
+// dweight by slot: the partial sums over the column tiles, in order; 0 for a slot with no expert.
+struct Dweight {
+  int64_t M;
+  int parts;
+  const float* part;
+  float* out;
+};
+__device__ __forceinline__ void dweight_of(const Dweight& d, const int32_t* place, const int32_t* index, int E) {
+  for (int64_t s = (int64_t)blockIdx.x * NT + threadIdx.x; s < d.M; s += (int64_t)gridDim.x * NT) {
+    const int p = place_of(place, index, E, s);
+    float t = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < d.parts; ++i) t += d.part[(int64_t)i * d.M + max(p, 0)];
+    d.out[s] = p >= 0 ? t : 0.f;
+  }
+}
+
+// Four slots' places, weights and products at a time are on their way together (a slot with none reads place 0).
 template <typename T>
 __global__ __launch_bounds__(NT) void combine_kernel(int64_t rows, int H, int ldo, int k,
                                                      const int32_t* __restrict__ place,
                                                      const int32_t* __restrict__ index, int E,
                                                      const float* __restrict__ weight, const float* __restrict__ o,
-                                                     T* __restrict__ y) {
+                                                     T* __restrict__ y, Dweight d) {
   const int nv = (H + 3) / 4;
   const int64_t n = rows * nv;
   for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
     const int64_t t = i / nv;
     const int c = (int)(i - t * nv) * 4;
     f4 s = {0.f, 0.f, 0.f, 0.f};
-    for (int j = 0; j < k; ++j) {
-      const int p = place_of(place, index, E, t * k + j);
-      if (p < 0) continue;
-      const float w = weight ? weight[t * k + j] : 1.f;
-      s += w * ld4(o + (int64_t)p * ldo + c);
+    for (int j0 = 0; j0 < k; j0 += 4) {
+      int p[4];
+      float w[4];
+      f4 v[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int64_t slot = t * k + min(j0 + j, k - 1);
+        p[j] = place_of(place, index, E, slot);
+        w[j] = weight ? weight[slot] : 1.f;
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j0 + j < k) v[j] = ld4(o + (int64_t)max(p[j], 0) * ldo + c);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (j0 + j < k && p[j] >= 0) s += w[j] * v[j];
     }
     store4(y + t * H + c, s, H - c);
   }
+  if (d.out) dweight_of(d, place, index, E);
 }
 
-// dweight by slot: the partial sums over the column tiles, in order; 0 for a slot with no expert.
-__global__ __launch_bounds__(NT) void dweight_kernel(int64_t M, int parts, const int32_t* __restrict__ place,
-                                                     const int32_t* __restrict__ index, int E, const float* __restrict__ part, float* __restrict__ dweight) {
-  const int64_t s = (int64_t)blockIdx.x * NT + threadIdx.x;
-  if (s >= M) return;
-  const int p = place_of(place, index, E, s);
-  float t = 0.f;
-  if (p >= 0)
-    for (int i = 0; i < parts; ++i) t += part[(int64_t)i * M + p];
-  dweight[s] = t;
+__global__ __launch_bounds__(NT) void dweight_kernel(Dweight d, const int32_t* __restrict__ place,
+                                                     const int32_t* __restrict__ index, int E) {
+  dweight_of(d, place, index, E);
 }
 
 // ---------------------------------------------------------------- host
@@ -644,17 +725,25 @@ inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 // kernels read an expert's weights once for 16 rows, the tiles once for up to 128.
 inline bool few(int64_t M, int E) { return M <= FEW_SLOTS && M <= 16 * (int64_t)E; }
 
-// Rows of a tile by the rows that an expert has on average: the weights are read once for each tile of an expert,
-// and rows that a tile lacks are still computed.
-inline int tile_rows(int64_t M, int E) {
-  const int64_t avg = M / std::max(1, E);
-  return avg > 64 ? 128 : avg > 32 ? 64 : 32;
+// Rows of a tile: 128 only where the products have enough tiles of 128 x 128 to fill the chip a few times (M rows by
+// F + H columns, up and down alike), else more blocks with fewer rows.
+inline int tile_rows(const FscExpertDims& d) {
+  const int64_t M = d.rows * d.k, avg = M / d.n_experts, tiles = M * (d.width + d.hidden) / (128 * 128);
+  return avg <= 32 || tiles < 224 ? 32 : avg <= 64 || tiles < 1024 ? 64 : 128;
 }
 
-// Whether rows at p can be read 16 bytes at a time through one buffer (all of them below kDropOffset bytes).
+// Whether rows at p can be read 16 bytes at a time through one buffer: whole 32-bit words, and all of them below
+// kDropOffset bytes.
 inline bool vec_ok(const void* p, int64_t rows, int64_t stride, int size, int n) {
-  return !p || ((uintptr_t)p % 16 == 0 && (stride * size) % 16 == 0 && n % (size == 1 ? 16 : 8) == 0 &&
+  return !p || ((uintptr_t)p % 4 == 0 && stride * size % 4 == 0 && n * size % 4 == 0 &&
                 ((rows - 1) * stride + n) * size < (int64_t)kDropOffset);
+}
+// The same for the few-rows kernels, which read 16 bytes through pointers as well, and step through an expert's matrix
+// with signed 32-bit offsets.
+inline bool few_vec_ok(const void* p, int64_t rows, int64_t stride, int size, int n) {
+  return vec_ok(p, rows, stride, size, n) &&
+         (!p || ((uintptr_t)p % 16 == 0 && stride * size % 16 == 0 && n % (size == 1 ? 16 : 8) == 0 &&
+                 ((rows - 1) * stride + n) * size < (1ll << 31)));
 }
 
 template <int KIND, typename S, int MODE>
@@ -667,9 +756,13 @@ void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
     if (vec) rows_kernel<KIND, S, MODE, nj, true><<<grid, 128 * WW, 0, st>>>(g);
     else rows_kernel<KIND, S, MODE, nj, false><<<grid, 128 * WW, 0, st>>>(g);
   };
-  if (tile == 128) go(std::integral_constant<int, 4>{});
-  else if (tile == 64) go(std::integral_constant<int, 2>{});
-  else go(std::integral_constant<int, 1>{});
+  if constexpr (KIND == FINE) {               // 32 rows a tile (fine)
+    go(std::integral_constant<int, 1>{});
+  } else {
+    if (tile == 128) go(std::integral_constant<int, 4>{});
+    else if (tile == 64) go(std::integral_constant<int, 2>{});
+    else go(std::integral_constant<int, 1>{});
+  }
 }
 
 // Tiles of a weight gradient, and how many parts its positions are split into: so many that about 512 blocks run, of
@@ -699,7 +792,7 @@ void launch_pass(const Pass& a, hipStream_t st) {
   int64_t rows = 0;
   for (int k = 0; k < a.arrays; ++k) rows += a.a[k].rows;
   if (rows == 0 && a.zeros == 0) return;
-  pass_kernel<S><<<(unsigned)std::max<int64_t>(1, (rows + 3) / 4), NT, 0, st>>>(a);
+  pass_kernel<S><<<(unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1 << 20)), NT, 0, st>>>(a);
 }
 
 // Adds an array to a pass if it has to be looked at: its largest magnitudes are wanted or its rows cannot be read in
@@ -713,6 +806,7 @@ bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int64_t outer, 
   if (copy || most) {
     a.a[a.arrays++] = Pass::Array{p, rows * outer, ld, n, most, copy ? room : nullptr, cld};
     if (copy) {
+      // (a copy of whole chunks from here on)
       p = room;
       ld = cld;
       room += align64(rows * outer * cld * (int64_t)sizeof(S));
@@ -722,10 +816,10 @@ bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int64_t outer, 
 }
 
 template <typename T>
-void launch_combine(const Args& g, const float* weight, T* y, hipStream_t st) {
+void launch_combine(const Args& g, const float* weight, T* y, const Dweight& d, hipStream_t st) {
   const int64_t n = g.T * ((g.H + 3) / 4);
   const unsigned grid = (unsigned)std::min<int64_t>((n + NT - 1) / NT, 1 << 20);
-  combine_kernel<T><<<grid, NT, 0, st>>>(g.T, g.H, g.ldo, g.k, g.place, g.index, g.E, weight, g.o, y);
+  combine_kernel<T><<<grid, NT, 0, st>>>(g.T, g.H, g.ldo, g.k, g.place, g.index, g.E, weight, g.o, y, d);
 }
 
 int check_dims(const FscExpertDims* d, bool q8) {
@@ -733,8 +827,8 @@ int check_dims(const FscExpertDims* d, bool q8) {
   FSC_CHECK_ARG(d->rows >= 0 && d->rows < (1ll << 31), "expert_mlp: rows must be below 2^31");
   FSC_CHECK_ARG(d->n_experts >= 1 && d->n_experts <= MAX_EXPERTS, "expert_mlp: 1 to 512 experts");
   FSC_CHECK_ARG(d->k >= 1 && d->k <= 64 && d->rows * d->k < (1ll << 31), "expert_mlp: 1 to 64 slots a row, fewer than 2^31 in all");
-  FSC_CHECK_ARG(d->width >= 1 && d->width <= (1 << 20) && d->hidden >= 1 && d->hidden <= (1 << 20),
-                "expert_mlp: width and hidden must be 1 to 2^20");
+  FSC_CHECK_ARG(d->width >= 1 && d->width <= (1 << 17) && d->hidden >= 1 && d->hidden <= (1 << 17),
+                "expert_mlp: width and hidden must be 1 to 2^17");
   if (q8) FSC_CHECK_ARG(d->dtype == FSC_I8, "expert_mlp_q8: rows and weights are int8");
   else FSC_CHECK_ARG(d->dtype == FSC_F32 || d->dtype == FSC_BF16, "expert_mlp: rows are float32 or bfloat16");
   return 0;
@@ -749,7 +843,7 @@ inline int ldo_of(const FscExpertDims& d) { return (d.width + 3) / 4 * 4; }
 // kernels stays in fp32 and the products run as those of fp32 rows do.
 inline bool fine(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k;
-  return d.dtype == FSC_BF16 && (few(M, d.n_experts) || tile_rows(M, d.n_experts) == 32);
+  return d.dtype == FSC_BF16 && (few(M, d.n_experts) || M <= 32 * (int64_t)d.n_experts);
 }
 // bytes of a value of the arrays between the kernels
 inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 : d.dtype == FSC_F32 || fine(d) ? 4 : 2; }
@@ -758,16 +852,16 @@ inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 
 struct Space {
   int64_t h, o, da, hw, part, hs, most, split, pad, total;
 };
-// whether the products are fp32 ones by tiles
+// fp32 rows by tiles: two scaled parts an operand (three products, and one pass over the weights for their scales), or
+// three parts (six products, no pass) where an expert has so few rows that the weights' bytes count for more.
 inline bool parts(const FscExpertDims& d) {
-  return !few(d.rows * d.k, d.n_experts) && (d.dtype == FSC_F32 || fine(d));
+  return !few(d.rows * d.k, d.n_experts) && d.dtype == FSC_F32 && d.rows * d.k > 80 * (int64_t)d.n_experts;
 }
 // room for padded copies of x (or x and dy) and of weights whose rows are no whole chunks
 inline int64_t pad_bytes(const FscExpertDims& d, int rows_arrays) {
   const int size = d.dtype == FSC_F32 ? 4 : d.dtype == FSC_BF16 ? 2 : 1, ce = size == 1 ? 16 : 8;
   const int64_t hp = whole_chunks(d.width, ce), fp = whole_chunks(d.hidden, ce), E = d.n_experts;
-  return rows_arrays * align64(d.rows * hp * size) + (hp != d.width ? align64(E * 2 * d.hidden * hp * size) : 0) +
-         (fp != d.hidden ? align64(E * d.width * fp * size) : 0);
+  return rows_arrays * align64(d.rows * hp * size) + align64(E * 2 * d.hidden * hp * size) + align64(E * d.width * fp * size);
 }
 inline Space forward_space(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, ldf = ldf_of(d), size = held_size(d);
@@ -838,8 +932,8 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
 template <int KIND, typename S>
 void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
   if (!g.place) {
-    const bool vin = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H) && vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H);
-    const bool vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
+    const bool vin = few_vec_ok(g.x, g.T, g.xs, sizeof(S), g.H) && few_vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H);
+    const bool vout = few_vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
     if constexpr (KIND == I8) {
       few_launch_q8(g, vin, vout, st);
     } else {
@@ -858,7 +952,7 @@ void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
     launch_rows<KIND, S, DOWN>(g, tile, vout, st);
   }
   using Y = std::conditional_t<KIND == I8, __bf16, S>;
-  launch_combine<Y>(g, g.weight, (Y*)y, st);
+  launch_combine<Y>(g, g.weight, (Y*)y, Dweight{}, st);
 }
 
 template <int KIND, typename S>
@@ -867,7 +961,9 @@ void backward(Args g, int tile, char* room, void* dx, float* dweight, hipStream_
   bool vdy = vec_ok(g.dy, g.T, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H);
   bool vin = vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
   if (by_slot) {
-    few_launch<S>(DH, g, vdy && vout, st);
+    const auto whole = [&](const void* p, int64_t rows, int64_t stride, int n) { return few_vec_ok(p, rows, stride, sizeof(S), n); };
+    few_launch<S>(DH, g, whole(g.dy, g.T, g.ds, g.H) && whole(g.w_out, g.H, g.F, g.F), st);
+    vin = whole(g.w_in, 2 * g.F, g.H, g.H);
   } else {
     Pass a{};
     if (g.out_col) {        // out_col, in_col and damost lie one after the other
@@ -887,21 +983,21 @@ void backward(Args g, int tile, char* room, void* dx, float* dweight, hipStream_
     }
     launch_rows<KIND, S, DH>(g, tile, vdy && vout, st);
   }
-  if (dweight)
-    dweight_kernel<<<(unsigned)((g.M + NT - 1) / NT), NT, 0, st>>>(
-        g.M, by_slot ? few_parts(g.F, sizeof(S)) : (g.F + BN - 1) / BN, g.place, g.index, g.E, g.dwpart, dweight);
+  const Dweight d{g.M, by_slot ? few_parts(g.F, sizeof(S)) : (g.F + BN - 1) / BN, g.dwpart, dweight};
   if (dx) {
     if (by_slot) few_launch<S>(DX, g, vin, st);
     else launch_rows<KIND, S, DX>(g, tile, vin, st);
-    launch_combine<S>(g, nullptr, (S*)dx, st);
+    launch_combine<S>(g, nullptr, (S*)dx, d, st);
+  } else if (dweight) {
+    dweight_kernel<<<(unsigned)((g.M + NT - 1) / NT), NT, 0, st>>>(d, g.place, g.index, g.E);
   }
+  constexpr int WK = KIND == F32 ? X6 : KIND;
   if (by_slot) {
-    if constexpr (KIND == F32) {
-      if (g.dw_in) launch_weights<X6, S, DWIN, true>(g, vx, st);
-      if (g.dw_out) launch_weights<X6, S, DWOUT, true>(g, vdy, st);
+    if constexpr (KIND != BF16) {
+      if (g.dw_in) launch_weights<WK, S, DWIN, true>(g, vx, st);
+      if (g.dw_out) launch_weights<WK, S, DWOUT, true>(g, vdy, st);
     }
   } else {
-    constexpr int WK = KIND == F32 ? X6 : KIND;
     if (g.dw_in) launch_weights<WK, S, DWIN>(g, vx, st);
     if (g.dw_out) launch_weights<WK, S, DWOUT>(g, vdy, st);
   }
@@ -918,7 +1014,7 @@ int fsc_expert_sizes(const FscExpertDims* dims, int64_t* plan_ints, int64_t* sav
   if (int rc = check_dims(dims, dims && dims->dtype == FSC_I8)) return rc;
   FSC_CHECK_ARG(plan_ints && saved_floats && forward_bytes && backward_bytes, "expert_sizes: null output");
   const int64_t M = dims->rows * dims->k;
-  *plan_ints = few(M, dims->n_experts) ? 0 : fsc::experts::plan_ints(M, dims->n_experts, tile_rows(M, dims->n_experts));
+  *plan_ints = few(M, dims->n_experts) ? 0 : fsc::experts::plan_ints(M, dims->n_experts, tile_rows(*dims));
   *saved_floats = dims->dtype == FSC_I8 ? 0 : M * 2 * ldf_of(*dims);
   *forward_bytes = forward_space(*dims).total;
   *backward_bytes = dims->dtype == FSC_I8 ? 0 : backward_space(*dims).total;
@@ -931,7 +1027,7 @@ int fsc_expert_plan(const FscExpertDims* dims, const int32_t* index, int32_t* pl
   const int64_t M = dims->rows * dims->k;
   if (few(M, dims->n_experts)) return 0;       // the products find their rows themselves
   FSC_CHECK_ARG(plan && index, "expert_plan: null array");
-  const int tile = tile_rows(M, dims->n_experts);
+  const int tile = tile_rows(*dims);
   launch_plan(plan_of(plan, M, dims->n_experts, tile), M, dims->n_experts, dims->k, tile, index, stream);
   return fsc::check_launch("expert_plan") ? 2 : 0;
 }
@@ -946,7 +1042,7 @@ int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const vo
   FSC_CHECK_ARG(x && index && (plan || few(M, dims->n_experts)) && weight && w_in && w_out && workspace && y,
                 "expert_mlp_forward: null array");
   FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_forward: negative row stride");
-  const int tile = tile_rows(M, dims->n_experts);
+  const int tile = tile_rows(*dims);
   const Plan p = plan_of(const_cast<int32_t*>(plan), M, dims->n_experts, tile);
   Args g = args_of(*dims, p);
   const Space s = forward_space(*dims);
@@ -961,8 +1057,9 @@ int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const vo
     g.in_row = g.hmost + g.M;
     g.out_row = g.in_row + (int64_t)g.E * 2 * g.F;
   }
-  if (dims->dtype == FSC_F32) forward<F32, float>(g, tile, ws + s.pad, y, stream);
-  else if (fine(*dims)) forward<F32, __bf16>(g, tile, ws + s.pad, y, stream);
+  if (parts(*dims)) forward<F32, float>(g, tile, ws + s.pad, y, stream);
+  else if (dims->dtype == FSC_F32) forward<X6, float>(g, tile, ws + s.pad, y, stream);
+  else if (fine(*dims)) forward<FINE, __bf16>(g, tile, ws + s.pad, y, stream);
   else forward<BF16, __bf16>(g, tile, ws + s.pad, y, stream);
   return fsc::check_launch("expert_mlp_forward") ? 2 : 0;
 }
@@ -977,7 +1074,7 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
   FSC_CHECK_ARG((plan || few(M, dims->n_experts)) && w_in && w_out, "expert_mlp_backward: null array");
   FSC_CHECK_ARG(M == 0 || (dy && x && index && weight && saved && workspace), "expert_mlp_backward: null array");
   FSC_CHECK_ARG(x_stride >= 0 && dy_stride >= 0, "expert_mlp_backward: negative row stride");
-  const int tile = tile_rows(M, dims->n_experts);
+  const int tile = tile_rows(*dims);
   const Plan p = plan_of(const_cast<int32_t*>(plan), M, dims->n_experts, tile);
   Args g = args_of(*dims, p);
   const Space s = backward_space(*dims);
@@ -1003,13 +1100,15 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
       if (dw_in) launch_weights<X6, float, DWIN, true>(g, false, stream);
       if (dw_out) launch_weights<X6, float, DWOUT, true>(g, false, stream);
     } else {
-      if (dw_in) launch_weights<X6, __bf16, DWIN, true>(g, false, stream);
-      if (dw_out) launch_weights<X6, __bf16, DWOUT, true>(g, false, stream);
+      if (dw_in) launch_weights<FINE, __bf16, DWIN, true>(g, false, stream);
+      if (dw_out) launch_weights<FINE, __bf16, DWOUT, true>(g, false, stream);
     }
-  } else if (dims->dtype == FSC_F32) {
+  } else if (parts(*dims)) {
     backward<F32, float>(g, tile, ws + s.pad, dx, dweight, stream);
+  } else if (dims->dtype == FSC_F32) {
+    backward<X6, float>(g, tile, ws + s.pad, dx, dweight, stream);
   } else if (fine(*dims)) {
-    backward<F32, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
+    backward<FINE, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
   } else {
     backward<BF16, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
   }
@@ -1026,7 +1125,7 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
   FSC_CHECK_ARG(x && x_scale && index && (plan || few(M, dims->n_experts)) && weight && w_in && w_in_scale && w_out && w_out_scale && workspace && y,
                 "expert_mlp_q8: null array");
   FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_q8: negative row stride");
-  const int tile = tile_rows(M, dims->n_experts);
+  const int tile = tile_rows(*dims);
   const Plan p = plan_of(const_cast<int32_t*>(plan), M, dims->n_experts, tile);
   Args g = args_of(*dims, p);
   const Space s = forward_space(*dims);

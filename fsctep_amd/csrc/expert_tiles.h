@@ -10,15 +10,38 @@ namespace experts {
 
 typedef int i4v __attribute__((ext_vector_type(4)));
 
-// F32: fp32 products from two scaled fp16 parts an operand (mfma_x3); X6: from three bf16 parts (mfma_x6)
-enum Kind { F32 = 0, BF16 = 1, I8 = 2, X6 = 3 };
+// F32: fp32 products from two scaled fp16 parts an operand (mfma_x3); X6: from three bf16 parts (mfma_x6); FINE: bf16
+// operands as they are, fp32 ones in three bf16 parts (one product, or three where the other operand is fp32)
+enum Kind { F32 = 0, BF16 = 1, I8 = 2, X6 = 3, FINE = 4 };
 
-// T: the type between the kernels; BK: reduction entries of a step; CE: those of a 16-byte LDS chunk; PL: LDS planes
+// T: the type between the kernels; BK: reduction entries of a step; CE: those of a 16-byte LDS chunk; planes<O>: LDS
+// planes of an operand that is an O in memory
 template <int KIND> struct El;
-template <> struct El<F32> { using T = float; static constexpr int BK = 32, CE = 8, PL = 2; };
-template <> struct El<X6> { using T = float; static constexpr int BK = 32, CE = 8, PL = 3; };
-template <> struct El<BF16> { using T = __bf16; static constexpr int BK = 64, CE = 8, PL = 1; };
-template <> struct El<I8> { using T = int8_t; static constexpr int BK = 128, CE = 16, PL = 1; };
+template <> struct El<F32> {
+  using T = float;
+  static constexpr int BK = 32, CE = 8;
+  template <typename O> static constexpr int planes = 2;
+};
+template <> struct El<X6> {
+  using T = float;
+  static constexpr int BK = 32, CE = 8;
+  template <typename O> static constexpr int planes = 3;
+};
+template <> struct El<FINE> {
+  using T = float;
+  static constexpr int BK = 32, CE = 8;
+  template <typename O> static constexpr int planes = sizeof(O) == 4 ? 3 : 1;
+};
+template <> struct El<BF16> {
+  using T = __bf16;
+  static constexpr int BK = 64, CE = 8;
+  template <typename O> static constexpr int planes = 1;
+};
+template <> struct El<I8> {
+  using T = int8_t;
+  static constexpr int BK = 128, CE = 16;
+  template <typename O> static constexpr int planes = 1;
+};
 
 template <int KIND> struct Acc { using V = f4; };
 template <> struct Acc<I8> { using V = i4v; };
@@ -201,7 +224,8 @@ __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, 
         float part = 0.f;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float sg = sigmoid(ga[s][v]), act = ga[s][v] * sg, h = act * up[s][v], pv = p.v[s][v], dh = pv * w[s];
+          const float sg = sigmoid(ga[s][v]), act = ga[s][v] * sg, h = act * up[s][v];
+          const float pv = n + v < g.F ? p.v[s][v] : 0.f, dh = pv * w[s];
           part += h * pv;
           hw[v] = h * w[s];
           du[v] = dh * act;

@@ -329,8 +329,8 @@ FscExpertDims expert_dims(const Tensor& x, const Tensor& index, const Tensor& we
   TORCH_CHECK(weight.scalar_type() == at::kFloat, name, ": weight must be float32, got ", weight.scalar_type());
   TORCH_CHECK(w_in.scalar_type() == x.scalar_type() && w_out.scalar_type() == x.scalar_type(), name,
               ": x, w_in and w_out must have one type");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= (1 << 20) && w_out.size(2) >= 1 && w_out.size(2) <= (1 << 20), name,
-              ": width and hidden must be 1 to 2^20");
+  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= (1 << 17) && w_out.size(2) >= 1 && w_out.size(2) <= (1 << 17), name,
+              ": width and hidden must be 1 to 2^17");
   TORCH_CHECK(w_out.size(0) >= 1 && w_out.size(0) <= 512, name, ": 1 to 512 experts, got ", w_out.size(0));
   TORCH_CHECK(index.size(1) <= 64, name, ": at most 64 slots a row, got ", index.size(1));
   const int32_t dt = x.scalar_type() == at::kChar ? FSC_I8 : code_of(x.scalar_type(), "x");
