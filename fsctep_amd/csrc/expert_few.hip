@@ -322,7 +322,7 @@ __device__ __forceinline__ i4v get16(const int8_t* p, int n) {
 template <bool VEC>
 __global__ __launch_bounds__(FT) void few_up_q8_kernel(Args g) {
   __shared__ int16_t list[FEW_SLOTS];
-  __shared__ float tops[FW][16];
+  __shared__ uint32_t tops[FW][16];
   const int ng = g.ldf / QG, grp = blockIdx.x;
   const int e = few_expert(g, blockIdx.y);
   if (e < 0) return;
@@ -380,31 +380,25 @@ __global__ __launch_bounds__(FT) void few_up_q8_kernel(Args g) {
       const int k = whole * 64 + 16 * q, n16 = g.H - k;
       mul(get16<VEC>(wg + k, n16), get16<VEC>(wg + up + k, n16), get16<VEC>(x + k, n16));
     }
-    float h[4], top = 0.f;
+    f4 h;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const float ga = n + j < g.F ? (float)ag[j] * (xs * sg[j]) : 0.f;
       const float u = n + j < g.F ? (float)au[j] * (xs * su[j]) : 0.f;
       h[j] = ga * sigmoid(ga) * u;
-      top = max_nan(top, fabsf(h[j]));
     }
-    top = max_nan(top, __shfl_xor(top, 16, 64));
-    top = max_nan(top, __shfl_xor(top, 32, 64));
+    uint32_t top = most4(h);
+    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
     __syncthreads();                                   // the last tile's maxima have been read
     if (q == 0) tops[wave][r] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < FW; ++w) top = max_nan(top, tops[w][r]);
-    const float inv = top > 0.f ? 127.f / top : 0.f;
+    for (int w = 0; w < FW; ++w) top = max(top, tops[w][r]);
+    const float most = __uint_as_float(top), inv = most > 0.f ? 127.f / most : 0.f;
     if (live) {
-      int8_t b[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float c = rintf(h[j] * inv);
-        b[j] = c >= -127.f && c <= 127.f ? (int8_t)c : (int8_t)0;
-      }
-      store_bytes<4>((int8_t*)g.h + (int64_t)slot * g.ldf + n, b);
-      if (wave == 0 && q == 0) g.hscale[(int64_t)slot * ng + grp] = top / 127.f;
+      *reinterpret_cast<uint32_t*>((int8_t*)g.h + (int64_t)slot * g.ldf + n) = codes4(h, inv);
+      if (wave == 0 && q == 0) g.hscale[(int64_t)slot * ng + grp] = most / 127.f;
     }
   }
 }

@@ -192,7 +192,7 @@ template <int KIND, int MODE>
 constexpr int waves_w() { return KIND == I8 && MODE == UP ? 4 : 2; }
 
 template <int KIND, typename S, int MODE, int NJ, bool VEC>
-__global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), 2) void rows_kernel(Args g) {
+__global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE == UP && VEC ? 4 : KIND == F32 && MODE == DH && VEC ? 3 : 2)) void rows_kernel(Args g) {
   using E = El<KIND>;
   using T = typename E::T;                                   // of the arrays between the kernels; S: the caller's
   using R = std::conditional_t<MODE == DOWN || MODE == DX, T, S>;

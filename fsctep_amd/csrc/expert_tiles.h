@@ -104,6 +104,15 @@ __device__ __forceinline__ void raise(uint32_t* most, uint32_t m, int width, boo
   if (in && (threadIdx.x & (width - 1)) == 0) atomicMax(most, m);
 }
 
+// Four codes rint(h inv), |h inv| <= 127: the sum with 1.5 * 2^23 has the whole number in its low bits.  (A NaN or an
+// infinity has some code: its group's unit is one too.)
+__device__ __forceinline__ uint32_t codes4(const f4& h, float inv) {
+  uint32_t w[4];
+#pragma unroll
+  for (int v = 0; v < 4; ++v) w[v] = __float_as_uint(__fadd_rn(__fmul_rn(h[v], inv), 12582912.f));
+  return __builtin_amdgcn_perm(__builtin_amdgcn_perm(w[3], w[2], 0x0c0c0400u), __builtin_amdgcn_perm(w[1], w[0], 0x0c0c0400u), 0x05040100u);
+}
+
 // What becomes of a tile's sums.  acc[i][j]: weight tile w0 + i (16 rows of the weight operand), row tile x0 + j; lane
 // (r, q) holds the weight rows 4 q .. 4 q + 3 of row r.  n0: the tile's first output column (up: a weight tile pair
 // is 16 hidden columns, gate then up).  buf: LDS that nobody reads any more, TURN floats for each wave, then WW * BM
@@ -131,48 +140,46 @@ __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, 
   } else if constexpr (MODE == UP && KIND == I8) {
     // the block holds whole groups of 128 columns: their largest values, then the codes
     static_assert(WW * NI == 16, "8-bit up: 128 hidden columns a tile");
-    f4 h[NI / 2][NJ];
-    float top[NJ];
+    f4 h[NI / 2][NJ], sg[NI / 2], su[NI / 2];
+    uint32_t top[NJ];
+#pragma unroll
+    for (int i = 0; i < NI / 2; ++i)
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {
+        const float* s = g.in_scale + (int64_t)t.e * 2 * g.F + min(n0 + (w0 / 2 + i) * 16 + 4 * q + v, g.F - 1);
+        sg[i][v] = s[0];
+        su[i][v] = s[g.F];
+      }
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int row = 16 * (x0 + j) + r;
       const float xs = g.xscale[t.rws[row]];               // a row past the tile: any row's, not stored
-      top[j] = 0.f;
+      top[j] = 0;
 #pragma unroll
       for (int i = 0; i < NI / 2; ++i) {
-        const int n = n0 + (w0 / 2 + i) * 16 + 4 * q;
 #pragma unroll
         for (int v = 0; v < 4; ++v) {
-          const float* s = g.in_scale + (int64_t)t.e * 2 * g.F + min(n + v, g.F - 1);
-          const float ga = (float)acc[2 * i][j][v] * (xs * s[0]), up = (float)acc[2 * i + 1][j][v] * (xs * s[g.F]);
+          const float ga = (float)acc[2 * i][j][v] * (xs * sg[i][v]), up = (float)acc[2 * i + 1][j][v] * (xs * su[i][v]);
           h[i][j][v] = ga * sigmoid(ga) * up;              // columns past the last have sums of zero
-          top[j] = max_nan(top[j], fabsf(h[i][j][v]));
         }
+        top[j] = max(top[j], most4(h[i][j]));
       }
-      top[j] = max_nan(top[j], __shfl_xor(top[j], 16, 64));
-      top[j] = max_nan(top[j], __shfl_xor(top[j], 32, 64));
-      if (q == 0) red[wn * BM + row] = top[j];
+      top[j] = max(top[j], (uint32_t)__shfl_xor((int)top[j], 16, 64));
+      top[j] = max(top[j], (uint32_t)__shfl_xor((int)top[j], 32, 64));
+      if (q == 0) reinterpret_cast<uint32_t*>(red)[wn * BM + row] = top[j];
     }
     __syncthreads();
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int row = 16 * (x0 + j) + r;
 #pragma unroll
-      for (int w = 0; w < WW; ++w) top[j] = max_nan(top[j], red[w * BM + row]);
+      for (int w = 0; w < WW; ++w) top[j] = max(top[j], reinterpret_cast<const uint32_t*>(red)[w * BM + row]);
       if (row >= t.rows) continue;
-      const float inv = top[j] > 0.f ? 127.f / top[j] : 0.f;
+      const float most = __uint_as_float(top[j]), inv = most > 0.f ? 127.f / most : 0.f;
 #pragma unroll
-      for (int i = 0; i < NI / 2; ++i) {
-        const int n = n0 + (w0 / 2 + i) * 16 + 4 * q;
-        int8_t b[4];
-#pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float c = rintf(h[i][j][v] * inv);
-          b[v] = c >= -127.f && c <= 127.f ? (int8_t)c : (int8_t)0;
-        }
-        store_bytes<4>((int8_t*)g.h + (t.p0 + row) * g.ldf + n, b);
-      }
-      if (wn == 0 && q == 0) g.hscale[(t.p0 + row) * (g.ldf / QG) + n0 / QG] = top[j] / 127.f;
+      for (int i = 0; i < NI / 2; ++i)
+        *reinterpret_cast<uint32_t*>((int8_t*)g.h + (t.p0 + row) * g.ldf + n0 + (w0 / 2 + i) * 16 + 4 * q) = codes4(h[i][j], inv);
+      if (wn == 0 && q == 0) g.hscale[(t.p0 + row) * (g.ldf / QG) + n0 / QG] = most / 127.f;
     }
   } else if constexpr (MODE == UP) {
     using U = Turned<NI / 2>;
