@@ -732,10 +732,13 @@ inline int tile_rows(const FscExpertDims& d) {
   return avg <= 32 || tiles < 224 ? 32 : avg <= 64 || tiles < 1024 ? 64 : 128;
 }
 
+// Rows that end inside a 32-bit word.
+inline bool odd_rows(int n, int size) { return n * (int64_t)size % 4 != 0; }
+
 // Whether rows at p can be read 16 bytes at a time through one buffer: whole 32-bit words, and all of them below
 // kDropOffset bytes.
 inline bool vec_ok(const void* p, int64_t rows, int64_t stride, int size, int n) {
-  return !p || ((uintptr_t)p % 4 == 0 && stride * size % 4 == 0 && n * size % 4 == 0 &&
+  return !p || ((uintptr_t)p % 4 == 0 && stride * size % 4 == 0 && !odd_rows(n, size) &&
                 ((rows - 1) * stride + n) * size < (int64_t)kDropOffset);
 }
 // The same for the few-rows kernels, which read 16 bytes through pointers as well, and step through an expert's matrix
@@ -795,18 +798,20 @@ void launch_pass(const Pass& a, hipStream_t st) {
   pass_kernel<S><<<(unsigned)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1 << 20)), NT, 0, st>>>(a);
 }
 
-// Adds an array to a pass if it has to be looked at: its largest magnitudes are wanted or its rows cannot be read in
-// whole chunks.  p and ld are then those of the padded copy at `room` (unless that were too large for one buffer:
-// returns false, and the products read single values).
+// Adds an array (E matrices of `rows` rows; E 0: the rows of x or dy) to a pass if it has to be looked at: its largest
+// magnitudes are wanted or its rows cannot be read in whole words.  p and ld are then those of a padded copy at `room`.
+// Returns false where the products read single values: arrays too large for one buffer, and weights whose rows are
+// whole words from an address that is none.
 template <typename S>
-bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int64_t outer, int n, uint32_t* most, char*& room) {
+bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int E, int n, uint32_t* most, char*& room) {
   constexpr int CE = sizeof(S) == 1 ? 16 : 8;
   const int cld = (int)whole_chunks(n, CE);
-  const bool ok = vec_ok(p, rows, ld, sizeof(S), n), copy = !ok && rows * cld * (int64_t)sizeof(S) < (int64_t)kDropOffset;
+  const int64_t outer = std::max(1, E);
+  const bool ok = vec_ok(p, rows, ld, sizeof(S), n);
+  const bool copy = !ok && (E == 0 || odd_rows(n, sizeof(S))) && rows * cld * (int64_t)sizeof(S) < (int64_t)kDropOffset;
   if (copy || most) {
     a.a[a.arrays++] = Pass::Array{p, rows * outer, ld, n, most, copy ? room : nullptr, cld};
     if (copy) {
-      // (a copy of whole chunks from here on)
       p = room;
       ld = cld;
       room += align64(rows * outer * cld * (int64_t)sizeof(S));
@@ -857,11 +862,14 @@ struct Space {
 inline bool parts(const FscExpertDims& d) {
   return !few(d.rows * d.k, d.n_experts) && d.dtype == FSC_F32 && d.rows * d.k > 80 * (int64_t)d.n_experts;
 }
-// room for padded copies of x (or x and dy) and of weights whose rows are no whole chunks
+// Room for padded copies of x (or x and dy: their strides and addresses are not known here) and of weights with odd rows;
+// fp32 rows are always whole words.
 inline int64_t pad_bytes(const FscExpertDims& d, int rows_arrays) {
   const int size = d.dtype == FSC_F32 ? 4 : d.dtype == FSC_BF16 ? 2 : 1, ce = size == 1 ? 16 : 8;
   const int64_t hp = whole_chunks(d.width, ce), fp = whole_chunks(d.hidden, ce), E = d.n_experts;
-  return rows_arrays * align64(d.rows * hp * size) + align64(E * 2 * d.hidden * hp * size) + align64(E * d.width * fp * size);
+  if (size == 4) return 0;
+  return rows_arrays * align64(d.rows * hp * size) + (odd_rows(d.width, size) ? align64(E * 2 * d.hidden * hp * size) : 0) +
+         (odd_rows(d.hidden, size) ? align64(E * d.width * fp * size) : 0);
 }
 inline Space forward_space(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, ldf = ldf_of(d), size = held_size(d);
@@ -942,7 +950,7 @@ void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
     }
   } else {
     Pass a{};
-    const bool vx = through<S>(a, g.x, g.xs, g.T, 1, g.H, g.xmost, room);
+    const bool vx = through<S>(a, g.x, g.xs, g.T, 0, g.H, g.xmost, room);
     const bool vin = through<S>(a, g.w_in, g.li, 2 * g.F, g.E, g.H, g.in_row, room) && vx;
     const bool vout = through<S>(a, g.w_out, g.lo, g.H, g.E, g.F, g.out_row, room);
     a.zero = g.hmost;
@@ -971,10 +979,10 @@ void backward(Args g, int tile, char* room, void* dx, float* dweight, hipStream_
       a.zeros = (int64_t)g.E * (g.F + g.H) + g.M;
     }
     const void *w_in = g.w_in, *w_out = g.w_out;
-    vdy = through<S>(a, g.dy, g.ds, g.T, 1, g.H, g.dymost, room);
+    vdy = through<S>(a, g.dy, g.ds, g.T, 0, g.H, g.dymost, room);
     vout = through<S>(a, g.w_out, g.lo, g.H, g.E, g.F, nullptr, room);
     if (dx) vin = through<S>(a, g.w_in, g.li, 2 * g.F, g.E, g.H, nullptr, room);
-    if (g.dw_in) vx = through<S>(a, g.x, g.xs, g.T, 1, g.H, nullptr, room);
+    if (g.dw_in) vx = through<S>(a, g.x, g.xs, g.T, 0, g.H, nullptr, room);
     launch_pass<S>(a, st);
     if (g.out_col) {
       col_most_kernel<S><<<dim3((g.F + 63) / 64, (g.H + 63) / 64, g.E), NT, 0, st>>>((const S*)w_out, g.H, g.F, g.out_col);

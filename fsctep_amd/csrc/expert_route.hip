@@ -376,6 +376,9 @@ int check_sizes(int64_t rows, int32_t experts, int32_t dtype, int32_t k, int32_t
   return 0;
 }
 
+// rows of a launch (a grid has fewer than 2^32 threads, and a row takes 16)
+constexpr int64_t MOST_ROWS = 1ll << 24;
+
 }  // namespace route
 }  // namespace fsc
 
@@ -397,13 +400,15 @@ int fsc_route_experts(int64_t rows, int32_t n_experts, int32_t dtype, int64_t lo
   FSC_CHECK_ARG(scale > 0.f && std::isfinite(scale), "route_experts: scale must be positive and finite");
   if (rows == 0) return 0;
   FSC_CHECK_ARG(logits && index && weight, "route_experts: null array");
-  const Args a{rows, logits_stride, n_experts, k, groups, groups_kept, group_best, renormalise != 0, scale,
-               logits, bias, index, weight};
-  const unsigned grid = (unsigned)((rows + NT / RL - 1) / (NT / RL));
   const int size = dtype == FSC_F32 ? 4 : 2;
   const bool vec = n_experts % 4 == 0 && logits_stride % 4 == 0 && (uintptr_t)logits % (4 * size) == 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += MOST_ROWS)
   by_experts(n_experts, [&](auto V) {
     constexpr int v = decltype(V)::value;
+    const Args a{std::min(rows - r0, MOST_ROWS), logits_stride, n_experts, k, groups, groups_kept, group_best,
+                 renormalise != 0, scale, (const char*)logits + r0 * logits_stride * size, bias, index + r0 * k,
+                 weight + r0 * k};
+    const unsigned grid = (unsigned)((a.rows + NT / RL - 1) / (NT / RL));
     // lanes of a group, 0 where groups do not lie in whole lanes, so many that they part the row's 16
     const int per = n_experts / groups, gl = per % v == 0 && RL % (per / v) == 0 ? per / v : 0;
     const size_t lds = groups > 1 && !gl ? NT / RL * (size_t)(n_experts + groups) * 4 : 0;
@@ -429,12 +434,15 @@ int fsc_route_experts_backward(int64_t rows, int32_t n_experts, int32_t dtype, i
   FSC_CHECK_ARG(scale > 0.f && std::isfinite(scale), "route_experts_backward: scale must be positive and finite");
   if (rows == 0) return 0;
   FSC_CHECK_ARG(logits && index && weight && dweight && dlogits, "route_experts_backward: null array");
-  const BackArgs a{rows, logits_stride, n_experts, k, renormalise != 0, scale, logits, index, weight, dweight, dlogits};
-  const unsigned grid = (unsigned)((rows + NT / RL - 1) / (NT / RL));
   const int size = dtype == FSC_F32 ? 4 : 2;
   const bool vec = n_experts % 4 == 0 && logits_stride % 4 == 0 && (uintptr_t)logits % (4 * size) == 0;
+  for (int64_t r0 = 0; r0 < rows; r0 += MOST_ROWS)
   by_experts(n_experts, [&](auto V) {
     constexpr int v = decltype(V)::value;
+    const BackArgs a{std::min(rows - r0, MOST_ROWS), logits_stride, n_experts, k, renormalise != 0, scale,
+                     (const char*)logits + r0 * logits_stride * size, index + r0 * k, weight + r0 * k, dweight + r0 * k,
+                     (char*)dlogits + r0 * n_experts * size};
+    const unsigned grid = (unsigned)((a.rows + NT / RL - 1) / (NT / RL));
     if (dtype == FSC_F32) {
       if (score == 0) route_back_kernel<float, v, true><<<grid, NT, 0, stream>>>(a, vec);
       else route_back_kernel<float, v, false><<<grid, NT, 0, stream>>>(a, vec);

@@ -363,7 +363,7 @@ bool by_width(int width, bool vec, F&& f) {
 }
 
 template <typename T, typename W>
-void launch_forward(const Args& a, bool q8, bool vec, hipStream_t st) {
+void launch_rows(const Args& a, bool q8, bool vec, hipStream_t st) {
   const unsigned grid = (unsigned)((a.rows + 3) / 4);
   const bool done = by_width<T, W>(a.width, vec, [&](auto V, auto CH) {
     constexpr int v = decltype(V)::value, ch = decltype(CH)::value;
@@ -373,6 +373,22 @@ void launch_forward(const Args& a, bool q8, bool vec, hipStream_t st) {
   if (done) return;
   if (q8) wide_kernel<T, W, true><<<(unsigned)a.rows, NT, 0, st>>>(a);
   else wide_kernel<T, W, false><<<(unsigned)a.rows, NT, 0, st>>>(a);
+}
+
+// At most 2^23 rows a launch: a grid has fewer than 2^32 threads, and a wide row takes 256.
+template <typename T, typename W>
+void launch_forward(const Args& all, bool q8, bool vec, hipStream_t st) {
+  constexpr int64_t MOST = 1ll << 23;
+  for (int64_t r0 = 0; r0 < all.rows; r0 += MOST) {
+    Args a = all;
+    a.rows = std::min(all.rows - r0, MOST);
+    a.x = (const T*)all.x + r0 * all.xs;
+    a.r = all.r ? (const T*)all.r + r0 * all.rs : nullptr;
+    a.y = (char*)all.y + r0 * all.width * (int64_t)(q8 ? 1 : sizeof(T));
+    a.z = all.z ? (T*)all.z + r0 * all.width : nullptr;
+    a.rstd = all.rstd + r0;
+    launch_rows<T, W>(a, q8, vec, st);
+  }
 }
 
 template <typename T, typename W>

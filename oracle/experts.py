@@ -27,7 +27,7 @@ def codes(y):
 def scores(logits, score):
     logits = logits.double()
     if score == "sigmoid":
-        return 1 / (1 + torch.exp(-logits))
+        return torch.sigmoid(logits)
     m = logits.max(1, keepdim=True).values
     e = torch.exp(logits - torch.where(m == -math.inf, torch.zeros_like(m), m))
     t = e.sum(1, keepdim=True)
@@ -84,7 +84,7 @@ def expert_mlp(x, index, weight, w_in, w_out, group=None):
         row, slot = torch.nonzero(index == e, as_tuple=True)
         a = x[row] @ w_in[e].T
         gate, up = a[:, :f], a[:, f:]
-        h = gate / (1 + torch.exp(-gate)) * up
+        h = gate * torch.sigmoid(gate) * up
         if group is not None:
             parts = []
             for lo in range(0, f, group):

@@ -386,3 +386,112 @@ def test_operators_on_a_side_stream_and_in_a_graph():
         eager = block(v)
         torch.cuda.synchronize()
         assert torch.equal(out, eager), seed
+
+
+# ------------------------------------------------------------------ every tile, ragged rows, neighbours, large arrays
+# Rows an expert has and columns in all choose the tile (32, 64 or 128 rows) and the fp32 products' form: sizes on both
+# sides of each choice, and widths that are odd, even and multiples of four.
+TILES = [(300, 331, 85, 8, 2), (300, 334, 86, 8, 2), (500, 70, 44, 8, 2), (1200, 640, 336, 30, 2), (1300, 642, 334, 20, 1),
+         (2000, 515, 330, 3, 2), (2000, 516, 332, 3, 2), (16100, 1042, 22, 3, 1), (16100, 1043, 23, 3, 1),
+         (9000, 22, 1042, 3, 2), (20, 16, 8, 512, 64), (10, 24, 12, 40, 20)]
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", TILES)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_products_of_every_tile(rows, width, hidden, experts, k, dtype):
+    test_products_and_gradients(rows, width, hidden, experts, k, dtype)
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", [(300, 334, 86, 8, 2), (2000, 516, 332, 3, 2), (16100, 1044, 24, 3, 1),
+                                                         (9000, 22, 1042, 3, 2), (2000, 515, 331, 3, 2), (16100, 1043, 24, 3, 1)])
+def test_8_bits_of_every_tile(rows, width, hidden, experts, k):
+    test_products_in_8_bits(rows, width, hidden, experts, k)
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", [(12, 70, 46, 4, 2), (150, 70, 46, 4, 2), (150, 71, 45, 4, 2), (700, 331, 202, 3, 2)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_ragged_rows_do_not_reach_into_the_next(rows, width, hidden, experts, k, dtype):
+    """Not-a-numbers in the rows, the gradients' rows and the experts beside: what is read past a row's end counts for
+    nothing, forward and backward."""
+    dt = DT[dtype]
+    x, index, weight, w_in, w_out, dy = problem(rows, width, hidden, experts, k, dt, rows, empty=False)
+    index = index.clamp(max=experts - 2)                # nobody has the last expert; a row may have one twice
+    leaf = [t.double().requires_grad_(True) for t in (x, weight)]
+    y0 = O.expert_mlp(leaf[0], index, leaf[1], w_in, w_out)
+    dx0, dw0 = torch.autograd.grad(y0, leaf, dy.double())
+    bad = torch.arange(rows) % 3 == 1
+    x[bad], dy[bad] = float("nan"), float("nan")
+    w_in[-1], w_out[-1] = float("nan"), float("nan")
+    dev = [t.to(DEV).requires_grad_(True) for t in (x, weight)]
+    y = X().expert_mlp(dev[0], index.to(DEV), dev[1], w_in.to(DEV), w_out.to(DEV))
+    dx, dw = torch.autograd.grad(y, dev, dy.to(DEV))
+    ok = ~bad
+    close(y[ok.to(DEV)], y0[ok], TOL[dt], "y")
+    close(dx[ok.to(DEV)], dx0[ok], TOL[dt], "dx")
+    close(dw[ok.to(DEV)], dw0[ok], TOL[dt], "dweight")
+    assert torch.isnan(y[bad.to(DEV)]).all()
+
+
+def test_products_of_very_different_sizes_by_tiles():
+    """As test_products_of_very_different_sizes, where the fp32 products scale each row and column."""
+    x, index, weight, w_in, w_out, dy = problem(900, 96, 64, 3, 1, torch.float32, 8, empty=False)
+    x = x * torch.exp2(torch.linspace(-30, 10, 900)).unsqueeze(1)
+    dy = dy * torch.exp2(torch.linspace(20, -25, 900)).unsqueeze(1)
+    leaf = x.double().requires_grad_(True)
+    y0 = O.expert_mlp(leaf, index, weight, w_in, w_out)
+    dx0, = torch.autograd.grad(y0, leaf, dy.double())
+    xd = x.to(DEV).requires_grad_(True)
+    y = X().expert_mlp(xd, index.to(DEV), weight.to(DEV), w_in.to(DEV), w_out.to(DEV))
+    dx, = torch.autograd.grad(y, xd, dy.to(DEV))
+    for a, b in ((y, y0), (dx, dx0)):
+        err = (a.detach().double().cpu() - b.detach()).abs().amax(1) / b.detach().abs().amax(1)
+        assert float(err.max()) < 1e-5
+
+
+def test_rows_far_apart():
+    """Row strides that put the last rows past 2^32 bytes."""
+    hold = torch.empty(300 * 4_000_004, device=DEV)      # 4.8 GB
+    for rows, stride in ((300, 4_000_004), (40, 30_000_004)):
+        x, index, weight, w_in, w_out, dy = problem(rows, 64, 40, 4, 2, torch.float32, rows)
+        v = hold.as_strided((rows, 64), (stride, 1))
+        v.copy_(x)
+        y0 = O.expert_mlp(x, index, weight, w_in, w_out)
+        close(X().expert_mlp(v, index.to(DEV), weight.to(DEV), w_in.to(DEV), w_out.to(DEV)), y0, TOL[torch.float32])
+        norm, _ = X().rms_norm(v, torch.ones(64, device=DEV))
+        close(norm, x.double() * (x.double().square().mean(1, keepdim=True) + 1e-6).rsqrt(), 1e-6, "norm")
+        idx, w = X().route_experts(v, 3)
+        assert torch.equal(idx.cpu().long(), x.topk(3, dim=1).indices)
+
+
+def test_rows_of_more_than_four_gigabytes():
+    """Rows that no buffer of 32-bit offsets holds, contiguous: values are read one by one through 64-bit addresses."""
+    rows, width, hidden = 1_100_000, 1000, 8
+    x = torch.empty(rows, width, device=DEV).normal_(generator=torch.Generator(device=DEV).manual_seed(1))
+    index = (torch.arange(rows, device=DEV, dtype=torch.int32) * 7 % 5 - 1).unsqueeze(1)   # experts 0 to 3 and none
+    weight = torch.rand(rows, 1, device=DEV) + 0.5
+    g = gen(3)
+    w_in = (rn(g, 4, 2 * hidden, width) / math.sqrt(width)).float()
+    w_out = (rn(g, 4, width, hidden) / math.sqrt(hidden)).float()
+    xd = x.requires_grad_(True)
+    y = X().expert_mlp(xd, index, weight, w_in.to(DEV), w_out.to(DEV))
+    dx, = torch.autograd.grad(y, xd, x.detach())
+    some = torch.cat([torch.arange(0, 50), torch.arange(rows - 300, rows), torch.arange(536_000, 537_200)])
+    leaf = x.detach()[some.to(DEV)].cpu().double().requires_grad_(True)
+    y0 = O.expert_mlp(leaf, index[some.to(DEV)].cpu(), weight[some.to(DEV)].cpu(), w_in, w_out)
+    dx0, = torch.autograd.grad(y0, leaf, leaf.detach())
+    close(y.detach()[some.to(DEV)], y0, TOL[torch.float32], "y")
+    close(dx[some.to(DEV)], dx0, TOL[torch.float32], "dx")
+
+
+def test_more_rows_than_a_launch():
+    rows = (1 << 23) + 5
+    x = torch.randn(rows, 2, device=DEV)
+    y, rstd = X().rms_norm(x, torch.ones(2, device=DEV))
+    want = x.double() * (x.double().square().mean(1, keepdim=True) + 1e-6).rsqrt()
+    assert float((y - want).abs().max()) < 1e-6
+    codes, scale, _ = X().rms_norm_q8(x, torch.ones(2, device=DEV))
+    assert float((codes * scale.unsqueeze(1) - want).abs().max()) < 1.5 / 127
+    rows = (1 << 24) + 3
+    l = torch.randn(rows, 3, device=DEV)
+    index, weight = X().route_experts(l, 1)
+    assert torch.equal(index[:, 0].long(), l.argmax(1)) and float((weight - 1).abs().max()) < 1e-6
