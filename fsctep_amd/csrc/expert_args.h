@@ -48,6 +48,10 @@ void few_launch(int mode, const Args& g, bool vec, hipStream_t st);
 int few_parts(int F, int size);
 // Few rows in 8 bits: up (codes of h) and down.
 void few_launch_q8(const Args& g, bool vin, bool vout, hipStream_t st);
+// A handful of slots (expert_one.hip): up, down and the rows from their experts.
+template <typename S>
+void one_launch(const Args& g, void* y, hipStream_t st);
+void one_launch_q8(const Args& g, void* y, hipStream_t st);
 
 // 1 / (1 + 2^(-v log2 e)) by the hardware's exponential and reciprocal: within 1e-7 |v| of the value where it is
 // small, within 1e-7 elsewhere; four instructions where expf and a division take about forty.

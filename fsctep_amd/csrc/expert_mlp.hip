@@ -725,6 +725,12 @@ inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 // kernels read an expert's weights once for 16 rows, the tiles once for up to 128.
 inline bool few(int64_t M, int E) { return M <= FEW_SLOTS && M <= 16 * (int64_t)E; }
 
+// Forward by dot products (expert_one.hip): eight slots, or no more than experts, so that hardly any weight is read twice.
+// Against the few-rows kernels, us, width and hidden 640, fp32 / bf16 / 8 bits: 2 slots 7.4 / 7.5 / 10.1 against 12.2 /
+// 11.2 / 13.3; 16 of 32 experts 16 / 13 / 11 against 26 / 17 / 14; 64 of 64 39 / 37 / 22 against 70 / 45 / 26; but four for
+// each of 16 experts 31 / 33 / 20 against 25 / 22 / 15, and two for each of 32 experts of 1,600 x 1,600 265 against 197.
+inline bool one(int64_t M, int E) { return M <= 8 || (M <= FEW_SLOTS && M <= E); }
+
 // Rows of a tile: 128 only where the products have enough tiles of 128 x 128 to fill the chip a few times (M rows by
 // F + H columns, up and down alike), else more blocks with fewer rows.
 inline int tile_rows(const FscExpertDims& d) {
@@ -940,6 +946,11 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
 template <int KIND, typename S>
 void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
   if (!g.place) {
+    if (one(g.M, g.E)) {
+      if constexpr (KIND == I8) one_launch_q8(g, y, st);
+      else one_launch<S>(g, y, st);
+      return;
+    }
     const bool vin = few_vec_ok(g.x, g.T, g.xs, sizeof(S), g.H) && few_vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H);
     const bool vout = few_vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
     if constexpr (KIND == I8) {

@@ -408,7 +408,23 @@ def test_8_bits_of_every_tile(rows, width, hidden, experts, k):
     test_products_in_8_bits(rows, width, hidden, experts, k)
 
 
-@pytest.mark.parametrize("rows,width,hidden,experts,k", [(12, 70, 46, 4, 2), (150, 70, 46, 4, 2), (150, 71, 45, 4, 2), (700, 331, 202, 3, 2)])
+# A handful of slots, each output a dot product: rows of fewer than 16 bytes, of one read and of several, odd and even.
+HANDFUL = [(1, 331, 203, 9, 1), (30, 70, 46, 64, 2), (3, 5, 3, 8, 2), (4, 1, 1, 3, 2), (6, 13, 200, 16, 2), (2, 1100, 520, 4, 3),
+           (8, 17, 15, 1, 1), (3, 259, 131, 60, 20)]
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", HANDFUL)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_products_of_a_handful(rows, width, hidden, experts, k, dtype):
+    test_products_and_gradients(rows, width, hidden, experts, k, dtype)
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", HANDFUL)
+def test_8_bits_of_a_handful(rows, width, hidden, experts, k):
+    test_products_in_8_bits(rows, width, hidden, experts, k)
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", [(3, 70, 46, 4, 2), (3, 71, 45, 4, 2), (12, 70, 46, 4, 2), (150, 70, 46, 4, 2), (150, 71, 45, 4, 2), (700, 331, 202, 3, 2)])
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
 def test_ragged_rows_do_not_reach_into_the_next(rows, width, hidden, experts, k, dtype):
     """Not-a-numbers in the rows, the gradients' rows and the experts beside: what is read past a row's end counts for
