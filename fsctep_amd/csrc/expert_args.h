@@ -31,8 +31,8 @@ struct Args {
   void* hw;                         // [M][ldf] weight h, for dw_out (null: not wanted)
   float* dwpart;                    // [column tiles of dh][M] partial dweight
   void *dw_in, *dw_out;
-  float* dwsplit;                   // [splits] partial weight gradients, where the positions are split
-  int splits;
+  float* dwsplit;                   // [shares] partial weight gradients of the experts with more than one share
+  int share;                        // positions of a share (an expert's positions are dealt into shares of so many)
   // fp32 products: largest magnitudes (bits) of the rows of x and dy [T], of h and da [M], of the weights along each
   // output: rows of w_in [E][2 F] and w_out [E][H] (up, down), columns of w_out [E][F] and w_in [E][H] (dh, dx)
   uint32_t *xmost, *dymost, *hmost, *damost, *in_row, *out_row, *out_col, *in_col;

@@ -438,6 +438,57 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE 
 }
 
 // ---------------------------------------------------------------- weight gradients
+// An expert's positions in shares of g.share, one after the other over the experts (one, empty, for an expert without
+// rows): the expert, which of its shares, how many it has, the number of its first.
+struct Share {
+  int e, at, n;
+  int64_t first;
+};
+constexpr int MANY_TILES = 64;
+
+// Runs f(e, shares of expert e, shares before the wave's 64 experts, inclusive sum over the lanes, all lanes) for 64
+// experts at a time until it returns true.
+template <typename F>
+__device__ __forceinline__ void scan_shares(const Args& g, F&& f) {
+  const int lane = threadIdx.x & 63;
+  int before = 0;
+  for (int e0 = 0; e0 < g.E; e0 += 64) {
+    const int e = e0 + lane;
+    const int rows = g.offsets[min(e + 1, g.E)] - g.offsets[min(e, g.E)];
+    const int n = e >= g.E ? 0 : rows > 0 ? (rows - 1) / g.share + 1 : 1;
+    int sum = n;
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+      const int u = __shfl_up(sum, off, 64);
+      if (lane >= off) sum += u;
+    }
+    const int all = __shfl(sum, 63, 64);
+    if (f(e0, n, before, sum, all)) return;
+    before += all;
+  }
+}
+// Every wave finds the same: the share of that number, false past the last.
+__device__ __forceinline__ bool find_share(const Args& g, int unit, Share& s) {
+  bool found = false;
+  scan_shares(g, [&](int e0, int n, int before, int sum, int all) {
+    if (unit >= before + all) return false;
+    const int l = __ffsll((unsigned long long)__ballot(before + sum > unit)) - 1;
+    const int ln = __shfl(n, l, 64), ls = __shfl(sum, l, 64);
+    s = Share{__builtin_amdgcn_readfirstlane(e0 + l), __builtin_amdgcn_readfirstlane(unit - (before + ls - ln)),
+              __builtin_amdgcn_readfirstlane(ln), __builtin_amdgcn_readfirstlane(before + ls - ln)};
+    return found = true;
+  });
+  return found;
+}
+__device__ __forceinline__ int count_shares(const Args& g) {
+  int total = 0;
+  scan_shares(g, [&](int, int, int before, int, int all) {
+    total = before + all;
+    return false;
+  });
+  return __builtin_amdgcn_readfirstlane(total);
+}
+
 // dw_in[e][m][n] = sum over expert e's positions of da[.][m] x[.][n]; dw_out[e][m][n] = that of dy[.][m] hw[.][n].
 // The matrix of the contiguous output index n is the MFMA's A operand; both are turned.
 // FEW: h's arrays lie by slot and the block finds the expert's slots itself.
@@ -454,11 +505,28 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   char* lb = lds + TT::BYTES;
   const int na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;   // columns of the operands
   const int ta = (na + BN - 1) / BN, tb = (nb + BN - 1) / BN;
-  // Workgroup w runs on XCD w % 8: every XCD takes a run of each expert's tiles, so that experts with many rows
-  // weigh on all of them
-  const int per = (ta * tb + 7) / 8, e = (int)(blockIdx.x >> 3) / per;
-  const int c = (int)(blockIdx.x & 7) * per + (int)(blockIdx.x >> 3) % per;
-  if (c >= ta * tb) return;
+  // Workgroup w runs on XCD w % 8.  With many tiles every XCD takes a run of each share's tiles, whatever the shares'
+  // sizes; with few a run of all tiles of all shares, which are then about equal.
+  const int tiles = ta * tb, w = (int)(blockIdx.x >> 3), x = (int)(blockIdx.x & 7);
+  Share sh;
+  int c;
+  if (FEW || g.M <= g.share) {                           // one share an expert
+    const int per = (tiles + 7) / 8;
+    sh = Share{w / per, 0, 1, 0};
+    c = x * per + w % per;
+    if (c >= tiles) return;
+  } else if (tiles >= MANY_TILES) {
+    const int per = (tiles + 7) / 8;
+    c = x * per + w % per;
+    if (c >= tiles || !find_share(g, w / per, sh)) return;
+  } else {
+    const int64_t all = (int64_t)count_shares(g) * tiles, per = (all + 7) / 8, i = x * per + w;
+    if (w >= per || i >= all) return;
+    const int unit = (int)(i / tiles);
+    c = (int)(i - (int64_t)unit * tiles);
+    if (!find_share(g, unit, sh)) return;
+  }
+  const int e = sh.e;
   const int b0 = (c / ta) * BN, a0 = (c % ta) * BN;
   __shared__ int16_t list[FEW ? FEW_SLOTS : 1];
   int64_t p0 = 0, cnt;
@@ -466,10 +534,8 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
     cnt = few_slots(g, e, few_first(g), list);
     __syncthreads();
   } else {
-    // the split's share of the expert's positions, in whole steps
-    const int64_t all = g.offsets[e + 1] - g.offsets[e], share = (all + g.splits * E::BK - 1) / (g.splits * E::BK) * E::BK;
-    p0 = g.offsets[e] + std::min<int64_t>(all, blockIdx.y * share);
-    cnt = std::min<int64_t>(share, g.offsets[e + 1] - p0);
+    p0 = g.offsets[e] + (int64_t)sh.at * g.share;
+    cnt = std::min<int64_t>(g.share, g.offsets[e + 1] - p0);
   }
   TT A;
   TB B;
@@ -551,25 +617,51 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
     if (out < 0) continue;
     const int len = MODE == DWIN ? g.H : g.F;
     S* dw = (S*)(MODE == DWIN ? g.dw_in : g.dw_out) + out;
-    float* part = g.dwsplit + blockIdx.y * ((int64_t)g.E * (MODE == DWIN ? 2 : 1) * g.F * g.H) + out;
+    // (out counts the experts before as well)
+    float* part = g.dwsplit + (sh.first + sh.at - e) * ((int64_t)(MODE == DWIN ? 2 : 1) * g.F * g.H) + out;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int n = a0 + (w0 + i) * 16 + 4 * q;
       if (n >= len) continue;
-      if (!FEW && g.splits > 1) store4(part + n, acc[i][j], len - n);
+      if (!FEW && sh.n > 1) store4(part + n, acc[i][j], len - n);
       else store4(dw + n, acc[i][j], len - n);
     }
   }
 }
 
-// A weight gradient from its splits, in their order.
+// The weight gradients (n entries an expert) of the experts with more than one share, in the shares' order; four entries
+// and four shares at a time are on their way together.  Blocks (., y) take every gridDim.y-th of these experts.
 template <typename S>
-__global__ __launch_bounds__(NT) void sum_splits_kernel(int64_t n, int splits, const float* __restrict__ part, S* __restrict__ dw) {
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT) {
-    float t = part[i];
-    for (int s = 1; s < splits; ++s) t += part[s * n + i];
-    dw[i] = from_f<S>(t);
-  }
+__global__ __launch_bounds__(NT) void sum_shares_kernel(Args g, int64_t n, S* __restrict__ dw) {
+  const int64_t step = (int64_t)gridDim.x * NT;
+  int turn = 0;
+  scan_shares(g, [&](int e0, int shares, int before, int sum, int) {
+    for (uint64_t some = __ballot(shares > 1); some; some &= some - 1) {
+      if (turn++ % gridDim.y != blockIdx.y) continue;
+      const int l = __ffsll((unsigned long long)some) - 1, k = __shfl(shares, l, 64);
+      const float* part = g.dwsplit + (int64_t)(before + __shfl(sum, l, 64) - k) * n;
+      S* out = dw + (e0 + l) * n;
+      for (int64_t i0 = (int64_t)blockIdx.x * NT + threadIdx.x; i0 < n; i0 += 4 * step) {
+        float t[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s0 = 0; s0 < k; s0 += 4) {
+          float v[4][4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) v[j][i] = part[min(s0 + j, k - 1) * n + min(i0 + i * step, n - 1)];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            if (s0 + j < k)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) t[i] += v[j][i];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (i0 + i * step < n) out[i0 + i * step] = from_f<S>(t[i]);
+      }
+    }
+    return false;
+  });
 }
 
 // ---------------------------------------------------------------- one pass over the rows of the caller's arrays
@@ -774,25 +866,35 @@ void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
   }
 }
 
-// Tiles of a weight gradient, and how many parts its positions are split into: so many that about 512 blocks run, of
-// at least 256 positions each on average.
+// Tiles of a weight gradient, and the positions of a share: so many that about 1,024 (fp32) or 512 tiles of shares run
+// whatever rows the experts have, of at least 128 (fp32: six products) or 256 positions, which outweigh writing and summing
+// them, and of 1,024 or 2,048 where the experts' tiles fill the chip without it and only the fullest experts are worth
+// dealing out.  Routing is uneven: 10,000 rows of 640, two of 16 experts, the fullest with three times the mean: forward
+// and all gradients 979 us against 1,553 with an expert's positions in one block (bf16 409 against 534).
 inline int64_t weight_tiles(int64_t na, int64_t nb) { return ((na + BN - 1) / BN) * ((nb + BN - 1) / BN); }
-inline int weight_splits(int64_t M, int E, int64_t tiles) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(16, 512 / (E * tiles)), M / E / 256));
+inline int weight_share(int64_t M, int E, int size, int64_t tiles) {
+  const int64_t least = (E * tiles >= 512 ? 1024 : 128) * (size == 4 ? 1 : 2);
+  const int64_t share = std::max(least, M * tiles / (size == 4 ? 1024 : 512));
+  return (int)std::min<int64_t>((share + 63) / 64 * 64, 1 << 30);
 }
+inline int64_t most_shares(int64_t M, int E, int share) { return M / share + E; }
+
+// bytes of a value of the arrays between the kernels
+template <int KIND> constexpr int held_bytes() { return sizeof(typename El<KIND>::T); }
 
 template <int KIND, typename S, int MODE, bool FEW = false>
 void launch_weights(Args g, bool vec, hipStream_t st) {
   const int64_t na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;
   const int64_t tiles = weight_tiles(na, nb);
-  g.splits = FEW ? 1 : weight_splits(g.M, g.E, tiles);
-  const dim3 grid((unsigned)(8 * g.E * ((tiles + 7) / 8)), g.splits);
+  g.share = FEW ? 0 : weight_share(g.M, g.E, held_bytes<KIND>(), tiles);
+  const int64_t shares = FEW ? g.E : most_shares(g.M, g.E, g.share);
+  const unsigned grid = (unsigned)(8 * (FEW || g.M <= g.share || tiles >= MANY_TILES ? shares * ((tiles + 7) / 8) : (shares * tiles + 7) / 8));
   if (vec) weights_kernel<KIND, S, MODE, true, FEW><<<grid, NT, 0, st>>>(g);
   else weights_kernel<KIND, S, MODE, false, FEW><<<grid, NT, 0, st>>>(g);
-  if (g.splits > 1) {
-    const int64_t n = (int64_t)g.E * (MODE == DWIN ? 2 : 1) * g.F * g.H;
-    sum_splits_kernel<S><<<(unsigned)std::min<int64_t>((n + NT - 1) / NT, 1 << 16), NT, 0, st>>>(
-        n, g.splits, g.dwsplit, (S*)(MODE == DWIN ? g.dw_in : g.dw_out));
+  if (!FEW && shares > g.E) {
+    const int64_t n = (int64_t)(MODE == DWIN ? 2 : 1) * g.F * g.H;
+    sum_shares_kernel<S><<<dim3((unsigned)std::min<int64_t>((n + 4 * NT - 1) / (4 * NT), 512), std::min(g.E, 8)), NT, 0, st>>>(
+        g, n, (S*)(MODE == DWIN ? g.dw_in : g.dw_out));
   }
 }
 
@@ -909,10 +1011,10 @@ inline Space backward_space(const FscExpertDims& d) {
   if (!few(M, d.n_experts)) {
     s.pad = at; at += pad_bytes(d, 2);
     // the two weight gradients use the same room, one after the other
-    const int64_t si = weight_splits(M, d.n_experts, weight_tiles(d.width, 2 * ldf));
-    const int64_t so = weight_splits(M, d.n_experts, weight_tiles(ldf, d.width));
-    const int64_t n = (int64_t)d.n_experts * d.hidden * d.width;
-    s.split = at; at += align64(std::max(si > 1 ? si * 2 * n : 0, so > 1 ? so * n : 0) * 4);
+    const int64_t si = most_shares(M, d.n_experts, weight_share(M, d.n_experts, (int)size, weight_tiles(d.width, 2 * ldf)));
+    const int64_t so = most_shares(M, d.n_experts, weight_share(M, d.n_experts, (int)size, weight_tiles(ldf, d.width)));
+    const int64_t n = (int64_t)d.hidden * d.width;
+    s.split = at; at += align64(std::max(si > d.n_experts ? si * 2 * n : 0, so > d.n_experts ? so * n : 0) * 4);
   }
   s.total = at;
   return s;
@@ -930,7 +1032,6 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
   g.k = d.k;
   g.li = d.width;
   g.lo = d.hidden;
-  g.splits = 1;
   g.k_inv = ((1u << 20) + d.k - 1) / d.k;
   if (!few(g.M, g.E)) {
     g.n_tiles = p.n_tiles;
