@@ -59,6 +59,9 @@ struct Raw {
   }
 };
 
+// 32 rows of 640, hidden 640, two of eight experts, fp32 (39 MB of weights, 9 us at a copy's rate, read once forward and once
+// backward): up 11.2, down 7.1, dh 11.8, dx 15.0 us; what bounds them is the chain index, weights, rows, LDS of a block.
+//
 // Whole steps of the reduction run without conditions: a lane past the last column or row reads the last one's
 // values, and what it computes is not stored.  The weights of a wave's first U steps are on their way before the
 // expert's slots are known.  Only the last, partial step looks at the bounds.
@@ -317,6 +320,8 @@ __device__ __forceinline__ i4v get16(const int8_t* p, int n) {
   return v;
 }
 
+// (32 rows of 640, hidden 640, two of eight experts: up 12.8, down 4.9 us for 10 MB of weights: a launch's time and the
+// chain of loads.)
 // up: a block an expert and a group of 128 hidden columns, a wave 16 of them (gate and up rows over all of K), so
 // the group's largest value is known in the block and h leaves it as codes.
 template <bool VEC>

@@ -10,10 +10,22 @@
 //     each output column's weights brought below 2^14 by a power of two of their own (from their largest magnitude,
 //     one pass before the products; h's and da's come from the products that make them) and the sums brought back
 //     exactly: 22 bits of every value down to 2^-17 of its row's largest, 2^-39 of that below;
-//   fp32 weight gradients: three bf16 parts and six products (split3, mfma_x6), 24 bits at any scale, since there the
-//     sum runs over rows of different scales.
+//   fp32 weight gradients, and all fp32 products where an expert has few rows: three bf16 parts and six products (split3,
+//     mfma_x6), 24 bits at any scale, since there the sum runs over rows of different scales, or a pass over the weights
+//     for their scales costs more than three products;
+//   bf16 rows where an expert has few: what is held between the kernels in fp32, its three bf16 parts against the weights
+//     as they are (three products; one where both operands are bf16).
 // The weights are the MFMA's A operand, the rows its B operand: a lane's four results are four neighbouring
 // columns of one row, stored by one access.
+//
+// Measured, us for all kernels of a call and what the products alone would take at a large library product's rate (1,125
+// TFLOP/s of 16-bit products): 10,000 x 640 fp32, hidden 640, two of eight experts, forward and rows' gradient 589 (262);
+// 16,384 x 1,600 bf16, hidden 800, two of 16, forward and all gradients 1,408 (671); 50,000 x 640 in 8 bits, hidden 1,280,
+// two of 16: 590 (219).  What bounds them is the step itself, a chain of loads, barrier, LDS and products in every block:
+// counters show the matrix units 40% busy, no other unit above 50%, half of a wave's time waiting for issue and a quarter
+// for loads.  Larger tiles (128 x 256; 256 x 256 with two LDS buffers), operands copied to LDS without registers or loaded
+// into them two or three steps ahead, four waves a SIMD, raised priorities in the products, and other orders of the tiles
+// took the same time or more.
 //
 // Rounding of what is held between the kernels: bf16 rows hold h, da and weight h in bf16 (each output passes one
 // such rounding and its own), or in fp32 where an expert has few rows; a, p and o stay in fp32.
@@ -39,7 +51,7 @@ constexpr int BN = 128;          // rows of the tile's weight operand
 // columns of padding and are read by ds_read_b64_tr_b16.
 constexpr int TRP = 128 + 16;
 
-template <int KIND, int ROWS, bool TR, typename T, int NT, int AHEAD = 1>
+template <int KIND, int ROWS, bool TR, typename T, int NT>
 struct Tile {                                                        // T: the type in memory
   using E = El<KIND>;
   static constexpr int CPR = E::BK / E::CE;                          // chunks of a straight row
@@ -52,7 +64,7 @@ struct Tile {                                                        // T: the t
   static constexpr int NV = E::CE * sizeof(T) / 16;                  // 16-byte parts of a chunk in memory
 
   struct Reg { u4v v[NV]; };
-  Reg reg[AHEAD][PER];                                               // AHEAD: steps on their way at once
+  Reg reg[PER];
   // F32: what the values are multiplied by, for each chunk (straight) or column of the thread's chunks (turned)
   static constexpr int NSC = KIND == F32 ? (TR ? 8 : PER) : 1;
   float scale[NSC];
@@ -62,33 +74,33 @@ struct Tile {                                                        // T: the t
   __device__ static constexpr int swz(int row) { return CPR == 4 ? (row >> 1) & 3 : row & 7; }
 
   // chunk c of the thread at byte off + more of a buffer (more the same for the wave), zeros outside it or with drop
-  __device__ __forceinline__ void fetch(int d, int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off, int more = 0, bool drop = false) {
+  __device__ __forceinline__ void fetch(int c, __amdgpu_buffer_rsrc_t rsrc, uint32_t off, int more = 0, bool drop = false) {
     const int o = (int)(drop ? kDropOffset : off);
 #pragma unroll
     for (int i = 0; i < NV; ++i)
-      reg[d][c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, o + 16 * i, more, 0));
+      reg[c].v[i] = __builtin_bit_cast(u4v, __builtin_amdgcn_raw_buffer_load_b128(rsrc, o + 16 * i, more, 0));
   }
   // chunk c of the thread from p (n values of it exist, the rest are zeros), of any alignment
-  __device__ __forceinline__ void fetch(int d, int c, const T* p, int n) {
+  __device__ __forceinline__ void fetch(int c, const T* p, int n) {
     alignas(16) T t[E::CE];
 #pragma unroll
     for (int i = 0; i < E::CE; ++i) t[i] = i < n ? p[i] : (T)0;
-    __builtin_memcpy(&reg[d][c], t, sizeof(t));
+    __builtin_memcpy(&reg[c], t, sizeof(t));
   }
-  // of step d's chunks, entries from `left` of the step's on become zeros (straight: along the reduction, where a row
+  // of the step's chunks, entries from `left` of the step's on become zeros (straight: along the reduction, where a row
   // ends inside a chunk and the loads have gone on into the next one)
-  __device__ __forceinline__ void cut(int d, int left) {
+  __device__ __forceinline__ void cut(int left) {
     static_assert(!TR);
     constexpr int EW = 4 / sizeof(T);                                // entries of a 32-bit word
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int l = left - chunk_of(threadIdx.x + i * NT) * E::CE;
 #pragma unroll
-      for (int w = 0; w < 4 * NV; ++w) reg[d][i].v[w / 4][w % 4] = w * EW < l ? reg[d][i].v[w / 4][w % 4] : 0;
+      for (int w = 0; w < 4 * NV; ++w) reg[i].v[w / 4][w % 4] = w * EW < l ? reg[i].v[w / 4][w % 4] : 0;
     }
   }
   // the thread's chunks into LDS
-  __device__ __forceinline__ void put(int d, char* lds) const {
+  __device__ __forceinline__ void put(char* lds) const {
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
       const int c = threadIdx.x + i * NT;
@@ -98,9 +110,9 @@ struct Tile {                                                        // T: the t
       if constexpr (KIND == F32 || KIND == X6 || PL == 3) {
         float v[8];
         if constexpr (sizeof(T) == 4) {
-          __builtin_memcpy(v, &reg[d][i], 32);
+          __builtin_memcpy(v, &reg[i], 32);
         } else {
-          const bf8 b = __builtin_bit_cast(bf8, reg[d][i].v[0]);
+          const bf8 b = __builtin_bit_cast(bf8, reg[i].v[0]);
 #pragma unroll
           for (int j = 0; j < 8; ++j) v[j] = (float)b[j];
         }
@@ -119,7 +131,7 @@ struct Tile {                                                        // T: the t
           *reinterpret_cast<bf8*>(lds + 2 * PLANE + at) = l;
         }
       } else {
-        *reinterpret_cast<u4v*>(lds + at) = reg[d][i].v[0];
+        *reinterpret_cast<u4v*>(lds + at) = reg[i].v[0];
       }
     }
   }
@@ -185,24 +197,32 @@ __device__ __forceinline__ int64_t whole_words(int n) { constexpr int w = 4 / si
 inline int64_t whole_chunks(int64_t n, int ce) { return (n + ce - 1) / ce * ce; }
 
 // ---------------------------------------------------------------- the products by row tiles
+// A block takes one tile: rows of one expert, read by their numbers (up, dh: the gather is the load), by columns.  Two
+// operands meet in LDS, double-buffered in registers, swizzled so that no read meets a bank twice; W_out and W_in of the
+// backward are turned by the transposing LDS reads.  The epilogues make h, da, dweight's parts and the codes from the sums in
+// registers, through LDS once into whole lines.  us at the sizes above (up, down, dh, dx): fp32 141, 86, 123, 158 (98, 49,
+// 49, 98 GFLOP of 16-bit products: 560 to 700 TFLOP/s, dh with 204 MB of a and da besides); bf16 233, 151, 191, 248 (168, 84,
+// 84, 168 GFLOP: 560 to 720 TFLOP/s, up with 210 MB of a, down and dx with 210 MB of o besides); 8 bits 311 and 200 (328
+// and 164 Gop; up's issue is half vector instructions: sigmoid, codes).
+//
 // up: 64 hidden columns a tile, their gate and up rows in turn by 16, so that a wave holds both of a column.
 // WW waves side by side along the weight operand, four (8-bit up: so many that 128 hidden columns make a tile)
-// 16-row tiles each, two along the rows.
+// 16-row tiles each, two along the rows.  Registers of 8-bit up are held to 128, so that two of its blocks of eight waves
+// share a CU (424 -> 333 us at 50,000 rows); those of fp32 dh to 168, three waves a SIMD (124 -> 118 us).
 template <int KIND, int MODE>
 constexpr int waves_w() { return KIND == I8 && MODE == UP ? 4 : 2; }
+template <int KIND, int MODE, bool VEC>                    // waves a SIMD that the registers leave room for
+constexpr int rows_waves() { return VEC && KIND == I8 && MODE == UP ? 4 : VEC && KIND == F32 && MODE == DH ? 3 : 2; }
 
 template <int KIND, typename S, int MODE, int NJ, bool VEC>
-__global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE == UP && VEC ? 4 : KIND == F32 && MODE == DH && VEC ? 3 : 2)) void rows_kernel(Args g) {
+__global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (rows_waves<KIND, MODE, VEC>())) void rows_kernel(Args g) {
   using E = El<KIND>;
   using T = typename E::T;                                   // of the arrays between the kernels; S: the caller's
   using R = std::conditional_t<MODE == DOWN || MODE == DX, T, S>;
   constexpr int BM = 32 * NJ, NI = 4, WW = waves_w<KIND, MODE>(), BN = 64 * WW, NT = 128 * WW;
   constexpr bool TR = MODE == DH || MODE == DX;
-  // one step of 128 rows is on its way during the products of another; with fewer rows a step's products are shorter
-  // than memory's answer, and more steps are
-  constexpr int AHEAD = !VEC || NJ == 4 ? 1 : NJ == 2 ? 2 : 3;
-  using TW = Tile<KIND, BN, TR, S, NT, AHEAD>;
-  using TX = Tile<KIND, BM, false, R, NT, AHEAD>;
+  using TW = Tile<KIND, BN, TR, S, NT>;
+  using TX = Tile<KIND, BM, false, R, NT>;
   // the operands; after the products the waves' rows and the sums across waves
   constexpr int OPERANDS = TW::BYTES + TX::BYTES, AFTER = (2 * WW * TURN + WW * BM) * 4;
   __shared__ __align__(16) char lds[OPERANDS > AFTER ? OPERANDS : AFTER];
@@ -293,7 +313,7 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE 
       tw.scale[i] = ldexpf(1.f, weight_exp(TR ? TW::chunk_of(threadIdx.x) * 8 + i : TW::row_of(threadIdx.x + i * NT)));
   }
   const int per_seg = (K + E::BK - 1) / E::BK, steps = SEG * per_seg;
-  auto fetch = [&](int d, int s) {
+  auto fetch = [&](int s) {
     const int seg = SEG == 2 && s >= per_seg, k0 = (s - seg * per_seg) * E::BK;
     const bool last = k0 + E::BK > K;                        // the same for the whole block
     const int64_t xat = seg * g.ldf + k0;
@@ -301,34 +321,34 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE 
     for (int i = 0; i < TX::PER; ++i) {
       const int left = KX - k0 - TX::chunk_of(threadIdx.x + i * NT) * E::CE;
       if constexpr (VEC) {
-        tx.fetch(d, i, xr, xo[i], (int)(xat * sizeof(R)), last && left <= 0);
+        tx.fetch(i, xr, xo[i], (int)(xat * sizeof(R)), last && left <= 0);
       } else {
-        tx.fetch(d, i, xbase + xo[i] + xat, xo[i] < 0 ? 0 : left);
+        tx.fetch(i, xbase + xo[i] + xat, xo[i] < 0 ? 0 : left);
       }
     }
     // turned: the buffer begins at row k0 of the segment and ends with it, rows past K are outside
     const int64_t wat = TR ? k0 * wld : k0;
     const __amdgpu_buffer_rsrc_t wr = buffer_rsrc_bytes(const_cast<S*>(wbase + seg * wseg + (TR ? wat : 0)),
-                                                        (uint32_t)(std::max<int64_t>(0, wseg - (TR ? wat : 0)) * sizeof(S)));
+                                                        (uint32_t)((wseg - (TR ? wat : 0)) * sizeof(S)));
 #pragma unroll
     for (int i = 0; i < TW::PER; ++i) {
       const int c = threadIdx.x + i * NT;
       const int left = TR ? K - k0 - TW::row_of(c) : K - k0 - TW::chunk_of(c) * E::CE;
       if constexpr (VEC) {
-        tw.fetch(d, i, wr, wo[i], TR ? 0 : (int)(wat * sizeof(S)), !TR && last && left <= 0);
+        tw.fetch(i, wr, wo[i], TR ? 0 : (int)(wat * sizeof(S)), !TR && last && left <= 0);
       } else {
         const int n = TR ? cols - n0 - TW::chunk_of(c) * 8 : left;
-        tw.fetch(d, i, wbase + seg * wseg + wo[i] + wat, wo[i] < 0 || left <= 0 ? 0 : n);
+        tw.fetch(i, wbase + seg * wseg + wo[i] + wat, wo[i] < 0 || left <= 0 ? 0 : n);
       }
     }
   };
 
   // (dx: da is padded and its reduction runs over W_in's rows)
-  auto trim = [&](int d, int s) {
+  auto trim = [&](int s) {
     if constexpr (VEC && MODE != DX) {
       if (K % E::CE == 0 || s + 1 < steps) return;
-      if constexpr (!TR) tw.cut(d, K - s * E::BK);
-      if constexpr (GATHER) tx.cut(d, K - s * E::BK);
+      if constexpr (!TR) tw.cut(K - s * E::BK);
+      if constexpr (GATHER) tx.cut(K - s * E::BK);
     }
   };
 
@@ -349,24 +369,25 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE 
       for (int j = 0; j < NJ; ++j) sum[i][j] = f4{0.f, 0.f, 0.f, 0.f};
     const int ng = g.ldf / QG;
     // the units, loaded before the operands of their step, since loads return in order; rows past the tile: the last's
-    float next[AHEAD][NJ];
-    auto units = [&](int d, int s) {
+    float next[NJ];
+    auto units = [&](int s) {
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
-        next[d][j] = g.hscale[(p0 + min(16 * (x0 + j) + r, rows - 1)) * ng + min(s, ng - 1)];
+      for (int j = 0; j < NJ; ++j) next[j] = g.hscale[(p0 + min(16 * (x0 + j) + r, rows - 1)) * ng + s];
     };
-    auto one = [&](int d, int s) {
-      trim(d, s);
+    units(0);
+    fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      trim(s);
       __syncthreads();
-      tw.put(d, lw);
-      tx.put(d, lx);
+      tw.put(lw);
+      tx.put(lx);
       __syncthreads();
       float u[NJ];
 #pragma unroll
-      for (int j = 0; j < NJ; ++j) u[j] = next[d][j];
-      if (AHEAD > 1 || s + AHEAD < steps) {
-        units(d, s + AHEAD);
-        fetch(d, s + AHEAD);
+      for (int j = 0; j < NJ; ++j) u[j] = next[j];
+      if (s + 1 < steps) {
+        units(s + 1);
+        fetch(s + 1);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
@@ -379,16 +400,7 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE 
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
           for (int v = 0; v < 4; ++v) sum[i][j][v] += (float)acc[i][j][v] * u[j];
-    };
-#pragma unroll
-    for (int d = 0; d < AHEAD; ++d) {
-      units(d, d);
-      fetch(d, d);
     }
-    for (int s = 0; s < steps; s += AHEAD)
-#pragma unroll
-      for (int d = 0; d < AHEAD; ++d)
-        if (s + d < steps) one(d, s + d);
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
       const int n = n0 + (w0 + i) * 16 + 4 * q;
@@ -402,21 +414,16 @@ __global__ __launch_bounds__((128 * waves_w<KIND, MODE>()), (KIND == I8 && MODE 
     finish<KIND, MODE, NI, NJ, WW, BM>(g, RowTile{e, rows, p0, slots, rws}, n0, ci, wave % WW, w0, x0, sum,
                                        reinterpret_cast<float*>(lds));
   } else {
-#pragma unroll
-    for (int d = 0; d < AHEAD; ++d) fetch(d, d);
-    for (int s = 0; s < steps; s += AHEAD)
-#pragma unroll
-      for (int d = 0; d < AHEAD; ++d) {
-        if (s + d >= steps) break;
-        trim(d, s + d);
-        __syncthreads();
-        tw.put(d, lw);
-        tx.put(d, lx);
-        __syncthreads();
-        // (past the last step: zeros; without a branch the wait for a step leaves the later ones on their way)
-        if (AHEAD > 1 || s + 1 < steps) fetch(d, s + d + AHEAD);
-        step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
-      }
+    fetch(0);
+    for (int s = 0; s < steps; ++s) {
+      trim(s);
+      __syncthreads();
+      tw.put(lw);
+      tx.put(lx);
+      __syncthreads();
+      if (s + 1 < steps) fetch(s + 1);
+      step<KIND, 4, NJ, TW, TX>(lw, lx, w0, x0, acc);
+    }
     if constexpr (KIND == F32) {
       const int r = lane & 15, q = lane >> 4;
       int xe[NJ];
@@ -490,7 +497,9 @@ __device__ __forceinline__ int count_shares(const Args& g) {
 }
 
 // dw_in[e][m][n] = sum over expert e's positions of da[.][m] x[.][n]; dw_out[e][m][n] = that of dy[.][m] hw[.][n].
-// The matrix of the contiguous output index n is the MFMA's A operand; both are turned.
+// The matrix of the contiguous output index n is the MFMA's A operand; both are turned.  The reduction runs over the rows,
+// whose numbers are loaded two steps ahead of their use, the rows themselves one step.  bf16 16,384 x 1,600, hidden 800:
+// 296 us dw_in, 184 us dw_out (570 and 460 TFLOP/s); fp32 4,099 x 331, hidden 203, with shares: 46 + 9 and 26 + 7 us.
 // FEW: h's arrays lie by slot and the block finds the expert's slots itself.
 template <int KIND, typename S, int MODE, bool VEC, bool FEW>
 __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
@@ -570,11 +579,11 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
       const bool gin = kr < left && ng < g.H, pin = kr < left && np < npc;
       auto load = [&](auto& gt, auto& pt) {
         if constexpr (VEC) {
-          gt.fetch(0, i, gr, gin ? (uint32_t)gat * (uint32_t)sizeof(S) : kDropOffset);
-          pt.fetch(0, i, pr, pin ? (uint32_t)pat * (uint32_t)sizeof(T) : kDropOffset);
+          gt.fetch(i, gr, gin ? (uint32_t)gat * (uint32_t)sizeof(S) : kDropOffset);
+          pt.fetch(i, pr, pin ? (uint32_t)pat * (uint32_t)sizeof(T) : kDropOffset);
         } else {
-          gt.fetch(0, i, gbase + gat, gin ? g.H - ng : 0);
-          pt.fetch(0, i, prow + pat, pin ? npc - np : 0);
+          gt.fetch(i, gbase + gat, gin ? g.H - ng : 0);
+          pt.fetch(i, prow + pat, pin ? npc - np : 0);
         }
       };
       if constexpr (MODE == DWIN) load(A, B);
@@ -595,8 +604,8 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   }
   for (int64_t k0 = 0; k0 < cnt; k0 += E::BK) {
     __syncthreads();
-    A.put(0, la);
-    B.put(0, lb);
+    A.put(la);
+    B.put(lb);
     __syncthreads();
     if (k0 + E::BK < cnt) {
       fetch(k0 + E::BK);
@@ -729,7 +738,8 @@ __global__ __launch_bounds__(NT) void pass_kernel(Pass a) {
   }
 }
 
-// Columns of an expert's matrix (R x n): 64 columns and 64 rows a block, raised in `out` [E][n], zeros before.
+// Columns of an expert's matrix (R x n): 64 columns and 64 rows a block, raised in `out` [E][n], zeros before.  One read of
+// the weights: 26 MB 6 us.
 template <typename S>
 __global__ __launch_bounds__(NT) void col_most_kernel(const S* __restrict__ w, int R, int n, uint32_t* __restrict__ out) {
   const int c = blockIdx.x * 64 + (threadIdx.x & 63), r0 = blockIdx.y * 64 + (threadIdx.x >> 6);
@@ -769,7 +779,9 @@ __device__ __forceinline__ void dweight_of(const Dweight& d, const int32_t* plac
   }
 }
 
-// Four slots' places, weights and products at a time are on their way together (a slot with none reads place 0).
+// y_t = sum_j weight_tj o_tj in the order of j, the same every time; o in 32 bits.  Four slots' places, weights and products
+// at a time are on their way together (a slot with none reads place 0).  Bound by memory: 16,384 x 1,600 bf16 from 210 MB of
+// o 45 us (5.8 TB/s), 50,000 x 640 57 us (5.6 TB/s).
 template <typename T>
 __global__ __launch_bounds__(NT) void combine_kernel(int64_t rows, int H, int ldo, int k,
                                                      const int32_t* __restrict__ place,
@@ -813,9 +825,14 @@ __global__ __launch_bounds__(NT) void dweight_kernel(Dweight d, const int32_t* _
 inline int up8(int v) { return (v + 7) / 8 * 8; }
 inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 
-// Few rows: at most 16 for each expert on average, and few enough slots for a block to look through.  The few-rows
-// kernels read an expert's weights once for 16 rows, the tiles once for up to 128.
-inline bool few(int64_t M, int E) { return M <= FEW_SLOTS && M <= 16 * (int64_t)E; }
+// Few rows: so few for each expert on average that reading the weights once, into registers, and no plan of the rows win
+// over the tiles' matrix products; and few enough slots for a block to look through.  Rows' step (8 bits: forward), us,
+// few against tiles, slots for each of eight experts: fp32 640 x 640 8: 72, 128; 38: 114, 131; 1,600 x 1,600 25: 292, 304.
+// bf16 640 8: 71, 75; 16: 81, 74; 1,600 12: 167, 143.  8 bits 640 8: 20, 22; 16: 25, 23; 1,600 12: 47, 36.
+inline bool few(const FscExpertDims& d) {
+  const int64_t M = d.rows * d.k;
+  return M <= FEW_SLOTS && M <= (d.dtype == FSC_F32 ? 32 : 8) * (int64_t)d.n_experts;
+}
 
 // Forward by dot products (expert_one.hip): eight slots, or no more than experts, so that hardly any weight is read twice.
 // Against the few-rows kernels, us, width and hidden 640, fp32 / bf16 / 8 bits: 2 slots 7.4 / 7.5 / 10.1 against 12.2 /
@@ -824,7 +841,9 @@ inline bool few(int64_t M, int E) { return M <= FEW_SLOTS && M <= 16 * (int64_t)
 inline bool one(int64_t M, int E) { return M <= 8 || (M <= FEW_SLOTS && M <= E); }
 
 // Rows of a tile: 128 only where the products have enough tiles of 128 x 128 to fill the chip a few times (M rows by
-// F + H columns, up and down alike), else more blocks with fewer rows.
+// F + H columns, up and down alike), else more blocks with fewer rows.  Forward and all gradients, us with 128, 64, 32 rows:
+// 1,024 tiles and more: 6,000 slots, 1,600 x 1,600, bf16 489, 576, 769; 625: 8,000 slots, 640 x 640, fp32 454, 455, 509, bf16
+// 211, 208, 220; 113: 1,371 slots, 949 x 406, fp32 371, 346, 326; 16: 270 slots, 872 x 95, fp32 153, 128, 116.
 inline int tile_rows(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, avg = M / d.n_experts, tiles = M * (d.width + d.hidden) / (128 * 128);
   return avg <= 32 || tiles < 224 ? 32 : avg <= 64 || tiles < 1024 ? 64 : 128;
@@ -956,7 +975,7 @@ inline int ldo_of(const FscExpertDims& d) { return (d.width + 3) / 4 * 4; }
 // kernels stays in fp32 and the products run as those of fp32 rows do.
 inline bool fine(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k;
-  return d.dtype == FSC_BF16 && (few(M, d.n_experts) || M <= 32 * (int64_t)d.n_experts);
+  return d.dtype == FSC_BF16 && (few(d) || M <= 32 * (int64_t)d.n_experts);
 }
 // bytes of a value of the arrays between the kernels
 inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 : d.dtype == FSC_F32 || fine(d) ? 4 : 2; }
@@ -966,9 +985,11 @@ struct Space {
   int64_t h, o, da, hw, part, hs, most, split, pad, total;
 };
 // fp32 rows by tiles: two scaled parts an operand (three products, and one pass over the weights for their scales), or
-// three parts (six products, no pass) where an expert has so few rows that the weights' bytes count for more.
+// three parts (six products, no pass) where an expert has so few rows that the weights' bytes count for more.  Forward and
+// all gradients of 640 x 640, us with two and three parts: 38 rows for each expert 193, 181; 62: 203, 191; 100: 241, 245; 250:
+// 339, 364.
 inline bool parts(const FscExpertDims& d) {
-  return !few(d.rows * d.k, d.n_experts) && d.dtype == FSC_F32 && d.rows * d.k > 80 * (int64_t)d.n_experts;
+  return !few(d) && d.dtype == FSC_F32 && d.rows * d.k > 80 * (int64_t)d.n_experts;
 }
 // Room for padded copies of x (or x and dy: their strides and addresses are not known here) and of weights with odd rows;
 // fp32 rows are always whole words.
@@ -991,7 +1012,7 @@ inline Space forward_space(const FscExpertDims& d) {
   if (d.dtype == FSC_I8) {
     s.hs = at; at += align64(M * (ldf / QG) * 4);
   }
-  if (!few(M, d.n_experts)) {
+  if (!few(d)) {
     s.pad = at; at += pad_bytes(d, 1);
   }
   s.total = at;
@@ -1008,7 +1029,7 @@ inline Space backward_space(const FscExpertDims& d) {
   if (parts(d)) {
     s.most = at; at += align64((d.rows + M + (int64_t)d.n_experts * (d.hidden + d.width)) * 4);
   }
-  if (!few(M, d.n_experts)) {
+  if (!few(d)) {
     s.pad = at; at += pad_bytes(d, 2);
     // the two weight gradients use the same room, one after the other
     const int64_t si = most_shares(M, d.n_experts, weight_share(M, d.n_experts, (int)size, weight_tiles(d.width, 2 * ldf)));
@@ -1033,7 +1054,7 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
   g.li = d.width;
   g.lo = d.hidden;
   g.k_inv = ((1u << 20) + d.k - 1) / d.k;
-  if (!few(g.M, g.E)) {
+  if (!few(d)) {
     g.n_tiles = p.n_tiles;
     g.offsets = p.offsets;
     g.slot_of = p.slot_of;
@@ -1134,7 +1155,7 @@ int fsc_expert_sizes(const FscExpertDims* dims, int64_t* plan_ints, int64_t* sav
   if (int rc = check_dims(dims, dims && dims->dtype == FSC_I8)) return rc;
   FSC_CHECK_ARG(plan_ints && saved_floats && forward_bytes && backward_bytes, "expert_sizes: null output");
   const int64_t M = dims->rows * dims->k;
-  *plan_ints = few(M, dims->n_experts) ? 0 : fsc::experts::plan_ints(M, dims->n_experts, tile_rows(*dims));
+  *plan_ints = few(*dims) ? 0 : fsc::experts::plan_ints(M, dims->n_experts, tile_rows(*dims));
   *saved_floats = dims->dtype == FSC_I8 ? 0 : M * 2 * ldf_of(*dims);
   *forward_bytes = forward_space(*dims).total;
   *backward_bytes = dims->dtype == FSC_I8 ? 0 : backward_space(*dims).total;
@@ -1145,7 +1166,7 @@ int fsc_expert_plan(const FscExpertDims* dims, const int32_t* index, int32_t* pl
   using namespace fsc::experts;
   if (int rc = check_dims(dims, dims && dims->dtype == FSC_I8)) return rc;
   const int64_t M = dims->rows * dims->k;
-  if (few(M, dims->n_experts)) return 0;       // the products find their rows themselves
+  if (few(*dims)) return 0;       // the products find their rows themselves
   FSC_CHECK_ARG(plan && index, "expert_plan: null array");
   const int tile = tile_rows(*dims);
   launch_plan(plan_of(plan, M, dims->n_experts, tile), M, dims->n_experts, dims->k, tile, index, stream);
@@ -1159,7 +1180,7 @@ int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const vo
   if (int rc = check_dims(dims, false)) return rc;
   if (dims->rows == 0) return 0;
   const int64_t M = dims->rows * dims->k;
-  FSC_CHECK_ARG(x && index && (plan || few(M, dims->n_experts)) && weight && w_in && w_out && workspace && y,
+  FSC_CHECK_ARG(x && index && (plan || few(*dims)) && weight && w_in && w_out && workspace && y,
                 "expert_mlp_forward: null array");
   FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_forward: negative row stride");
   const int tile = tile_rows(*dims);
@@ -1191,7 +1212,7 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
   using namespace fsc::experts;
   if (int rc = check_dims(dims, false)) return rc;
   const int64_t M = dims->rows * dims->k;
-  FSC_CHECK_ARG((plan || few(M, dims->n_experts)) && w_in && w_out, "expert_mlp_backward: null array");
+  FSC_CHECK_ARG((plan || few(*dims)) && w_in && w_out, "expert_mlp_backward: null array");
   FSC_CHECK_ARG(M == 0 || (dy && x && index && weight && saved && workspace), "expert_mlp_backward: null array");
   FSC_CHECK_ARG(x_stride >= 0 && dy_stride >= 0, "expert_mlp_backward: negative row stride");
   const int tile = tile_rows(*dims);
@@ -1242,7 +1263,7 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
   if (int rc = check_dims(dims, true)) return rc;
   if (dims->rows == 0) return 0;
   const int64_t M = dims->rows * dims->k;
-  FSC_CHECK_ARG(x && x_scale && index && (plan || few(M, dims->n_experts)) && weight && w_in && w_in_scale && w_out && w_out_scale && workspace && y,
+  FSC_CHECK_ARG(x && x_scale && index && (plan || few(*dims)) && weight && w_in && w_in_scale && w_out && w_out_scale && workspace && y,
                 "expert_mlp_q8: null array");
   FSC_CHECK_ARG(x_stride >= 0, "expert_mlp_q8: negative row stride");
   const int tile = tile_rows(*dims);

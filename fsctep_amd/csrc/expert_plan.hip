@@ -8,6 +8,9 @@
 //   tiles   [2 n]     (expert, first sorted position) of each tile of `tile` rows, expert -1 past the last one
 //                     (n = ceil(M / tile) + min(E, M) bounds their number)
 //   counts  [blocks E] rows of each expert before each block of slots, with many slots
+//
+// Bound by latency (4 bytes in, 16 out for each slot): up to 4,096 slots one launch, 3 to 5 us; above that three, 15 us at
+// 20,000 slots and 20 us at 100,000 (one block alone: 33 and 146 us).
 #include <algorithm>
 
 #include "common.h"

@@ -9,6 +9,10 @@
 // across them are four DPP steps, "the lowest expert" is the lowest lane of a ballot, and the work of a round of
 // the selection is spread over four rows.  Reads T E logits, writes 8 T k bytes.  The softmax's sum runs in 64
 // bits and is rounded once, so that no choice hangs on the order of its terms.
+//
+// Measured: 100,000 x 256 fp32, sigmoid with a bias, 4 of 8 groups, k = 8: 72 us forward (109 MB: 25 us at a copy's
+// rate; what bounds it is the issue of the selection's k rounds and the groups' ranks), 40 us backward (211 MB,
+// 5.3 TB/s); 32 x 8: 2.7 us, a launch.
 #include <cmath>
 
 #include "common.h"
@@ -142,7 +146,8 @@ __device__ __forceinline__ float score_of(float l, float m, float total) {
 // The value of the lane s places further round in the row (s the same for all): a step of a loop.
 __device__ __forceinline__ float next_lane(float v) { return ror<1>(v); }
 
-// group_lanes: lanes of a group where groups lie in whole lanes that part the row's 16, so that ranks stay in registers;
+// A round: the largest of the row's remaining c (four DPP steps), the lowest lane that has it (a ballot), which writes
+// the choice and drops it.  group_lanes: lanes of a group where groups lie in whole lanes that part the row's 16, so that ranks stay in registers;
 // 0: through LDS.
 template <typename T, int V, bool SOFTMAX>
 __global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec, int group_lanes) {

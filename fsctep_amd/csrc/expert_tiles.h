@@ -169,17 +169,24 @@ __device__ __forceinline__ void finish(const Args& g, const RowTile& t, int n0, 
       if (q == 0) reinterpret_cast<uint32_t*>(red)[wn * BM + row] = top[j];
     }
     __syncthreads();
+    // a row's 128 codes are one line: through LDS, so that eight lanes store it
+    constexpr int LD = QG + 16;
+    int8_t* const line = reinterpret_cast<int8_t*>(buf);
 #pragma unroll
     for (int j = 0; j < NJ; ++j) {
       const int row = 16 * (x0 + j) + r;
 #pragma unroll
       for (int w = 0; w < WW; ++w) top[j] = max(top[j], reinterpret_cast<const uint32_t*>(red)[w * BM + row]);
-      if (row >= t.rows) continue;
       const float most = __uint_as_float(top[j]), inv = most > 0.f ? 127.f / most : 0.f;
 #pragma unroll
       for (int i = 0; i < NI / 2; ++i)
-        *reinterpret_cast<uint32_t*>((int8_t*)g.h + (t.p0 + row) * g.ldf + n0 + (w0 / 2 + i) * 16 + 4 * q) = codes4(h[i][j], inv);
-      if (wn == 0 && q == 0) g.hscale[(t.p0 + row) * (g.ldf / QG) + n0 / QG] = most / 127.f;
+        *reinterpret_cast<uint32_t*>(line + row * LD + (w0 / 2 + i) * 16 + 4 * q) = codes4(h[i][j], inv);
+      if (wn == 0 && q == 0 && row < t.rows) g.hscale[(t.p0 + row) * (g.ldf / QG) + n0 / QG] = most / 127.f;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.rows * (QG / 16); i += blockDim.x) {
+      const int row = i / (QG / 16), c = i % (QG / 16) * 16;
+      *reinterpret_cast<u4v*>((int8_t*)g.h + (t.p0 + row) * g.ldf + n0 + c) = *reinterpret_cast<const u4v*>(line + row * LD + c);
     }
   } else if constexpr (MODE == UP) {
     using U = Turned<NI / 2>;

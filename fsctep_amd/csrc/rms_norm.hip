@@ -9,6 +9,10 @@
 // The sum of squares runs in 64 bits (a square of a float is exact there) and the root is rounded to 32 bits once,
 // so rstd, and with it every 8-bit code, is the same for any order of the sum.  At the sizes here the 64-bit
 // operations hide behind the loads.
+//
+// Measured (a copy of this size moves 4.4 TB/s; smaller arrays come in part from the last-level cache): 100,000 x 640
+// bf16 with a residual 91 us forward (512 MB, 5.6 TB/s) and 108 us backward (512 MB, 4.7 TB/s) with 5 us for the
+// weight's gradient; 10,007 x 1,600 bf16 to codes 25 us (112 MB, 4.4 TB/s); 32 x 640 3.7 us, a launch.
 #include <algorithm>
 
 #include "common.h"
@@ -51,7 +55,8 @@ __device__ __forceinline__ int8_t code_of(float y, float inv) {
   return c >= -127.f && c <= 127.f ? (int8_t)c : (int8_t)0;
 }
 
-// One wave a row; lane l holds the chunks l, l + 64, .. of V values each (CH of them).
+// One wave a row; lane l holds the chunks l, l + 64, .. of V values each (CH of them): 16 bytes a lane and load, a row
+// read once.  Figures: top of the file.
 template <typename T, typename W, int V, int CH, bool Q8>
 __global__ __launch_bounds__(NT) void row_kernel(Args a) {
   const int64_t row = (int64_t)blockIdx.x * (NT / 64) + (threadIdx.x >> 6);
@@ -136,7 +141,8 @@ __device__ __forceinline__ double block_sum64(double v, double* red) {
   return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-// One block a row, any width and alignment: the row is read from memory once and from the caches again.
+// One block a row, any width and alignment: the row is read from memory once and from the caches again.  For rows that
+// a wave's registers do not hold (above 2,048 values, unaligned rows too): 2 x 5,000 takes a launch's time.
 template <typename T, typename W, bool Q8>
 __global__ __launch_bounds__(NT) void wide_kernel(Args a) {
   __shared__ double red[NT / 64];
@@ -185,7 +191,10 @@ struct BackArgs {
   float* part;                   // [gridDim.x][width] partial dw, or null
 };
 
-// NARROW: at most 64 columns.
+// dx = rstd (w dy - zhat mean(w dy zhat)) + dz, dweight = sum over rows of dy zhat (zhat = z rstd).  A wave takes every
+// gridDim.x * 4-th row and keeps its part of dweight in registers, so that a block writes one partial row.  NARROW: at most 64 columns, where dx is a
+// difference of nearly equal numbers (exactly zero at one column) and is formed in 64 bits; the other instance does not
+// carry those registers.
 template <typename T, typename W, int V, int CH, bool NARROW>
 __global__ __launch_bounds__(NT) void row_back_kernel(BackArgs a) {
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -319,7 +328,8 @@ __global__ __launch_bounds__(NT) void wide_back_kernel(BackArgs a) {
     for (int i = threadIdx.x; i < a.width; i += NT) part[i] = 0.f;
 }
 
-// dw[c] = sum over the blocks' partial rows: 32 columns a block, 32 threads a column, then a fixed tree.
+// dw[c] = sum over the blocks' partial rows: 32 columns a block, 32 threads a column, then a fixed tree (the same sum
+// every time).  1,024 x 640 partial sums: 5 us, in part the launch.
 template <typename W>
 __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ part, int n, int width, W* __restrict__ dw) {
   __shared__ float red[32][33];
@@ -335,8 +345,8 @@ __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ par
 }
 
 // Blocks of the backward: enough waves to fill the chip, few enough that the partial rows stay small beside the
-// rows themselves.
-inline int back_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 2048)); }
+// rows themselves (100,000 x 640 bf16, forward and backward with 512, 1,024, 2,048, 4,096 blocks: 252, 199, 208, 223 us).
+inline int back_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1024)); }
 
 inline bool aligned(const void* p, int64_t stride, int size, int vec) {
   return !p || ((uintptr_t)p % (size * vec) == 0 && stride % vec == 0);
