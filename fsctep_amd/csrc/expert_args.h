@@ -46,7 +46,7 @@ template <typename S>
 void few_launch(int mode, const Args& g, bool vec, hipStream_t st);
 // Columns of dh that share a partial dweight there.
 int few_parts(int F, int size);
-// Few rows in 8 bits: up (codes of h) and down.
+// Few rows in 8 bits: up (h in 32 bits) and down (from its codes).
 void few_launch_q8(const Args& g, bool vin, bool vout, hipStream_t st);
 // A handful of slots (expert_one.hip): up, down and the rows from their experts.
 template <typename S>

@@ -320,32 +320,30 @@ __device__ __forceinline__ i4v get16(const int8_t* p, int n) {
   return v;
 }
 
-// (32 rows of 640, hidden 640, two of eight experts: up 12.8, down 4.9 us for 10 MB of weights: a launch's time and the
-// chain of loads.)
-// up: a block an expert and a group of 128 hidden columns, a wave 16 of them (gate and up rows over all of K), so
-// the group's largest value is known in the block and h leaves it as codes.
+// up: a block an expert and 16 hidden columns, gate and up rows; its waves split the reduction and meet in LDS as whole
+// numbers.  h stays in 32 bits here: its codes need the largest value of 128 columns, which no block holds (blocks of whole
+// groups, a tenth as many, took 12 us where this takes 4.9 at 32 rows of 640, hidden 640, two of eight experts).
 template <bool VEC>
-__global__ __launch_bounds__(FT) void few_up_q8_kernel(Args g) {
+__global__ __launch_bounds__(256) void few_up_q8_kernel(Args g) {
   __shared__ int16_t list[FEW_SLOTS];
-  __shared__ uint32_t tops[FW][16];
-  const int ng = g.ldf / QG, grp = blockIdx.x;
-  const int e = few_expert(g, blockIdx.y);
+  __shared__ i4v red[4][2][64];
+  const int e = few_expert(g, blockIdx.y), n0 = blockIdx.x * 16;
   if (e < 0) return;
   const int first = few_first(g);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
-  const int nr = grp * QG + wave * 16 + r, n = grp * QG + wave * 16 + 4 * q;
-  const int8_t* wg = (const int8_t*)g.w_in + ((int64_t)e * 2 * g.F + min(nr, g.F - 1)) * g.H;
+  const int n = n0 + 4 * q;
+  const int8_t* wg = (const int8_t*)g.w_in + ((int64_t)e * 2 * g.F + min(n0 + r, g.F - 1)) * g.H;
   const int64_t up = (int64_t)g.F * g.H;
   // the first U steps' weights and the columns' scales (a column past the last: the last one's), before the slots
   // are known
-  constexpr int U = VEC ? 10 : 1;
+  constexpr int U = VEC ? 4 : 1;
   const int whole = g.H / 64;
   Raw<16, VEC> a[U], b[U];
   auto load_chunk = [&](int s0) {
 #pragma unroll
     for (int u = 0; u < U; ++u)
-      if (s0 + u < whole) {
-        const int k = (s0 + u) * 64 + 16 * q;
+      if (wave + 4 * (s0 + u) < whole) {
+        const int k = (wave + 4 * (s0 + u)) * 64 + 16 * q;
         a[u].load(wg + k);
         b[u].load(wg + up + k);
       }
@@ -371,72 +369,99 @@ __global__ __launch_bounds__(FT) void few_up_q8_kernel(Args g) {
       ag = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, xv, ag, 0, 0, 0);
       au = __builtin_amdgcn_mfma_i32_16x16x64_i8(b, xv, au, 0, 0, 0);
     };
-    for (int s0 = 0; s0 < whole; s0 += U) {
+    for (int s0 = 0; wave + 4 * s0 < whole; s0 += U) {
       Raw<16, VEC> xv[U];
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (s0 + u < whole) xv[u].load(x + (s0 + u) * 64 + 16 * q);
-      if (s0 > 0 || (t0 > 0 && U < whole)) load_chunk(s0);
+        if (wave + 4 * (s0 + u) < whole) xv[u].load(x + (wave + 4 * (s0 + u)) * 64 + 16 * q);
+      if (s0 > 0 || (t0 > 0 && wave + 4 * U < whole)) load_chunk(s0);
 #pragma unroll
       for (int u = 0; u < U; ++u)
-        if (s0 + u < whole) mul(__builtin_bit_cast(i4v, a[u]), __builtin_bit_cast(i4v, b[u]), __builtin_bit_cast(i4v, xv[u]));
+        if (wave + 4 * (s0 + u) < whole)
+          mul(__builtin_bit_cast(i4v, a[u]), __builtin_bit_cast(i4v, b[u]), __builtin_bit_cast(i4v, xv[u]));
     }
-    if (whole * 64 < g.H) {
+    if (wave == 3 && whole * 64 < g.H) {
       const int k = whole * 64 + 16 * q, n16 = g.H - k;
       mul(get16<VEC>(wg + k, n16), get16<VEC>(wg + up + k, n16), get16<VEC>(x + k, n16));
     }
-    f4 h;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float ga = n + j < g.F ? (float)ag[j] * (xs * sg[j]) : 0.f;
-      const float u = n + j < g.F ? (float)au[j] * (xs * su[j]) : 0.f;
-      h[j] = ga * sigmoid(ga) * u;
-    }
-    uint32_t top = most4(h);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
-    __syncthreads();                                   // the last tile's maxima have been read
-    if (q == 0) tops[wave][r] = top;
+    __syncthreads();                                   // the last tile's sums have been read
+    red[wave][0][lane] = ag;
+    red[wave][1][lane] = au;
     __syncthreads();
+    if (wave == 0 && live) {
+      ag = (red[0][0][lane] + red[1][0][lane]) + (red[2][0][lane] + red[3][0][lane]);
+      au = (red[0][1][lane] + red[1][1][lane]) + (red[2][1][lane] + red[3][1][lane]);
+      f4 h;
 #pragma unroll
-    for (int w = 0; w < FW; ++w) top = max(top, tops[w][r]);
-    const float most = __uint_as_float(top), inv = most > 0.f ? 127.f / most : 0.f;
-    if (live) {
-      *reinterpret_cast<uint32_t*>((int8_t*)g.h + (int64_t)slot * g.ldf + n) = codes4(h, inv);
-      if (wave == 0 && q == 0) g.hscale[(int64_t)slot * ng + grp] = most / 127.f;
+      for (int j = 0; j < 4; ++j) {
+        const float ga = (float)ag[j] * (xs * sg[j]), u = (float)au[j] * (xs * su[j]);
+        h[j] = n + j < g.F ? ga * sigmoid(ga) * u : 0.f;
+      }
+      st4((float*)g.h + (int64_t)slot * g.ldf + n, h);
     }
   }
 }
 
-// down: a block an expert and 16 columns, the groups of h dealt to its waves.
+// down: a block an expert and 16 columns, the groups of h dealt to its waves.  Lane (r, q) makes the codes of its 32 values
+// of slot r's group, which are its part of the matrix operand.  32 rows of 640, hidden 640: 6.2 us.
 template <bool VEC>
-__global__ __launch_bounds__(256) void few_down_q8_kernel(Args g) {
+__global__ __launch_bounds__(FT) void few_down_q8_kernel(Args g) {
   __shared__ int16_t list[FEW_SLOTS];
-  __shared__ f4 red[4][64];
+  __shared__ f4 red[FW][64];
   const int n0 = blockIdx.x * 16, ng = g.ldf / QG;
   const int e = few_expert(g, blockIdx.y);
   if (e < 0) return;
-  const int cnt = few_slots(g, e, few_first(g), list);
-  if (cnt == 0) return;
-  __syncthreads();
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
+  const int first = few_first(g);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, r = lane & 15, q = lane >> 4;
   const int8_t* w = (const int8_t*)g.w_out + ((int64_t)e * g.H + min(n0 + r, g.H - 1)) * g.F;
   const int n = n0 + 4 * q;
+  // the first group's weights and the columns' scales, before the slots are known
+  i4v a[2];
+  auto weights = [&](int grp) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      const int k = grp * QG + 64 * s + 16 * q;
+      a[s] = get16<VEC>(w + k, g.F - k);
+    }
+  };
+  weights(wave);
+  f4 scale;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) scale[j] = g.out_scale[(int64_t)e * g.H + min(n + j, g.H - 1)];
+  const int cnt = few_slots(g, e, first, list);
+  if (cnt == 0) return;
+  __syncthreads();
   for (int t0 = 0; t0 < cnt; t0 += 16) {
     const bool live = t0 + r < cnt;
     const int slot = list[live ? t0 + r : 0];
-    const int8_t* h = (const int8_t*)g.h + (int64_t)slot * g.ldf;
+    const float* h = (const float*)g.h + (int64_t)slot * g.ldf;
     f4 sum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-    for (int grp = wave; grp < ng; grp += 4) {
-      i4v acc = {0, 0, 0, 0};
+    for (int grp = wave; grp < ng; grp += FW) {
+      f4 v[2][4];
+      uint32_t top = 0;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const int k = grp * QG + 64 * s + 16 * q;
-        const i4v a = get16<VEC>(w + k, g.F - k), b = get16<true>(h + k, 16);
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[s][j] = ld4(h + k + 4 * j);
       }
-      const float u = g.hscale[(int64_t)slot * ng + grp];
+      if (grp != wave || (t0 > 0 && ng > FW)) weights(grp);   // else the first group's are still there
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top = max(top, most4(v[s][j]));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 16, 64));
+      top = max(top, (uint32_t)__shfl_xor((int)top, 32, 64));
+      const float most = __uint_as_float(top), inv = most > 0.f ? 127.f / most : 0.f;
+      i4v acc = {0, 0, 0, 0};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        i4v b;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) b[j] = (int)codes4(v[s][j], inv);
+        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[s], b, acc, 0, 0, 0);
+      }
+      const float u = most / 127.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) sum[j] += (float)acc[j] * u;
     }
@@ -444,20 +469,21 @@ __global__ __launch_bounds__(256) void few_down_q8_kernel(Args g) {
     red[wave][lane] = sum;
     __syncthreads();
     if (wave == 0 && live) {
-      sum = (red[0][lane] + red[1][lane]) + (red[2][lane] + red[3][lane]);
+      f4 t[FW];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sum[j] *= g.out_scale[(int64_t)e * g.H + min(n + j, g.H - 1)];
+      for (int u = 0; u < FW; ++u) t[u] = red[u][lane];
+      sum = (((t[0] + t[1]) + (t[2] + t[3])) + ((t[4] + t[5]) + (t[6] + t[7]))) * scale;
       store4(g.o + (int64_t)slot * g.ldo + n, sum, g.H - n);
     }
   }
 }
 
 void few_launch_q8(const Args& g, bool vin, bool vout, hipStream_t st) {
-  const dim3 up(g.ldf / QG, few_blocks(g)), down((g.H + 15) / 16, few_blocks(g));
-  if (vin) few_up_q8_kernel<true><<<up, FT, 0, st>>>(g);
-  else few_up_q8_kernel<false><<<up, FT, 0, st>>>(g);
-  if (vout) few_down_q8_kernel<true><<<down, 256, 0, st>>>(g);
-  else few_down_q8_kernel<false><<<down, 256, 0, st>>>(g);
+  const dim3 up(g.ldf / 16, few_blocks(g)), down((g.H + 15) / 16, few_blocks(g));
+  if (vin) few_up_q8_kernel<true><<<up, 256, 0, st>>>(g);
+  else few_up_q8_kernel<false><<<up, 256, 0, st>>>(g);
+  if (vout) few_down_q8_kernel<true><<<down, FT, 0, st>>>(g);
+  else few_down_q8_kernel<false><<<down, FT, 0, st>>>(g);
 }
 
 }  // namespace experts

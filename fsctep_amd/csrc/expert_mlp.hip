@@ -828,10 +828,10 @@ inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 // Few rows: so few for each expert on average that reading the weights once, into registers, and no plan of the rows win
 // over the tiles' matrix products; and few enough slots for a block to look through.  Rows' step (8 bits: forward), us,
 // few against tiles, slots for each of eight experts: fp32 640 x 640 8: 72, 128; 38: 114, 131; 1,600 x 1,600 25: 292, 304.
-// bf16 640 8: 71, 75; 16: 81, 74; 1,600 12: 167, 143.  8 bits 640 8: 20, 22; 16: 25, 23; 1,600 12: 47, 36.
+// bf16 640 8: 71, 75; 16: 81, 74; 1,600 12: 167, 143.  8 bits 640 16: 19, 23; 25: 24, 22; 1,600 8: 28, 36; 12: 37, 37.
 inline bool few(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k;
-  return M <= FEW_SLOTS && M <= (d.dtype == FSC_F32 ? 32 : 8) * (int64_t)d.n_experts;
+  return M <= FEW_SLOTS && M <= (d.dtype == FSC_F32 ? 32 : d.dtype == FSC_I8 ? 16 : 8) * (int64_t)d.n_experts;
 }
 
 // Forward by dot products (expert_one.hip): eight slots, or no more than experts, so that hardly any weight is read twice.
@@ -978,7 +978,9 @@ inline bool fine(const FscExpertDims& d) {
   return d.dtype == FSC_BF16 && (few(d) || M <= 32 * (int64_t)d.n_experts);
 }
 // bytes of a value of the arrays between the kernels
-inline int64_t held_size(const FscExpertDims& d) { return d.dtype == FSC_I8 ? 1 : d.dtype == FSC_F32 || fine(d) ? 4 : 2; }
+inline int64_t held_size(const FscExpertDims& d) {
+  return d.dtype == FSC_I8 ? few(d) ? 4 : 1 : d.dtype == FSC_F32 || fine(d) ? 4 : 2;   // (few: h before its codes)
+}
 
 // Parts of a workspace, in bytes.
 struct Space {
