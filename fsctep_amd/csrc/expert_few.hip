@@ -21,7 +21,9 @@ namespace experts {
 constexpr int FT = 512;             // eight waves
 constexpr int FW = FT / 64;
 
-// B bytes from p, by 16- or 8-byte loads where ALIGNED
+// B bytes from p, by 16- or 8-byte loads where ALIGNED (to four bytes)
+typedef unsigned u4w __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u2w __attribute__((ext_vector_type(2), aligned(4)));
 template <int B, bool ALIGNED>
 struct Raw {
   uint32_t v[B / 4];
@@ -30,11 +32,11 @@ struct Raw {
     if constexpr (ALIGNED && B % 16 == 0) {
 #pragma unroll
       for (int i = 0; i < B / 16; ++i) {
-        const u4v t = *(reinterpret_cast<const u4v*>(p) + i);
+        const u4w t = *(reinterpret_cast<const u4w*>(p) + i);
         v[4 * i] = t.x; v[4 * i + 1] = t.y; v[4 * i + 2] = t.z; v[4 * i + 3] = t.w;
       }
     } else if constexpr (ALIGNED) {
-      const u2v t = *reinterpret_cast<const u2v*>(p);
+      const u2w t = *reinterpret_cast<const u2w*>(p);
       v[0] = t.x; v[1] = t.y;
     } else {
       T t[B / sizeof(T)];
@@ -93,7 +95,8 @@ __global__ __launch_bounds__(FT, MODE == UP || MODE == DOWN ? 4 : 2) void few_ke
   const int K = MODE == UP || MODE == DH ? g.H : g.F;
   const int whole = K / STEP, steps = PARTS * whole;
   const int n = n0 + (ALONG ? r : CE * r);
-  const int nc = ALONG ? min(n, cols - 1) : VEC ? min(n, cols - CE) : n;
+  // (a lane whose columns reach past the last one reads on into the next row, zeros past the matrix: not stored)
+  const int nc = ALONG ? min(n, cols - 1) : VEC && n >= cols ? cols - CE : n;
   const S* wbase = MODE == UP ? (const S*)g.w_in + ((int64_t)e * 2 * g.F + nc) * g.H
                    : MODE == DOWN ? (const S*)g.w_out + ((int64_t)e * g.H + nc) * g.F
                    : MODE == DH ? (const S*)g.w_out + (int64_t)e * g.H * g.F
@@ -134,7 +137,7 @@ __global__ __launch_bounds__(FT, MODE == UP || MODE == DOWN ? 4 : 2) void few_ke
         const int kk = 4 * q + c;
         const int row = part * K + k + (kk < left ? kk : left - 1);
         const S* p = wbase + (int64_t)row * cols + nc;
-        if (VEC) w[c].load(p);
+        if (VEC && cols % CE == 0) w[c].load(p);
         else w[c].load(p, cols - nc);
       }
     }

@@ -827,11 +827,13 @@ inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 
 // Few rows: so few for each expert on average that reading the weights once, into registers, and no plan of the rows win
 // over the tiles' matrix products; and few enough slots for a block to look through.  Rows' step (8 bits: forward), us,
-// few against tiles, slots for each of eight experts: fp32 640 x 640 8: 72, 128; 38: 114, 131; 1,600 x 1,600 25: 292, 304.
+// few against tiles, slots for each of eight experts: fp32 640 x 640 8: 72, 128; 30: 99, 129; 1,600 x 1,600 25: 292, 304; but
+// for each of 32 experts 576 x 808 11: 145, 164; 21: 219, 188.
 // bf16 640 8: 71, 75; 16: 81, 74; 1,600 12: 167, 143.  8 bits 640 16: 19, 23; 25: 24, 22; 1,600 8: 28, 36; 12: 37, 37.
 inline bool few(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k;
-  return M <= FEW_SLOTS && M <= (d.dtype == FSC_F32 ? 32 : d.dtype == FSC_I8 ? 16 : 8) * (int64_t)d.n_experts;
+  const int most = d.dtype == FSC_BF16 ? 8 : d.dtype == FSC_F32 && M <= 256 ? 32 : 16;
+  return M <= FEW_SLOTS && M <= most * (int64_t)d.n_experts;
 }
 
 // Forward by dot products (expert_one.hip): eight slots, or no more than experts, so that hardly any weight is read twice.
@@ -858,12 +860,12 @@ inline bool vec_ok(const void* p, int64_t rows, int64_t stride, int size, int n)
   return !p || ((uintptr_t)p % 4 == 0 && stride * size % 4 == 0 && !odd_rows(n, size) &&
                 ((rows - 1) * stride + n) * size < (int64_t)kDropOffset);
 }
-// The same for the few-rows kernels, which read 16 bytes through pointers as well, and step through an expert's matrix
-// with signed 32-bit offsets.
+// The same for the few-rows kernels, which read 16 bytes through pointers as well and step through an expert's matrix with
+// signed 32-bit offsets; 8-bit rows in whole 16 bytes.
 inline bool few_vec_ok(const void* p, int64_t rows, int64_t stride, int size, int n) {
   return vec_ok(p, rows, stride, size, n) &&
-         (!p || ((uintptr_t)p % 16 == 0 && stride * size % 16 == 0 && n % (size == 1 ? 16 : 8) == 0 &&
-                 ((rows - 1) * stride + n) * size < (1ll << 31)));
+         (!p || (n >= 8 && ((rows - 1) * stride + n) * size < (1ll << 31) &&
+                 (size > 1 || ((uintptr_t)p % 16 == 0 && stride % 16 == 0 && n % 16 == 0))));
 }
 
 template <int KIND, typename S, int MODE>
