@@ -35,6 +35,7 @@
 
 #include "common.h"
 #include "expert_plan.h"
+#include "expert_shares.h"
 #include "expert_tiles.h"
 #include "fsctep.h"
 
@@ -43,6 +44,7 @@ namespace experts {
 
 constexpr int NT = 256;          // four waves, two by two
 constexpr int BN = 128;          // rows of the tile's weight operand
+static_assert(BN == WEIGHT_TILE, "the weight gradients' tiles");
 
 // ---------------------------------------------------------------- tiles of the operands
 // A chunk is 16 bytes of an LDS plane: 8 values (16 in 8 bits) along the row.  Straight operands (rows of the tile
@@ -451,7 +453,6 @@ struct Share {
   int e, at, n;
   int64_t first;
 };
-constexpr int MANY_TILES = 64;
 
 // Runs f(e, shares of expert e, shares before the wave's 64 experts, inclusive sum over the lanes, all lanes) for 64
 // experts at a time until it returns true.
@@ -514,17 +515,15 @@ __global__ __launch_bounds__(NT, 2) void weights_kernel(Args g) {
   char* lb = lds + TT::BYTES;
   const int na = MODE == DWIN ? g.H : g.ldf, nb = MODE == DWIN ? 2 * g.ldf : g.H;   // columns of the operands
   const int ta = (na + BN - 1) / BN, tb = (nb + BN - 1) / BN;
-  // Workgroup w runs on XCD w % 8.  With many tiles every XCD takes a run of each share's tiles, whatever the shares'
-  // sizes; with few a run of all tiles of all shares, which are then about equal.
   const int tiles = ta * tb, w = (int)(blockIdx.x >> 3), x = (int)(blockIdx.x & 7);
   Share sh;
   int c;
-  if (FEW || g.M <= g.share) {                           // one share an expert
+  if (FEW || one_share_each(g.M, g.share)) {
     const int per = (tiles + 7) / 8;
     sh = Share{w / per, 0, 1, 0};
     c = x * per + w % per;
-    if (c >= tiles) return;
-  } else if (tiles >= MANY_TILES) {
+    if (c >= tiles || sh.e >= g.E) return;
+  } else if (runs_by_share(false, tiles)) {
     const int per = (tiles + 7) / 8;
     c = x * per + w % per;
     if (c >= tiles || !find_share(g, w / per, sh)) return;
@@ -887,19 +886,6 @@ void launch_rows(const Args& g, int tile, bool vec, hipStream_t st) {
   }
 }
 
-// Tiles of a weight gradient, and the positions of a share: so many that about 1,024 (fp32) or 512 tiles of shares run
-// whatever rows the experts have, of at least 128 (fp32: six products) or 256 positions, which outweigh writing and summing
-// them, and of 1,024 or 2,048 where the experts' tiles fill the chip without it and only the fullest experts are worth
-// dealing out.  Routing is uneven: 10,000 rows of 640, two of 16 experts, the fullest with three times the mean: forward
-// and all gradients 979 us against 1,553 with an expert's positions in one block (bf16 409 against 534).
-inline int64_t weight_tiles(int64_t na, int64_t nb) { return ((na + BN - 1) / BN) * ((nb + BN - 1) / BN); }
-inline int weight_share(int64_t M, int E, int size, int64_t tiles) {
-  const int64_t least = (E * tiles >= 512 ? 1024 : 128) * (size == 4 ? 1 : 2);
-  const int64_t share = std::max(least, M * tiles / (size == 4 ? 1024 : 512));
-  return (int)std::min<int64_t>((share + 63) / 64 * 64, 1 << 30);
-}
-inline int64_t most_shares(int64_t M, int E, int share) { return M / share + E; }
-
 // bytes of a value of the arrays between the kernels
 template <int KIND> constexpr int held_bytes() { return sizeof(typename El<KIND>::T); }
 
@@ -909,7 +895,7 @@ void launch_weights(Args g, bool vec, hipStream_t st) {
   const int64_t tiles = weight_tiles(na, nb);
   g.share = FEW ? 0 : weight_share(g.M, g.E, held_bytes<KIND>(), tiles);
   const int64_t shares = FEW ? g.E : most_shares(g.M, g.E, g.share);
-  const unsigned grid = (unsigned)(8 * (FEW || g.M <= g.share || tiles >= MANY_TILES ? shares * ((tiles + 7) / 8) : (shares * tiles + 7) / 8));
+  const unsigned grid = (unsigned)weight_blocks(shares, tiles, runs_by_share(FEW || one_share_each(g.M, g.share), tiles));
   if (vec) weights_kernel<KIND, S, MODE, true, FEW><<<grid, NT, 0, st>>>(g);
   else weights_kernel<KIND, S, MODE, false, FEW><<<grid, NT, 0, st>>>(g);
   if (!FEW && shares > g.E) {

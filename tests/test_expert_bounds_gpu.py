@@ -1,0 +1,81 @@
+"""The experts' products through the C ABI with every output and workspace of the size that is asked for inside a larger
+buffer whose bytes around it have to stay; values against the 64-bit oracle within the bounds of test_experts_gpu.py (fp32
+1e-5, bf16 2^-7 of the largest value)."""
+
+import ctypes
+
+import pytest
+import torch
+
+from oracle import experts as O
+from test_experts_gpu import DEV, DT, TOL, close, problem
+from test_experts_host import Dims
+
+pytestmark = pytest.mark.gpu
+GUARD = 8 << 20            # bytes on each side: more than any expert's matrices here
+FILL = 0xA5
+
+
+class Guarded:
+    """`shape` values of a type between guard bytes."""
+
+    def __init__(self, shape, dtype):
+        self.n = torch.empty(0, dtype=dtype).element_size() * int(torch.Size(shape).numel())
+        self.buf = torch.full((2 * GUARD + self.n,), FILL, dtype=torch.uint8, device=DEV)
+        self.t = self.buf[GUARD:GUARD + self.n].view(dtype).view(shape)
+
+    @property
+    def ptr(self):
+        return self.buf.data_ptr() + GUARD
+
+    def check(self, what):
+        assert int((self.buf[:GUARD] != FILL).sum()) == 0, f"{what}: bytes before"
+        assert int((self.buf[GUARD + self.n:] != FILL).sum()) == 0, f"{what}: bytes after"
+
+
+def run(x, index, weight, w_in, w_out, dy):
+    """(y, dx, dweight, dw_in, dw_out) of rows x, dy with their own strides; guards checked."""
+    from fsctep_amd import _lib
+    rows, width = x.shape
+    E, hidden, k = w_out.shape[0], w_out.shape[2], index.shape[1]
+    d = Dims(rows, width, hidden, E, k, 0 if x.dtype == torch.float32 else 1)
+    n = [ctypes.c_int64() for _ in range(4)]
+    _lib.call("fsc_expert_sizes", ctypes.byref(d), *(ctypes.byref(v) for v in n))
+    plan, saved, fwd, bwd = (v.value for v in n)
+    g = dict(plan=Guarded((plan,), torch.int32), saved=Guarded((saved,), torch.float32), forward=Guarded((fwd,), torch.uint8),
+             backward=Guarded((bwd,), torch.uint8), y=Guarded(x.shape, x.dtype), dx=Guarded(x.shape, x.dtype),
+             dweight=Guarded(weight.shape, torch.float32), dw_in=Guarded(w_in.shape, x.dtype),
+             dw_out=Guarded(w_out.shape, x.dtype))
+    p, st = {name: b.ptr for name, b in g.items()}, _lib.stream_handle(DEV)
+    _lib.call("fsc_expert_plan", ctypes.byref(d), index.data_ptr(), p["plan"], st)
+    _lib.call("fsc_expert_mlp_forward", ctypes.byref(d), x.stride(0), x.data_ptr(), index.data_ptr(), p["plan"],
+              weight.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), p["saved"], p["forward"], p["y"], st)
+    _lib.call("fsc_expert_mlp_backward", ctypes.byref(d), x.stride(0), dy.stride(0), dy.data_ptr(), x.data_ptr(),
+              index.data_ptr(), p["plan"], weight.data_ptr(), w_in.data_ptr(), w_out.data_ptr(), p["saved"], p["backward"],
+              p["dx"], p["dweight"], p["dw_in"], p["dw_out"], st)
+    torch.cuda.synchronize()
+    for name, b in g.items():
+        b.check(name)
+    return [g[name].t for name in ("y", "dx", "dweight", "dw_in", "dw_out")]
+
+
+def reference(x, index, weight, w_in, w_out, dy):
+    leaf = [t.double().requires_grad_(True) for t in (x, weight, w_in, w_out)]
+    y = O.expert_mlp(leaf[0], index, leaf[1], leaf[2], leaf[3])
+    return [y.detach(), *torch.autograd.grad(y, leaf, dy.double())]
+
+
+# Slots as many as the share of a weight gradient, one fewer and one more: of both gradients (fp32 128, bf16 256 and, few
+# for each expert, 128) or of dw_in alone (1,024 and 2,048).
+SHARES = [("fp32", 64, 640, 640, 2, 2), ("fp32", 64, 640, 640, 3, 2), ("fp32", 127, 330, 203, 2, 1), ("fp32", 128, 330, 203, 2, 1),
+          ("fp32", 129, 330, 203, 2, 1), ("fp32", 512, 640, 640, 16, 2), ("bf16", 64, 640, 640, 8, 2),
+          ("bf16", 128, 640, 640, 4, 2), ("bf16", 255, 200, 72, 3, 1), ("bf16", 256, 200, 72, 3, 1), ("bf16", 257, 200, 72, 3, 1),
+          ("bf16", 1024, 640, 640, 16, 2)]
+
+
+@pytest.mark.parametrize("dtype,rows,width,hidden,experts,k", SHARES)
+def test_weight_gradients_stay_inside_their_arrays(dtype, rows, width, hidden, experts, k):
+    p = problem(rows, width, hidden, experts, k, DT[dtype], rows + experts)
+    got = run(*(t.to(DEV) for t in p))
+    for a, b, n in zip(got, reference(*p), ("y", "dx", "dweight", "dw_in", "dw_out")):
+        close(a, b, TOL[DT[dtype]], n)
