@@ -35,6 +35,7 @@
 
 #include "common.h"
 #include "expert_plan.h"
+#include "expert_room.h"
 #include "expert_shares.h"
 #include "expert_tiles.h"
 #include "fsctep.h"
@@ -196,7 +197,6 @@ __device__ __forceinline__ void step(const char* lw, const char* lx, int w0, int
 // n entries in whole 32-bit words (rows that end inside one are read from padded copies)
 template <typename T>
 __device__ __forceinline__ int64_t whole_words(int n) { constexpr int w = 4 / sizeof(T); return (n + w - 1) / w * w; }
-inline int64_t whole_chunks(int64_t n, int ce) { return (n + ce - 1) / ce * ce; }
 
 // ---------------------------------------------------------------- the products by row tiles
 // A block takes one tile: rows of one expert, read by their numbers (up, dh: the gather is the load), by columns.  Two
@@ -822,7 +822,6 @@ __global__ __launch_bounds__(NT) void dweight_kernel(Dweight d, const int32_t* _
 
 // ---------------------------------------------------------------- host
 inline int up8(int v) { return (v + 7) / 8 * 8; }
-inline int64_t align64(int64_t b) { return (b + 63) / 64 * 64; }
 
 // Few rows: so few for each expert on average that reading the weights once, into registers, and no plan of the rows win
 // over the tiles' matrix products; and few enough slots for a block to look through.  Rows' step (8 bits: forward), us,
@@ -849,9 +848,6 @@ inline int tile_rows(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, avg = M / d.n_experts, tiles = M * (d.width + d.hidden) / (128 * 128);
   return avg <= 32 || tiles < 224 ? 32 : avg <= 64 || tiles < 1024 ? 64 : 128;
 }
-
-// Rows that end inside a 32-bit word.
-inline bool odd_rows(int n, int size) { return n * (int64_t)size % 4 != 0; }
 
 // Whether rows at p can be read 16 bytes at a time through one buffer: whole 32-bit words, and all of them below
 // kDropOffset bytes.
@@ -914,22 +910,22 @@ void launch_pass(const Pass& a, hipStream_t st) {
 }
 
 // Adds an array (E matrices of `rows` rows; E 0: the rows of x or dy) to a pass if it has to be looked at: its largest
-// magnitudes are wanted or its rows cannot be read in whole words.  p and ld are then those of a padded copy at `room`.
-// Returns false where the products read single values: arrays too large for one buffer, and weights whose rows are
-// whole words from an address that is none.
+// magnitudes are wanted or its rows cannot be read 16 bytes at a time and may be copied.  p and ld are then those of a
+// padded copy in `room`.  Returns false where the products read single values: arrays too large for one buffer, fp32 rows
+// too far apart for one, and weights whose rows are whole words from an address that is none.
 template <typename S>
-bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int E, int n, uint32_t* most, char*& room) {
-  constexpr int CE = sizeof(S) == 1 ? 16 : 8;
-  const int cld = (int)whole_chunks(n, CE);
+bool through(Pass& a, const void*& p, int64_t& ld, int64_t rows, int E, int n, uint32_t* most, Room& room) {
+  const int cld = (int)copy_row(n, sizeof(S));
   const int64_t outer = std::max(1, E);
   const bool ok = vec_ok(p, rows, ld, sizeof(S), n);
-  const bool copy = !ok && (E == 0 || odd_rows(n, sizeof(S))) && rows * cld * (int64_t)sizeof(S) < (int64_t)kDropOffset;
+  void* const copy = !ok && copies(E > 0, n, sizeof(S)) && rows * cld * (int64_t)sizeof(S) < (int64_t)kDropOffset
+                         ? room.take(copy_bytes(rows * outer, n, sizeof(S)))
+                         : nullptr;
   if (copy || most) {
-    a.a[a.arrays++] = Pass::Array{p, rows * outer, ld, n, most, copy ? room : nullptr, cld};
+    a.a[a.arrays++] = Pass::Array{p, rows * outer, ld, n, most, copy, cld};
     if (copy) {
-      p = room;
+      p = copy;
       ld = cld;
-      room += align64(rows * outer * cld * (int64_t)sizeof(S));
     }
   }
   return ok || copy;
@@ -972,7 +968,8 @@ inline int64_t held_size(const FscExpertDims& d) {
 
 // Parts of a workspace, in bytes.
 struct Space {
-  int64_t h, o, da, hw, part, hs, most, split, pad, total;
+  int64_t h, o, da, hw, part, hs, most, split, pad, pad_end, total;
+  Room room(char* ws) const { return Room{ws + pad, ws + pad_end}; }
 };
 // fp32 rows by tiles: two scaled parts an operand (three products, and one pass over the weights for their scales), or
 // three parts (six products, no pass) where an expert has so few rows that the weights' bytes count for more.  Forward and
@@ -981,14 +978,9 @@ struct Space {
 inline bool parts(const FscExpertDims& d) {
   return !few(d) && d.dtype == FSC_F32 && d.rows * d.k > 80 * (int64_t)d.n_experts;
 }
-// Room for padded copies of x (or x and dy: their strides and addresses are not known here) and of weights with odd rows;
-// fp32 rows are always whole words.
 inline int64_t pad_bytes(const FscExpertDims& d, int rows_arrays) {
-  const int size = d.dtype == FSC_F32 ? 4 : d.dtype == FSC_BF16 ? 2 : 1, ce = size == 1 ? 16 : 8;
-  const int64_t hp = whole_chunks(d.width, ce), fp = whole_chunks(d.hidden, ce), E = d.n_experts;
-  if (size == 4) return 0;
-  return rows_arrays * align64(d.rows * hp * size) + (odd_rows(d.width, size) ? align64(E * 2 * d.hidden * hp * size) : 0) +
-         (odd_rows(d.hidden, size) ? align64(E * d.width * fp * size) : 0);
+  const int size = d.dtype == FSC_F32 ? 4 : d.dtype == FSC_BF16 ? 2 : 1;
+  return copies_bytes(d.rows, d.width, d.hidden, d.n_experts, size, rows_arrays);
 }
 inline Space forward_space(const FscExpertDims& d) {
   const int64_t M = d.rows * d.k, ldf = ldf_of(d), size = held_size(d);
@@ -1003,7 +995,7 @@ inline Space forward_space(const FscExpertDims& d) {
     s.hs = at; at += align64(M * (ldf / QG) * 4);
   }
   if (!few(d)) {
-    s.pad = at; at += pad_bytes(d, 1);
+    s.pad = at; at += pad_bytes(d, 1); s.pad_end = at;
   }
   s.total = at;
   return s;
@@ -1020,7 +1012,7 @@ inline Space backward_space(const FscExpertDims& d) {
     s.most = at; at += align64((d.rows + M + (int64_t)d.n_experts * (d.hidden + d.width)) * 4);
   }
   if (!few(d)) {
-    s.pad = at; at += pad_bytes(d, 2);
+    s.pad = at; at += pad_bytes(d, 2); s.pad_end = at;
     // the two weight gradients use the same room, one after the other
     const int64_t si = most_shares(M, d.n_experts, weight_share(M, d.n_experts, (int)size, weight_tiles(d.width, 2 * ldf)));
     const int64_t so = most_shares(M, d.n_experts, weight_share(M, d.n_experts, (int)size, weight_tiles(ldf, d.width)));
@@ -1056,7 +1048,7 @@ Args args_of(const FscExpertDims& d, const Plan& p) {
 }
 
 template <int KIND, typename S>
-void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
+void forward(Args g, int tile, Room room, void* y, hipStream_t st) {
   if (!g.place) {
     if (one(g.M, g.E)) {
       if constexpr (KIND == I8) one_launch_q8(g, y, st);
@@ -1087,7 +1079,7 @@ void forward(Args g, int tile, char* room, void* y, hipStream_t st) {
 }
 
 template <int KIND, typename S>
-void backward(Args g, int tile, char* room, void* dx, float* dweight, hipStream_t st) {
+void backward(Args g, int tile, Room room, void* dx, float* dweight, hipStream_t st) {
   const bool by_slot = !g.place;
   bool vdy = vec_ok(g.dy, g.T, g.ds, sizeof(S), g.H), vx = vec_ok(g.x, g.T, g.xs, sizeof(S), g.H);
   bool vin = vec_ok(g.w_in, 2 * g.F, g.H, sizeof(S), g.H), vout = vec_ok(g.w_out, g.H, g.F, sizeof(S), g.F);
@@ -1188,10 +1180,10 @@ int fsc_expert_mlp_forward(const FscExpertDims* dims, int64_t x_stride, const vo
     g.in_row = g.hmost + g.M;
     g.out_row = g.in_row + (int64_t)g.E * 2 * g.F;
   }
-  if (parts(*dims)) forward<F32, float>(g, tile, ws + s.pad, y, stream);
-  else if (dims->dtype == FSC_F32) forward<X6, float>(g, tile, ws + s.pad, y, stream);
-  else if (fine(*dims)) forward<FINE, __bf16>(g, tile, ws + s.pad, y, stream);
-  else forward<BF16, __bf16>(g, tile, ws + s.pad, y, stream);
+  if (parts(*dims)) forward<F32, float>(g, tile, s.room(ws), y, stream);
+  else if (dims->dtype == FSC_F32) forward<X6, float>(g, tile, s.room(ws), y, stream);
+  else if (fine(*dims)) forward<FINE, __bf16>(g, tile, s.room(ws), y, stream);
+  else forward<BF16, __bf16>(g, tile, s.room(ws), y, stream);
   return fsc::check_launch("expert_mlp_forward") ? 2 : 0;
 }
 
@@ -1235,13 +1227,13 @@ int fsc_expert_mlp_backward(const FscExpertDims* dims, int64_t x_stride, int64_t
       if (dw_out) launch_weights<FINE, __bf16, DWOUT, true>(g, false, stream);
     }
   } else if (parts(*dims)) {
-    backward<F32, float>(g, tile, ws + s.pad, dx, dweight, stream);
+    backward<F32, float>(g, tile, s.room(ws), dx, dweight, stream);
   } else if (dims->dtype == FSC_F32) {
-    backward<X6, float>(g, tile, ws + s.pad, dx, dweight, stream);
+    backward<X6, float>(g, tile, s.room(ws), dx, dweight, stream);
   } else if (fine(*dims)) {
-    backward<FINE, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
+    backward<FINE, __bf16>(g, tile, s.room(ws), dx, dweight, stream);
   } else {
-    backward<BF16, __bf16>(g, tile, ws + s.pad, dx, dweight, stream);
+    backward<BF16, __bf16>(g, tile, s.room(ws), dx, dweight, stream);
   }
   return fsc::check_launch("expert_mlp_backward") ? 2 : 0;
 }
@@ -1267,7 +1259,7 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
   g.h = ws + s.h;
   g.o = (float*)(ws + s.o);
   g.hscale = (float*)(ws + s.hs);
-  forward<I8, int8_t>(g, tile, ws + s.pad, y, stream);
+  forward<I8, int8_t>(g, tile, s.room(ws), y, stream);
   return fsc::check_launch("expert_mlp_q8") ? 2 : 0;
 }
 

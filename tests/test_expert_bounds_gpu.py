@@ -79,3 +79,48 @@ def test_weight_gradients_stay_inside_their_arrays(dtype, rows, width, hidden, e
     got = run(*(t.to(DEV) for t in p))
     for a, b, n in zip(got, reference(*p), ("y", "dx", "dweight", "dw_in", "dw_out")):
         close(a, b, TOL[DT[dtype]], n)
+
+
+def held_rows(hold, t, stride, at):
+    """Rows t as a view of `hold` (uint8) with a row stride in elements, from element `at` on."""
+    v = hold.view(t.dtype).as_strided(t.shape, (stride, 1), at)
+    v.copy_(t)
+    return v
+
+
+# Row strides that put the last rows past what a buffer of 32-bit offsets reaches (0xF0000000 bytes), rows by tiles and few;
+# and rows at odd places, whole words or not, which are copied.
+@pytest.mark.parametrize("rows,width,far", [(300, 64, True), (40, 64, True), (300, 65, True), (300, 64, False), (300, 65, False)])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_strided_rows_stay_inside_the_workspaces(rows, width, far, dtype):
+    dt = DT[dtype]
+    size = 4 if dtype == "fp32" else 2
+    x, index, weight, w_in, w_out, dy = problem(rows, width, 40, 4, 2, dt, rows + width)
+    stride = (0xF0000000 // (rows - 1) // size + 4) // 4 * 4 + 4 if far else 203
+    hold = torch.empty(rows * stride * size + 1024, dtype=torch.uint8, device=DEV)
+    xs, dys = held_rows(hold, x.to(DEV), stride, 1), held_rows(hold, dy.to(DEV), stride, 101)
+    got = run(xs, index.to(DEV), weight.to(DEV), w_in.to(DEV), w_out.to(DEV), dys)
+    for a, b, n in zip(got, reference(x, index, weight, w_in, w_out, dy), ("y", "dx", "dweight", "dw_in", "dw_out")):
+        close(a, b, TOL[dt], n)
+
+
+@pytest.mark.parametrize("rows,width,hidden", [(300, 65, 41), (300, 64, 40), (20, 65, 41), (2, 65, 41)])
+def test_8_bit_products_stay_inside_the_workspaces(rows, width, hidden):
+    from fsctep_amd import _lib, expert_ops as X
+    x, index, weight, w_in, w_out, _ = problem(rows, width, hidden, 4, 2, torch.float32, rows + width)
+    (q, s), (qi, si), (qo, so) = X.to_codes(x.to(DEV)), X.to_codes(w_in.to(DEV)), X.to_codes(w_out.to(DEV))
+    hold = torch.zeros(rows * 203 + 1024, dtype=torch.uint8, device=DEV)
+    v = held_rows(hold, q, 203, 3)
+    d = Dims(rows, width, hidden, 4, 2, 2)
+    n = [ctypes.c_int64() for _ in range(4)]
+    _lib.call("fsc_expert_sizes", ctypes.byref(d), *(ctypes.byref(t) for t in n))
+    plan, ws = Guarded((n[0].value,), torch.int32), Guarded((n[2].value,), torch.uint8)
+    y, st = Guarded(x.shape, torch.bfloat16), _lib.stream_handle(DEV)
+    i, w = index.to(DEV), weight.to(DEV)
+    _lib.call("fsc_expert_plan", ctypes.byref(d), i.data_ptr(), plan.ptr, st)
+    _lib.call("fsc_expert_mlp_q8", ctypes.byref(d), 203, v.data_ptr(), s.data_ptr(), i.data_ptr(), plan.ptr, w.data_ptr(),
+              qi.data_ptr(), si.data_ptr(), qo.data_ptr(), so.data_ptr(), ws.ptr, y.ptr, st)
+    torch.cuda.synchronize()
+    for b, name in ((plan, "plan"), (ws, "workspace"), (y, "y")):
+        b.check(name)
+    assert torch.equal(y.t, X.expert_mlp_q8(q, s, i, w, qi, si, qo, so))
