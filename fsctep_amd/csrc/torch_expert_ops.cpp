@@ -57,6 +57,14 @@ auto op_handle(const char* name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<Sig>();
 }
 
+// Whether a call goes through its autograd function: a gradient is wanted, or an input carries a forward-mode tangent,
+// which the function refuses (below autograd it would be lost).
+bool differentiates(std::initializer_list<std::reference_wrapper<const Tensor>> ts) {
+  for (const Tensor& t : ts)
+    if (t.defined() && ((at::GradMode::is_enabled() && t.requires_grad()) || t._fw_grad(0).defined())) return true;
+  return false;
+}
+
 // A backward op's call: below autograd unless a gradient of the gradient may be asked for, which then raises.
 struct BackwardGuard {
   optional<at::AutoDispatchBelowADInplaceOrView> below;
@@ -203,7 +211,7 @@ struct RmsNormFn : public torch::autograd::Function<RmsNormFn> {
 
 std::tuple<Tensor, Tensor, Tensor> rms_norm_autograd(const Tensor& x, const Tensor& weight,
                                                      const optional<Tensor>& residual, double eps) {
-  if (at::GradMode::is_enabled() && (x.requires_grad() || weight.requires_grad() || some(residual).requires_grad())) {
+  if (differentiates({x, weight, some(residual)})) {
     auto r = RmsNormFn::apply(x, weight, residual, eps);
     return {r[0], r[1], r[2]};
   }
@@ -302,7 +310,7 @@ struct RouteFn : public torch::autograd::Function<RouteFn> {
 std::tuple<Tensor, Tensor> route_experts_autograd(const Tensor& logits, const optional<Tensor>& bias, int64_t k,
                                                   int64_t score, int64_t groups, int64_t kept, int64_t best,
                                                   bool renormalise, double scale) {
-  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+  if (differentiates({logits})) {
     auto r = RouteFn::apply(logits, bias, k, score, groups, kept, best, renormalise, scale);
     return {r[0], r[1]};
   }
@@ -458,8 +466,7 @@ Tensor expert_mlp(const Tensor& x, const Tensor& index, const Tensor& weight, co
 // The values before the activation are kept only where a gradient will ask for them.
 Tensor expert_mlp_autograd(const Tensor& x, const Tensor& index, const Tensor& weight, const Tensor& w_in,
                            const Tensor& w_out) {
-  if (at::GradMode::is_enabled() &&
-      (x.requires_grad() || weight.requires_grad() || w_in.requires_grad() || w_out.requires_grad()))
+  if (differentiates({x, weight, w_in, w_out}))
     return ExpertMlpFn::apply(x, index, weight, w_in, w_out)[0];
   at::AutoDispatchBelowADInplaceOrView guard;
   return expert_mlp(x, index, weight, w_in, w_out);
