@@ -16,7 +16,9 @@ without one run as before.
 * training on forces (the trunks' ``train()`` step): ``differentiable=True``, the twice differentiable torch form
   on the experts that the fused router chose;
 * energies alone of many candidates (screening, Monte Carlo): ``ExpertReadout.to_8_bits()``, rows and weights in 8
-  bits, no gradient.
+  bits, no gradient;
+* the layers in bfloat16: ``ExpertReadout.bfloat16()``, on float32 rows too (what a layer adds is bfloat16, the rows
+  themselves stay as they are).
 """
 
 from __future__ import annotations
@@ -29,11 +31,25 @@ import torch.nn.functional as F
 
 from . import expert_ops as X
 
+ROW_TYPES = (torch.float32, torch.bfloat16)
 
-class ExpertLayer(nn.Module):
+
+class _OwnTypes(nn.Module):
+    """Buffers that keep their types where a program casts the parameters (``.bfloat16()`` and the like)."""
+
+    def _apply(self, fn, recurse=True):
+        before = dict(self._buffers)
+        super()._apply(fn, recurse)
+        for name, b in before.items():
+            if self._buffers[name].dtype != b.dtype:
+                self._buffers[name] = b.to(self._buffers[name].device)
+        return self
+
+
+class ExpertLayer(_OwnTypes):
     """Parameters of one layer: norm weight (width,), gate (n_experts, width) or, by atomic number, (n_species,
     n_experts), w_in (n_experts, 2 hidden, width), w_out (n_experts, width, hidden, zero at first) and the balance
-    bias (n_experts,), a buffer that moves which experts are chosen and not what they weigh."""
+    bias (n_experts,), a float32 buffer that moves which experts are chosen and not what they weigh."""
 
     def __init__(self, width: int, hidden: int, n_experts: int, n_species: int | None = None):
         super().__init__()
@@ -83,7 +99,8 @@ class Router:
 class ExpertReadout(nn.Module):
     """``layers`` expert layers on rows (N, width); ``k`` of ``n_experts`` experts a row, scores ``softmax`` or
     ``sigmoid``, optional groups (``groups``, ``groups_kept``, ``group_best``), weights renormalised and scaled as
-    ``expert_ops.route_experts`` does; ``n_species``: choice by atomic number."""
+    ``expert_ops.route_experts`` does; ``n_species``: choice by atomic number.  Parameters in float32 or, after
+    ``.bfloat16()``, in bfloat16; rows in either."""
 
     def __init__(self, width: int, hidden: int, n_experts: int, k: int = 2, layers: int = 1, score: str = "softmax",
                  groups: int = 1, groups_kept: int = 1, group_best: int = 1, renormalise: bool = True,
@@ -98,8 +115,18 @@ class ExpertReadout(nn.Module):
     def forward(self, x, species=None, differentiable: bool = False):
         """(N, width) -> (N, width); ``species``: atomic numbers (N,), below n_species.  ``differentiable``: twice
         differentiable (force losses)."""
+        if x.dtype not in ROW_TYPES:
+            raise ValueError(f"expert readout: rows are float32 or bfloat16, got {x.dtype}")
         if differentiable:
             return self._forward_train(x, species)
+        own = self.layers[0].norm.dtype
+        if x.dtype != own:
+            out = x
+            for layer in self.layers:
+                y, _ = X.rms_norm(out.to(own), layer.norm, eps=self.eps)
+                index, weight = self.router.choose(layer, self.router.logits(layer, y, species))
+                out = out + X.expert_mlp(y, index, weight, layer.w_in, layer.w_out)
+            return out.to(x.dtype)
         z, add = x, None
         for layer in self.layers:
             y, z = X.rms_norm(x, layer.norm, eps=self.eps) if add is None else X.rms_norm(add, layer.norm, z, self.eps)
@@ -109,15 +136,16 @@ class ExpertReadout(nn.Module):
 
     def _forward_train(self, x, species):
         from . import train_ops as T
+        own, rows = self.layers[0].norm.dtype, x.dtype
         for layer in self.layers:
-            y, _ = T.rms_norm(x, layer.norm, eps=self.eps)
+            y, _ = T.rms_norm(x.to(own), layer.norm, eps=self.eps)
             logits = self.router.logits(layer, y, species)
             with torch.no_grad():
                 index, _ = self.router.choose(layer, logits.detach())
             weight = T.route_weights(logits, index, self.router.score, self.router.renormalise,
                                      self.router.scale)
             x = x + T.expert_mlp(y, index, weight, layer.w_in, layer.w_out)
-        return x
+        return x.to(rows)
 
     def to_8_bits(self) -> "ExpertReadoutQ8":
         return ExpertReadoutQ8(self)
@@ -132,7 +160,7 @@ class ExpertReadoutQ8(nn.Module):
         self.router, self.eps = full.router, full.eps
         self.layers = nn.ModuleList()
         for layer in full.layers:
-            m = nn.Module()
+            m = _OwnTypes()
             m.register_buffer("norm", layer.norm.detach().float().clone())
             m.register_buffer("gate", layer.gate.detach().float().clone())
             m.register_buffer("balance", layer.balance.detach().clone())

@@ -219,15 +219,22 @@ def readout_features(feats, Ws, scales, maps):
 
 
 # ------------------------------------------------------------------ expert readout (rms_norm.hip, expert_mlp.hip)
+def _wide(t):
+    """16-bit values in 32 bits, in which they are multiplied and summed."""
+    return t.float() if t.dtype == torch.bfloat16 else t
+
+
 def rms_norm(x, weight, residual=None, eps: float = 1e-6):
     """(y, z) of ``expert_ops.rms_norm``, differentiable to any order."""
     z = x if residual is None else x + residual
-    return z * torch.rsqrt((z * z).mean(-1, keepdim=True) + eps) * weight, z
+    v = _wide(z)
+    return (v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps) * _wide(weight)).to(z.dtype), z
 
 
 def route_weights(logits, index, score: str, renormalise: bool, scale: float):
     """The routing weights of the experts already chosen (``expert_ops.route_experts``' index), differentiable
     in the logits to any order; 0 where the index is -1."""
+    logits = _wide(logits)
     s = torch.softmax(logits, -1) if score == "softmax" else torch.sigmoid(logits)
     there = index >= 0
     picked = torch.where(there, s.gather(1, index.clamp(min=0).long()), torch.zeros((), device=s.device, dtype=s.dtype))
@@ -244,8 +251,9 @@ def expert_mlp(x, index, weight, w_in, w_out):
     there = index >= 0
     share = weight.new_zeros(x.shape[0], E).scatter_add(1, index.clamp(min=0).long(),
                                                         torch.where(there, weight, torch.zeros_like(weight)))
-    y = torch.zeros_like(x)
+    v = _wide(x)
+    y = torch.zeros_like(v)
     for e in range(E):
-        a = x @ w_in[e].t()
-        y = y + share[:, e:e + 1] * ((F.silu(a[:, :f]) * a[:, f:]) @ w_out[e].t())
-    return y
+        a = v @ _wide(w_in[e]).t()
+        y = y + share[:, e:e + 1] * ((F.silu(a[:, :f]) * a[:, f:]) @ _wide(w_out[e]).t())
+    return y.to(x.dtype)
