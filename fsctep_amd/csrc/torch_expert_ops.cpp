@@ -10,6 +10,8 @@
 #include <torch/csrc/autograd/autograd_not_implemented_fallback.h>
 #include <torch/library.h>
 
+#include <cmath>
+
 #include "fsctep.h"
 
 namespace {
@@ -220,23 +222,34 @@ std::tuple<Tensor, Tensor, Tensor> rms_norm_autograd(const Tensor& x, const Tens
 }
 
 // ============================================================== router
+// What the router takes, the same on the GPU and on Meta tensors.
+void check_route(const Tensor& l, const Tensor& bias, int64_t k, int64_t score, int64_t groups, int64_t kept, int64_t best,
+                 double scale) {
+  TORCH_CHECK(l.dim() == 2, "route_experts: logits must be (rows, experts), got ", l.dim(), " dimensions");
+  code_of(l.scalar_type(), "logits");
+  const auto experts = l.sym_size(1);
+  TORCH_CHECK(experts >= 1 && experts <= 512, "route_experts: 1 to 512 experts, got ", experts);
+  if (bias.defined()) {
+    TORCH_CHECK(bias.dim() == 1 && bias.sym_size(0) == experts, "route_experts: bias must be (", experts, ",)");
+    TORCH_CHECK(bias.scalar_type() == at::kFloat, "route_experts: bias must be float32, got ", bias.scalar_type());
+  }
+  TORCH_CHECK(score == 0 || score == 1, "route_experts: score is 0 (softmax) or 1 (sigmoid), got ", score);
+  TORCH_CHECK(k >= 1 && k <= 16 && experts >= k, "route_experts: k must be 1 to 16 and at most the experts, got ", k);
+  TORCH_CHECK(groups >= 1 && groups <= 128 && kept >= 1 && kept <= groups,
+              "route_experts: groups must be 1 to 128 and groups_kept 1 to groups, got ", groups, " and ", kept);
+  TORCH_CHECK(experts % groups == 0, "route_experts: groups must divide the experts, got ", groups, " and ", experts);
+  TORCH_CHECK(experts / groups * kept >= k, "route_experts: k is more than the kept groups' experts, got ", k);
+  TORCH_CHECK(best == 1 || best == 2, "route_experts: group_best is 1 or 2, got ", best);
+  TORCH_CHECK(scale > 0 && std::isfinite((float)scale), "route_experts: scale must be positive and finite, got ", scale);
+}
+
 std::tuple<Tensor, Tensor> route_experts(const Tensor& logits_, const optional<Tensor>& bias_, int64_t k, int64_t score,
                                          int64_t groups, int64_t groups_kept, int64_t group_best, bool renormalise,
                                          double scale) {
   require_gpu({logits_, some(bias_)}, "route_experts");
-  const Tensor l = rows2d(logits_, "logits");
+  check_route(logits_, some(bias_), k, score, groups, groups_kept, group_best, scale);
+  const Tensor l = rows2d(logits_, "logits"), b = bias_.has_value() ? bias_->contiguous() : Tensor();
   const int32_t dt = code_of(l.scalar_type(), "logits");
-  Tensor b;
-  if (bias_.has_value()) {
-    TORCH_CHECK(bias_->dim() == 1 && bias_->size(0) == l.size(1), "route_experts: bias must be (", l.size(1), ",)");
-    TORCH_CHECK(bias_->scalar_type() == at::kFloat, "route_experts: bias must be float32, got ", bias_->scalar_type());
-    b = bias_->contiguous();
-  }
-  TORCH_CHECK(k >= 1 && k <= 16, "route_experts: k must be 1 to 16, got ", k);
-  TORCH_CHECK(groups >= 1 && groups <= 128 && groups_kept >= 1 && groups_kept <= groups,
-              "route_experts: groups must be 1 to 128 and groups_kept 1 to groups, got ", groups, " and ", groups_kept);
-  TORCH_CHECK(group_best == 1 || group_best == 2, "route_experts: group_best is 1 or 2, got ", group_best);
-  TORCH_CHECK(l.size(1) >= 1 && l.size(1) <= 512, "route_experts: 1 to 512 experts, got ", l.size(1));
   Tensor index = at::empty({l.size(0), k}, l.options().dtype(at::kInt));
   Tensor weight = at::empty({l.size(0), k}, l.options().dtype(at::kFloat));
   check(fsc_route_experts(l.size(0), (int32_t)l.size(1), dt, stride_of(l), ptr(l), (const float*)ptr(b), (int32_t)k,
@@ -246,8 +259,9 @@ std::tuple<Tensor, Tensor> route_experts(const Tensor& logits_, const optional<T
   return {index, weight};
 }
 
-std::tuple<Tensor, Tensor> route_experts_meta(const Tensor& l, const optional<Tensor>&, int64_t k, int64_t, int64_t,
-                                              int64_t, int64_t, bool, double) {
+std::tuple<Tensor, Tensor> route_experts_meta(const Tensor& l, const optional<Tensor>& bias, int64_t k, int64_t score,
+                                              int64_t groups, int64_t kept, int64_t best, bool, double scale) {
+  check_route(l, some(bias), k, score, groups, kept, best, scale);
   return {at::empty_symint({l.sym_size(0), k}, l.options().dtype(at::kInt)),
           at::empty_symint({l.sym_size(0), k}, l.options().dtype(at::kFloat))};
 }
@@ -323,25 +337,36 @@ struct Sizes {
   int64_t plan = 0, saved = 0, fwd = 0, bwd = 0;
 };
 
-FscExpertDims expert_dims(const Tensor& x, const Tensor& index, const Tensor& weight, const Tensor& w_in,
-                          const Tensor& w_out, const char* name) {
+// What the products take, the same on the GPU and on Meta tensors (of sizes that a trace does not know yet, too).
+void check_products(const Tensor& x, const Tensor& index, const Tensor& weight, const Tensor& w_in, const Tensor& w_out,
+                    const char* name, bool q8 = false) {
   TORCH_CHECK(x.dim() == 2, name, ": x must be (rows, width), got ", x.dim(), " dimensions");
-  TORCH_CHECK(w_out.dim() == 3 && w_out.size(1) == x.size(1), name, ": w_out must be (experts, ", x.size(1), ", hidden)");
-  TORCH_CHECK(w_in.dim() == 3 && w_in.size(0) == w_out.size(0) && w_in.size(1) == 2 * w_out.size(2) &&
-                  w_in.size(2) == x.size(1),
-              name, ": w_in must be (", w_out.size(0), ", ", 2 * w_out.size(2), ", ", x.size(1), ")");
-  TORCH_CHECK(index.dim() == 2 && index.size(0) == x.size(0) && index.size(1) >= 1, name, ": index must be (",
-              x.size(0), ", k)");
+  if (q8) {
+    TORCH_CHECK(x.scalar_type() == at::kChar, name, ": x must be int8 codes, got ", x.scalar_type());
+  } else {
+    code_of(x.scalar_type(), "x");
+  }
+  const auto rows = x.sym_size(0), width = x.sym_size(1);
+  TORCH_CHECK(w_out.dim() == 3 && w_out.sym_size(1) == width, name, ": w_out must be (experts, ", width, ", hidden)");
+  const auto experts = w_out.sym_size(0), hidden = w_out.sym_size(2);
+  TORCH_CHECK(w_in.dim() == 3 && w_in.sym_size(0) == experts && w_in.sym_size(1) == hidden * 2 && w_in.sym_size(2) == width,
+              name, ": w_in must be (", experts, ", ", hidden * 2, ", ", width, ")");
+  TORCH_CHECK(index.dim() == 2 && index.sym_size(0) == rows && index.sym_size(1) >= 1, name, ": index must be (", rows, ", k)");
   TORCH_CHECK(index.scalar_type() == at::kInt, name, ": index must be int32, got ", index.scalar_type());
-  TORCH_CHECK(weight.sizes() == index.sizes(), name, ": weight must have index's shape");
+  TORCH_CHECK(weight.sym_sizes() == index.sym_sizes(), name, ": weight must have index's shape");
   TORCH_CHECK(weight.scalar_type() == at::kFloat, name, ": weight must be float32, got ", weight.scalar_type());
   TORCH_CHECK(w_in.scalar_type() == x.scalar_type() && w_out.scalar_type() == x.scalar_type(), name,
               ": x, w_in and w_out must have one type");
-  TORCH_CHECK(x.size(1) >= 1 && x.size(1) <= (1 << 17) && w_out.size(2) >= 1 && w_out.size(2) <= (1 << 17), name,
+  TORCH_CHECK(width >= 1 && width <= (1 << 17) && hidden >= 1 && hidden <= (1 << 17), name,
               ": width and hidden must be 1 to 2^17");
-  TORCH_CHECK(w_out.size(0) >= 1 && w_out.size(0) <= 512, name, ": 1 to 512 experts, got ", w_out.size(0));
-  TORCH_CHECK(index.size(1) <= 64, name, ": at most 64 slots a row, got ", index.size(1));
-  const int32_t dt = x.scalar_type() == at::kChar ? FSC_I8 : code_of(x.scalar_type(), "x");
+  TORCH_CHECK(experts >= 1 && experts <= 512, name, ": 1 to 512 experts, got ", experts);
+  TORCH_CHECK(index.sym_size(1) <= 64, name, ": at most 64 slots a row, got ", index.sym_size(1));
+}
+
+FscExpertDims expert_dims(const Tensor& x, const Tensor& index, const Tensor& weight, const Tensor& w_in,
+                          const Tensor& w_out, const char* name, bool q8 = false) {
+  check_products(x, index, weight, w_in, w_out, name, q8);
+  const int32_t dt = q8 ? FSC_I8 : code_of(x.scalar_type(), "x");
   return {x.size(0), (int32_t)x.size(1), (int32_t)w_out.size(2), (int32_t)w_out.size(0), (int32_t)index.size(1), dt};
 }
 
@@ -472,19 +497,21 @@ Tensor expert_mlp_autograd(const Tensor& x, const Tensor& index, const Tensor& w
   return expert_mlp(x, index, weight, w_in, w_out);
 }
 
+// A scale for each row of codes.
+void check_scales(const Tensor& scale, const Tensor& codes, const char* name) {
+  const auto shape = codes.sym_sizes().slice(0, codes.dim() - 1);
+  TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.sym_sizes() == shape, "expert_mlp_q8: ", name,
+              " must be float32 of shape ", shape);
+}
+
 Tensor expert_mlp_q8(const Tensor& x_, const Tensor& x_scale_, const Tensor& index_, const Tensor& weight_,
                      const Tensor& w_in_, const Tensor& w_in_scale_, const Tensor& w_out_, const Tensor& w_out_scale_) {
   require_gpu({x_, x_scale_, index_, weight_, w_in_, w_in_scale_, w_out_, w_out_scale_}, "expert_mlp_q8");
-  TORCH_CHECK(x_.scalar_type() == at::kChar, "expert_mlp_q8: x must be int8 codes, got ", x_.scalar_type());
-  const FscExpertDims d = expert_dims(x_, index_, weight_, w_in_, w_out_, "expert_mlp_q8");
-  auto scales = [](const Tensor& t, at::IntArrayRef shape, const char* name) {
-    TORCH_CHECK(t.scalar_type() == at::kFloat && t.sizes() == shape, "expert_mlp_q8: ", name,
-                " must be float32 of shape ", shape);
-    return t.contiguous();
-  };
-  const Tensor xs = scales(x_scale_, {d.rows}, "x_scale");
-  const Tensor is = scales(w_in_scale_, {d.n_experts, 2 * (int64_t)d.hidden}, "w_in_scale");
-  const Tensor os = scales(w_out_scale_, {d.n_experts, d.width}, "w_out_scale");
+  const FscExpertDims d = expert_dims(x_, index_, weight_, w_in_, w_out_, "expert_mlp_q8", true);
+  check_scales(x_scale_, x_, "x_scale");
+  check_scales(w_in_scale_, w_in_, "w_in_scale");
+  check_scales(w_out_scale_, w_out_, "w_out_scale");
+  const Tensor xs = x_scale_.contiguous(), is = w_in_scale_.contiguous(), os = w_out_scale_.contiguous();
   const Tensor x = rows2d(x_, "x"), index = index_.contiguous(), weight = weight_.contiguous();
   const Tensor w_in = w_in_.contiguous(), w_out = w_out_.contiguous();
   const Sizes s = sizes_of(d);
@@ -499,12 +526,17 @@ Tensor expert_mlp_q8(const Tensor& x_, const Tensor& x_scale_, const Tensor& ind
   return y;
 }
 
-Tensor expert_mlp_q8_meta(const Tensor& x, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
-                          const Tensor&, const Tensor&) {
+Tensor expert_mlp_q8_meta(const Tensor& x, const Tensor& x_scale, const Tensor& index, const Tensor& weight,
+                          const Tensor& w_in, const Tensor& w_in_scale, const Tensor& w_out, const Tensor& w_out_scale) {
+  check_products(x, index, weight, w_in, w_out, "expert_mlp_q8", true);
+  check_scales(x_scale, x, "x_scale");
+  check_scales(w_in_scale, w_in, "w_in_scale");
+  check_scales(w_out_scale, w_out, "w_out_scale");
   return at::empty_symint(x.sym_sizes(), x.options().dtype(at::kBFloat16));
 }
 
-Tensor expert_mlp_meta(const Tensor& x, const Tensor&, const Tensor&, const Tensor&, const Tensor&) {
+Tensor expert_mlp_meta(const Tensor& x, const Tensor& index, const Tensor& weight, const Tensor& w_in, const Tensor& w_out) {
+  check_products(x, index, weight, w_in, w_out, "expert_mlp");
   return at::empty_symint(x.sym_sizes(), x.options());
 }
 
