@@ -66,7 +66,7 @@ class ExpertLayer(_OwnTypes):
         it (``index``: the router's choices of a batch)."""
         n = self.balance.shape[0]
         flat = index.reshape(-1).long()
-        count = self.balance.new_zeros(n + 1).index_add_(0, torch.where(flat < 0, n, flat),
+        count = self.balance.new_zeros(n + 1).index_add_(0, torch.where((flat < 0) | (flat > n), n, flat),
                                                          torch.ones_like(flat, dtype=self.balance.dtype))[:n]
         self.balance += rate * torch.sign(count.mean() - count)
 

@@ -231,13 +231,19 @@ def rms_norm(x, weight, residual=None, eps: float = 1e-6):
     return (v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps) * _wide(weight)).to(z.dtype), z
 
 
+def _slots(index, n_experts: int):
+    """Which slots have an expert, and an expert to look up for each (0 where there is none)."""
+    there = (index >= 0) & (index < n_experts)
+    return there, torch.where(there, index, torch.zeros_like(index)).long()
+
+
 def route_weights(logits, index, score: str, renormalise: bool, scale: float):
     """The routing weights of the experts already chosen (``expert_ops.route_experts``' index), differentiable
-    in the logits to any order; 0 where the index is -1."""
+    in the logits to any order; 0 where the index is none of the experts."""
+    there, at = _slots(index, logits.shape[1])
     logits = _wide(logits)
     s = torch.softmax(logits, -1) if score == "softmax" else torch.sigmoid(logits)
-    there = index >= 0
-    picked = torch.where(there, s.gather(1, index.clamp(min=0).long()), torch.zeros((), device=s.device, dtype=s.dtype))
+    picked = torch.where(there, s.gather(1, at), torch.zeros((), device=s.device, dtype=s.dtype))
     if renormalise:
         total = picked.sum(-1, keepdim=True)
         picked = picked / torch.where(total > 0, total, torch.ones_like(total))
@@ -248,9 +254,8 @@ def expert_mlp(x, index, weight, w_in, w_out):
     """``expert_ops.expert_mlp``, differentiable to any order: every expert on every row (training
     configurations are small; the sizes follow from the tensors, so nothing waits for the GPU)."""
     E, H, f = w_out.shape
-    there = index >= 0
-    share = weight.new_zeros(x.shape[0], E).scatter_add(1, index.clamp(min=0).long(),
-                                                        torch.where(there, weight, torch.zeros_like(weight)))
+    there, at = _slots(index, E)
+    share = weight.new_zeros(x.shape[0], E).scatter_add(1, at, torch.where(there, weight, torch.zeros_like(weight)))
     v = _wide(x)
     y = torch.zeros_like(v)
     for e in range(E):

@@ -52,3 +52,21 @@ def test_twice_differentiable_forms_sum_in_32_bits(score):
     y = T.expert_mlp(x, index, weight, w_in, w_out)
     y0 = O.expert_mlp(x, index, weight, w_in, w_out)
     assert y.dtype == torch.bfloat16 and float((y.double() - y0).abs().max()) <= 2.0 ** -8 * float(y0.abs().max())
+
+
+def test_an_index_outside_the_experts_adds_nothing():
+    """As the fused operator has it: below 0 and from n_experts on."""
+    g = torch.Generator().manual_seed(5)
+    rn = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    x, w_in, w_out, weight = rn(4, 12), rn(3, 10, 12), rn(3, 12, 5), torch.rand(4, 2, generator=g, dtype=torch.float64)
+    index = torch.tensor([[0, 3], [7, 2], [-1, 2 ** 30], [1, -9]], dtype=torch.int32)
+    x.requires_grad_(True)
+    y, y0 = T.expert_mlp(x, index, weight, w_in, w_out), O.expert_mlp(x, index, weight, w_in, w_out)
+    assert torch.allclose(y, y0, rtol=1e-12, atol=1e-14) and float(y[2].detach().abs().max()) == 0
+    logits = rn(4, 3).requires_grad_(True)
+    picked = T.route_weights(logits, index, "softmax", False, 2.0)
+    want = torch.where((index >= 0) & (index < 3), 2 * torch.softmax(logits, -1).gather(1, index.clamp(0, 2).long()), 0.0)
+    assert torch.allclose(picked, want, rtol=1e-12, atol=0)
+    layer = ExpertReadout(20, 8, 4).layers[0]
+    layer.rebalance(torch.tensor([[0, 4], [9, -1], [0, 2]], dtype=torch.int32), rate=0.5)    # counts 2, 0, 1, 0
+    assert layer.balance.tolist() == [-0.5, 0.5, -0.5, 0.5]
