@@ -241,7 +241,8 @@ def route_weights(logits, index, score: str, renormalise: bool, scale: float):
     """The routing weights of the experts already chosen (``expert_ops.route_experts``' index), differentiable
     in the logits to any order; 0 where the index is none of the experts."""
     there, at = _slots(index, logits.shape[1])
-    logits = _wide(logits)
+    # a row without an expert has no weights, whatever its logits (all -inf have no softmax)
+    logits = torch.where(there.any(1, keepdim=True), _wide(logits), torch.zeros((), device=logits.device))
     s = torch.softmax(logits, -1) if score == "softmax" else torch.sigmoid(logits)
     picked = torch.where(there, s.gather(1, at), torch.zeros((), device=s.device, dtype=s.dtype))
     if renormalise:

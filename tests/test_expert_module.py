@@ -70,3 +70,25 @@ def test_an_index_outside_the_experts_adds_nothing():
     layer = ExpertReadout(20, 8, 4).layers[0]
     layer.rebalance(torch.tensor([[0, 4], [9, -1], [0, 2]], dtype=torch.int32), rate=0.5)    # counts 2, 0, 1, 0
     assert layer.balance.tolist() == [-0.5, 0.5, -0.5, 0.5]
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("renormalise", [False, True])
+def test_rows_with_nothing_to_choose_have_no_gradient(score, renormalise):
+    """A row whose logits are all -inf (and one barred in part) beside ordinary rows: zeros, and so through the second
+    derivative; the other rows' gradient is the formula's."""
+    g = torch.Generator().manual_seed(6)
+    logits = torch.randn(4, 5, generator=g, dtype=torch.float64)
+    logits[1] = -math.inf
+    logits[2, :3] = -math.inf
+    index = O.choose(torch.where(logits > -math.inf, O.scores(logits, score), -math.inf), 2)   # a barred expert is not chosen
+    assert index[1].tolist() == [-1, -1]
+    u = torch.randn(4, 2, generator=g, dtype=torch.float64)
+    leaf = logits.clone().requires_grad_(True)
+    w = T.route_weights(leaf, index, score, renormalise, 1.5)
+    dl, = torch.autograd.grad((w * u).sum(), leaf, create_graph=True)
+    second, = torch.autograd.grad((dl ** 2).sum(), leaf)
+    assert float(w[1].detach().abs().max()) == 0 and float(dl[1].detach().abs().max()) == 0
+    assert torch.isfinite(second).all() and float(second[1].abs().max()) == 0
+    want = O.route_gradient(logits, index, score, renormalise, 1.5, u)
+    assert torch.allclose(dl, want, rtol=1e-12, atol=1e-14)
