@@ -79,16 +79,28 @@ class Router:
             raise ValueError("expert readout: k must be 1 to n_experts")
         if score not in X.SCORES:
             raise ValueError(f"score {score!r}: expected one of {sorted(X.SCORES)}")
-        self.k, self.score, self.n_species = int(k), score, n_species
+        self.k, self.score, self.n_species = int(k), score, None if n_species is None else int(n_species)
         self.groups, self.groups_kept, self.group_best = int(groups), int(groups_kept), int(group_best)
         self.renormalise, self.scale = bool(renormalise), float(scale)
 
-    def logits(self, layer, y, species):
+    def rows_of(self, species, below):
+        """Rows of the layers' tables for the atoms and which atoms have none (None: all have one).  ``below``: what the
+        caller's atomic numbers are known to lie under; where that is not within the tables they are looked at."""
         if self.n_species is None:
-            return F.linear(y, layer.gate)
+            return None, None
         if species is None:
             raise ValueError("this expert readout chooses by atomic number: pass species (N,)")
-        return layer.gate.index_select(0, species)
+        if below is not None and below <= self.n_species:
+            return species, None
+        none = (species < 0) | (species >= self.n_species)
+        return species.masked_fill(none, 0), none.unsqueeze(1)
+
+    def logits(self, layer, y, species, none=None):
+        """Of an atom without a row NaN, which the router passes on to what the atom becomes."""
+        if self.n_species is None:
+            return F.linear(y, layer.gate)
+        l = layer.gate.index_select(0, species)
+        return l if none is None else l.masked_fill(none, math.nan)
 
     def choose(self, layer, logits):
         return X.route_experts(logits, self.k, score=self.score, bias=layer.balance, groups=self.groups,
@@ -112,40 +124,42 @@ class ExpertReadout(nn.Module):
         self.eps = float(eps)
         self.layers = nn.ModuleList([ExpertLayer(width, hidden, n_experts, n_species) for _ in range(layers)])
 
-    def forward(self, x, species=None, differentiable: bool = False):
-        """(N, width) -> (N, width); ``species``: atomic numbers (N,), below n_species.  ``differentiable``: twice
-        differentiable (force losses)."""
+    def forward(self, x, species=None, differentiable: bool = False, species_below: int | None = None):
+        """(N, width) -> (N, width); ``species``: atomic numbers (N,), below n_species (an atom with another becomes NaN).
+        ``differentiable``: twice differentiable (force losses).  ``species_below``: what the caller knows ``species`` to
+        lie under from 0 on, so that they need not be looked at."""
         if x.dtype not in ROW_TYPES:
             raise ValueError(f"expert readout: rows are float32 or bfloat16, got {x.dtype}")
+        rows = self.router.rows_of(species, species_below)
         if differentiable:
-            return self._forward_train(x, species)
+            return self._forward_train(x, rows)
         own = self.layers[0].norm.dtype
         if x.dtype != own:
             out = x
             for layer in self.layers:
                 y, _ = X.rms_norm(out.to(own), layer.norm, eps=self.eps)
-                index, weight = self.router.choose(layer, self.router.logits(layer, y, species))
+                index, weight = self.router.choose(layer, self.router.logits(layer, y, *rows))
                 out = out + X.expert_mlp(y, index, weight, layer.w_in, layer.w_out)
             return out.to(x.dtype)
         z, add = x, None
         for layer in self.layers:
             y, z = X.rms_norm(x, layer.norm, eps=self.eps) if add is None else X.rms_norm(add, layer.norm, z, self.eps)
-            index, weight = self.router.choose(layer, self.router.logits(layer, y, species))
+            index, weight = self.router.choose(layer, self.router.logits(layer, y, *rows))
             add = X.expert_mlp(y, index, weight, layer.w_in, layer.w_out)
         return z + add
 
-    def _forward_train(self, x, species):
+    def _forward_train(self, x, rows):
         from . import train_ops as T
-        own, rows = self.layers[0].norm.dtype, x.dtype
+        own, given = self.layers[0].norm.dtype, x.dtype
         for layer in self.layers:
             y, _ = T.rms_norm(x.to(own), layer.norm, eps=self.eps)
-            logits = self.router.logits(layer, y, species)
+            logits = self.router.logits(layer, y, *rows)
             with torch.no_grad():
                 index, _ = self.router.choose(layer, logits.detach())
             weight = T.route_weights(logits, index, self.router.score, self.router.renormalise,
                                      self.router.scale)
             x = x + T.expert_mlp(y, index, weight, layer.w_in, layer.w_out)
-        return x.to(rows)
+        return x.to(given)
 
     def to_8_bits(self) -> "ExpertReadoutQ8":
         return ExpertReadoutQ8(self)
@@ -171,13 +185,14 @@ class ExpertReadoutQ8(nn.Module):
             self.layers.append(m)
 
     @torch.no_grad()
-    def forward(self, x, species=None, differentiable: bool = False):
+    def forward(self, x, species=None, differentiable: bool = False, species_below: int | None = None):
         if differentiable:
             raise RuntimeError("the 8-bit expert readout has no gradient; train the ExpertReadout it was made from")
+        rows = self.router.rows_of(species, species_below)
         z, add = x.to(torch.bfloat16), None
         for m in self.layers:
             q, scale, z = X.rms_norm_q8(z, m.norm, None, self.eps) if add is None else \
                 X.rms_norm_q8(add, m.norm, z, self.eps)
-            index, weight = self.router.choose(m, self.router.logits(m, q * scale.unsqueeze(-1), species))
+            index, weight = self.router.choose(m, self.router.logits(m, q * scale.unsqueeze(-1), *rows))
             add = X.expert_mlp_q8(q, scale, index, weight, m.w_in, m.w_in_scale, m.w_out, m.w_out_scale)
         return (z.float() + add.float()).to(x.dtype)

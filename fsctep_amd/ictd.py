@@ -314,7 +314,7 @@ class _ICTDTrunk(nn.Module):
             outs.append(sq * factors[i])
         f = torch.cat(outs, dim=-1)
         if self.readout_experts is not None:
-            f = self.readout_experts(f, species, differentiable=train)
+            f = self.readout_experts(f, species, differentiable=train, species_below=self.n_species)
         e = self.weighted_sum(self.proj_total(f)) if train else readout_energy(self.proj_total, self.weighted_sum, f)
         dip = None
         if self._dipole and with_dipole:

@@ -349,7 +349,7 @@ class PureCartesianSparseTransformerLayer(nn.Module):
         invs = (sq.view(-1, len(_COMPS), nL, self.channels) * self._readout_cache[skey]).transpose(1, 2)
         f5 = torch.cat([invs.flatten(1), f3 * f3], dim=-1)
         if self.readout_experts is not None:
-            f5 = self.readout_experts(f5, species, differentiable=train)
+            f5 = self.readout_experts(f5, species, differentiable=train, species_below=self.n_species)
         if train:
             return self.weighted_sum(self.proj_total(f5))
         return readout_energy(self.proj_total, self.weighted_sum, f5)

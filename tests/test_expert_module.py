@@ -92,3 +92,22 @@ def test_rows_with_nothing_to_choose_have_no_gradient(score, renormalise):
     assert torch.isfinite(second).all() and float(second[1].abs().max()) == 0
     want = O.route_gradient(logits, index, score, renormalise, 1.5, u)
     assert torch.allclose(dl, want, rtol=1e-12, atol=1e-14)
+
+
+def test_atomic_numbers_without_a_row():
+    """Looked up nowhere: NaN logits, unless the caller's bound lies within the table."""
+    r = ExpertReadout(20, 8, 4, n_species=5)
+    layer = r.layers[0]
+    species = torch.tensor([0, 4, 5, -1, 2 ** 40, 3])
+    l = r.router.logits(layer, None, *r.router.rows_of(species, None))
+    ok = torch.tensor([True, True, False, False, False, True])
+    assert torch.equal(l[ok], layer.gate.detach()[species[ok]]) and torch.isnan(l[~ok]).all()
+    g, = torch.autograd.grad(l[ok].sum(), layer.gate)
+    assert torch.isfinite(g).all()
+    assert torch.equal(r.router.logits(layer, None, *r.router.rows_of(species[ok], 5)), l[ok])
+    assert r.router.rows_of(species[ok], 5)[1] is None and r.router.rows_of(species[ok], 4)[1] is None
+    l = r.router.logits(layer, None, *r.router.rows_of(species, 100))       # a bound beyond the table: looked at
+    assert torch.isnan(l[~ok]).all() and torch.isfinite(l[ok]).all()
+    for m in (r, r.to_8_bits()):
+        with pytest.raises(ValueError, match="pass species"):
+            m(torch.zeros(6, 20))

@@ -84,3 +84,39 @@ def test_trunk_with_experts_in_bf16():
     assert float((gp + f).detach().norm()) < 2.0 ** -6 * float((f32 - f0).norm()) + 2e-5 * float(f0.norm())
     grads = torch.autograd.grad((gp ** 2).sum(), list(model.readout_experts.parameters()))
     assert all(t.dtype == torch.bfloat16 and torch.isfinite(t).all() and float(t.abs().max()) > 0 for t in grads)
+
+
+@pytest.mark.parametrize("differentiable", [False, True])
+def test_atoms_without_a_row_become_nan(differentiable):
+    """Atomic numbers outside the table, and only they."""
+    m = readout(96, 40, 6, 2, k=2, layers=2, n_species=5)
+    x = torch.randn(64, 96, device=DEV)
+    species = torch.arange(64, device=DEV) % 5
+    want = m(x, species, differentiable=differentiable)
+    for other in (5, -1, 2 ** 40):
+        bad = species.clone()
+        bad[7] = other
+        y = m(x, bad, differentiable=differentiable)
+        assert torch.isnan(y[7]).all()
+        y[7] = want[7]
+        assert rel_inf(y, want) < 2e-5
+    assert torch.isnan(m.to_8_bits()(x, bad)[7]).all()
+
+
+def test_a_trunk_with_experts_that_know_fewer_elements():
+    """Its own elements as with a table of all; an atom of an element beyond the table NaN, no other atom's."""
+    g, model, pos, A, batch, cell, (src, dst, sh) = _system()
+    graph = model.prepare(src, dst, sh, pos.shape[0], A)
+    _attach(model)
+    with torch.no_grad():
+        e0 = model.forward_graph(pos, batch, cell, graph)
+        for known in (int(A.max()) + 1, int(A.max())):
+            full = model.readout_experts
+            few = readout(model.proj_total.input_norm.normalized_shape[0], 48, 4, 3, n_species=known)
+            few.load_state_dict({k: v[:known] if k.endswith("gate") else v for k, v in full.state_dict().items()})
+            model.readout_experts = few
+            e = model.forward_graph(pos, batch, cell, graph)
+            model.readout_experts = full
+            has = A < known
+            assert torch.equal(e[has], e0[has]) and torch.isnan(e[~has]).all()
+    assert not has.all() and has.any()
