@@ -75,4 +75,5 @@ def to_codes(w):
     to half a code."""
     w = w.detach().float()
     scale = w.abs().amax(-1) / 127
-    return torch.round(w / torch.where(scale > 0, scale, 1.0).unsqueeze(-1)).to(torch.int8), scale
+    # (a scale next to the smallest number is a rounded one: its codes may come out above 127)
+    return torch.round(w / torch.where(scale > 0, scale, 1.0).unsqueeze(-1)).clamp(-127, 127).to(torch.int8), scale

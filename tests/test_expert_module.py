@@ -111,3 +111,13 @@ def test_atomic_numbers_without_a_row():
     for m in (r, r.to_8_bits()):
         with pytest.raises(ValueError, match="pass species"):
             m(torch.zeros(6, 20))
+
+
+def test_codes_of_the_smallest_numbers_keep_their_sign():
+    from fsctep_amd.expert_ops import to_codes
+    w = torch.tensor([[190.0, 3.0, -190.0], [127.0, 1.0, -2.0], [0.0, 0.0, 0.0]]) * 2.0 ** -149
+    q, s = to_codes(w)
+    assert q.tolist() == [[127, 3, -127], [127, 1, -2], [0, 0, 0]]
+    q, s = to_codes(w * 2.0 ** 120)
+    assert q.tolist() == [[127, 2, -127], [127, 1, -2], [0, 0, 0]]
+    assert float((q * s.unsqueeze(1) - w * 2.0 ** 120).abs().max()) <= 0.5 * float(s.max())
