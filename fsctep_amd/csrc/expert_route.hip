@@ -281,7 +281,8 @@ __global__ __launch_bounds__(NT) void route_kernel(Args a, bool vec, int group_l
 }
 
 // Gradient of the weights with respect to the logits.  With u the weights' gradient and w = scale s / S:
-//   renormalised: ds_j s_j = w_j (u_j - sum u w / scale); else ds_j s_j = scale s_j u_j = w_j u_j
+//   renormalised: ds_j s_j = w_j (u_j - sum u (w / scale)); else ds_j s_j = scale s_j u_j = w_j u_j
+// (a single choice has w / scale = 1 to the bit, and no gradient)
 //   sigmoid: dl_j = (ds_j s_j)(1 - s_j);  softmax: dl_i = (ds_i s_i) - s_i sum_j ds_j s_j
 // The last sum is zero for renormalised weights, so only sigmoid (the chosen logits) and softmax without
 // renormalisation (all) read the logits again.  The chosen experts' gradients meet the rest of the row in LDS.
@@ -314,7 +315,7 @@ __global__ __launch_bounds__(NT) void route_back_kernel(BackArgs a, bool vec) {
       u = a.dweight[row * a.k + lane];
     }
   }
-  if (a.renorm) u -= row_sum(u * w) / a.scale;
+  if (a.renorm) u -= row_sum(u * (w / a.scale));
   float d = w * u;                             // ds_j s_j
   float o[V];
 #pragma unroll

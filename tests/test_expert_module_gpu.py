@@ -120,3 +120,15 @@ def test_a_trunk_with_experts_that_know_fewer_elements():
             has = A < known
             assert torch.equal(e[has], e0[has]) and torch.isnan(e[~has]).all()
     assert not has.all() and has.any()
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("scale", [1.0, 1.5, 0.3, 2.7])
+def test_a_single_renormalised_choice_has_no_gradient(score, scale):
+    """Its weight is the scale whatever the logits: zero to the bit."""
+    from fsctep_amd import expert_ops as X
+    for experts in (1, 7, 40):
+        l = torch.randn(500, experts, device=DEV, requires_grad=True)
+        index, w = X.route_experts(l, 1, score=score, scale=scale)
+        dl, = torch.autograd.grad(w, l, torch.randn(500, 1, device=DEV))
+        assert torch.equal(w, torch.full_like(w, scale)) and float(dl.abs().max()) == 0
