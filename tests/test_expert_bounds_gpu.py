@@ -8,7 +8,7 @@ import pytest
 import torch
 
 from oracle import experts as O
-from test_experts_gpu import DEV, DT, TOL, close, problem
+from test_experts_gpu import DEV, DT, HANDFUL, MLP, NORM, ROUTE, TILES, TOL, close, problem
 from test_experts_host import Dims
 
 pytestmark = pytest.mark.gpu
@@ -124,3 +124,70 @@ def test_8_bit_products_stay_inside_the_workspaces(rows, width, hidden):
     for b, name in ((plan, "plan"), (ws, "workspace"), (y, "y")):
         b.check(name)
     assert torch.equal(y.t, X.expert_mlp_q8(q, s, i, w, qi, si, qo, so))
+
+
+@pytest.mark.parametrize("rows,width,hidden,experts,k", MLP + TILES + HANDFUL)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_products_stay_inside_their_arrays(rows, width, hidden, experts, k, dtype):
+    p = problem(rows, width, hidden, experts, k, DT[dtype], rows + width)
+    got = run(*(t.to(DEV) for t in p))
+    for a, b, n in zip(got, reference(*p), ("y", "dx", "dweight", "dw_in", "dw_out")):
+        close(a, b, TOL[DT[dtype]], n)
+
+
+@pytest.mark.parametrize("rows,width", NORM)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("residual", [False, True])
+def test_norm_stays_inside_its_arrays(rows, width, dtype, residual):
+    from fsctep_amd import _lib
+    dt, code = DT[dtype], 0 if dtype == "fp32" else 1
+    x, r, dy, dz = (torch.randn(rows, width + 3, device=DEV).to(dt)[:, 1:width + 1] for _ in range(4))
+    w, eps, st = torch.randn(width, device=DEV).to(dt), 1e-6, _lib.stream_handle(DEV)
+    n = ctypes.c_int64()
+    _lib.call("fsc_rms_norm_workspace", rows, width, ctypes.byref(n))
+    like = lambda t=dt, shape=(rows, width): Guarded(shape, t)
+    g = dict(y=like(), z=like(), rstd=like(torch.float32, (rows,)), codes=like(torch.int8), scale=like(torch.float32, (rows,)),
+             z8=like(), dx=like(), dw=like(dt, (width,)), workspace=like(torch.float32, (n.value,)))
+    rp, zp = (r.data_ptr(), g["z"].ptr) if residual else (0, 0)
+    s = width + 3
+    _lib.call("fsc_rms_norm_forward", rows, width, code, code, s, s, x.data_ptr(), rp, w.data_ptr(), eps, g["y"].ptr, zp,
+              g["rstd"].ptr, st)
+    _lib.call("fsc_rms_norm_q8", rows, width, code, code, s, s, x.data_ptr(), rp, w.data_ptr(), eps, g["codes"].ptr,
+              g["scale"].ptr, g["z8"].ptr if residual else 0, st)
+    z, zs = (g["z"].ptr, width) if residual else (x.data_ptr(), s)
+    _lib.call("fsc_rms_norm_backward", rows, width, code, code, zs, s, s, z, w.data_ptr(), g["rstd"].ptr, eps, dy.data_ptr(),
+              dz.data_ptr() if residual else 0, g["dx"].ptr, g["dw"].ptr, g["workspace"].ptr, st)
+    torch.cuda.synchronize()
+    for name, b in g.items():
+        b.check(name)
+    leaf = [t.cpu().double().requires_grad_(True) for t in (x, w, r)]
+    y0, z0 = O.rms_norm(leaf[0], leaf[1], leaf[2] if residual else None, held=dt)
+    heads, gs = ((y0, z0), (dy, dz)) if residual else ((y0,), (dy,))
+    dx0, dw0 = torch.autograd.grad(heads, leaf[:2], [t.cpu().double() for t in gs])
+    for a, b, name in ((g["y"], y0, "y"), (g["dx"], dx0, "dx"), (g["dw"], dw0, "dw")):
+        close(a.t, b, TOL[dt], name)
+
+
+@pytest.mark.parametrize("rows,experts,k,groups,kept,best", ROUTE)
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_router_stays_inside_its_arrays(rows, experts, k, groups, kept, best, dtype):
+    from fsctep_amd import _lib, expert_ops as X
+    dt, code, st = DT[dtype], 0 if dtype == "fp32" else 1, _lib.stream_handle(DEV)
+    l = torch.randn(rows, experts + 5, device=DEV).to(dt)[:, 2:experts + 2]
+    bias = 0.1 * torch.randn(experts, device=DEV)
+    u = torch.randn(rows, k, device=DEV)
+    for score, name in ((0, "softmax"), (1, "sigmoid")):
+        for renormalise in (0, 1):
+            g = dict(index=Guarded((rows, k), torch.int32), weight=Guarded((rows, k), torch.float32), dl=Guarded((rows, experts), dt))
+            _lib.call("fsc_route_experts", rows, experts, code, experts + 5, l.data_ptr(), bias.data_ptr(), k, score, groups, kept,
+                      best, renormalise, 1.5, g["index"].ptr, g["weight"].ptr, st)
+            _lib.call("fsc_route_experts_backward", rows, experts, code, experts + 5, l.data_ptr(), g["index"].ptr,
+                      g["weight"].ptr, u.data_ptr(), k, score, renormalise, 1.5, g["dl"].ptr, st)
+            torch.cuda.synchronize()
+            for what, b in g.items():
+                b.check(what)
+            i, w = X.route_experts(l, k, score=name, bias=bias, groups=groups, groups_kept=kept, group_best=best,
+                                   renormalise=bool(renormalise), scale=1.5)
+            assert torch.equal(i, g["index"].t) and torch.equal(w, g["weight"].t)
+            want = O.route_gradient(l.cpu().double(), i.cpu(), name, bool(renormalise), 1.5, u.cpu().double())
+            close(g["dl"].t, want, 2e-5 if dtype == "fp32" else TOL[dt], "dlogits")

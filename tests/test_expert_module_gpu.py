@@ -4,6 +4,7 @@ layer rounds its rows, hidden values and output, its gradient as many: 2^-6 of t
 import pytest
 import torch
 
+from oracle import experts as O
 from sparse_helpers import rel_inf
 from test_expert_readout_gpu import DEV, _attach, _system, oracle, readout
 
@@ -120,6 +121,78 @@ def test_a_trunk_with_experts_that_know_fewer_elements():
             has = A < known
             assert torch.equal(e[has], e0[has]) and torch.isnan(e[~has]).all()
     assert not has.all() and has.any()
+
+
+@pytest.mark.parametrize("kw", [dict(k=2, layers=2, score="sigmoid", n_species=7), dict(k=2, layers=1),
+                                dict(k=1, layers=2, renormalise=False, scale=2.0, n_species=7)])
+def test_parameter_gradients_of_a_force_loss(kw):
+    """The gradient of sum (d(m(x) . dy)/dx)^2 with respect to every parameter, against 64 bits (1e-4 of the largest value:
+    two derivatives of fp32 sums of 130 x 96 products, 1e-6 of each term)."""
+    m = readout(96, 40, 6, 1, **kw)
+    g = torch.Generator().manual_seed(4)
+    x, dy = torch.randn(130, 96, generator=g), torch.randn(130, 96, generator=g)
+    species = torch.randint(0, 7, (130,), generator=g) if kw.get("n_species") else None
+    p0 = [{n: p.detach().double().cpu().requires_grad_(True) for n, p in layer.named_parameters()} for layer in m.layers]
+    leaf, r = x.double().requires_grad_(True), m.router
+    out = leaf
+    for p, layer in zip(p0, m.layers):
+        y, _ = O.rms_norm(out, p["norm"], eps=m.eps)
+        logits = y @ p["gate"].T if species is None else p["gate"][species]
+        index = O.choose(O.scores(logits.detach(), r.score) + layer.balance.double().cpu(), r.k)
+        out = out + O.expert_mlp(y, index, O.weights(logits, index, r.score, r.renormalise, r.scale), p["w_in"], p["w_out"])
+    f0, = torch.autograd.grad((out * dy.double()).sum(), leaf, create_graph=True)
+    ref = torch.autograd.grad((f0 ** 2).sum(), [p[n] for p in p0 for n in p], allow_unused=True)
+    xd = x.to(DEV).requires_grad_(True)
+    y = m(xd, None if species is None else species.to(DEV), differentiable=True)
+    f, = torch.autograd.grad((y * dy.to(DEV)).sum(), xd, create_graph=True)
+    got = torch.autograd.grad((f ** 2).sum(), [q for layer in m.layers for q in layer.parameters()], allow_unused=True)
+    assert rel_inf(f.detach(), f0.detach()) < 1e-5
+    names = [n for layer in m.layers for n, _ in layer.named_parameters()]
+    assert names == [n for p in p0 for n in p]
+    for n, a, b in zip(names, got, ref):
+        assert (a is None) == (b is None) and (a is None or rel_inf(a, b) < 1e-4), n
+
+
+def test_trunk_energies_in_8_bits_are_near():
+    """The energies' change by 8-bit experts, against what the experts change: their outputs are within 5 %, the head's
+    response to an error that of any direction, four times that at most."""
+    g, model, pos, A, batch, cell, (src, dst, sh) = _system()
+    graph = model.prepare(src, dst, sh, pos.shape[0], A)
+    with torch.no_grad():
+        e0 = model.forward_graph(pos, batch, cell, graph)
+        _attach(model, layers=2)
+        e = model.forward_graph(pos, batch, cell, graph)
+        model.readout_experts = model.readout_experts.to_8_bits()
+        e8 = model.forward_graph(pos, batch, cell, graph)
+    assert float((e8 - e).norm()) < 0.2 * float((e - e0).norm())
+
+
+def test_ictd_forces_with_experts():
+    """The fused path's energies and forces against the twice differentiable torch form of the training step, and against
+    differences of the energy."""
+    from conftest import load_golden
+    from fsctep_amd.ictd import energy_forces
+    from test_ictd_gpu import _model
+    g = load_golden("ictd_open32_c32_l2")
+    model = _attach(_model(g))
+    t = lambda k, dt=None: torch.tensor(g[k], device=DEV, dtype=dt)
+    pos, A, cell = t("pos", torch.float32), t("species"), t("cell", torch.float32)
+    batch = torch.zeros(pos.shape[0], dtype=torch.long, device=DEV)
+    src, dst, sh = t("edge_src"), t("edge_dst"), t("edge_shifts", torch.float32)
+    graph = model.prepare(src, dst, sh, pos.shape[0], A)
+    e, f, _ = energy_forces(model, pos, batch, cell, graph)
+    h, d = 1e-2, torch.randn(pos.shape, generator=torch.Generator().manual_seed(2)).to(DEV)
+    sums = [float(energy_forces(model, pos + s * h * d, batch, cell, graph)[0].double().sum()) for s in (2, 1, -1, -2)]
+    slope = (-sums[0] + 8 * sums[1] - 8 * sums[2] + sums[3]) / (12 * h)
+    assert abs(slope + float((f.double() * d.double()).sum())) < 2e-2 * float(f.double().norm() * d.double().norm())
+    model.train().requires_grad_(True)
+    p = pos.clone().requires_grad_(True)
+    et = model(p, A, batch, src, dst, sh, cell)
+    et = et[0] if isinstance(et, tuple) else et
+    gp, = torch.autograd.grad(et.sum(), p, create_graph=True)
+    assert rel_inf(et.detach().squeeze(-1), e.squeeze(-1) if e.dim() > 1 else e) < 2e-5 and rel_inf(-gp.detach(), f) < 2e-5
+    grads = torch.autograd.grad((gp ** 2).sum(), list(model.readout_experts.parameters()))
+    assert all(torch.isfinite(q).all() and float(q.abs().max()) > 0 for q in grads)
 
 
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
