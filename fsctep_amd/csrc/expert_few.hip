@@ -62,7 +62,8 @@ struct Raw {
 };
 
 // 32 rows of 640, hidden 640, two of eight experts, fp32 (39 MB of weights, 9 us at a copy's rate, read once forward and once
-// backward): up 11.2, down 7.1, dh 11.8, dx 15.0 us; what bounds them is the chain index, weights, rows, LDS of a block.
+// backward): up 11.2, down 7.1, dh 11.8, dx 15.0 us (bf16: 9.4, 6.4, 16.6, 20.6, whose dh and dx strips of 64 columns make 80
+// blocks where fp32's make 160); what bounds them is the chain index, weights, rows, LDS of a block.
 //
 // Whole steps of the reduction run without conditions: a lane past the last column or row reads the last one's
 // values, and what it computes is not stored.  The weights of a wave's first U steps are on their way before the

@@ -22,8 +22,8 @@
 // TFLOP/s of 16-bit products): 10,000 x 640 fp32, hidden 640, two of eight experts, forward and rows' gradient 589 (262);
 // 16,384 x 1,600 bf16, hidden 800, two of 16, forward and all gradients 1,408 (671); 50,000 x 640 in 8 bits, hidden 1,280,
 // two of 16: 590 (219).  What bounds them is the step itself, a chain of loads, barrier, LDS and products in every block:
-// counters show the matrix units 40% busy, no other unit above 50%, half of a wave's time waiting for issue and a quarter
-// for loads.  Larger tiles (128 x 256; 256 x 256 with two LDS buffers), operands copied to LDS without registers or loaded
+// counters show the matrix units 18 to 34% busy, LDS as much, no unit above 50%, a third to a half of a wave's time waiting
+// for issue and a quarter for loads.  Larger tiles (128 x 256; 256 x 256 with two LDS buffers), operands copied to LDS without registers or loaded
 // into them two or three steps ahead, four waves a SIMD, raised priorities in the products, and other orders of the tiles
 // took the same time or more.
 //

@@ -9,7 +9,7 @@
 //                     (n = ceil(M / tile) + min(E, M) bounds their number)
 //   counts  [blocks E] rows of each expert before each block of slots, with many slots
 //
-// Bound by latency (4 bytes in, 16 out for each slot): up to 4,096 slots one launch, 3 to 5 us; above that three, 15 us at
+// Bound by latency (4 bytes in, 16 out for each slot): up to 4,096 slots one launch, 3 to 5 us; above that three, 17 us at
 // 20,000 slots and 20 us at 100,000 (one block alone: 33 and 146 us).
 #include <algorithm>
 
@@ -23,7 +23,7 @@ namespace experts {
 
 constexpr int PT = 1024;            // threads: 16 waves
 constexpr int PW = PT / 64;
-// Slots of a block; up to so many, one block does all (one launch: 20,000 slots took it 33 us, three launches 12 us).
+// Slots of a block; up to so many, one block does all.
 constexpr int BLOCK = 4096;
 
 // The lanes of the wave with the same expert as this one (bits of lanes without an expert clear).

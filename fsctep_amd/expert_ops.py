@@ -60,7 +60,13 @@ def route_experts(logits, k: int, score: str = "softmax", bias=None, groups: int
 def expert_mlp(x, index, weight, w_in, w_out):
     """``y_t = sum_j weight_tj w_out[e] (silu(w_in[e][:F] x_t) * (w_in[e][F:] x_t))`` with e = index_tj, for rows
     x (T, H), index (int32) and weight (float32) (T, k), w_in (E, 2F, H) and w_out (E, H, F) of x's type (float32
-    or bfloat16).  An index outside [0, E) adds nothing."""
+    or bfloat16).  An index outside [0, E) adds nothing.
+
+    Sums are held in 32 bits.  float32 products are made of 16-bit parts: 24 bits of every operand, or, where an expert has
+    more than about 80 rows, 22 bits of values down to 2^-17 of the largest of their row (of the rows) or output column (of
+    the weights).  In bfloat16 the hidden values and their gradients are rounded to bfloat16 between the products where an
+    expert has more than about 32 rows, which makes the error about 1.4 times that of the one rounding at the end; with
+    fewer rows they stay in float32."""
     return torch.ops.fsctep.expert_mlp(x, index, weight, w_in, w_out)
 
 

@@ -12,7 +12,8 @@ at zero, so a trained trunk keeps its energies when one is attached.  The refere
 without one run as before.
 
 * energies and forces: the fused operators, whose gradient with respect to the rows gives the forces;
-* training on energies: the same with the parameters' gradients;
+* training the experts on energies: the same with the parameters' gradients (a trunk in ``eval()`` mode, whose own
+  parameters have none there);
 * training on forces (the trunks' ``train()`` step): ``differentiable=True``, the twice differentiable torch form
   on the experts that the fused router chose;
 * energies alone of many candidates (screening, Monte Carlo): ``ExpertReadout.to_8_bits()``, rows and weights in 8

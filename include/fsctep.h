@@ -566,7 +566,9 @@ int fsc_route_experts_backward(int64_t rows, int32_t n_experts, int32_t dtype, i
 /* The experts' products: y_t = sum_j weight_tj W_out[e] (silu(W_in[e][:F] x_t) * (W_in[e][F:] x_t)), e = index_tj,
  * with w_in [n_experts][2 hidden][width], w_out [n_experts][width][hidden] and index, weight [rows][k]; an index
  * outside [0, n_experts) adds nothing.  dtype of x, w_in, w_out, y and the gradients: FSC_F32 (products as accurate
- * as fp32 ones) or FSC_BF16 (32-bit sums); weight and dweight are fp32.
+ * as fp32 ones) or FSC_BF16 (32-bit sums; hidden values and their gradients held in bf16 where an expert has more than
+ * 32 rows on average, in fp32 otherwise); weight and dweight are fp32.  Rows of x and dy may lie at any stride; fp32
+ * rows by tiles that span 0xF0000000 bytes or more are read value by value.
  * fsc_expert_sizes: int32 of a plan, floats that the forward keeps for the backward, bytes of the two workspaces
  * (64-byte aligned).  fsc_expert_plan sorts the slots by expert (stable); one plan serves forward and backward
  * (with few rows its size is 0 and it may be null).
