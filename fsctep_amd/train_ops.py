@@ -257,9 +257,12 @@ def expert_mlp(x, index, weight, w_in, w_out):
     E, H, f = w_out.shape
     there, at = _slots(index, E)
     share = weight.new_zeros(x.shape[0], E).scatter_add(1, at, torch.where(there, weight, torch.zeros_like(weight)))
-    v = _wide(x)
+    # what no product asks for counts for nothing, infinities and NaN included: rows without an expert, experts without a row
+    zero = torch.zeros((), device=x.device, dtype=x.dtype)
+    v = _wide(torch.where(there.any(1, keepdim=True), x, zero))
+    chosen = torch.zeros(E, device=x.device).scatter_add(0, at.reshape(-1), there.reshape(-1).float()).view(E, 1, 1) > 0
     y = torch.zeros_like(v)
-    for e in range(E):
-        a = v @ _wide(w_in[e]).t()
-        y = y + share[:, e:e + 1] * ((F.silu(a[:, :f]) * a[:, f:]) @ _wide(w_out[e]).t())
+    for e, (wi, wo) in enumerate(zip(*(_wide(torch.where(chosen, w, zero)).unbind(0) for w in (w_in, w_out)))):
+        a = v @ wi.t()
+        y = y + share[:, e:e + 1] * ((F.silu(a[:, :f]) * a[:, f:]) @ wo.t())
     return y.to(x.dtype)

@@ -121,3 +121,24 @@ def test_codes_of_the_smallest_numbers_keep_their_sign():
     q, s = to_codes(w * 2.0 ** 120)
     assert q.tolist() == [[127, 2, -127], [127, 1, -2], [0, 0, 0]]
     assert float((q * s.unsqueeze(1) - w * 2.0 ** 120).abs().max()) <= 0.5 * float(s.max())
+
+
+def test_twice_differentiable_products_keep_what_nobody_asks_for_out():
+    """NaN and infinities in an expert that nobody chose and in a row without an expert: not in the products, not in any
+    gradient of theirs, first or second."""
+    g = torch.Generator().manual_seed(8)
+    rn = lambda *s: torch.randn(*s, generator=g, dtype=torch.float64)
+    x, w_in, w_out, weight = rn(5, 12), rn(3, 10, 12), rn(3, 12, 5), torch.rand(5, 2, generator=g, dtype=torch.float64)
+    index = torch.tensor([[0, 2], [2, -1], [-1, 3], [0, 0], [2, 0]], dtype=torch.int32)
+    dy = rn(5, 12)
+    leaf0 = [t.clone().requires_grad_(True) for t in (x, weight, w_in, w_out)]
+    y0 = O.expert_mlp(leaf0[0], index, *leaf0[1:])
+    first0 = torch.autograd.grad((y0 * dy).sum(), leaf0, create_graph=True)
+    second0 = torch.autograd.grad((first0[0] ** 2).sum(), leaf0)
+    x[2], w_in[1], w_out[1], weight[2, 0] = math.nan, math.inf, math.nan, math.nan
+    leaf = [t.clone().requires_grad_(True) for t in (x, weight, w_in, w_out)]
+    y = T.expert_mlp(leaf[0], index, *leaf[1:])
+    first = torch.autograd.grad((y * dy).sum(), leaf, create_graph=True)
+    second = torch.autograd.grad((first[0] ** 2).sum(), leaf)
+    for a, b in zip((y, *first, *second), (y0, *first0, *second0)):
+        assert torch.allclose(a, b, rtol=1e-11, atol=1e-13)
