@@ -87,6 +87,17 @@ SIGNATURES = {
     "fsc_expert_mlp_forward": [_p, _i64] + [_p] * 10,
     "fsc_expert_mlp_backward": [_p, _i64, _i64] + [_p] * 14,
     "fsc_expert_mlp_q8": [_p, _i64] + [_p] * 12,
+    "fsc_layer_norm_forward": [_i64, _i32, _i32, _i32, _i32, _i64, _p, _p, _p, _f32, _p, _p, _p, _p],
+    "fsc_layer_norm_workspace": [_i64, _i32, _pi64],
+    "fsc_layer_norm_backward": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _p, _p, _p, _f32] + [_p] * 8,
+    "fsc_layer_norm_backward_twice": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _f32] + [_p] * 12,
+    "fsc_embedding_forward": [_i64, _i32, _i64, _i32, _i32, _i64, _p, _p, _f32, _p, _p],
+    "fsc_embedding_workspace": [_i64, _i32, _i64, _pi64],
+    "fsc_embedding_backward": [_i64, _i32, _i64, _i32, _i32, _i64, _p, _p, _f32, _p, _p, _p],
+    "fsc_adamw_workspace": [_i32, _p, _pi64, _pi64],
+    "fsc_grad_norm": [_i32, _p, _p, _p, _p],
+    "fsc_adamw_step": [_i32, _p, _p, _p, _p],
+    "fsc_adamw_values": [_i64, _i32, _p, _p, _p, _p],
 }
 # the fp64 twins of the bucket functions take the same arguments (double arrays)
 SIGNATURES.update({n + "_f64": SIGNATURES[n] for n in (

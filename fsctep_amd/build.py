@@ -57,7 +57,7 @@ def build(verbose: bool = False) -> str:
     tmp = LIB + ".tmp"
     hip_cmd = [hipcc, *HIP_FLAGS, *inc, *sources(), "-o", tmp]
     tinc, tlib = _torch_dirs()
-    torch_srcs = ["torch_ops.cpp", "torch_bucket_ops.cpp", "torch_expert_ops.cpp"]
+    torch_srcs = ["torch_ops.cpp", "torch_bucket_ops.cpp", "torch_expert_ops.cpp", "torch_learn_ops.cpp"]
     objs = [os.path.join(PKG, src.replace(".cpp", ".o.tmp")) for src in torch_srcs]
     torch_ccs = [[hipcc, "-std=c++17", "-O2", "-fPIC", "-c", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                   "-D_GLIBCXX_USE_CXX11_ABI=1", "-I", tinc, "-I", os.path.join(tinc, "torch", "csrc", "api", "include"),

@@ -1,0 +1,168 @@
+"""AdamW on the GPU: one launch for a model's tensors, the gradients clipped by their common norm on the way, states in
+32 or in 8 bits.
+
+    opt = AdamW(model.parameters(), lr=1e-3, weight_decay=0.01, max_norm=1.0)       # a torch.optim.Optimizer
+    loss.backward(); opt.step(); opt.zero_grad()
+    opt.grad_norm                                                                    # of the last step, on the GPU
+
+The formulas are torch.optim.AdamW's (the reference's trainer, training/trainer.py), states of 32 bits have its names,
+so that its checkpoints load.  Parameters are float32, or bfloat16 with a float32 copy ("master") in the state that
+is stepped and rounded.  Step counts live on the GPU and nothing waits for it, so a step can be captured into a graph
+(``lr`` as a float32 tensor then changes between replays).  The ops are registered in C++
+(``csrc/torch_learn_ops.cpp``, kernels ``csrc/adamw.hip``).
+
+States in 8 bits (``state_bits=8``): m and sqrt(v) as 8-bit floats with a float32 scale for each 256 values, rounded
+up or down by a hash of the value's number and the step, so that small changes add up over the steps instead of being
+rounded away.  16 bytes a value are moved in place of 28.
+
+    adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay, max_norm, masters, norm)
+    adamw_step_q8(params, grads, exp_avgs, exp_avg_scales, roots, root_scales, steps, ...)
+    grad_norm(grads) -> norm
+    moment_values(codes, scale), root_values(codes, scale) -> what 8-bit states stand for
+"""
+
+from __future__ import annotations
+
+from . import _lib
+
+_lib.load_torch_ops()
+
+import math  # noqa: E402
+
+import torch  # noqa: E402
+
+GROUP = 256            # values that share a scale
+
+
+@torch.no_grad()
+def grad_norm(grads):
+    """The 2-norm of all values of the gradients (float32 or bfloat16), a float32 on the GPU; sums in 64 bits."""
+    grads = list(grads)
+    if not grads:
+        raise ValueError("grad_norm: no gradients")
+    return torch.ops.fsctep.grad_norm(grads)
+
+
+def _settings(grads, lr, betas, eps, weight_decay, max_norm, norm):
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError(f"betas must lie in [0, 1), got {betas}")
+    if eps < 0 or weight_decay < 0 or (not isinstance(lr, torch.Tensor) and lr < 0):
+        raise ValueError("lr, eps and weight_decay must not be negative")
+    if max_norm is not None and not max_norm > 0:
+        raise ValueError(f"max_norm must be positive, got {max_norm}")
+    if max_norm is None:
+        norm = None
+    elif norm is None and len(grads):
+        norm = torch.ops.fsctep.grad_norm(grads)
+    t = lr if isinstance(lr, torch.Tensor) else None
+    return norm, (norm, t, 0.0 if t is not None else float(lr), float(betas[0]), float(betas[1]), float(eps),
+                  float(weight_decay), 0.0 if max_norm is None else float(max_norm))
+
+
+@torch.no_grad()
+def adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8,
+               weight_decay: float = 1e-2, max_norm: float | None = None, masters=None, norm=None):
+    """One AdamW step in place on lists of contiguous tensors: ``params`` float32 or bfloat16, ``grads`` of their types,
+    moments float32, ``steps`` one float32 value each on the GPU (the steps taken before), ``masters`` float32 copies
+    where a parameter is bfloat16.  ``lr``: a number or one float32 value on the GPU.  ``max_norm``: the gradients
+    count as scaled by min(1, max_norm / (norm + 1e-6)), ``norm`` their norm where the caller has it (of more tensors,
+    say).  Returns the norm (None without ``max_norm``)."""
+    grads = list(grads)
+    norm, rest = _settings(grads, lr, betas, eps, weight_decay, max_norm, norm)
+    lists = [list(t) for t in (params, grads, exp_avgs, exp_avg_sqs, steps, masters or [])]
+    if any(lists):
+        torch.ops.fsctep.adamw_(*lists, *rest)
+    return norm
+
+
+@torch.no_grad()
+def adamw_step_q8(params, grads, exp_avgs, exp_avg_scales, roots, root_scales, steps, lr=1e-3, betas=(0.9, 0.999),
+                  eps: float = 1e-8, weight_decay: float = 1e-2, max_norm: float | None = None, masters=None, norm=None):
+    """``adamw_step`` with states in 8 bits: codes (uint8, as many as values) and scales (float32, one for each 256) of
+    the first moment and of the second moment's root; all zeros at the start."""
+    grads = list(grads)
+    norm, rest = _settings(grads, lr, betas, eps, weight_decay, max_norm, norm)
+    lists = [list(t) for t in (params, grads, exp_avgs, exp_avg_scales, roots, root_scales, steps, masters or [])]
+    if any(lists):
+        torch.ops.fsctep.adamw_q8_(*lists, *rest)
+    return norm
+
+
+def moment_values(codes, scale):
+    """The first moments that 8-bit codes stand for, float32."""
+    return torch.ops.fsctep.adamw_values(codes, scale, False)
+
+
+def root_values(codes, scale):
+    """The second moments' roots that 8-bit codes stand for, float32."""
+    return torch.ops.fsctep.adamw_values(codes, scale, True)
+
+
+class AdamW(torch.optim.Optimizer):
+    """``torch.optim.AdamW`` without its variants, on the GPU, for float32 and bfloat16 parameters (contiguous).
+    ``max_norm`` clips by the norm of all groups' gradients together (``grad_norm`` holds the last one's; a norm that is
+    not finite makes the step what the formulas say, NaN and all).  ``state_bits``: 32 or 8."""
+
+    def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 max_norm: float | None = None, state_bits: int = 32):
+        if state_bits not in (32, 8):
+            raise ValueError(f"state_bits must be 32 or 8, got {state_bits}")
+        _settings([], lr, betas, eps, weight_decay, max_norm, None)
+        self.max_norm, self.state_bits, self.grad_norm = max_norm, int(state_bits), None
+        super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
+
+    def _state(self, p):
+        s = self.state[p]
+        if not s:
+            s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
+            if self.state_bits == 32:
+                for name in ("exp_avg", "exp_avg_sq"):
+                    s[name] = torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+            else:
+                for name in ("exp_avg", "root"):
+                    s[name] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
+                    s[name + "_scale"] = torch.zeros(math.ceil(p.numel() / GROUP), dtype=torch.float32, device=p.device)
+            if p.dtype == torch.bfloat16:
+                s["master"] = p.detach().float()
+        return s
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        groups = [(g, [p for p in g["params"] if p.grad is not None]) for g in self.param_groups]
+        if self.max_norm is not None:
+            grads = [p.grad for _, ps in groups for p in ps]
+            self.grad_norm = grad_norm(grads) if grads else None
+        names = ("exp_avg", "exp_avg_sq") if self.state_bits == 32 else ("exp_avg", "exp_avg_scale", "root", "root_scale")
+        call = adamw_step if self.state_bits == 32 else adamw_step_q8
+        for g, ps in groups:
+            if not ps:
+                continue
+            states = [self._state(p) for p in ps]
+            call(ps, [p.grad for p in ps], *([s[n] for s in states] for n in names), [s["step"] for s in states],
+                 lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], max_norm=self.max_norm,
+                 masters=[s.get("master", p) for s, p in zip(states, ps)], norm=self.grad_norm)
+        return loss
+
+    def load_state_dict(self, state_dict):
+        """Also a checkpoint of ``torch.optim.AdamW`` (states in 32 bits).  States keep their own types, which the base
+        class would cast to the parameter's."""
+        super().load_state_dict(state_dict)
+        held = state_dict["state"]
+        number = {}
+        for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
+            number.update(zip(mine["params"], theirs["params"]))
+        for p, s in self.state.items():
+            for name, value in held[number[p]].items():
+                if name == "step":
+                    s[name] = torch.as_tensor(value, dtype=torch.float32).to(p.device).reshape(()).clone()
+                elif isinstance(value, torch.Tensor):
+                    s[name] = value.detach().to(p.device).clone(memory_format=torch.contiguous_format)
+            if p.dtype == torch.bfloat16 and "master" not in s:
+                s["master"] = p.detach().float()
+            want = {"exp_avg_sq"} if self.state_bits == 32 else {"root", "root_scale", "exp_avg_scale"}
+            if not want <= set(s):
+                raise ValueError(f"the checkpoint's states do not have {self.state_bits} bits")

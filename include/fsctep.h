@@ -595,6 +595,79 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
                       const int32_t* index, const int32_t* plan, const float* weight, const int8_t* w_in, const float* w_in_scale,
                       const int8_t* w_out, const float* w_out_scale, void* workspace, void* y, hipStream_t stream);
 
+/* ------------------------------------------------------------------ training step
+ * What a training step needs beside the tensor products: layer norm, lookups by token, the optimiser.
+ *
+ * Layer norm of `rows` rows of `width` values (last dimension contiguous, row strides in elements), with an optional
+ * SiLU: y = act((x - mean) rstd weight + bias), rstd = 1 / sqrt(mean (x - mean)^2 + eps).  Replaces LayerNorm and SiLU of
+ * MainNet (models/mlp.py:8-66) in the training step.  dtype of x, y, dy, dx, v, grad_x, grad_dy: FSC_F32 or FSC_BF16;
+ * weight, bias and what belongs to them FSC_F32 or the rows' type (weight null: 1, bias null: 0).  Outputs are contiguous.
+ * mean [rows] (64 bits) and rstd [rows] are kept for the gradients (both null: not kept).
+ * Backward: dx (null: not wanted), dweight and dbias (each null: not wanted; either needs the workspace).
+ * Backward of the backward: from cotangents v of dx, v_weight of dweight, v_bias of dbias (each null: 0) the gradients of
+ * x, dy, weight and bias (each null: not wanted).  Sums over rows are in a fixed order. */
+#define FSC_ACT_NONE 0
+#define FSC_ACT_SILU 1
+int fsc_layer_norm_forward(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
+                           int64_t x_stride, const void* x, const void* weight, const void* bias, float eps, void* y,
+                           double* mean, float* rstd, hipStream_t stream);
+int fsc_layer_norm_workspace(int64_t rows, int32_t width, int64_t* floats);
+int fsc_layer_norm_backward(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
+                            int64_t x_stride, int64_t dy_stride, const void* x, const void* weight, const void* bias,
+                            float eps, const double* mean, const float* rstd, const void* dy, void* dx, void* dweight,
+                            void* dbias, float* workspace, hipStream_t stream);
+int fsc_layer_norm_backward_twice(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
+                                  int64_t x_stride, int64_t dy_stride, int64_t v_stride, const void* x,
+                                  const void* weight, const void* bias, float eps, const double* mean,
+                                  const float* rstd, const void* dy, const void* v, const void* v_weight,
+                                  const void* v_bias, void* grad_x, void* grad_dy, void* grad_weight, void* grad_bias,
+                                  float* workspace, hipStream_t stream);
+
+/* Lookup: out[i] = scale table[index[i]] for `rows` tokens (index contiguous, int32 or int64 by index_bits), zeros where
+ * the index lies outside [0, table_rows).  dtype of table and out: FSC_F32 or FSC_BF16; rows of the table at any stride, out
+ * [rows][width] contiguous.  Backward: dtable [table_rows][width] (contiguous, every row written) = scale times the sum
+ * of dy's rows by token, in 32 bits and a fixed order.  The workspace (bytes, 16-byte aligned) is the backward's. */
+int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits,
+                          int64_t table_stride, const void* table, const void* index, float scale, void* out,
+                          hipStream_t stream);
+int fsc_embedding_workspace(int64_t rows, int32_t width, int64_t table_rows, int64_t* bytes);
+int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits,
+                           int64_t dy_stride, const void* dy, const void* index, float scale, void* dtable,
+                           void* workspace, hipStream_t stream);
+
+/* AdamW on `count` tensors at once.  Of each: n values p (dtype FSC_F32, or FSC_BF16 with the float32 copy `master` that is
+ * stepped and rounded to p), the gradient g of p's type, the states, and the number of steps taken, a float32 on the
+ * GPU that the call raises by one.  All arrays contiguous.  With c = min(1, max_norm / (norm + 1e-6)) (norm null: 1):
+ *   g = c g, m = beta1 m + (1 - beta1) g, v = beta2 v + (1 - beta2) g g
+ *   p = p (1 - lr weight_decay) - lr / (1 - beta1^step) m / (sqrt(v) / sqrt(1 - beta2^step) + eps)
+ * bits 32: m and v are float32 [n].  bits 8: m and sqrt(v) are uint8 codes [n] with a float32 scale for each 256 values
+ * ([ceil(n / 256)]), the block's largest.  A code is a floating number, for m a sign, 4 exponent and 3 fraction bits, for
+ * sqrt(v) 4 and 4, the largest code standing for 1 and code 0 for 0; values are rounded up or down by a hash of their
+ * number and the step, so that the mean of the roundings is the value; sqrt(v) above zero has a code above zero, and
+ * a block whose largest is below 2^-100 is zeros.
+ * lr_tensor (a float32 on the GPU, null: lr) takes the place of lr.  workspace: fsc_adamw_workspace bytes.
+ * fsc_grad_norm: norm = sqrt of the sum of all gradients' squares (64-bit sums), a float32 on the GPU.
+ * fsc_adamw_values: the values that codes stand for (root 0: m's, 1: sqrt(v)'s). */
+typedef struct FscAdamTensor {
+  int64_t n;
+  int32_t dtype, pad;
+  void* p;
+  const void* g;
+  void *m, *v;
+  float *m_scale, *v_scale, *master, *step;
+} FscAdamTensor;
+typedef struct FscAdamSettings {
+  double lr, beta1, beta2, eps, weight_decay, max_norm;
+  const float *lr_tensor, *norm;
+  int32_t bits, pad;
+} FscAdamSettings;
+int fsc_adamw_workspace(int32_t count, const FscAdamTensor* tensors, int64_t* step_bytes, int64_t* norm_bytes);
+int fsc_grad_norm(int32_t count, const FscAdamTensor* tensors, void* workspace, float* norm, hipStream_t stream);
+int fsc_adamw_step(int32_t count, const FscAdamTensor* tensors, const FscAdamSettings* settings, void* workspace,
+                   hipStream_t stream);
+int fsc_adamw_values(int64_t n, int32_t root, const uint8_t* codes, const float* scale, float* values,
+                     hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
