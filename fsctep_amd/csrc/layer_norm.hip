@@ -239,6 +239,405 @@ __global__ __launch_bounds__(NT) void wide_twice_kernel(Args a) {
   }
 }
 
+// ---------------------------------------------------------------- a row in the registers of L lanes
+// Lane l of a row's L holds the vectors of 16 bytes c L + l, c < CH; a row is read once.  The last vector of a row whose
+// width no vector divides is read from the row's end back, and its lane takes the values from `skip` on as its own; lanes
+// past the end own none.  Values that are not a lane's own are zeros in every sum.
+template <typename T>
+struct alignas(sizeof(T)) Vec {          // at any address a value may lie at
+  static constexpr int N = 16 / sizeof(T);
+  T t[N];
+};
+
+template <typename T, int L, int CH>
+struct Row {
+  static constexpr int V = Vec<T>::N;
+  int width, lane;
+  bool ragged;                           // some lane owns less than CH vectors
+  __device__ __forceinline__ Row(int w) : width(w), lane(threadIdx.x & (L - 1)), ragged(w != L * CH * V) {}
+  __device__ __forceinline__ int base(int c) const { return std::min((c * L + lane) * V, width - V); }
+  __device__ __forceinline__ int skip(int c) const { return (c * L + lane) * V - base(c); }
+
+  template <typename S>
+  __device__ __forceinline__ void load_one(const S* p, int c, float (&v)[V]) const {
+    if constexpr (sizeof(S) == sizeof(T)) {
+      const Vec<S> k = *reinterpret_cast<const Vec<S>*>(p + base(c));
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = to_f(k.t[j]);
+    } else {                             // float32 weights of bfloat16 rows
+#pragma unroll
+      for (int h = 0; h < V; h += 4) {
+        const Vec<float> k = *reinterpret_cast<const Vec<float>*>(p + base(c) + h);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[h + j] = k.t[j];
+      }
+    }
+  }
+  template <typename S>
+  __device__ __forceinline__ void load(const S* p, float (&v)[CH][V]) const {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) load_one(p, c, v[c]);
+  }
+  template <typename S>
+  __device__ __forceinline__ void load_or(const S* p, float other, float (&v)[CH][V]) const {
+    if (p) {
+      load(p, v);
+      return;
+    }
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[c][j] = other;
+  }
+  // zeros for what is not the lane's own
+  template <typename F>
+  __device__ __forceinline__ void own(F (&v)[CH][V]) const {
+    if (!ragged) return;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[c][j] = j >= skip(c) ? v[c][j] : F(0);
+  }
+  template <typename F>
+  __device__ __forceinline__ void store(T* p, int c, const F (&v)[V]) const {
+    const int s = skip(c);
+    if (s == 0) {
+      Vec<T> k;
+#pragma unroll
+      for (int j = 0; j < V; ++j) k.t[j] = from_f<T>((float)v[j]);
+      *reinterpret_cast<Vec<T>*>(p + base(c)) = k;
+    } else if (s < V) {
+#pragma unroll
+      for (int j = 1; j < V; ++j)
+        if (j >= s) p[base(c) + j] = from_f<T>((float)v[j]);
+    }
+  }
+};
+
+// Sums of N values over a row's lanes, the same in each.  A row of a whole block's lanes meets in LDS, in two places by
+// turns: who still reads the one has not passed the barrier before the next but one sum.
+template <int L, typename F>
+struct RowAdd {
+  F* red;                                // [2][5][NW] where a row takes the block
+  int turn = 0;
+  __device__ __forceinline__ explicit RowAdd(F* r) : red(r) {}
+  template <int N>
+  __device__ __forceinline__ void operator()(F (&v)[N]) {
+#pragma unroll
+    for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off, 64);
+    if constexpr (L == NT) {
+      F* at = red + turn * 5 * NW;
+      turn ^= 1;
+      if ((threadIdx.x & 63) == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) at[i * NW + (threadIdx.x >> 6)] = v[i];
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = (at[i * NW] + at[i * NW + 1]) + (at[i * NW + 2] + at[i * NW + 3]);
+    }
+  }
+};
+
+// A 64-bit mean in two 32-bit parts: deviations keep their own accuracy, far from zero and next to the mean.
+__device__ __forceinline__ void parts_of(double mean, float& hi, float& lo) {
+  hi = (float)mean;
+  lo = (float)(mean - (double)hi);
+}
+
+template <typename T, typename W, bool SILU, int L, int CH>
+__global__ __launch_bounds__(NT) void row_kernel(Args a) {
+  using R = Row<T, L, CH>;
+  constexpr int V = R::V;
+  __shared__ double red64[L == NT ? 2 * 5 * NW : 1];
+  __shared__ float red32[L == NT ? 2 * 5 * NW : 1];
+  RowAdd<L, double> add64(red64);
+  RowAdd<L, float> add32(red32);
+  const int64_t row = ((int64_t)blockIdx.x * NT + threadIdx.x) / L;
+  if (row >= a.rows) return;
+  const R at(a.width);
+  float x[CH][V], w[CH][V], b[CH][V];
+  at.load((const T*)a.x + row * a.xs, x);
+  at.load_or((const W*)a.w, 1.f, w);
+  at.load_or((const W*)a.b, 0.f, b);
+  double s[1] = {0.0};
+  float t[1] = {0.f}, hi, lo;
+  at.own(x);
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) s[0] += (double)x[c][j];
+  add64(s);
+  const double mean = s[0] / a.width;
+  parts_of(mean, hi, lo);
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) x[c][j] = (x[c][j] - hi) - lo;
+  at.own(x);
+#pragma unroll
+  for (int c = 0; c < CH; ++c)
+#pragma unroll
+    for (int j = 0; j < V; ++j) t[0] += x[c][j] * x[c][j];
+  add32(t);
+  const float rstd = 1.f / sqrtf(t[0] / a.width + a.eps);
+  T* y = (T*)a.y + row * a.width;
+#pragma unroll
+  for (int c = 0; c < CH; ++c) {
+    float o[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) o[j] = act0<SILU>(x[c][j] * rstd * w[c][j] + b[c][j]);
+    at.store(y, c, o);
+  }
+  if (at.lane == 0 && a.mean) {
+    a.mean[row] = mean;
+    a.rstd[row] = rstd;
+  }
+}
+
+// (x - mean) and the root's factor of the row in x; own values alone
+template <typename T, typename F, int L, int CH, int V>
+__device__ __forceinline__ F deviations(const Args& a, const Row<T, L, CH>& at, RowAdd<L, F>& row_add, int64_t row,
+                                        const float (&x)[CH][V], F (&c_)[CH][V]) {
+  const double mean = a.mean[row];
+  if constexpr (sizeof(F) == 4) {
+    float hi, lo;
+    parts_of(mean, hi, lo);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) c_[c][j] = (x[c][j] - hi) - lo;
+    return a.rstd[row];
+  } else {
+    double s[1] = {0.0};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) c_[c][j] = (double)x[c][j] - mean;
+    at.own(c_);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[0] += c_[c][j] * c_[c][j];
+    row_add(s);
+    return 1.0 / sqrt(s[0] / a.width + (double)a.eps);
+  }
+}
+
+// Adds a lane's sums of the weight's and the bias' gradients over the wave's rows and the block's waves: a partial row
+// for the block.
+template <typename T, int L, int CH, int V>
+__device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at, float (&gw)[CH][V], float (&gb)[CH][V],
+                                         float* buf) {
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.width;
+  if constexpr (L == NT) {               // the block's rows were this thread's own
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        if (j >= at.skip(c)) {
+          part[at.base(c) + j] = gw[c][j];
+          part[a.width + at.base(c) + j] = gb[c][j];
+        }
+    return;
+  }
+  const int wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = L; off < 64; off <<= 1)
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        gw[c][j] += __shfl_xor(gw[c][j], off, 64);
+        gb[c][j] += __shfl_xor(gb[c][j], off, 64);
+      }
+#pragma unroll 1
+  for (int k = 0; k < NW; ++k) {
+    if (wave == k && (threadIdx.x & 63) < L) {
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j >= at.skip(c)) {
+            const int i = at.base(c) + j;
+            buf[i] = k ? buf[i] + gw[c][j] : gw[c][j];
+            buf[a.width + i] = k ? buf[a.width + i] + gb[c][j] : gb[c][j];
+          }
+    }
+    __syncthreads();
+  }
+  for (int i = threadIdx.x; i < 2 * a.width; i += NT) part[i] = buf[i];
+}
+
+template <typename T, typename W, bool SILU, typename F, int L, int CH>
+__global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
+  using R = Row<T, L, CH>;
+  constexpr int V = R::V;
+  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
+  __shared__ F red[L == NT ? 2 * 5 * NW : 1];
+  RowAdd<L, F> row_add(red);
+  const R at(a.width);
+  float w[CH][V], b[CH][V], gw[CH][V] = {}, gb[CH][V] = {};
+  at.load_or((const W*)a.w, 1.f, w);
+  if (SILU) at.load_or((const W*)a.b, 0.f, b);
+  const int64_t step = (int64_t)gridDim.x * (NT / L);
+  // every lane of a wave goes round as often: rows past the last one count as zeros and are not stored
+  const int64_t r0 = ((int64_t)blockIdx.x * NT + threadIdx.x) / L, lead = ((int64_t)blockIdx.x * NT + (threadIdx.x & ~63)) / L;
+  for (int64_t k = 0; lead + k < a.rows; k += step) {
+    const bool there = r0 + k < a.rows;
+    const int64_t row = there ? r0 + k : a.rows - 1;
+    float x[CH][V], d[CH][V];
+    at.load((const T*)a.x + row * a.xs, x);
+    at.load((const T*)a.dy + row * a.ys, d);
+    F z[CH][V], g[CH][V];
+    const F r = deviations<T, F, L, CH, V>(a, at, row_add, row, x, z);
+    at.own(d);
+    at.own(z);
+    F s[2] = {F(0), F(0)};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        z[c][j] *= r;
+        F d1, d2, du = (F)d[c][j];
+        if (SILU) {
+          act12<SILU>(z[c][j] * (F)w[c][j] + (F)b[c][j], d1, d2);
+          du *= d1;
+        }
+        if (there) {
+          gw[c][j] += (float)(du * z[c][j]);
+          gb[c][j] += (float)du;
+        }
+        g[c][j] = du * (F)w[c][j];
+        s[0] += g[c][j];
+        s[1] += g[c][j] * z[c][j];
+      }
+    if (!a.dx) continue;
+    row_add(s);
+    const F mg = s[0] / (F)a.width, mgz = s[1] / (F)a.width;
+    if (there)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        F o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = r * (g[c][j] - mg - z[c][j] * mgz);
+        at.store((T*)a.dx + row * a.width, c, o);
+      }
+  }
+  if (a.part) put_part<T, L, CH, V>(a, at, gw, gb, buf);
+}
+
+template <typename T, typename W, bool SILU, typename F, int L, int CH>
+__global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
+  using R = Row<T, L, CH>;
+  constexpr int V = R::V;
+  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
+  __shared__ F red[L == NT ? 2 * 5 * NW : 1];
+  RowAdd<L, F> row_add(red);
+  const R at(a.width);
+  float w[CH][V], b[CH][V], gw[CH][V] = {}, gb[CH][V] = {};
+  at.load_or((const W*)a.w, 1.f, w);
+  if (SILU) at.load_or((const W*)a.b, 0.f, b);
+  const F n = (F)a.width;
+  const int64_t step = (int64_t)gridDim.x * (NT / L);
+  const int64_t r0 = ((int64_t)blockIdx.x * NT + threadIdx.x) / L, lead = ((int64_t)blockIdx.x * NT + (threadIdx.x & ~63)) / L;
+  for (int64_t i = 0; lead + i < a.rows; i += step) {
+    const bool there = r0 + i < a.rows;
+    const int64_t row = there ? r0 + i : a.rows - 1;
+    float x[CH][V], d[CH][V], v[CH][V];
+    at.load((const T*)a.x + row * a.xs, x);
+    at.load((const T*)a.dy + row * a.ys, d);
+    at.load_or(a.v ? (const T*)a.v + row * a.vs : nullptr, 0.f, v);
+    F z[CH][V];
+    const F r = deviations<T, F, L, CH, V>(a, at, row_add, row, x, z);
+    at.own(d);
+    at.own(v);
+    at.own(z);
+    F s[5] = {F(0), F(0), F(0), F(0), F(0)};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        z[c][j] *= r;
+        F d1, d2, g = (F)d[c][j] * (F)w[c][j];
+        if (SILU) {
+          act12<SILU>(z[c][j] * (F)w[c][j] + (F)b[c][j], d1, d2);
+          g *= d1;
+        }
+        const F q = (F)v[c][j];
+        s[0] += g;
+        s[1] += g * z[c][j];
+        s[2] += q;
+        s[3] += q * z[c][j];
+        s[4] += g * q;
+      }
+    row_add(s);
+    const F mg = s[0] / n, mgz = s[1] / n, mv = s[2] / n, mvz = s[3] / n;
+    const F turn = r * (s[4] / n - mg * mv - mgz * mvz);
+    F k[CH][V], t[2] = {F(0), F(0)};
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      F gdy[V];
+      float vw[V] = {}, vb[V] = {};
+      if (a.vw) at.load_one((const W*)a.vw, c, vw);
+      if (a.vb) at.load_one((const W*)a.vb, c, vb);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        F d1 = F(1), d2 = F(0);
+        const F wi = (F)w[c][j], dj = (F)d[c][j], zj = z[c][j];
+        if (SILU) act12<SILU>(zj * wi + (F)b[c][j], d1, d2);
+        const F du = dj * d1, q = r * ((F)v[c][j] - mv - zj * mvz);
+        const F aa = wi * q + (F)vw[j] * zj + (F)vb[j], e = dj * d2 * aa;
+        gdy[j] = d1 * aa;
+        if (there) {
+          gw[c][j] += (float)(du * q + e * zj);
+          gb[c][j] += (float)e;
+        }
+        k[c][j] = e * wi + du * (F)vw[j] - r * (du * wi * mvz + (F)v[c][j] * mgz);
+        t[0] += k[c][j];
+        t[1] += k[c][j] * zj;
+      }
+      if (a.gdy && there) at.store((T*)a.gdy + row * a.width, c, gdy);
+    }
+    if (!a.gx) continue;
+    row_add(t);
+    const F mk = t[0] / n, mkz = t[1] / n + turn;
+    if (there)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        F o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = r * (k[c][j] - mk - z[c][j] * mkz);
+        at.store((T*)a.gx + row * a.width, c, o);
+      }
+  }
+  if (a.part) put_part<T, L, CH, V>(a, at, gw, gb, buf);
+}
+
+// Calls f(L, CH) for the fewest lanes and vectors that hold a row; false where none do (a row shorter than a vector, or too wide).
+template <typename T, typename F>
+bool by_shape(int width, F&& f) {
+  constexpr int V = Vec<T>::N;
+#define FSC_LN_SHAPE(L_, CH_)                                                               \
+  if (width <= L_ * CH_ * V) {                                                              \
+    f(std::integral_constant<int, L_>{}, std::integral_constant<int, CH_>{});               \
+    return true;                                                                            \
+  }
+  if (width < V) return false;
+  FSC_LN_SHAPE(16, 1)
+  FSC_LN_SHAPE(32, 1)
+  FSC_LN_SHAPE(64, 1)
+  FSC_LN_SHAPE(64, 2)
+  if constexpr (V == 4) {
+    FSC_LN_SHAPE(64, 3)
+  }
+  FSC_LN_SHAPE(256, 1)
+  FSC_LN_SHAPE(256, 2)
+#undef FSC_LN_SHAPE
+  return false;
+}
+
 // Column sums of the blocks' partial rows, the weight's gradient and the bias': 32 columns a block, 32 threads a column,
 // then a fixed tree (the same sum every time).  blockIdx.y: which of the two.
 template <typename W>
@@ -273,17 +672,35 @@ void launch_forward(const Args& all, hipStream_t st) {
       a.mean = all.mean + r0;
       a.rstd = all.rstd + r0;
     }
-    wide_kernel<T, W, SILU><<<(unsigned)a.rows, NT, 0, st>>>(a);
+    if (!by_shape<T>(a.width, [&](auto L, auto CH) {
+          constexpr int l = decltype(L)::value, ch = decltype(CH)::value;
+          row_kernel<T, W, SILU, l, ch><<<(unsigned)((a.rows * l + NT - 1) / NT), NT, 0, st>>>(a);
+        }))
+      wide_kernel<T, W, SILU><<<(unsigned)a.rows, NT, 0, st>>>(a);
   }
 }
 
 template <typename T, typename W, bool SILU>
 void launch_backward(const Args& a, bool twice, W* dw, W* db, hipStream_t st) {
   const int blocks = back_blocks(a.rows);
-  if (a.width <= 64) {
+  const bool done = by_shape<T>(a.width, [&](auto L, auto CH) {
+    constexpr int l = decltype(L)::value, ch = decltype(CH)::value;
+    if constexpr (l == 16) {
+      if (a.width <= 64) {
+        if (twice) row_twice_kernel<T, W, SILU, double, l, ch><<<blocks, NT, 0, st>>>(a);
+        else row_back_kernel<T, W, SILU, double, l, ch><<<blocks, NT, 0, st>>>(a);
+        return;
+      }
+    }
+    if constexpr (l > 16 || sizeof(T) == 2) {
+      if (twice) row_twice_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
+      else row_back_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
+    }
+  });
+  if (!done && a.width <= 64) {
     if (twice) wide_twice_kernel<T, W, SILU, double><<<blocks, NT, 0, st>>>(a);
     else wide_back_kernel<T, W, SILU, double><<<blocks, NT, 0, st>>>(a);
-  } else {
+  } else if (!done) {
     if (twice) wide_twice_kernel<T, W, SILU, float><<<blocks, NT, 0, st>>>(a);
     else wide_back_kernel<T, W, SILU, float><<<blocks, NT, 0, st>>>(a);
   }
