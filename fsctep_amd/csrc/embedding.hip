@@ -15,6 +15,13 @@ namespace embed {
 
 constexpr int NT = 256;
 
+// runs the statement with FULL whether the condition holds
+#define FSC_EMBED_FULL(condition, ...)                           \
+  {                                                              \
+    if (condition) { constexpr bool FULL = true; __VA_ARGS__; }  \
+    else { constexpr bool FULL = false; __VA_ARGS__; }           \
+  }
+
 struct Args {
   int64_t rows, stride;        // row stride of the table (forward) or of dy (backward), in elements
   int64_t table_rows;
@@ -24,98 +31,85 @@ struct Args {
   void* out;
 };
 
-// A vector of 16 bytes at any address a value may lie at.
 template <typename T>
-struct alignas(sizeof(T)) Vec {
-  static constexpr int N = 16 / sizeof(T);
-  T t[N];
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);     // values of a vector
 };
-// n values from p on (all of them by one load where n is a vector's), zeros behind them
-template <typename T>
-__device__ __forceinline__ void load_some(const T* p, int n, float (&v)[Vec<T>::N]) {
-  constexpr int N = Vec<T>::N;
-  if (n >= N) {
-    const Vec<T> k = *reinterpret_cast<const Vec<T>*>(p);
+// A vector of M values from p on, by one load; not FULL: a row shorter than a vector, n values and zeros behind them.  FULL is known
+// when the kernel is compiled: a branch at every load would have each wait for the one before.
+template <bool FULL, int M, typename T>
+__device__ __forceinline__ void load_some(const T* p, int n, float (&v)[M]) {
+  if constexpr (FULL) {
+    struct alignas(sizeof(T)) Pack { T t[M]; };
+    const Pack k = *reinterpret_cast<const Pack*>(p);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = to_f(k.t[j]);
+    for (int j = 0; j < M; ++j) v[j] = to_f(k.t[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = j < n ? to_f(p[j]) : 0.f;
+    for (int j = 0; j < M; ++j) v[j] = j < n ? to_f(p[j < n ? j : 0]) : 0.f;
   }
 }
-template <typename T>
-__device__ __forceinline__ void store_some(T* p, int n, const float (&v)[Vec<T>::N]) {
-  constexpr int N = Vec<T>::N;
-  if (n >= N) {
-    Vec<T> k;
+template <bool FULL, int M, typename T>
+__device__ __forceinline__ void store_some(T* p, int n, const float (&v)[M]) {
+  if constexpr (FULL) {
+    struct alignas(sizeof(T)) Pack { T t[M]; };
+    Pack k;
 #pragma unroll
-    for (int j = 0; j < N; ++j) k.t[j] = from_f<T>(v[j]);
-    *reinterpret_cast<Vec<T>*>(p) = k;
+    for (int j = 0; j < M; ++j) k.t[j] = from_f<T>(v[j]);
+    *reinterpret_cast<Pack*>(p) = k;
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+    for (int j = 0; j < M; ++j)
       if (j < n) p[j] = from_f<T>(v[j]);
   }
 }
 
 // ---------------------------------------------------------------- lookup
-// The output is written as one array, 16 bytes a thread and store whatever the width: a thread's values lie in one row
-// and come by one load, but for those that a row's end parts.  STEPS stores a thread, a block's width apart.
+// A row's vector a thread, STEPS of them a block's width apart.  Where no vector divides the width, a row's last one lies at
+// its end and writes some of the values before it once more (the same ones); rows shorter than a vector are one
+// vector that is not full.
 constexpr int STEPS = 4;
-template <typename T, typename I>
-__global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first) {
+template <typename T, typename I, bool FULL>
+__global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint32_t vectors) {
   constexpr int N = Vec<T>::N;
-  const int64_t total = a.rows * a.width;
-  const int64_t f0 = first + (int64_t)blockIdx.x * (NT * N * STEPS);      // the block's first value, in row r0
-  const int64_t r0 = f0 / a.width;
-  const uint32_t c0 = (uint32_t)(f0 - r0 * a.width), width = a.width;
+  const int64_t total = a.rows * vectors;
+  const int64_t f0 = first + (int64_t)blockIdx.x * (NT * STEPS);         // the block's first vector, in row r0
+  const int64_t r0 = f0 / vectors;
+  const uint32_t c0 = (uint32_t)(f0 - r0 * vectors);
+  const int n = FULL ? N : a.width;
+  float v[STEPS][N];
+  int64_t row[STEPS], t[STEPS];
+  int col[STEPS];
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s) {      // vectors past the last one: the last one again, not stored
+    const int64_t f = std::min<int64_t>(f0 + s * NT + threadIdx.x, total - 1);
+    const uint32_t local = c0 + (uint32_t)(f - f0), up = local / vectors;
+    row[s] = r0 + up;
+    col[s] = std::min((int)(local - up * vectors) * N, a.width - n);
+    t[s] = ((const I*)a.index)[row[s]];
+  }
 #pragma unroll
   for (int s = 0; s < STEPS; ++s) {
-    const uint32_t local = c0 + (s * NT + threadIdx.x) * N;
-    const int64_t f = f0 + (s * NT + threadIdx.x) * N;
-    if (f >= total) return;
-    const uint32_t up = local / width;
-    int64_t row = r0 + up;
-    uint32_t col = local - up * width;
-    const int n = (int)std::min<int64_t>(N, total - f);
-    float v[N];
-    if (col + n <= width) {
-      const int64_t t = ((const I*)a.index)[row];
-      if (t >= 0 && t < a.table_rows) {
-        load_some((const T*)a.in + t * a.stride + col, n, v);
+    const bool there = t[s] >= 0 && t[s] < a.table_rows;
+    load_some<FULL, N>((const T*)a.in + (there ? t[s] : 0) * a.stride + col[s], n, v[s]);
 #pragma unroll
-        for (int j = 0; j < N; ++j) v[j] *= a.scale;
-      } else {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = 0.f;
-      }
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        v[j] = 0.f;
-        if (j >= n) continue;
-        const int64_t t = ((const I*)a.index)[row];
-        if (t >= 0 && t < a.table_rows) v[j] = a.scale * to_f(((const T*)a.in)[t * a.stride + col]);
-        if (++col == width) {
-          col = 0;
-          ++row;
-        }
-      }
-    }
-    store_some((T*)a.out + f, n, v);
+    for (int j = 0; j < N; ++j) v[s][j] = there ? a.scale * v[s][j] : 0.f;
   }
+#pragma unroll
+  for (int s = 0; s < STEPS; ++s)
+    if (f0 + s * NT + threadIdx.x < total) store_some<FULL, N>((T*)a.out + row[s] * a.width + col[s], n, v[s]);
 }
 
 // ---------------------------------------------------------------- gradient, few tokens
 // Up to FEW tokens: a block owns a row of the table and a vector a lane of its columns, its four waves look through a
 // quarter of the tokens each, 64 at a time, and add the rows they find; one launch, no sort.
 constexpr int FEW = 1024;
-template <typename T, typename I>
+template <typename T, typename I, bool FULL>
 __global__ __launch_bounds__(NT) void few_kernel(Args a) {
   constexpr int N = Vec<T>::N, AHEAD = 4;
   __shared__ float red[NT / 64][64 * N];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int col = (blockIdx.y * 64 + lane) * N, n = std::max(0, std::min(N, a.width - col));
+  const int n = FULL ? N : a.width, first = (blockIdx.y * 64 + lane) * N, col = std::min(first, a.width - n);
   const int per = (int)((a.rows + 255) / 256) * 64;
   const int i0 = std::min<int>(a.rows, wave * per), i1 = std::min<int>(a.rows, i0 + per);
   for (int64_t v = blockIdx.x; v < a.table_rows; v += gridDim.x) {
@@ -125,35 +119,105 @@ __global__ __launch_bounds__(NT) void few_kernel(Args a) {
     for (int b = i0; b < i1; b += 64) {
       const int i = b + lane;
       uint64_t hits = __ballot(i < i1 && (int64_t)((const I*)a.index)[std::min(i, i1 - 1)] == v);
-      while (hits) {                     // AHEAD rows on their way together
-        int at[AHEAD], m = 0;
-#pragma unroll
-        for (int k = 0; k < AHEAD; ++k) {
-          at[k] = hits ? b + __ffsll((unsigned long long)hits) - 1 : -1;
-          m += hits != 0;
-          hits &= hits - 1;
-        }
+      while (hits) {                     // AHEAD rows on their way together, the last one again where there are fewer
+        int at = 0, m = 0;
         float u[AHEAD][N];
 #pragma unroll
-        for (int k = 0; k < AHEAD; ++k)
-          if (at[k] >= 0) load_some((const T*)a.in + at[k] * a.stride + col, n, u[k]);
+        for (int k = 0; k < AHEAD; ++k) {
+          at = hits ? b + __ffsll((unsigned long long)hits) - 1 : at;
+          m += hits != 0;
+          hits &= hits - 1;
+          load_some<FULL, N>((const T*)a.in + at * a.stride + col, n, u[k]);
+        }
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k)
-          if (k < m)
 #pragma unroll
-            for (int j = 0; j < N; ++j) s[j] += u[k][j];
+          for (int j = 0; j < N; ++j) s[j] = k < m ? s[j] + u[k][j] : s[j];
       }
     }
 #pragma unroll
     for (int j = 0; j < N; ++j) red[wave][lane * N + j] = s[j];
     __syncthreads();
-    if (wave == 0 && n > 0) {
+    if (wave == 0 && first < a.width) {
 #pragma unroll
       for (int j = 0; j < N; ++j)
         s[j] = a.scale * ((red[0][lane * N + j] + red[1][lane * N + j]) + (red[2][lane * N + j] + red[3][lane * N + j]));
-      store_some((T*)a.out + v * a.width + col, n, s);
+      store_some<FULL, N>((T*)a.out + v * a.width + col, n, s);
     }
     __syncthreads();
+  }
+}
+
+// ---------------------------------------------------------------- gradient, small tables
+// Up to SMALL table rows: no sort.  Every group of lanes adds the rows it streams through, in order and AHEAD on their way, to its
+// own copy of 256 columns of the table in LDS; a block's copies are added to a partial table, and those by small_join_kernel.
+constexpr int SMALL = 32;
+inline int small_waves(int64_t table_rows) { return table_rows <= 16 ? 4 : 2; }       // at most 64 KB of copies a block
+struct Stream {
+  int lanes;                             // of a row's columns: four values each, 256 at most for the group
+  int64_t range;                         // rows of a block
+  float* part;                           // [gridDim.x][table_rows][width]
+};
+
+template <typename T, typename I, bool FULL>
+__global__ __launch_bounds__(NT) void small_kernel(Args a, Stream s) {
+  extern __shared__ __align__(16) float copies[];
+  constexpr int AHEAD = 8;
+  const int lane = threadIdx.x & 63, L = s.lanes, rows = (int)a.table_rows;
+  const int group = threadIdx.x / L, groups = blockDim.x / L;
+  const int n = FULL ? 4 : a.width, first = 4 * (lane & (L - 1)), c0 = blockIdx.y * 256;
+  const int col = std::min(c0 + first, a.width - n);                     // a row's last vector lies at its end
+  float* mine = copies + (int64_t)group * rows * L * 4 + first;          // a row of a copy: L vectors
+  for (int i = threadIdx.x; i < groups * rows * L * 4; i += blockDim.x) copies[i] = 0.f;
+  __syncthreads();
+  const int64_t r0 = blockIdx.x * s.range, r1 = std::min<int64_t>(r0 + s.range, a.rows);
+  const T* in = (const T*)a.in + col;
+  for (int64_t r = r0 + group; r < r1; r += groups * AHEAD) {
+    int64_t t[AHEAD];
+    float v[AHEAD][4];
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k) {    // rows past the last one: the last one again, not added
+      const int64_t q = std::min<int64_t>(r + k * groups, r1 - 1);
+      t[k] = (int64_t)((const I*)a.index)[q];
+      load_some<FULL, 4>(in + q * a.stride, n, v[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < AHEAD; ++k)
+      if (r + k * groups < r1 && t[k] >= 0 && t[k] < rows) {
+        f4* at = reinterpret_cast<f4*>(mine + (int)t[k] * (L * 4));
+        *at = *at + f4{v[k][0], v[k][1], v[k][2], v[k][3]};
+      }
+  }
+  __syncthreads();
+  float* part = s.part + (int64_t)blockIdx.x * rows * a.width;
+  const int vectors = std::min(64, (a.width - c0 + 3) / 4);
+  for (int i = threadIdx.x; i < rows * L; i += blockDim.x) {
+    const int row = i / L, k = i - row * L;
+    if (k >= vectors) continue;
+    f4 x = {0.f, 0.f, 0.f, 0.f};
+    for (int g = 0; g < groups; ++g) x += *reinterpret_cast<const f4*>(copies + ((int64_t)(g * rows + row) * L + k) * 4);
+    const float o[4] = {x.x, x.y, x.z, x.w};
+    store_some<FULL, 4>(part + (int64_t)row * a.width + std::min(c0 + 4 * k, a.width - n), n, o);
+  }
+}
+
+// Adds the partial tables: 64 values a block, 16 waves over the tables, in a fixed order.
+template <typename T>
+__global__ __launch_bounds__(1024) void small_join_kernel(Args a, const float* __restrict__ part, int n) {
+  __shared__ float red[16][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t values = a.table_rows * a.width, at = (int64_t)blockIdx.x * 64 + lane;
+  float x = 0.f;
+  if (at < values)
+#pragma unroll 8
+    for (int i = wave; i < n; i += 16) x += part[i * values + at];
+  red[wave][lane] = x;
+  __syncthreads();
+  if (wave == 0 && at < values) {
+    x = 0.f;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) x += red[w][lane];
+    ((T*)a.out)[at] = from_f<T>(a.scale * x);
   }
 }
 
@@ -161,8 +225,9 @@ __global__ __launch_bounds__(NT) void few_kernel(Args a) {
 // The tokens' numbers sorted by token (a stable radix sort, 8 bits a pass, tokens outside the table last), so that
 // sums are over runs of the sorted list.  A pass: counts by digit and block, each digit's counts scanned over the blocks, and
 // the places: a digit's first place (all smaller digits' totals), the blocks before, the waves before, the lanes before.
-constexpr int TILE = 4096, PER = TILE / NT;       // tokens of a block, and of a thread
+// A block takes PER tokens a thread: 16 where that leaves a block for every CU, 4 otherwise.
 constexpr int DIGITS = 256;
+inline int per_thread(int64_t rows) { return rows >= (int64_t)256 * 16 * NT ? 16 : 4; }
 
 // key of token i for the sort, from the index (first pass) or the pass before
 template <typename I>
@@ -179,7 +244,7 @@ struct Source {
 };
 
 // Blocks from `blocks` on fill the table's gradient with zeros (rows that no token names).
-template <typename I, typename T>
+template <int PER, typename I, typename T>
 __global__ __launch_bounds__(NT) void count_kernel(Source<I> src, int shift, int blocks, int32_t* __restrict__ counts,
                                                    T* __restrict__ table, int64_t values) {
   if ((int)blockIdx.x >= blocks) {
@@ -187,13 +252,14 @@ __global__ __launch_bounds__(NT) void count_kernel(Source<I> src, int shift, int
     const float zero[N] = {};
     const int64_t step = (int64_t)(gridDim.x - blocks) * NT * N;
     for (int64_t f = ((int64_t)(blockIdx.x - blocks) * NT + threadIdx.x) * N; f < values; f += step)
-      store_some(table + f, (int)std::min<int64_t>(N, values - f), zero);
+      if (f + N <= values) store_some<true, N>(table + f, N, zero);
+      else store_some<false, N>(table + f, (int)(values - f), zero);
     return;
   }
   __shared__ int cnt[DIGITS];
   cnt[threadIdx.x] = 0;
   __syncthreads();
-  const int64_t b0 = (int64_t)blockIdx.x * TILE;
+  const int64_t b0 = (int64_t)blockIdx.x * (NT * PER);
 #pragma unroll
   for (int k = 0; k < PER; ++k) {
     const int64_t i = b0 + k * NT + threadIdx.x;
@@ -237,7 +303,7 @@ __device__ __forceinline__ uint64_t peers(int digit, bool ok) {
   return m;
 }
 
-template <typename I>
+template <int PER, typename I>
 __global__ __launch_bounds__(NT) void place_kernel(Source<I> src, int shift, int blocks, const int32_t* __restrict__ counts,
                                                    const int32_t* __restrict__ totals, int32_t* __restrict__ key,
                                                    int32_t* __restrict__ pos) {
@@ -252,7 +318,7 @@ __global__ __launch_bounds__(NT) void place_kernel(Source<I> src, int shift, int
   __syncthreads();
   int base = run - total + counts[(int64_t)d * blocks + blockIdx.x];
   for (int w = 0; w < wave; ++w) base += sums[w];
-  const int64_t w0 = (int64_t)blockIdx.x * TILE + wave * (TILE / (NT / 64));
+  const int64_t w0 = ((int64_t)blockIdx.x * NT + wave * 64) * PER;
   int32_t k[PER];
 #pragma unroll
   for (int j = 0; j < PER; ++j) {
@@ -296,15 +362,15 @@ struct Sums {
   float* part;                           // [shares][2][width]
 };
 
-template <typename T>
+template <typename T, bool FULL>
 __global__ __launch_bounds__(NT) void sum_kernel(Args a, Sums s) {
   constexpr int N = Vec<T>::N, AHEAD = 8;
   const int64_t g = ((int64_t)blockIdx.x * NT + threadIdx.x) / s.lanes;
   const int64_t share = g / s.columns;
   if (share >= s.shares) return;
-  const int col = ((int)(g - share * s.columns) * s.lanes + (threadIdx.x & (s.lanes - 1))) * N;
-  const int n = std::min(N, a.width - col);
-  if (n <= 0) return;
+  const int first_col = ((int)(g - share * s.columns) * s.lanes + (threadIdx.x & (s.lanes - 1))) * N;
+  if (first_col >= a.width) return;
+  const int n = FULL ? N : a.width, col = std::min(first_col, a.width - n);     // a row's last vector lies at its end
   const int64_t p0 = share * s.share, p1 = std::min<int64_t>(p0 + s.share, s.rows);
   const T* in = (const T*)a.in + col;
   float acc[N];
@@ -319,15 +385,12 @@ __global__ __launch_bounds__(NT) void sum_kernel(Args a, Sums s) {
     const bool head = first && before, tail = end && behind == now;
     if (head || tail) {
       float* out = s.part + (2 * share + (head ? 0 : 1)) * a.width + col;
-      store_some(out, std::min(n, 4), *(float(*)[4])&acc[0]);
-      if constexpr (N == 8) {
-        if (n > 4) store_some(out + 4, n - 4, *(float(*)[4])&acc[4]);
-      }
+      store_some<FULL, N>(out, n, acc);
     } else {
       float o[N];
 #pragma unroll
       for (int j = 0; j < N; ++j) o[j] = a.scale * acc[j];
-      store_some((T*)a.out + now * (int64_t)a.width + col, n, o);
+      store_some<FULL, N>((T*)a.out + now * (int64_t)a.width + col, n, o);
     }
   };
   for (int64_t p = p0; p < p1; p += AHEAD) {
@@ -338,7 +401,7 @@ __global__ __launch_bounds__(NT) void sum_kernel(Args a, Sums s) {
     for (int i = 0; i < AHEAD; ++i) {
       const int64_t q = std::min<int64_t>(p + i, last);
       k[i] = s.key[q];
-      load_some(in + s.pos[q] * a.stride, n, v[i]);
+      load_some<FULL, N>(in + s.pos[q] * a.stride, n, v[i]);
     }
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) {
@@ -373,60 +436,75 @@ __device__ __forceinline__ int64_t count_below(const int32_t* key, int64_t n, in
   return lo;
 }
 
-// Adds the partial rows of one token: 64 columns a block, 16 waves over the rows, narrow rows several to a wave.  BY_TOKEN: a
-// block a token, which writes the zeros of one that is not there; otherwise a block a share, which does nothing unless a
-// token's run begins in it and goes on.
-constexpr int JT = 1024;
-template <typename T, bool BY_TOKEN>
+// Adds the partial rows of one token: 256 columns a block, four a lane, eight waves over the rows, narrow rows several
+// to a wave.  BY_TOKEN: a block a token, which writes the zeros of one that is not there; otherwise a block a share, which does
+// nothing unless a token's run begins in it and goes on.
+constexpr int JT = 512, JW = JT / 64;
+template <typename T, bool BY_TOKEN, bool FULL>
 __global__ __launch_bounds__(JT) void join_kernel(Args a, Sums s) {
-  __shared__ float red[JT / 64][64];
+  __shared__ float red[JW][256];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int c0 = blockIdx.y * 64, wide = std::min(64, a.width - c0);
+  const int c0 = blockIdx.y * 256, wide = std::min(256, a.width - c0);
+  T* out = (T*)a.out + c0;
   int32_t v;
   int64_t s0, s1;                        // the shares it lies in
   if (BY_TOKEN) {
     v = (int32_t)blockIdx.x;
     const int64_t b = count_below<false>(s.key, s.rows, v, lane);
     if (b >= s.rows || s.key[b] != v) {
-      if ((int)threadIdx.x < wide) ((T*)a.out)[v * (int64_t)a.width + c0 + threadIdx.x] = from_f<T>(0.f);
+      if ((int)threadIdx.x < wide) out[v * (int64_t)a.width + threadIdx.x] = from_f<T>(0.f);
       return;
     }
-    const int64_t e = b + count_below<true>(s.key + b, s.rows - b, v, lane);
     s0 = b / s.share;
-    s1 = (e - 1) / s.share;
-    if (s0 == s1) return;
+    const int64_t p1 = (s0 + 1) * s.share;
+    if (p1 >= s.rows || s.key[p1] != v) return;
+    s1 = (p1 + count_below<true>(s.key + p1, s.rows - p1, v, lane) - 1) / s.share;
   } else {
     s0 = blockIdx.x;
     const int64_t p0 = s0 * s.share, p1 = p0 + s.share;
     if (p1 >= s.rows) return;
     v = s.key[p1 - 1];
     if (v >= a.table_rows || s.key[p1] != v || (p0 > 0 && s.key[p0 - 1] == v)) return;
-    const int64_t e = p1 + count_below<true>(s.key + p1, s.rows - p1, v, lane);
-    s1 = (e - 1) / s.share;
+    s1 = (p1 + count_below<true>(s.key + p1, s.rows - p1, v, lane) - 1) / s.share;
   }
+  const int vectors = (wide + 3) / 4;
   int cols = 1;                          // lanes of a row: a power of two
-  while (cols < wide) cols <<= 1;
-  const int per = 64 / cols, sub = lane / cols, c = lane & (cols - 1);
+  while (cols < vectors) cols <<= 1;
+  const int per = 64 / cols, sub = lane / cols, n = FULL ? 4 : a.width;
+  const int col = std::min(c0 + 4 * (lane & (cols - 1)), a.width - n);   // a row's last vector lies at its end
   const int64_t m = s1 - s0 + 1;         // partial rows: the second of s0, the first of the others
-  float x = 0.f;
-  if (c < wide) {
-    const float* part = s.part + c0 + c;
-    // a run that goes on from the share's first token on has its partial row in the first share's second place as well
-#pragma unroll 8
-    for (int64_t i = (int64_t)wave * per + sub; i < m; i += (JT / 64) * per)
-      x += part[(2 * (s0 + i) + (i == 0 ? 1 : 0)) * a.width];
+  float x[4] = {0.f, 0.f, 0.f, 0.f};
+  const float* part = s.part + col;
+  for (int64_t i = (int64_t)wave * per + sub; i < m; i += 8 * JW * per) {
+    float u[8][4];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {        // rows past the last one: the last one again, not added
+      const int64_t r = std::min<int64_t>(i + k * JW * per, m - 1);
+      load_some<FULL, 4>(part + (2 * (s0 + r) + (r == 0 ? 1 : 0)) * a.width, n, u[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (i + k * JW * per < m)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[j] += u[k][j];
   }
-  for (int off = cols; off < 64; off <<= 1) x += __shfl_xor(x, off, 64);
-  red[wave][lane] = x;
+  for (int off = cols; off < 64; off <<= 1)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] += __shfl_xor(x[j], off, 64);
+  if (sub == 0)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < n && col + j >= c0) red[wave][col + j - c0] = x[j];
   __syncthreads();
-  if (wave == 0 && lane < wide) {
-    x = 0.f;
-    for (int w = 0; w < JT / 64; ++w) x += red[w][lane];
-    ((T*)a.out)[v * (int64_t)a.width + c0 + lane] = from_f<T>(a.scale * x);
+  if ((int)threadIdx.x < wide) {
+    float y = 0.f;
+    for (int w = 0; w < JW; ++w) y += red[w][threadIdx.x];
+    out[v * (int64_t)a.width + threadIdx.x] = from_f<T>(a.scale * y);
   }
 }
 
 // Workspace of the gradient: the sorted tokens and their numbers, twice, the counts, and the partial rows.
+constexpr int64_t WAVES = 16384;         // of the sums
 struct Layout {
   int passes, share, lanes, columns;
   int64_t blocks, shares, key[2], pos[2], counts, totals, part, bytes;
@@ -434,15 +512,18 @@ struct Layout {
 Layout layout_of(int64_t rows, int width, int64_t table_rows, int size) {
   Layout l{};
   const int64_t vectors = (width + 16 / size - 1) / (16 / size);
+  // a row's vectors go to groups of 16, 32 or 64 lanes, whichever leaves the fewest lanes idle; short rows take fewer lanes
   l.lanes = 4;
   while (l.lanes < 64 && l.lanes < vectors) l.lanes *= 2;
+  for (int k = l.lanes / 2; k >= 16; k /= 2)
+    if ((vectors + k - 1) / k * k < (vectors + l.lanes - 1) / l.lanes * l.lanes) l.lanes = k;
   l.columns = (int)((vectors + l.lanes - 1) / l.lanes);
   l.passes = 1;
   while (l.passes < 4 && (table_rows >> (8 * l.passes))) ++l.passes;
-  l.blocks = (rows + TILE - 1) / TILE;
+  l.blocks = (rows + NT * per_thread(rows) - 1) / (NT * per_thread(rows));
   // enough shares to fill the chip with waves, not so many that a token's partial rows take long to join
   const int64_t waves = rows * l.columns * l.lanes / 64;
-  l.share = (int)std::min<int64_t>(1024, std::max<int64_t>({16, waves / 8192, rows / 8192}));
+  l.share = (int)std::min<int64_t>(1024, std::max<int64_t>({16, waves / WAVES, rows / 8192}));
   l.shares = (rows + l.share - 1) / l.share;
   int64_t at = 0;
   auto take = [&](int64_t n) {
@@ -461,12 +542,33 @@ Layout layout_of(int64_t rows, int width, int64_t table_rows, int size) {
   return l;
 }
 
+// Blocks of a small table's sums: as many as the copies let the chip hold, four waves a SIMD at most.
+struct SmallLayout {
+  int lanes, chunks, waves, blocks;
+  int64_t range, bytes;
+};
+SmallLayout small_layout(int64_t rows, int width, int64_t table_rows) {
+  SmallLayout l{};
+  l.chunks = (width + 255) / 256;
+  l.lanes = 1;
+  while (l.lanes < 64 && 4 * l.lanes < width) l.lanes *= 2;
+  l.waves = small_waves(table_rows);
+  const int64_t fit = std::max<int64_t>(1, std::min<int64_t>(16 / l.waves, 160 / (l.waves * table_rows)));
+  const int64_t most = std::max<int64_t>(1, 256 * fit / l.chunks);
+  const int64_t least = (int64_t)l.waves * 64 / l.lanes * 8;               // rows that a block has on their way
+  l.range = std::max(least, (rows + most - 1) / most);
+  l.blocks = (int)((rows + l.range - 1) / l.range);
+  l.bytes = (int64_t)l.blocks * table_rows * width * 4;
+  return l;
+}
+
 template <typename T, typename I>
 void launch_lookup(const Args& a, hipStream_t st) {
-  constexpr int64_t BLOCK = (int64_t)NT * Vec<T>::N * STEPS, MOST = BLOCK << 23;    // fewer than 2^32 threads a launch
-  const int64_t total = a.rows * a.width;
+  constexpr int64_t BLOCK = (int64_t)NT * STEPS, MOST = BLOCK << 23;     // fewer than 2^32 threads a launch
+  const int64_t vectors = (a.width + Vec<T>::N - 1) / Vec<T>::N, total = a.rows * vectors;
   for (int64_t f = 0; f < total; f += MOST)
-    lookup_kernel<T, I><<<(unsigned)((std::min(total - f, MOST) + BLOCK - 1) / BLOCK), NT, 0, st>>>(a, f);
+    FSC_EMBED_FULL(a.width >= Vec<T>::N, (lookup_kernel<T, I, FULL><<<(unsigned)((std::min(total - f, MOST) + BLOCK - 1) / BLOCK),
+                                                                      NT, 0, st>>>(a, f, (uint32_t)vectors)));
 }
 
 template <typename T, typename I>
@@ -474,7 +576,15 @@ void launch_backward(const Args& a, char* ws, hipStream_t st) {
   constexpr int N = Vec<T>::N;
   if (a.rows <= FEW) {
     const dim3 grid((unsigned)std::min<int64_t>(a.table_rows, 1 << 16), (a.width + 64 * N - 1) / (64 * N));
-    few_kernel<T, I><<<grid, NT, 0, st>>>(a);
+    FSC_EMBED_FULL(a.width >= N, (few_kernel<T, I, FULL><<<grid, NT, 0, st>>>(a)));
+    return;
+  }
+  if (a.table_rows <= SMALL) {
+    const SmallLayout l = small_layout(a.rows, a.width, a.table_rows);
+    const Stream s{l.lanes, l.range, (float*)ws};
+    FSC_EMBED_FULL(a.width >= 4, (small_kernel<T, I, FULL><<<dim3(l.blocks, l.chunks), 64 * l.waves,
+                                                             l.waves * a.table_rows * 1024, st>>>(a, s)));
+    small_join_kernel<T><<<(unsigned)((a.table_rows * a.width + 63) / 64), 1024, 0, st>>>(a, s.part, l.blocks);
     return;
   }
   const Layout l = layout_of(a.rows, a.width, a.table_rows, sizeof(T));
@@ -489,18 +599,23 @@ void launch_backward(const Args& a, char* ws, hipStream_t st) {
   for (int p = 0; p < l.passes; ++p) {
     const int64_t values = p == 0 && !by_token ? a.table_rows * a.width : 0;
     const unsigned fill = (unsigned)std::min<int64_t>((values + NT * N - 1) / (NT * N), 2048);
-    count_kernel<I, T><<<(unsigned)l.blocks + fill, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, (T*)a.out, values);
-    scan_kernel<<<DIGITS, 64, 0, st>>>((int)l.blocks, counts, totals);
-    place_kernel<I><<<(unsigned)l.blocks, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, totals, key[p & 1], pos[p & 1]);
+    auto sort = [&](auto per) {
+      constexpr int PER = decltype(per)::value;
+      count_kernel<PER, I, T><<<(unsigned)l.blocks + fill, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, (T*)a.out, values);
+      scan_kernel<<<DIGITS, 64, 0, st>>>((int)l.blocks, counts, totals);
+      place_kernel<PER, I><<<(unsigned)l.blocks, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, totals, key[p & 1], pos[p & 1]);
+    };
+    if (per_thread(a.rows) == 16) sort(std::integral_constant<int, 16>{});
+    else sort(std::integral_constant<int, 4>{});
     src.key = key[p & 1];
     src.pos = pos[p & 1];
   }
   const Sums s{src.key, src.pos, a.rows, l.shares, l.share, l.lanes, l.columns, (float*)(ws + l.part)};
   const int64_t threads = l.shares * l.columns * l.lanes;
-  sum_kernel<T><<<(unsigned)((threads + NT - 1) / NT), NT, 0, st>>>(a, s);
-  const dim3 grid((unsigned)(by_token ? a.table_rows : l.shares), (a.width + 63) / 64);
-  if (by_token) join_kernel<T, true><<<grid, JT, 0, st>>>(a, s);
-  else join_kernel<T, false><<<grid, JT, 0, st>>>(a, s);
+  FSC_EMBED_FULL(a.width >= N, (sum_kernel<T, FULL><<<(unsigned)((threads + NT - 1) / NT), NT, 0, st>>>(a, s)));
+  const dim3 grid((unsigned)(by_token ? a.table_rows : l.shares), (a.width + 255) / 256);
+  if (by_token) FSC_EMBED_FULL(a.width >= 4, (join_kernel<T, true, FULL><<<grid, JT, 0, st>>>(a, s)))
+  else FSC_EMBED_FULL(a.width >= 4, (join_kernel<T, false, FULL><<<grid, JT, 0, st>>>(a, s)))
 }
 
 int check_sizes(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits) {
@@ -534,7 +649,8 @@ int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32
   if (rows == 0) return 0;
   FSC_CHECK_ARG(index && out && (table || table_rows == 0), "embedding: null array");
   FSC_CHECK_ARG(table_stride >= 0, "embedding: negative row stride");
-  const Args a{rows, table_stride, table_rows, width, scale, table, index, out};
+  // without a table no row is read for its values: any array does
+  const Args a{rows, table_rows ? table_stride : 0, table_rows, width, scale, table_rows ? table : out, index, out};
   FSC_EMBED_TYPES((launch_lookup<T, I>(a, stream)));
   return check_launch("embedding") ? 2 : 0;
 }
@@ -543,9 +659,9 @@ int fsc_embedding_workspace(int64_t rows, int32_t width, int64_t table_rows, int
   FSC_CHECK_ARG(bytes != nullptr, "embedding: null output");
   if (int rc = fsc::embed::check_sizes(rows, width, table_rows, FSC_F32, 32)) return rc;
   // the layout depends on the type: room for either
-  *bytes = rows <= fsc::embed::FEW || table_rows == 0
-               ? 0
-               : std::max(fsc::embed::layout_of(rows, width, table_rows, 4).bytes,
+  if (rows <= fsc::embed::FEW || table_rows == 0) *bytes = 0;
+  else if (table_rows <= fsc::embed::SMALL) *bytes = fsc::embed::small_layout(rows, width, table_rows).bytes;
+  else *bytes = std::max(fsc::embed::layout_of(rows, width, table_rows, 4).bytes,
                           fsc::embed::layout_of(rows, width, table_rows, 2).bytes);
   return 0;
 }
