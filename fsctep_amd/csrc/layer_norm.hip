@@ -33,7 +33,8 @@ struct Args {
   // backward: dx null: not wanted
   const void* dy;
   void* dx;
-  float* part;                 // [gridDim.x][2][width] partial sums of the weight's and the bias' gradients, or null
+  void *dw, *db;               // null: not wanted
+  float* part;                 // [gridDim.x][2][width] partial sums of the two
   // twice: v, vw, vb null: 0; gx, gdy null: not wanted
   const void *v, *vw, *vb;
   void *gx, *gdy;
@@ -133,7 +134,7 @@ template <typename T, typename W, bool SILU, typename F>
 __global__ __launch_bounds__(NT) void wide_back_kernel(Args a) {
   __shared__ double red[2 * NW];
   const W *w = (const W*)a.w, *b = (const W*)a.b;
-  float* part = a.part ? a.part + (int64_t)blockIdx.x * 2 * a.width : nullptr;
+  float* part = a.dw || a.db ? a.part + (int64_t)blockIdx.x * 2 * a.width : nullptr;
   if (part)                              // a thread's own columns from here on
     for (int i = threadIdx.x; i < a.width; i += NT) part[i] = part[a.width + i] = 0.f;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -176,7 +177,7 @@ template <typename T, typename W, bool SILU, typename F>
 __global__ __launch_bounds__(NT) void wide_twice_kernel(Args a) {
   __shared__ double red[5 * NW];
   const W *w = (const W*)a.w, *b = (const W*)a.b, *vw = (const W*)a.vw, *vb = (const W*)a.vb;
-  float* part = a.part ? a.part + (int64_t)blockIdx.x * 2 * a.width : nullptr;
+  float* part = a.dw || a.db ? a.part + (int64_t)blockIdx.x * 2 * a.width : nullptr;
   if (part)
     for (int i = threadIdx.x; i < a.width; i += NT) part[i] = part[a.width + i] = 0.f;
   for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
@@ -243,6 +244,9 @@ __global__ __launch_bounds__(NT) void wide_twice_kernel(Args a) {
 // Lane l of a row's L holds the vectors of 16 bytes c L + l, c < CH; a row is read once.  The last vector of a row whose
 // width no vector divides is read from the row's end back, and its lane takes the values from `skip` on as its own; lanes
 // past the end own none.  Values that are not a lane's own are zeros in every sum.
+//
+// Bound by the vector units as much as by memory (a wave's instruction takes four cycles): shapes leave few lanes
+// idle, sums within 16 lanes are DPP additions, and a value takes about a dozen instructions in each pass.
 template <typename T>
 struct alignas(sizeof(T)) Vec {          // at any address a value may lie at
   static constexpr int N = 16 / sizeof(T);
@@ -298,14 +302,17 @@ struct Row {
 #pragma unroll
       for (int j = 0; j < V; ++j) v[c][j] = j >= skip(c) ? v[c][j] : F(0);
   }
+  // Past the caches' own keeping: what a pass writes is read by another kernel, on other XCDs (10,000 x 1,600: 34 -> 27 us
+  // forward, 39 -> 37 us backward).
   template <typename F>
   __device__ __forceinline__ void store(T* p, int c, const F (&v)[V]) const {
+    typedef unsigned u4s __attribute__((ext_vector_type(4), aligned(2)));
     const int s = skip(c);
     if (s == 0) {
       Vec<T> k;
 #pragma unroll
       for (int j = 0; j < V; ++j) k.t[j] = from_f<T>((float)v[j]);
-      *reinterpret_cast<Vec<T>*>(p + base(c)) = k;
+      __builtin_nontemporal_store(__builtin_bit_cast(u4s, k), reinterpret_cast<u4s*>(p + base(c)));
     } else if (s < V) {
 #pragma unroll
       for (int j = 1; j < V; ++j)
@@ -313,6 +320,19 @@ struct Row {
     }
   }
 };
+
+// v of the lane that DPP's CTRL names
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
+}
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const int2 u = __builtin_bit_cast(int2, v);
+  const int2 w = {__builtin_amdgcn_update_dpp(0, u.x, CTRL, 0xf, 0xf, true),
+                  __builtin_amdgcn_update_dpp(0, u.y, CTRL, 0xf, 0xf, true)};
+  return __builtin_bit_cast(double, w);
+}
 
 // Sums of N values over a row's lanes, the same in each.  A row of a whole block's lanes meets in LDS, in two places by
 // turns: who still reads the one has not passed the barrier before the next but one sum.
@@ -323,8 +343,16 @@ struct RowAdd {
   __device__ __forceinline__ explicit RowAdd(F* r) : red(r) {}
   template <int N>
   __device__ __forceinline__ void operator()(F (&v)[N]) {
+    static_assert(L >= 16, "whole DPP rows");
 #pragma unroll
-    for (int off = (L < 64 ? L : 64) / 2; off > 0; off >>= 1)
+    for (int i = 0; i < N; ++i) {
+      v[i] += dpp<0xB1>(v[i]);           // neighbours, then pairs, then (both halves alike) mirrored in 8 and in 16
+      v[i] += dpp<0x4E>(v[i]);
+      v[i] += dpp<0x141>(v[i]);
+      v[i] += dpp<0x140>(v[i]);
+    }
+#pragma unroll
+    for (int off = 16; off < (L < 64 ? L : 64); off <<= 1)
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off, 64);
     if constexpr (L == NT) {
@@ -396,65 +424,60 @@ __global__ __launch_bounds__(NT) void row_kernel(Args a) {
   }
 }
 
-// (x - mean) and the root's factor of the row in x; own values alone
+// zh of the row in x: zeros where a value is not the lane's own.  Returns the root's factor.
 template <typename T, typename F, int L, int CH, int V>
-__device__ __forceinline__ F deviations(const Args& a, const Row<T, L, CH>& at, RowAdd<L, F>& row_add, int64_t row,
-                                        const float (&x)[CH][V], F (&c_)[CH][V]) {
-  const double mean = a.mean[row];
+__device__ __forceinline__ F normalised(const Args& a, const Row<T, L, CH>& at, RowAdd<L, F>& row_add, double mean, float rstd,
+                                        const float (&x)[CH][V], F (&z)[CH][V]) {
   if constexpr (sizeof(F) == 4) {
     float hi, lo;
     parts_of(mean, hi, lo);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < V; ++j) c_[c][j] = (x[c][j] - hi) - lo;
-    return a.rstd[row];
+      for (int j = 0; j < V; ++j) z[c][j] = ((x[c][j] - hi) - lo) * rstd;
+    at.own(z);
+    return rstd;
   } else {
     double s[1] = {0.0};
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < V; ++j) c_[c][j] = (double)x[c][j] - mean;
-    at.own(c_);
+      for (int j = 0; j < V; ++j) z[c][j] = (double)x[c][j] - mean;
+    at.own(z);
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < V; ++j) s[0] += c_[c][j] * c_[c][j];
+      for (int j = 0; j < V; ++j) s[0] += z[c][j] * z[c][j];
     row_add(s);
-    return 1.0 / sqrt(s[0] / a.width + (double)a.eps);
+    const F r = 1.0 / sqrt(s[0] / a.width + (double)a.eps);
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) z[c][j] *= r;
+    return r;
   }
 }
 
 // Adds a lane's sums of the weight's and the bias' gradients over the wave's rows and the block's waves: a partial row
-// for the block.
-template <typename T, int L, int CH, int V>
+// for the block, or the gradients themselves where there is one block.
+template <typename T, typename W, int L, int CH, int V>
 __device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at, float (&gw)[CH][V], float (&gb)[CH][V],
                                          float* buf) {
-  float* part = a.part + (int64_t)blockIdx.x * 2 * a.width;
-  if constexpr (L == NT) {               // the block's rows were this thread's own
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j)
-        if (j >= at.skip(c)) {
-          part[at.base(c) + j] = gw[c][j];
-          part[a.width + at.base(c) + j] = gb[c][j];
-        }
-    return;
-  }
   const int wave = threadIdx.x >> 6;
+  if constexpr (L < 64)
 #pragma unroll
-  for (int off = L; off < 64; off <<= 1)
+    for (int off = L; off < 64; off <<= 1)
 #pragma unroll
-    for (int c = 0; c < CH; ++c)
+      for (int c = 0; c < CH; ++c)
 #pragma unroll
-      for (int j = 0; j < V; ++j) {
-        gw[c][j] += __shfl_xor(gw[c][j], off, 64);
-        gb[c][j] += __shfl_xor(gb[c][j], off, 64);
-      }
+        for (int j = 0; j < V; ++j) {
+          gw[c][j] += __shfl_xor(gw[c][j], off, 64);
+          gb[c][j] += __shfl_xor(gb[c][j], off, 64);
+        }
+  // a row of the block's lanes: every column is one thread's own
 #pragma unroll 1
-  for (int k = 0; k < NW; ++k) {
-    if (wave == k && (threadIdx.x & 63) < L) {
+  for (int k = 0; k < (L == NT ? 1 : NW); ++k) {
+    if (L == NT || (wave == k && (threadIdx.x & 63) < L)) {
 #pragma unroll
       for (int c = 0; c < CH; ++c)
 #pragma unroll
@@ -467,72 +490,22 @@ __device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at,
     }
     __syncthreads();
   }
+  if (gridDim.x == 1) {
+    for (int i = threadIdx.x; i < a.width; i += NT) {
+      if (a.dw) ((W*)a.dw)[i] = from_f<W>(buf[i]);
+      if (a.db) ((W*)a.db)[i] = from_f<W>(buf[a.width + i]);
+    }
+    return;
+  }
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.width;
   for (int i = threadIdx.x; i < 2 * a.width; i += NT) part[i] = buf[i];
 }
 
 template <typename T, typename W, bool SILU, typename F, int L, int CH>
 __global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
   using R = Row<T, L, CH>;
-  constexpr int V = R::V;
-  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
-  __shared__ F red[L == NT ? 2 * 5 * NW : 1];
-  RowAdd<L, F> row_add(red);
-  const R at(a.width);
-  float w[CH][V], b[CH][V], gw[CH][V] = {}, gb[CH][V] = {};
-  at.load_or((const W*)a.w, 1.f, w);
-  if (SILU) at.load_or((const W*)a.b, 0.f, b);
-  const int64_t step = (int64_t)gridDim.x * (NT / L);
-  // every lane of a wave goes round as often: rows past the last one count as zeros and are not stored
-  const int64_t r0 = ((int64_t)blockIdx.x * NT + threadIdx.x) / L, lead = ((int64_t)blockIdx.x * NT + (threadIdx.x & ~63)) / L;
-  for (int64_t k = 0; lead + k < a.rows; k += step) {
-    const bool there = r0 + k < a.rows;
-    const int64_t row = there ? r0 + k : a.rows - 1;
-    float x[CH][V], d[CH][V];
-    at.load((const T*)a.x + row * a.xs, x);
-    at.load((const T*)a.dy + row * a.ys, d);
-    F z[CH][V], g[CH][V];
-    const F r = deviations<T, F, L, CH, V>(a, at, row_add, row, x, z);
-    at.own(d);
-    at.own(z);
-    F s[2] = {F(0), F(0)};
-#pragma unroll
-    for (int c = 0; c < CH; ++c)
-#pragma unroll
-      for (int j = 0; j < V; ++j) {
-        z[c][j] *= r;
-        F d1, d2, du = (F)d[c][j];
-        if (SILU) {
-          act12<SILU>(z[c][j] * (F)w[c][j] + (F)b[c][j], d1, d2);
-          du *= d1;
-        }
-        if (there) {
-          gw[c][j] += (float)(du * z[c][j]);
-          gb[c][j] += (float)du;
-        }
-        g[c][j] = du * (F)w[c][j];
-        s[0] += g[c][j];
-        s[1] += g[c][j] * z[c][j];
-      }
-    if (!a.dx) continue;
-    row_add(s);
-    const F mg = s[0] / (F)a.width, mgz = s[1] / (F)a.width;
-    if (there)
-#pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        F o[V];
-#pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = r * (g[c][j] - mg - z[c][j] * mgz);
-        at.store((T*)a.dx + row * a.width, c, o);
-      }
-  }
-  if (a.part) put_part<T, L, CH, V>(a, at, gw, gb, buf);
-}
-
-template <typename T, typename W, bool SILU, typename F, int L, int CH>
-__global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
-  using R = Row<T, L, CH>;
-  constexpr int V = R::V;
-  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
+  constexpr int V = R::V, ROWS = NT / L;
+  __shared__ float buf[2 * L * CH * V];
   __shared__ F red[L == NT ? 2 * 5 * NW : 1];
   RowAdd<L, F> row_add(red);
   const R at(a.width);
@@ -540,26 +513,85 @@ __global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
   at.load_or((const W*)a.w, 1.f, w);
   if (SILU) at.load_or((const W*)a.b, 0.f, b);
   const F n = (F)a.width;
-  const int64_t step = (int64_t)gridDim.x * (NT / L);
-  const int64_t r0 = ((int64_t)blockIdx.x * NT + threadIdx.x) / L, lead = ((int64_t)blockIdx.x * NT + (threadIdx.x & ~63)) / L;
-  for (int64_t i = 0; lead + i < a.rows; i += step) {
-    const bool there = r0 + i < a.rows;
-    const int64_t row = there ? r0 + i : a.rows - 1;
+  // every lane goes round as often: rows past the last one are the last one again, with zeros for what is added and stored nowhere
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t mine = r0 + threadIdx.x / L, row = std::min<int64_t>(mine, a.rows - 1);
+    const bool there = mine < a.rows;
+    float x[CH][V], d[CH][V];
+    at.load((const T*)a.x + row * a.xs, x);
+    at.load((const T*)a.dy + row * a.ys, d);
+    F z[CH][V], g[CH][V];
+    const F r = normalised<T, F, L, CH, V>(a, at, row_add, a.mean[row], a.rstd[row], x, z);
+    at.own(d);
+    if (r0 + ROWS > a.rows && !there)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[c][j] = F(0), d[c][j] = 0.f;
+    F s[2] = {F(0), F(0)};
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        F d1, d2, du = (F)d[c][j];
+        if (SILU) {
+          act12<SILU>(z[c][j] * (F)w[c][j] + (F)b[c][j], d1, d2);
+          du *= d1;
+        }
+        gw[c][j] += (float)(du * z[c][j]);
+        gb[c][j] += (float)du;
+        g[c][j] = du * (F)w[c][j];
+        s[0] += g[c][j];
+        s[1] += g[c][j] * z[c][j];
+      }
+    if (!a.dx) continue;
+    row_add(s);
+    const F mg = s[0] / n, mgz = s[1] / n;
+    if (there)
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        F o[V];
+#pragma unroll
+        for (int j = 0; j < V; ++j) o[j] = r * ((g[c][j] - mg) - z[c][j] * mgz);
+        at.store((T*)a.dx + row * a.width, c, o);
+      }
+  }
+  if (a.dw || a.db) put_part<T, W, L, CH, V>(a, at, gw, gb, buf);
+}
+
+template <typename T, typename W, bool SILU, typename F, int L, int CH>
+__global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
+  using R = Row<T, L, CH>;
+  constexpr int V = R::V, ROWS = NT / L;
+  __shared__ float buf[2 * L * CH * V];
+  __shared__ F red[L == NT ? 2 * 5 * NW : 1];
+  RowAdd<L, F> row_add(red);
+  const R at(a.width);
+  float w[CH][V], b[CH][V], gw[CH][V] = {}, gb[CH][V] = {};
+  at.load_or((const W*)a.w, 1.f, w);
+  if (SILU) at.load_or((const W*)a.b, 0.f, b);
+  const F n = (F)a.width;
+  for (int64_t r0 = (int64_t)blockIdx.x * ROWS; r0 < a.rows; r0 += (int64_t)gridDim.x * ROWS) {
+    const int64_t mine = r0 + threadIdx.x / L, row = std::min<int64_t>(mine, a.rows - 1);
+    const bool there = mine < a.rows;
     float x[CH][V], d[CH][V], v[CH][V];
     at.load((const T*)a.x + row * a.xs, x);
     at.load((const T*)a.dy + row * a.ys, d);
     at.load_or(a.v ? (const T*)a.v + row * a.vs : nullptr, 0.f, v);
     F z[CH][V];
-    const F r = deviations<T, F, L, CH, V>(a, at, row_add, row, x, z);
+    const F r = normalised<T, F, L, CH, V>(a, at, row_add, a.mean[row], a.rstd[row], x, z);
     at.own(d);
     at.own(v);
-    at.own(z);
+    if (r0 + ROWS > a.rows && !there)
+#pragma unroll
+      for (int c = 0; c < CH; ++c)
+#pragma unroll
+        for (int j = 0; j < V; ++j) z[c][j] = F(0), d[c][j] = v[c][j] = 0.f;
     F s[5] = {F(0), F(0), F(0), F(0), F(0)};
 #pragma unroll
     for (int c = 0; c < CH; ++c)
 #pragma unroll
       for (int j = 0; j < V; ++j) {
-        z[c][j] *= r;
         F d1, d2, g = (F)d[c][j] * (F)w[c][j];
         if (SILU) {
           act12<SILU>(z[c][j] * (F)w[c][j] + (F)b[c][j], d1, d2);
@@ -587,13 +619,12 @@ __global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
         F d1 = F(1), d2 = F(0);
         const F wi = (F)w[c][j], dj = (F)d[c][j], zj = z[c][j];
         if (SILU) act12<SILU>(zj * wi + (F)b[c][j], d1, d2);
-        const F du = dj * d1, q = r * ((F)v[c][j] - mv - zj * mvz);
+        // a value that is not the lane's own has d 0: nothing of it reaches a sum
+        const F du = dj * d1, q = r * (((F)v[c][j] - mv) - zj * mvz);
         const F aa = wi * q + (F)vw[j] * zj + (F)vb[j], e = dj * d2 * aa;
         gdy[j] = d1 * aa;
-        if (there) {
-          gw[c][j] += (float)(du * q + e * zj);
-          gb[c][j] += (float)e;
-        }
+        gw[c][j] += (float)(du * q + e * zj);
+        gb[c][j] += (float)e;
         k[c][j] = e * wi + du * (F)vw[j] - r * (du * wi * mvz + (F)v[c][j] * mgz);
         t[0] += k[c][j];
         t[1] += k[c][j] * zj;
@@ -608,34 +639,11 @@ __global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
       for (int c = 0; c < CH; ++c) {
         F o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = r * (k[c][j] - mk - z[c][j] * mkz);
+        for (int j = 0; j < V; ++j) o[j] = r * ((k[c][j] - mk) - z[c][j] * mkz);
         at.store((T*)a.gx + row * a.width, c, o);
       }
   }
-  if (a.part) put_part<T, L, CH, V>(a, at, gw, gb, buf);
-}
-
-// Calls f(L, CH) for the fewest lanes and vectors that hold a row; false where none do (a row shorter than a vector, or too wide).
-template <typename T, typename F>
-bool by_shape(int width, F&& f) {
-  constexpr int V = Vec<T>::N;
-#define FSC_LN_SHAPE(L_, CH_)                                                               \
-  if (width <= L_ * CH_ * V) {                                                              \
-    f(std::integral_constant<int, L_>{}, std::integral_constant<int, CH_>{});               \
-    return true;                                                                            \
-  }
-  if (width < V) return false;
-  FSC_LN_SHAPE(16, 1)
-  FSC_LN_SHAPE(32, 1)
-  FSC_LN_SHAPE(64, 1)
-  FSC_LN_SHAPE(64, 2)
-  if constexpr (V == 4) {
-    FSC_LN_SHAPE(64, 3)
-  }
-  FSC_LN_SHAPE(256, 1)
-  FSC_LN_SHAPE(256, 2)
-#undef FSC_LN_SHAPE
-  return false;
+  if (a.dw || a.db) put_part<T, W, L, CH, V>(a, at, gw, gb, buf);
 }
 
 // Column sums of the blocks' partial rows, the weight's gradient and the bias': 32 columns a block, 32 threads a column,
@@ -657,8 +665,44 @@ __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ par
   if (c == 0 && blockIdx.x * 32 + k < width) out[blockIdx.x * 32 + k] = from_f<W>(s);
 }
 
-// Blocks of the two backward passes.
-inline int back_blocks(int64_t rows) { return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 3) / 4, 1024)); }
+// Calls f(L, CH) for the fewest vectors of L lanes that hold a row; false where none do (a row shorter than a vector, or too
+// wide).  FORWARD shapes may have the registers of five vectors of 16 bits a lane, the backward passes three (100,000 x 640 in
+// bf16 backward, five vectors of 16 lanes: 130 us, three of 32: 88 us), the second one three of either type.
+enum Pass { FORWARD, BACK, TWICE };
+template <typename T, Pass P, typename F>
+bool by_shape(int width, F&& f) {
+  constexpr int V = Vec<T>::N;
+  constexpr bool FIVE = P == FORWARD || (P == BACK && V == 4);
+#define FSC_LN_SHAPE(L_, CH_)                                                               \
+  if (width <= L_ * CH_ * V) {                                                              \
+    f(std::integral_constant<int, L_>{}, std::integral_constant<int, CH_>{});               \
+    return true;                                                                            \
+  }
+  if (width < V) return false;
+  FSC_LN_SHAPE(16, 1)
+  FSC_LN_SHAPE(16, 2)
+  FSC_LN_SHAPE(16, 3)
+  if constexpr (FIVE) {
+    FSC_LN_SHAPE(16, 5)
+  }
+  FSC_LN_SHAPE(32, 3)
+  FSC_LN_SHAPE(64, 2)
+  if constexpr (FIVE) {
+    FSC_LN_SHAPE(32, 5)
+  }
+  FSC_LN_SHAPE(64, 3)
+  FSC_LN_SHAPE(256, 1)
+  FSC_LN_SHAPE(256, 2)
+#undef FSC_LN_SHAPE
+  return false;
+}
+
+// Blocks of the two backward passes on rows of L lanes: four rows in turn at least, so that few rows take one block, which needs
+// no partial rows (32 x 128, both passes: 2 launches in place of 4); at most 1,024.
+inline int back_blocks(int64_t rows, int L) {
+  const int64_t at_once = NT / L;
+  return (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 4 * at_once ? 1 : (rows + at_once - 1) / at_once, 1024));
+}
 
 template <typename T, typename W, bool SILU>
 void launch_forward(const Args& all, hipStream_t st) {
@@ -672,7 +716,7 @@ void launch_forward(const Args& all, hipStream_t st) {
       a.mean = all.mean + r0;
       a.rstd = all.rstd + r0;
     }
-    if (!by_shape<T>(a.width, [&](auto L, auto CH) {
+    if (!by_shape<T, FORWARD>(a.width, [&](auto L, auto CH) {
           constexpr int l = decltype(L)::value, ch = decltype(CH)::value;
           row_kernel<T, W, SILU, l, ch><<<(unsigned)((a.rows * l + NT - 1) / NT), NT, 0, st>>>(a);
         }))
@@ -680,31 +724,36 @@ void launch_forward(const Args& all, hipStream_t st) {
   }
 }
 
-template <typename T, typename W, bool SILU>
-void launch_backward(const Args& a, bool twice, W* dw, W* db, hipStream_t st) {
-  const int blocks = back_blocks(a.rows);
-  const bool done = by_shape<T>(a.width, [&](auto L, auto CH) {
+template <typename T, typename W, bool SILU, Pass P>
+void launch_backward(const Args& a, hipStream_t st) {
+  int blocks = 0;
+  const bool done = by_shape<T, P>(a.width, [&](auto L, auto CH) {
     constexpr int l = decltype(L)::value, ch = decltype(CH)::value;
-    if constexpr (l == 16) {
+    blocks = back_blocks(a.rows, l);
+    if constexpr (l * ch <= 16) {
       if (a.width <= 64) {
-        if (twice) row_twice_kernel<T, W, SILU, double, l, ch><<<blocks, NT, 0, st>>>(a);
+        if constexpr (P == TWICE) row_twice_kernel<T, W, SILU, double, l, ch><<<blocks, NT, 0, st>>>(a);
         else row_back_kernel<T, W, SILU, double, l, ch><<<blocks, NT, 0, st>>>(a);
         return;
       }
     }
-    if constexpr (l > 16 || sizeof(T) == 2) {
-      if (twice) row_twice_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
+    if constexpr (l * ch > 16 || sizeof(T) == 2) {
+      if constexpr (P == TWICE) row_twice_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
       else row_back_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
     }
   });
-  if (!done && a.width <= 64) {
-    if (twice) wide_twice_kernel<T, W, SILU, double><<<blocks, NT, 0, st>>>(a);
-    else wide_back_kernel<T, W, SILU, double><<<blocks, NT, 0, st>>>(a);
-  } else if (!done) {
-    if (twice) wide_twice_kernel<T, W, SILU, float><<<blocks, NT, 0, st>>>(a);
-    else wide_back_kernel<T, W, SILU, float><<<blocks, NT, 0, st>>>(a);
+  if (!done) {
+    blocks = back_blocks(a.rows, NT);
+    if (a.width <= 64) {
+      if constexpr (P == TWICE) wide_twice_kernel<T, W, SILU, double><<<blocks, NT, 0, st>>>(a);
+      else wide_back_kernel<T, W, SILU, double><<<blocks, NT, 0, st>>>(a);
+    } else {
+      if constexpr (P == TWICE) wide_twice_kernel<T, W, SILU, float><<<blocks, NT, 0, st>>>(a);
+      else wide_back_kernel<T, W, SILU, float><<<blocks, NT, 0, st>>>(a);
+    }
   }
-  if (a.part) sum_kernel<W><<<dim3((a.width + 31) / 32, 2), 1024, 0, st>>>(a.part, blocks, a.width, dw, db);
+  if ((a.dw || a.db) && (blocks > 1 || !done))
+    sum_kernel<W><<<dim3((a.width + 31) / 32, 2), 1024, 0, st>>>(a.part, blocks, a.width, (W*)a.dw, (W*)a.db);
 }
 
 // runs the statement with (T, W, SILU)
@@ -725,15 +774,17 @@ int check_types(int64_t rows, int32_t width, int32_t dtype, int32_t wtype, int32
   return 0;
 }
 
-int backward(const Args& a, int32_t dtype, int32_t wtype, int32_t act, bool twice, void* dw, void* db, hipStream_t st) {
+int backward(const Args& a, int32_t dtype, int32_t wtype, int32_t act, bool twice, hipStream_t st) {
   if (int rc = check_types(a.rows, a.width, dtype, wtype, act)) return rc;
   FSC_CHECK_ARG(a.rows == 0 || (a.x && a.mean && a.rstd && a.dy), "layer_norm_backward: null array");
   FSC_CHECK_ARG(a.xs >= 0 && a.ys >= 0 && a.vs >= 0, "layer_norm_backward: negative row stride");
-  FSC_CHECK_ARG(!(dw || db) || a.part, "layer_norm_backward: the weight's and the bias' gradients need a workspace");
-  Args k = a;
-  if (!dw && !db) k.part = nullptr;
-  if (!k.part && (a.rows == 0 || !(a.dx || a.gx || a.gdy))) return 0;
-  FSC_LN_TYPES(launch_backward<T, W, SILU>(k, twice, (W*)dw, (W*)db, st));
+  FSC_CHECK_ARG(!(a.dw || a.db) || a.part, "layer_norm_backward: the weight's and the bias' gradients need a workspace");
+  if (!a.dw && !a.db && (a.rows == 0 || !(a.dx || a.gx || a.gdy))) return 0;
+  if (twice) {
+    FSC_LN_TYPES((launch_backward<T, W, SILU, TWICE>(a, st)));
+  } else {
+    FSC_LN_TYPES((launch_backward<T, W, SILU, BACK>(a, st)));
+  }
   return check_launch("layer_norm_backward") ? 2 : 0;
 }
 
@@ -762,7 +813,7 @@ int fsc_layer_norm_forward(int64_t rows, int32_t width, int32_t dtype, int32_t w
 int fsc_layer_norm_workspace(int64_t rows, int32_t width, int64_t* floats) {
   FSC_CHECK_ARG(floats != nullptr, "layer_norm: null output");
   FSC_CHECK_ARG(rows >= 0 && width >= 1, "layer_norm: negative size");
-  *floats = (int64_t)fsc::lnorm::back_blocks(rows) * 2 * width;
+  *floats = (int64_t)fsc::lnorm::back_blocks(rows, fsc::lnorm::NT) * 2 * width;   // no shape takes more blocks
   return 0;
 }
 
@@ -773,8 +824,8 @@ int fsc_layer_norm_backward(int64_t rows, int32_t width, int32_t dtype, int32_t 
   fsc::lnorm::Args a{};
   a.rows = rows; a.xs = x_stride; a.ys = dy_stride; a.width = width; a.eps = eps;
   a.x = x; a.w = weight; a.b = bias; a.mean = const_cast<double*>(mean); a.rstd = const_cast<float*>(rstd);
-  a.dy = dy; a.dx = dx; a.part = workspace;
-  return fsc::lnorm::backward(a, dtype, weight_dtype, activation, false, dweight, dbias, stream);
+  a.dy = dy; a.dx = dx; a.dw = dweight; a.db = dbias; a.part = workspace;
+  return fsc::lnorm::backward(a, dtype, weight_dtype, activation, false, stream);
 }
 
 int fsc_layer_norm_backward_twice(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
@@ -786,8 +837,9 @@ int fsc_layer_norm_backward_twice(int64_t rows, int32_t width, int32_t dtype, in
   fsc::lnorm::Args a{};
   a.rows = rows; a.xs = x_stride; a.ys = dy_stride; a.vs = v_stride; a.width = width; a.eps = eps;
   a.x = x; a.w = weight; a.b = bias; a.mean = const_cast<double*>(mean); a.rstd = const_cast<float*>(rstd);
-  a.dy = dy; a.v = v; a.vw = v_weight; a.vb = v_bias; a.gx = grad_x; a.gdy = grad_dy; a.part = workspace;
-  return fsc::lnorm::backward(a, dtype, weight_dtype, activation, true, grad_weight, grad_bias, stream);
+  a.dy = dy; a.v = v; a.vw = v_weight; a.vb = v_bias; a.gx = grad_x; a.gdy = grad_dy;
+  a.dw = grad_weight; a.db = grad_bias; a.part = workspace;
+  return fsc::lnorm::backward(a, dtype, weight_dtype, activation, true, stream);
 }
 
 }  // extern "C"
