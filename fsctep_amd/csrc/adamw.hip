@@ -29,7 +29,7 @@ struct Entry {
 struct Table {
   int count;
   int32_t first[MOST + 1];           // first block of each tensor
-  uint8_t bf16[MOST], wide[MOST];    // type of p and g; whether every array is aligned for four values a load
+  uint8_t bf16[MOST];                // type of p and g
   Entry t[MOST];
 };
 static_assert(sizeof(Table) <= 3800, "kernel arguments");
@@ -59,7 +59,7 @@ __device__ __forceinline__ int tensor_of(const Table& tab, int block) {
   return lo;
 }
 
-// One value.  Every operation rounds by itself, root and quotient correctly (the compiler's default; no fused
+// One value.  Every operation that reaches a state rounds by itself, the root correctly (the compiler's default; no fused
 // multiply-add): the codes of the 8-bit states then depend on
 // nothing but the formula.
 __device__ __forceinline__ void update(const Rule& k, float decay, float size, float over, float g, float& p, float& m,
@@ -68,12 +68,12 @@ __device__ __forceinline__ void update(const Rule& k, float decay, float size, f
   m = k.b1 * m + k.a1 * g;
   v = k.b2 * v + (k.a2 * g) * g;
   root = sqrtf(v);
-  p = p * decay - size * (m / (root * over + k.eps));
+  // the parameter alone takes the hardware's reciprocal, off by 2^-23: of the step, which is far below the parameter
+  p = p * decay - size * (m * __builtin_amdgcn_rcpf(root * over + k.eps));
 }
 
-// 32 bits from a value's number and the step: two rounds of multiplying and folding.
-__device__ __forceinline__ uint32_t hash(uint32_t place, uint32_t step) {
-  uint32_t h = place * 0x9E3779B1u + step * 0x6A09E667u;
+// 32 bits from place * 0x9E3779B1 + step * 0x6A09E667, place the value's number: two rounds of folding and multiplying.
+__device__ __forceinline__ uint32_t hash(uint32_t h) {
   h ^= h >> 16;
   h *= 0xBB67AE85u;
   h ^= h >> 15;
@@ -105,10 +105,20 @@ __device__ __forceinline__ uint32_t encode(float x, float over, uint32_t bits) {
   return (uint32_t)max(c, 0) | (x < 0.f ? 128u : 0u);
 }
 
-__device__ __forceinline__ float wave_top(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = max_nan(v, __shfl_xor(v, off, 64));
-  return v;
+// The wave's largest of values at and above zero, by their bits, which order as they do, NaN last; 0 below 2^-100.
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+__device__ __forceinline__ float wave_top(uint32_t v) {
+  v = max(v, dpp<0xB1>(v));              // neighbours, pairs, then mirrored in 8 and in 16 lanes
+  v = max(v, dpp<0x4E>(v));
+  v = max(v, dpp<0x141>(v));
+  v = max(v, dpp<0x140>(v));
+  v = max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+  v = max(v, (uint32_t)__shfl_xor((int)v, 32, 64));
+  const float top = __uint_as_float(v);
+  return top < 0x1p-100f ? 0.f : top;
 }
 
 // The step counts go up by one; decay, clip and each tensor's factors from them, in 64 bits.  One block.
@@ -133,146 +143,168 @@ __global__ __launch_bounds__(64) void prepare_kernel(Steps s, FscAdamSettings k,
   }
 }
 
-// N values from `at` on, those past n zeros; V: by one load (N * size aligned)
-template <int N, typename T>
-__device__ __forceinline__ void read(const T* p, int64_t at, int64_t n, bool wide, float (&v)[N]) {
-  if (wide && at + N <= n) {
-    struct alignas(N * sizeof(T)) Pack { T t[N]; };
-    const Pack k = *reinterpret_cast<const Pack*>(p + at);
+// Four values at any address; `last`: the tensor ends among them, those past n are zeros and not written.
+template <typename T>
+struct alignas(sizeof(T)) Four { T t[4]; };
+template <typename T>
+__device__ __forceinline__ void read(const T* p, int64_t at, int64_t n, bool last, float (&v)[4]) {
+  if (!last) {
+    const Four<T> k = *reinterpret_cast<const Four<T>*>(p + at);
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = to_f(k.t[j]);
+    for (int j = 0; j < 4; ++j) v[j] = to_f(k.t[j]);
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = at + j < n ? to_f(p[at + j]) : 0.f;
+    for (int j = 0; j < 4; ++j) v[j] = at + j < n ? to_f(p[at + j]) : 0.f;
   }
 }
-template <int N, typename T>
-__device__ __forceinline__ void write(T* p, int64_t at, int64_t n, bool wide, const float (&v)[N]) {
-  if (wide && at + N <= n) {
-    struct alignas(N * sizeof(T)) Pack { T t[N]; };
-    Pack k;
+template <typename T>
+__device__ __forceinline__ void write(T* p, int64_t at, int64_t n, bool last, const float (&v)[4]) {
+  if (!last) {
+    Four<T> k;
 #pragma unroll
-    for (int j = 0; j < N; ++j) k.t[j] = from_f<T>(v[j]);
-    *reinterpret_cast<Pack*>(p + at) = k;
+    for (int j = 0; j < 4; ++j) k.t[j] = from_f<T>(v[j]);
+    *reinterpret_cast<Four<T>*>(p + at) = k;
   } else {
 #pragma unroll
-    for (int j = 0; j < N; ++j)
+    for (int j = 0; j < 4; ++j)
       if (at + j < n) p[at + j] = from_f<T>(v[j]);
   }
 }
+__device__ __forceinline__ uint32_t read_codes(const uint8_t* p, int64_t at, int64_t n, bool last) {
+  uint32_t c = 0;
+  if (!last) {
+    const Four<uint8_t> k = *reinterpret_cast<const Four<uint8_t>*>(p + at);
+    c = __builtin_bit_cast(uint32_t, k);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (at + j < n) c |= (uint32_t)p[at + j] << (8 * j);
+  }
+  return c;
+}
+__device__ __forceinline__ void write_codes(uint8_t* p, int64_t at, int64_t n, bool last, uint32_t c) {
+  if (!last) {
+    *reinterpret_cast<Four<uint8_t>*>(p + at) = __builtin_bit_cast(Four<uint8_t>, c);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (at + j < n) p[at + j] = (uint8_t)(c >> (8 * j));
+  }
+}
 
-// Four values a lane, 256 a wave: the values that share a scale.
+// Four values a lane, 256 a wave: the values that share a scale.  LAST: the group that the tensor ends in.
+template <bool Q8, typename T, bool LAST>
+__device__ __forceinline__ void step_group(const Entry& e, int64_t group, int lane, const Rule& rule, const Factors& f, int i) {
+  const int64_t at = group * GROUP + lane * 4;
+  const bool last = LAST && at + 4 > e.n;
+  T* const p_ = (T*)e.p;
+  float* const own = sizeof(T) == 2 ? e.master : (float*)e.p;   // the value that is stepped
+  float p[4], g[4], m[4], v[4], root[4];
+  read((const T*)e.g, at, e.n, last, g);
+  read(own, at, e.n, last, p);
+  if (Q8) {
+    const float ms = e.m_scale[group], vs = e.v_scale[group];
+    const uint32_t mc = read_codes((const uint8_t*)e.m, at, e.n, last), vc = read_codes((const uint8_t*)e.v, at, e.n, last);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      m[j] = decode<false>(mc >> (8 * j) & 255u, ms);
+      const float r = decode<true>(vc >> (8 * j) & 255u, vs);
+      v[j] = r * r;
+    }
+  } else {
+    read((const float*)e.m, at, e.n, last, m);
+    read((const float*)e.v, at, e.n, last, v);
+  }
+  const float clip = f.clip, size = f.of[i].size, over = f.of[i].over;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) update(rule, f.decay, size, over, g[j] * clip, p[j], m[j], v[j], root[j]);
+  write(own, at, e.n, last, p);
+  if (sizeof(T) == 2) write(p_, at, e.n, last, p);
+  if (Q8) {
+    uint32_t mt = 0, vt = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      mt = max(mt, __float_as_uint(fabsf(m[j])));
+      vt = max(vt, __float_as_uint(root[j]));
+    }
+    const float ml = wave_top(mt), vl = wave_top(vt);
+    const float mo = ml > 0.f ? 1.f / ml : 0.f, vo = vl > 0.f ? 1.f / vl : 0.f;
+    const uint32_t step = (uint32_t)(int64_t)f.of[i].step, salt = (uint32_t)at * 0x9E3779B1u + step * 0x6A09E667u;
+    uint32_t mc = 0, vc = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t bits = hash(salt + j * 0x9E3779B1u);
+      mc |= encode<false>(m[j], mo, bits) << (8 * j);
+      vc |= encode<true>(root[j], vo, bits) << (8 * j);
+    }
+    write_codes((uint8_t*)e.m, at, e.n, last, mc);
+    write_codes((uint8_t*)e.v, at, e.n, last, vc);
+    if (lane == 0) {
+      e.m_scale[group] = ml;
+      e.v_scale[group] = vl;
+    }
+  } else {
+    write((float*)e.m, at, e.n, last, m);
+    write((float*)e.v, at, e.n, last, v);
+  }
+}
+
 template <bool Q8>
 __global__ __launch_bounds__(NT) void step_kernel(Table tab, Rule rule, const Factors* __restrict__ f) {
   const int i = tensor_of(tab, blockIdx.x);
   const Entry& e = tab.t[i];
   const int lane = threadIdx.x & 63;
-  const bool wide = tab.wide[i], bf16 = tab.bf16[i];
-  const float decay = f->decay, clip = f->clip, size = f->of[i].size, over = f->of[i].over;
-  const uint32_t step = (uint32_t)(int64_t)f->of[i].step;
-  const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * SHARE;
-  for (int part = threadIdx.x >> 6; part < SHARE / GROUP; part += NT / 64) {
-    const int64_t b0 = base + part * GROUP, at = b0 + lane * 4;
-    if (b0 >= e.n) break;
-    float p[4], g[4], m[4], v[4], root[4];
-    if (bf16) {
-      read<4>((const __bf16*)e.g, at, e.n, wide, g);
-      read<4>(e.master, at, e.n, wide, p);
+  const int64_t g0 = (int64_t)(blockIdx.x - tab.first[i]) * (SHARE / GROUP) + (threadIdx.x >> 6);
+#pragma unroll
+  for (int k = 0; k < SHARE / GROUP; k += NT / 64) {
+    const int64_t group = g0 + k;
+    if (group * GROUP >= e.n) break;
+    const bool whole = (group + 1) * GROUP <= e.n;
+    if (tab.bf16[i]) {
+      if (whole) step_group<Q8, __bf16, false>(e, group, lane, rule, *f, i);
+      else step_group<Q8, __bf16, true>(e, group, lane, rule, *f, i);
     } else {
-      read<4>((const float*)e.g, at, e.n, wide, g);
-      read<4>((const float*)e.p, at, e.n, wide, p);
-    }
-    const int64_t group = b0 / GROUP;
-    if (Q8) {
-      const float ms = e.m_scale[group], vs = e.v_scale[group];
-      uint32_t mc = 0, vc = 0;
-      if (wide && at + 4 <= e.n) {
-        mc = *reinterpret_cast<const uint32_t*>((const uint8_t*)e.m + at);
-        vc = *reinterpret_cast<const uint32_t*>((const uint8_t*)e.v + at);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (at + j < e.n) {
-            mc |= (uint32_t)((const uint8_t*)e.m)[at + j] << (8 * j);
-            vc |= (uint32_t)((const uint8_t*)e.v)[at + j] << (8 * j);
-          }
-      }
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        m[j] = decode<false>(mc >> (8 * j) & 255u, ms);
-        const float r = decode<true>(vc >> (8 * j) & 255u, vs);
-        v[j] = r * r;
-      }
-    } else {
-      read<4>((const float*)e.m, at, e.n, wide, m);
-      read<4>((const float*)e.v, at, e.n, wide, v);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) update(rule, decay, size, over, g[j] * clip, p[j], m[j], v[j], root[j]);
-    if (bf16) {
-      write<4>(e.master, at, e.n, wide, p);
-      write<4>((__bf16*)e.p, at, e.n, wide, p);
-    } else {
-      write<4>((float*)e.p, at, e.n, wide, p);
-    }
-    if (Q8) {
-      float mt = 0.f, vt = 0.f;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        mt = max_nan(mt, fabsf(m[j]));
-        vt = max_nan(vt, root[j]);
-      }
-      mt = wave_top(mt);
-      vt = wave_top(vt);
-      if (mt < 0x1p-100f) mt = 0.f;
-      if (vt < 0x1p-100f) vt = 0.f;
-      const float mo = mt > 0.f ? 1.f / mt : 0.f, vo = vt > 0.f ? 1.f / vt : 0.f;
-      uint32_t mc = 0, vc = 0;
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const uint32_t bits = hash((uint32_t)(at + j), step);
-        mc |= encode<false>(m[j], mo, bits) << (8 * j);
-        vc |= encode<true>(root[j], vo, bits) << (8 * j);
-      }
-      if (wide && at + 4 <= e.n) {
-        *reinterpret_cast<uint32_t*>((uint8_t*)e.m + at) = mc;
-        *reinterpret_cast<uint32_t*>((uint8_t*)e.v + at) = vc;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (at + j < e.n) {
-            ((uint8_t*)e.m)[at + j] = (uint8_t)(mc >> (8 * j));
-            ((uint8_t*)e.v)[at + j] = (uint8_t)(vc >> (8 * j));
-          }
-      }
-      if (lane == 0) {
-        e.m_scale[group] = mt;
-        e.v_scale[group] = vt;
-      }
-    } else {
-      write<4>((float*)e.m, at, e.n, wide, m);
-      write<4>((float*)e.v, at, e.n, wide, v);
+      if (whole) step_group<Q8, float, false>(e, group, lane, rule, *f, i);
+      else step_group<Q8, float, true>(e, group, lane, rule, *f, i);
     }
   }
 }
 
 // ---------------------------------------------------------------- the gradients' norm
-constexpr int NORM_SHARE = 8192;
+constexpr int NORM_SHARE = 8192, NORM_STEPS = NORM_SHARE / (NT * 4);
 
-// Sum of squares of a block's share, in 64 bits (a square of a float is exact there).
+// Sum of squares of a block's share, in 64 bits (a square of a float is exact there).  A whole share's loads are on their way
+// together (314 MB: one at a time 95 us, eight 72 us).
+template <typename T>
+__device__ __forceinline__ double squares(const T* g, int64_t base, int64_t n) {
+  double s = 0.0;
+  if (n >= 4) {
+    // vectors past the end: the last four values again, those that are not a lane's own left out
+    Four<T> v[NORM_STEPS];
+#pragma unroll
+    for (int k = 0; k < NORM_STEPS; ++k)
+      v[k] = *reinterpret_cast<const Four<T>*>(g + std::min<int64_t>(base + (k * NT + threadIdx.x) * 4, n - 4));
+#pragma unroll
+    for (int k = 0; k < NORM_STEPS; ++k) {
+      const int64_t at = base + (k * NT + threadIdx.x) * 4, skip = at - std::min<int64_t>(at, n - 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const double x = j >= skip ? (double)to_f(v[k].t[j]) : 0.0;
+        s += x * x;
+      }
+    }
+  } else if (threadIdx.x < n) {
+    const double x = (double)to_f(g[threadIdx.x]);
+    s = x * x;
+  }
+  return s;
+}
 __global__ __launch_bounds__(NT) void square_kernel(Table tab, double* __restrict__ part) {
   __shared__ double red[NT / 64];
   const int i = tensor_of(tab, blockIdx.x);
   const Entry& e = tab.t[i];
   const int64_t base = (int64_t)(blockIdx.x - tab.first[i]) * NORM_SHARE;
-  double s = 0.0;
-  for (int64_t at = base + threadIdx.x * 4; at < std::min<int64_t>(base + NORM_SHARE, e.n); at += NT * 4) {
-    float g[4];
-    if (tab.bf16[i]) read<4>((const __bf16*)e.g, at, e.n, tab.wide[i], g);
-    else read<4>((const float*)e.g, at, e.n, tab.wide[i], g);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s += (double)g[j] * (double)g[j];
-  }
+  double s = tab.bf16[i] ? squares((const __bf16*)e.g, base, e.n) : squares((const float*)e.g, base, e.n);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) s += __shfl_xor(s, off, 64);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
@@ -294,11 +326,33 @@ __global__ __launch_bounds__(1024) void norm_kernel(const double* __restrict__ p
   }
 }
 
+// Four codes a thread, which share a scale, VALUE_STEPS times a block's width apart; stored past the caches.
+constexpr int VALUE_STEPS = 4, VALUE_SHARE = NT * 4 * VALUE_STEPS;
 template <bool ROOT>
 __global__ __launch_bounds__(NT) void values_kernel(int64_t n, const uint8_t* __restrict__ c,
-                                                    const float* __restrict__ scale, float* __restrict__ v) {
-  for (int64_t i = (int64_t)blockIdx.x * NT + threadIdx.x; i < n; i += (int64_t)gridDim.x * NT)
-    v[i] = decode<ROOT>(c[i], scale[i / GROUP]);
+                                                    const float* __restrict__ scale, float* __restrict__ v, int64_t first) {
+  const int64_t base = first + (int64_t)blockIdx.x * VALUE_SHARE;
+  if (base + VALUE_SHARE <= n) {
+    struct alignas(1) Pack { uint8_t t[4]; };
+    Pack k[VALUE_STEPS];
+    float s[VALUE_STEPS];
+#pragma unroll
+    for (int j = 0; j < VALUE_STEPS; ++j) {
+      const int64_t at = base + (j * NT + threadIdx.x) * 4;
+      k[j] = *reinterpret_cast<const Pack*>(c + at);
+      s[j] = scale[at / GROUP];
+    }
+#pragma unroll
+    for (int j = 0; j < VALUE_STEPS; ++j) {
+      typedef float f4s __attribute__((ext_vector_type(4), aligned(4)));
+      f4s x;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x[i] = decode<ROOT>(k[j].t[i], s[j]);
+      __builtin_nontemporal_store(x, reinterpret_cast<f4s*>(v + base + (j * NT + threadIdx.x) * 4));
+    }
+  } else {
+    for (int64_t i = base + threadIdx.x; i < n; i += NT) v[i] = decode<ROOT>(c[i], scale[i / GROUP]);
+  }
 }
 
 inline int64_t blocks_of(int64_t n, int share) { return (n + share - 1) / share; }
@@ -320,8 +374,6 @@ int by_tables(int32_t count, const FscAdamTensor* t, int share, F&& f) {
       tab.first[k] = (int32_t)blocks;
       blocks += b;
       tab.bf16[k] = s.dtype == FSC_BF16;
-      const uintptr_t half = (uintptr_t)s.g | (uintptr_t)s.p, full = (uintptr_t)s.master | (uintptr_t)s.m | (uintptr_t)s.v;
-      tab.wide[k] = half % (s.dtype == FSC_BF16 ? 8 : 16) == 0 && full % 16 == 0;
       tab.t[k] = Entry{s.n, s.p, s.g, s.m, s.v, s.m_scale, s.v_scale, s.master};
     }
     tab.first[tab.count] = (int32_t)blocks;
@@ -417,9 +469,12 @@ int fsc_adamw_values(int64_t n, int32_t root, const uint8_t* codes, const float*
   FSC_CHECK_ARG(n >= 0, "adamw_values: negative size");
   if (n == 0) return 0;
   FSC_CHECK_ARG(codes && scale && values, "adamw_values: null array");
-  const unsigned grid = (unsigned)std::min<int64_t>((n + NT - 1) / NT, 1 << 16);
-  if (root) values_kernel<true><<<grid, NT, 0, stream>>>(n, codes, scale, values);
-  else values_kernel<false><<<grid, NT, 0, stream>>>(n, codes, scale, values);
+  constexpr int64_t MOST_VALUES = (int64_t)VALUE_SHARE << 23;             // fewer than 2^32 threads a launch
+  for (int64_t f = 0; f < n; f += MOST_VALUES) {
+    const unsigned grid = (unsigned)((std::min(n - f, MOST_VALUES) + VALUE_SHARE - 1) / VALUE_SHARE);
+    if (root) values_kernel<true><<<grid, NT, 0, stream>>>(n, codes, scale, values, f);
+    else values_kernel<false><<<grid, NT, 0, stream>>>(n, codes, scale, values, f);
+  }
   return check_launch("adamw_values") ? 2 : 0;
 }
 
