@@ -65,39 +65,33 @@ __device__ __forceinline__ void store_some(T* p, int n, const float (&v)[M]) {
 }
 
 // ---------------------------------------------------------------- lookup
-// A row's vector a thread, STEPS of them a block's width apart.  Where no vector divides the width, a row's last one lies at
-// its end and writes some of the values before it once more (the same ones); rows shorter than a vector are one
-// vector that is not full.
-constexpr int STEPS = 4;
+// A row's vector a thread.  Where no vector divides the width, a row's last one lies at its end and writes some of the values
+// before it once more (the same ones); rows shorter than a vector are one vector that is not full.  Bound by the stores,
+// which go past the caches: what they write is read by other kernels, on other XCDs (520,000 x 192: 58 us, a fill of that
+// size 59 us; ordinary stores 95 us; four vectors a thread 69 and 86 us).
 template <typename T, typename I, bool FULL>
 __global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint32_t vectors) {
   constexpr int N = Vec<T>::N;
-  const int64_t total = a.rows * vectors;
-  const int64_t f0 = first + (int64_t)blockIdx.x * (NT * STEPS);         // the block's first vector, in row r0
-  const int64_t r0 = f0 / vectors;
-  const uint32_t c0 = (uint32_t)(f0 - r0 * vectors);
-  const int n = FULL ? N : a.width;
-  float v[STEPS][N];
-  int64_t row[STEPS], t[STEPS];
-  int col[STEPS];
+  const int64_t f0 = first + (int64_t)blockIdx.x * NT, r0 = f0 / vectors;     // the block's first vector, in row r0
+  if (f0 + threadIdx.x >= a.rows * vectors) return;
+  const uint32_t local = (uint32_t)(f0 - r0 * vectors) + threadIdx.x, up = local / vectors;
+  const int n = FULL ? N : a.width, col = std::min((int)(local - up * vectors) * N, a.width - n);
+  const int64_t row = r0 + up, t = ((const I*)a.index)[row];
+  const bool there = t >= 0 && t < a.table_rows;
+  float v[N];
+  load_some<FULL, N>((const T*)a.in + (there ? t : 0) * a.stride + col, n, v);
 #pragma unroll
-  for (int s = 0; s < STEPS; ++s) {      // vectors past the last one: the last one again, not stored
-    const int64_t f = std::min<int64_t>(f0 + s * NT + threadIdx.x, total - 1);
-    const uint32_t local = c0 + (uint32_t)(f - f0), up = local / vectors;
-    row[s] = r0 + up;
-    col[s] = std::min((int)(local - up * vectors) * N, a.width - n);
-    t[s] = ((const I*)a.index)[row[s]];
+  for (int j = 0; j < N; ++j) v[j] = there ? a.scale * v[j] : 0.f;
+  T* out = (T*)a.out + row * a.width + col;
+  if constexpr (FULL) {
+    typedef unsigned u4s __attribute__((ext_vector_type(4), aligned(2)));
+    struct Pack { T t[N]; } k;
+#pragma unroll
+    for (int j = 0; j < N; ++j) k.t[j] = from_f<T>(v[j]);
+    __builtin_nontemporal_store(__builtin_bit_cast(u4s, k), reinterpret_cast<u4s*>(out));
+  } else {
+    store_some<false, N>(out, n, v);
   }
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s) {
-    const bool there = t[s] >= 0 && t[s] < a.table_rows;
-    load_some<FULL, N>((const T*)a.in + (there ? t[s] : 0) * a.stride + col[s], n, v[s]);
-#pragma unroll
-    for (int j = 0; j < N; ++j) v[s][j] = there ? a.scale * v[s][j] : 0.f;
-  }
-#pragma unroll
-  for (int s = 0; s < STEPS; ++s)
-    if (f0 + s * NT + threadIdx.x < total) store_some<FULL, N>((T*)a.out + row[s] * a.width + col[s], n, v[s]);
 }
 
 // ---------------------------------------------------------------- gradient, few tokens
@@ -523,7 +517,7 @@ Layout layout_of(int64_t rows, int width, int64_t table_rows, int size) {
   l.blocks = (rows + NT * per_thread(rows) - 1) / (NT * per_thread(rows));
   // enough shares to fill the chip with waves, not so many that a token's partial rows take long to join
   const int64_t waves = rows * l.columns * l.lanes / 64;
-  l.share = (int)std::min<int64_t>(1024, std::max<int64_t>({16, waves / WAVES, rows / 8192}));
+  l.share = (int)std::min<int64_t>(1024, std::max<int64_t>({32, waves / WAVES, rows / 8192}));
   l.shares = (rows + l.share - 1) / l.share;
   int64_t at = 0;
   auto take = [&](int64_t n) {
@@ -564,7 +558,7 @@ SmallLayout small_layout(int64_t rows, int width, int64_t table_rows) {
 
 template <typename T, typename I>
 void launch_lookup(const Args& a, hipStream_t st) {
-  constexpr int64_t BLOCK = (int64_t)NT * STEPS, MOST = BLOCK << 23;     // fewer than 2^32 threads a launch
+  constexpr int64_t BLOCK = NT, MOST = BLOCK << 23;                      // fewer than 2^32 threads a launch
   const int64_t vectors = (a.width + Vec<T>::N - 1) / Vec<T>::N, total = a.rows * vectors;
   for (int64_t f = 0; f < total; f += MOST)
     FSC_EMBED_FULL(a.width >= Vec<T>::N, (lookup_kernel<T, I, FULL><<<(unsigned)((std::min(total - f, MOST) + BLOCK - 1) / BLOCK),
