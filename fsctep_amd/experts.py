@@ -100,7 +100,8 @@ class Router:
         """Of an atom without a row NaN, which the router passes on to what the atom becomes."""
         if self.n_species is None:
             return F.linear(y, layer.gate)
-        l = layer.gate.index_select(0, species)
+        from . import train_ops as T
+        l = T.lookup(layer.gate, species)
         return l if none is None else l.masked_fill(none, math.nan)
 
     def choose(self, layer, logits):

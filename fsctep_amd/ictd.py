@@ -315,7 +315,8 @@ class _ICTDTrunk(nn.Module):
         f = torch.cat(outs, dim=-1)
         if self.readout_experts is not None:
             f = self.readout_experts(f, species, differentiable=train, species_below=self.n_species)
-        e = self.weighted_sum(self.proj_total(f)) if train else readout_energy(self.proj_total, self.weighted_sum, f)
+        head = T.readout_energy if train else readout_energy
+        e = head(self.proj_total, self.weighted_sum, f)
         dip = None
         if self._dipole and with_dipole:
             # the (1, -1) Gram input, (N, d, n*C), by the same column map (differentiable gather)

@@ -15,6 +15,7 @@ States in 8 bits (``state_bits=8``): m and sqrt(v) as 8-bit floats with a float3
 up or down by a hash of the value's number and the step, so that small changes add up over the steps instead of being
 rounded away.  16 bytes a value are moved in place of 28.
 
+    train_step(model, optimizer, pos, batch, cell, graph, energy, forces, ...)       # a trunk's step on energies and forces
     adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay, max_norm, masters, norm)
     adamw_step_q8(params, grads, exp_avgs, exp_avg_scales, roots, root_scales, steps, ...)
     grad_norm(grads) -> norm
@@ -166,3 +167,29 @@ class AdamW(torch.optim.Optimizer):
             want = {"exp_avg_sq"} if self.state_bits == 32 else {"root", "root_scale", "exp_avg_scale"}
             if not want <= set(s):
                 raise ValueError(f"the checkpoint's states do not have {self.state_bits} bits")
+
+
+def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy_weight: float = 1.0,
+               force_weight: float = 1.0, external_tensor=None):
+    """One training step of a trunk in ``train()`` mode on a prepared graph (``sparse.energy_and_forces`` and
+    ``ictd.energy_forces`` are the same evaluation without the step): energies (G,) of the structures and forces F = -dE/dpos
+    (N, 3), loss = energy_weight mean (E - energy)^2 + force_weight mean (F - forces)^2 (training/trainer.py:1292-1297),
+    its gradients, and the optimiser's step.  Returns (loss, E, F), detached; nothing waits for the GPU."""
+    optimizer.zero_grad(set_to_none=True)
+    pos = pos.detach().requires_grad_(True)
+    if external_tensor is None:
+        out = model.forward_graph(pos, batch, cell, graph)
+    else:
+        out = model.forward_graph(pos, batch, cell, graph, external_tensor=external_tensor)
+    atoms = (out[0] if isinstance(out, tuple) else out).squeeze(-1)
+    # the sum by structure is the gradient of a lookup of each atom's structure
+    total = torch.ops.fsctep.embedding_backward(atoms.unsqueeze(1), batch, cell.shape[0], 1.0).squeeze(1)
+    gradient, = torch.autograd.grad(atoms.sum(), pos, create_graph=True)
+    loss = (energy_weight * (total - energy).square().mean()
+            + force_weight * (gradient + forces).square().mean())
+    # of the parameters alone: the positions are not trained
+    params = [p for group in optimizer.param_groups for p in group["params"]]
+    for p, g in zip(params, torch.autograd.grad(loss, params, allow_unused=True)):
+        p.grad = g
+    optimizer.step()
+    return loss.detach(), total.detach(), -gradient.detach()

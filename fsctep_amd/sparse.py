@@ -351,7 +351,7 @@ class PureCartesianSparseTransformerLayer(nn.Module):
         if self.readout_experts is not None:
             f5 = self.readout_experts(f5, species, differentiable=train, species_below=self.n_species)
         if train:
-            return self.weighted_sum(self.proj_total(f5))
+            return T.readout_energy(self.proj_total, self.weighted_sum, f5)
         return readout_energy(self.proj_total, self.weighted_sum, f5)
 
 

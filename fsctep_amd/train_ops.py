@@ -7,6 +7,8 @@ build the step from:
 * the conv2..n tensor products on their HIP kernels (``sparse_conv`` / ``ictd_conv``), whose C++ autograd
   gives the parameter gradients and a differentiable backward (the analogues of the reference's
   double-backward kernels, csrc/ictd_tp_cuda.cu:536-971): these carry almost all of the step's work;
+* the layer norms of the energy head, with their SiLU, on the HIP op that differentiates twice, and the lookups
+  by species pair on the HIP op whose gradient sums by pair (``learn_ops``);
 * the functions below for the rest: edge geometry, radial basis and radial MLP, ICTD direction harmonics,
   the conv1 species-pair contraction and the readout's Gram bilinear and squared norms.  They are the same
   formulas as the inference kernels (``edge_radial.hip``, ``sparse_conv.hip`` conv1, ``ictd_conv.hip`` conv1,
@@ -22,9 +24,24 @@ from __future__ import annotations
 import math
 
 import torch
+import torch.nn as nn
 import torch.nn.functional as F
 
 from .graph import Graph
+
+
+def _on_ops(t) -> bool:
+    """Whether a tensor is one that the HIP ops take (others, the host's and 64-bit ones, stay with torch)."""
+    return t.is_cuda and t.dtype in (torch.float32, torch.bfloat16)
+
+
+# ------------------------------------------------------------------ lookups (embedding.hip)
+def lookup(table, index):
+    """``table.index_select(0, index)`` of a table of any shape, its gradient summed by row in a fixed order."""
+    if not _on_ops(table) or table.numel() == 0:
+        return table.index_select(0, index)
+    from . import learn_ops
+    return learn_ops.embedding(table.reshape(table.shape[0], -1), index).view(-1, *table.shape[1:])
 
 
 # ------------------------------------------------------------------ edge geometry (edge_radial.hip)
@@ -143,10 +160,10 @@ def sparse_conv1(h, n, w_last, b_last, atab, g: Graph, channels: int):
     tile_pair = g.pair_tiles[16 * nt:].long()
     valid = ids >= 0
     ht = h.index_select(0, ids.clamp(min=0).reshape(-1)).view(nt, 16, K) * valid.unsqueeze(-1).to(h.dtype)
-    qt = torch.bmm(ht, T.index_select(0, tile_pair))                            # (nt, 16, 3C)
+    qt = torch.bmm(ht, lookup(T, tile_pair))                                    # (nt, 16, 3C)
     slot = torch.where(valid, ids, torch.full_like(ids, E)).reshape(-1)
     Q = h.new_zeros(E + 1, 3 * C).index_copy(0, slot, qt.reshape(-1, 3 * C))[:E]
-    Q = (Q + Tb.index_select(0, g.edge_pair.long())).view(E, 3, C)
+    Q = (Q + lookup(Tb, g.edge_pair)).view(E, 3, C)
     nn_ = (n.unsqueeze(-1) * n.unsqueeze(-2)).reshape(E, 9)
     msg = torch.cat([Q[:, 0:1, :], Q[:, 1:2, :] * n.unsqueeze(-1), Q[:, 2:3, :] * nn_.unsqueeze(-1)], dim=1)
     return _receiver_mean(msg, g)
@@ -159,7 +176,7 @@ def ictd_conv1(Fe, gates, qtab, g: Graph, layout):
     A_dst[j]; summed to receivers / max(in-degree, 1)."""
     E = Fe.shape[0]
     C = qtab.shape[2]
-    Qe = qtab.index_select(0, g.edge_pair.long())                                 # (E, NP1, C)
+    Qe = lookup(qtab, g.edge_pair)                                                # (E, NP1, C)
     msg = Fe.new_zeros(E, layout.M, C)
     parts = []
     for i, p in enumerate(layout.conv1_paths()):
@@ -216,6 +233,36 @@ def readout_features(feats, Ws, scales, maps):
         sqs.append(torch.cat([(f[:, comp:comp + d, :] ** 2).sum(1) for f in feats], dim=1))
         comp += d
     return scalars, torch.stack(sqs, dim=1)
+
+
+# ------------------------------------------------------------------ energy head (layer_norm.hip)
+def _plain_norm(ln) -> bool:
+    """A LayerNorm over the last dimension as it was made, with nothing hooked to its call."""
+    return (type(ln) is nn.LayerNorm and len(ln.normalized_shape) == 1 and not ln._forward_hooks
+            and not ln._forward_pre_hooks and not ln._backward_hooks and not ln._backward_pre_hooks)
+
+
+def _norm(ln, x, activation=None):
+    params = [p for p in (ln.weight, ln.bias) if p is not None]
+    if _on_ops(x) and x.dim() == 2 and x.shape[1] == ln.normalized_shape[0] and all(p.dtype == x.dtype for p in params):
+        from . import learn_ops
+        return learn_ops.layer_norm(x, ln.weight, ln.bias, ln.eps, activation)
+    y = ln(x)
+    return F.silu(y) if activation else y
+
+
+def readout_energy(net, weighted_sum, x):
+    """``weighted_sum(net(x))`` of the energy head (models/mlp.py:8-66, :117-133), differentiable twice: the layer norms and
+    their SiLU on the HIP op, the products in torch.  Heads that are not as ``sparse.MainNet`` makes them run as the modules."""
+    from .sparse import MainNet
+    norms = [net.input_norm, *net.layer_norms] if type(net) is MainNet else []
+    if (not norms or not all(_plain_norm(ln) for ln in norms) or net._forward_hooks or net._forward_pre_hooks
+            or net._backward_hooks or net._backward_pre_hooks or torch.is_autocast_enabled()):
+        return weighted_sum(net(x))
+    y = _norm(net.input_norm, x)
+    for lin, ln in zip(net.layers, net.layer_norms):
+        y = _norm(ln, lin(y), "silu")
+    return weighted_sum(net.output(y))
 
 
 # ------------------------------------------------------------------ expert readout (rms_norm.hip, expert_mlp.hip)
