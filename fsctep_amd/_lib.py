@@ -89,7 +89,7 @@ SIGNATURES = {
     "fsc_expert_mlp_q8": [_p, _i64] + [_p] * 12,
     "fsc_layer_norm_forward": [_i64, _i32, _i32, _i32, _i32, _i64, _p, _p, _p, _f32, _p, _p, _p, _p],
     "fsc_layer_norm_workspace": [_i64, _i32, _pi64],
-    "fsc_layer_norm_backward": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _p, _p, _p, _f32] + [_p] * 8,
+    "fsc_layer_norm_backward": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _f32] + [_p] * 9,
     "fsc_layer_norm_backward_twice": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _f32] + [_p] * 12,
     "fsc_embedding_forward": [_i64, _i32, _i64, _i32, _i32, _i64, _p, _p, _f32, _p, _p],
     "fsc_embedding_workspace": [_i64, _i32, _i64, _pi64],

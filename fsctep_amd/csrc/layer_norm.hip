@@ -32,6 +32,8 @@ struct Args {
   void* y;
   // backward: dx null: not wanted
   const void* dy;
+  const void* plus;            // added to dx, or null
+  int64_t ps;                  // its row stride
   void* dx;
   void *dw, *db;               // null: not wanted
   float* part;                 // [gridDim.x][2][width] partial sums of the two
@@ -165,10 +167,11 @@ __global__ __launch_bounds__(NT) void wide_back_kernel(Args a) {
     block_add(s, (F*)red);
     const F mg = s[0] / a.width, mgz = s[1] / a.width;
     T* dx = (T*)a.dx + row * a.width;
+    const T* plus = a.plus ? (const T*)a.plus + row * a.ps : nullptr;
     for (int i = threadIdx.x; i < a.width; i += NT) {
       F zh, du;
       terms(i, zh, du);
-      dx[i] = from_f<T>((float)(r * (du * (F)at_or(w, i, 1.f) - mg - zh * mgz)));
+      dx[i] = from_f<T>((float)((F)at_or(plus, i, 0.f) + r * (du * (F)at_or(w, i, 1.f) - mg - zh * mgz)));
     }
   }
 }
@@ -545,6 +548,7 @@ __global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
         s[1] += g[c][j] * z[c][j];
       }
     if (!a.dx) continue;
+    at.load_or(a.plus ? (const T*)a.plus + row * a.ps : nullptr, 0.f, d);
     row_add(s);
     const F mg = s[0] / n, mgz = s[1] / n;
     if (there)
@@ -552,7 +556,7 @@ __global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
       for (int c = 0; c < CH; ++c) {
         F o[V];
 #pragma unroll
-        for (int j = 0; j < V; ++j) o[j] = r * ((g[c][j] - mg) - z[c][j] * mgz);
+        for (int j = 0; j < V; ++j) o[j] = (F)d[c][j] + r * ((g[c][j] - mg) - z[c][j] * mgz);
         at.store((T*)a.dx + row * a.width, c, o);
       }
   }
@@ -777,7 +781,7 @@ int check_types(int64_t rows, int32_t width, int32_t dtype, int32_t wtype, int32
 int backward(const Args& a, int32_t dtype, int32_t wtype, int32_t act, bool twice, hipStream_t st) {
   if (int rc = check_types(a.rows, a.width, dtype, wtype, act)) return rc;
   FSC_CHECK_ARG(a.rows == 0 || (a.x && a.mean && a.rstd && a.dy), "layer_norm_backward: null array");
-  FSC_CHECK_ARG(a.xs >= 0 && a.ys >= 0 && a.vs >= 0, "layer_norm_backward: negative row stride");
+  FSC_CHECK_ARG(a.xs >= 0 && a.ys >= 0 && a.vs >= 0 && a.ps >= 0, "layer_norm_backward: negative row stride");
   FSC_CHECK_ARG(!(a.dw || a.db) || a.part, "layer_norm_backward: the weight's and the bias' gradients need a workspace");
   if (!a.dw && !a.db && (a.rows == 0 || !(a.dx || a.gx || a.gdy))) return 0;
   if (twice) {
@@ -818,13 +822,13 @@ int fsc_layer_norm_workspace(int64_t rows, int32_t width, int64_t* floats) {
 }
 
 int fsc_layer_norm_backward(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
-                            int64_t x_stride, int64_t dy_stride, const void* x, const void* weight, const void* bias,
-                            float eps, const double* mean, const float* rstd, const void* dy, void* dx, void* dweight,
-                            void* dbias, float* workspace, hipStream_t stream) {
+                            int64_t x_stride, int64_t dy_stride, int64_t plus_stride, const void* x, const void* weight,
+                            const void* bias, float eps, const double* mean, const float* rstd, const void* dy,
+                            const void* plus, void* dx, void* dweight, void* dbias, float* workspace, hipStream_t stream) {
   fsc::lnorm::Args a{};
   a.rows = rows; a.xs = x_stride; a.ys = dy_stride; a.width = width; a.eps = eps;
   a.x = x; a.w = weight; a.b = bias; a.mean = const_cast<double*>(mean); a.rstd = const_cast<float*>(rstd);
-  a.dy = dy; a.dx = dx; a.dw = dweight; a.db = dbias; a.part = workspace;
+  a.dy = dy; a.plus = plus; a.ps = plus_stride; a.dx = dx; a.dw = dweight; a.db = dbias; a.part = workspace;
   return fsc::lnorm::backward(a, dtype, weight_dtype, activation, false, stream);
 }
 

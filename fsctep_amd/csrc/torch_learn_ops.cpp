@@ -91,12 +91,15 @@ NormGrad norm_grad(const Tensor& x, const Tensor& w, const Tensor& b, double eps
   return g;
 }
 
-// (dx, dweight, dbias), empty where not wanted
+// (dx + plus, dweight, dbias), empty where not wanted.  `through` has x's shape and no values: the gradient of x takes its way
+// where it is given (LayerNormFn).
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy_, const Tensor& x_, const optional<Tensor>& w_,
                                                        const optional<Tensor>& b_, const Tensor& mean_, const Tensor& rstd_,
-                                                       double eps, int64_t act, bool want_x, bool want_w, bool want_b) {
+                                                       double eps, int64_t act, bool want_x, bool want_w, bool want_b,
+                                                       const optional<Tensor>& plus_, const optional<Tensor>&) {
   const char* op = "layer_norm_backward";
-  require_gpu({x_, dy_, some(w_), some(b_), mean_, rstd_}, op);
+  require_gpu({x_, dy_, some(w_), some(b_), mean_, rstd_, some(plus_)}, op);
+  check_rows_like(some(plus_), x_, op, "plus");
   check_norm(x_, some(w_), some(b_), eps, act, op);
   check_rows_like(dy_, x_, op, "dy");
   check_stats(x_, mean_, rstd_, op);
@@ -104,11 +107,12 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy_, const 
   const c10::OptionalDeviceGuard device(x_.device());
   NormGrad g = norm_grad(x_, some(w_), some(b_), eps, act, want_w || want_b, op);
   const Tensor dy = rows2d(dy_, "dy"), mean = mean_.contiguous(), rstd = rstd_.contiguous();
+  const Tensor plus = plus_.has_value() ? rows2d(*plus_, "plus") : Tensor();
   Tensor dx = out_if(want_x, g.x);
   Tensor dw = out_if(want_w, want_w ? g.w : g.x), db = out_if(want_b, want_b ? g.b : g.x);
   check(fsc_layer_norm_backward(g.x.size(0), (int32_t)g.x.size(1), g.dt, g.wt, (int32_t)act, stride_of(g.x), stride_of(dy),
-                                ptr(g.x), ptr(g.w), ptr(g.b), (float)eps, (const double*)ptr(mean), (const float*)ptr(rstd),
-                                ptr(dy), want_x ? mptr(dx) : nullptr, want_w ? mptr(dw) : nullptr,
+                                stride_or_0(plus), ptr(g.x), ptr(g.w), ptr(g.b), (float)eps, (const double*)ptr(mean),
+                                (const float*)ptr(rstd), ptr(dy), ptr(plus), want_x ? mptr(dx) : nullptr, want_w ? mptr(dw) : nullptr,
                                 want_b ? mptr(db) : nullptr, (float*)mptr(g.ws), stream_of(g.x)),
         "fsc_layer_norm_backward");
   return {dx, dw, db};
@@ -116,10 +120,12 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward(const Tensor& dy_, const 
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_meta(const Tensor& dy, const Tensor& x, const optional<Tensor>& w,
                                                             const optional<Tensor>& b, const Tensor& mean, const Tensor& rstd,
-                                                            double eps, int64_t act, bool want_x, bool want_w, bool want_b) {
+                                                            double eps, int64_t act, bool want_x, bool want_w, bool want_b,
+                                                            const optional<Tensor>& plus, const optional<Tensor>&) {
   const char* op = "layer_norm_backward";
   check_norm(x, some(w), some(b), eps, act, op);
   check_rows_like(dy, x, op, "dy");
+  check_rows_like(some(plus), x, op, "plus");
   check_stats(x, mean, rstd, op);
   check_wanted(some(w), some(b), want_w, want_b, op);
   return {out_if(want_x, x), out_if(want_w, want_w ? some(w) : x), out_if(want_b, want_b ? some(b) : x)};
@@ -177,20 +183,25 @@ auto& layer_norm_op() {
 auto& layer_norm_backward_op() {
   static auto op = op_handle<std::tuple<Tensor, Tensor, Tensor>(
       const Tensor&, const Tensor&, const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, double,
-      int64_t, bool, bool, bool)>("fsctep::layer_norm_backward");
+      int64_t, bool, bool, bool, const optional<Tensor>&, const optional<Tensor>&)>("fsctep::layer_norm_backward");
   return op;
 }
 optional<Tensor> opt(const Tensor& t) { return t.defined() ? optional<Tensor>(t) : std::nullopt; }
 
-// The backward as a function of dy, x, weight and bias (the statistics are x's own): its backward is an op without one.
+// The backward as a function of dy, x, weight and bias (the statistics are x's own), and of plus: its backward is an op without
+// one.
 struct LayerNormBackwardFn : public torch::autograd::Function<LayerNormBackwardFn> {
   static variable_list forward(AutogradContext* ctx, Tensor dy, Tensor x, optional<Tensor> w, optional<Tensor> b, Tensor mean,
-                               Tensor rstd, double eps, int64_t act, bool want_x, bool want_w, bool want_b) {
+                               Tensor rstd, double eps, int64_t act, bool want_x, bool want_w, bool want_b,
+                               optional<Tensor> plus, optional<Tensor> through) {
     at::AutoDispatchBelowADInplaceOrView guard;
-    auto [dx, dw, db] = layer_norm_backward_op().call(dy, x, w, b, mean, rstd, eps, act, want_x, want_w, want_b);
+    auto [dx, dw, db] =
+        layer_norm_backward_op().call(dy, x, w, b, mean, rstd, eps, act, want_x, want_w, want_b, plus, std::nullopt);
     ctx->save_for_backward({dy, x, some(w), some(b), mean, rstd});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["act"] = act;
+    ctx->saved_data["plus"] = plus.has_value();
+    ctx->saved_data["through"] = through.has_value();
     ctx->set_materialize_grads(false);
     variable_list none;
     if (!want_x) none.push_back(dx);
@@ -200,22 +211,28 @@ struct LayerNormBackwardFn : public torch::autograd::Function<LayerNormBackwardF
     return {dx, dw, db};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(11);
+    variable_list out(13);
     if (!grads[0].defined() && !grads[1].defined() && !grads[2].defined()) return out;
     auto s = ctx->get_saved_variables();
     static auto op = op_handle<std::tuple<Tensor, Tensor, Tensor, Tensor>(
         const optional<Tensor>&, const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&,
         const optional<Tensor>&, const optional<Tensor>&, const Tensor&, const Tensor&, double, int64_t, bool, bool, bool, bool)>(
         "fsctep::layer_norm_backward_twice");
-    const bool want_dy = ctx->needs_input_grad(0), want_x = ctx->needs_input_grad(1);
-    const bool want_w = s[2].defined() && ctx->needs_input_grad(2);
-    const bool want_b = s[3].defined() && ctx->needs_input_grad(s[2].defined() ? 3 : 2);    // counts the tensors there are
+    // needs_input_grad counts the tensors there are: dy, x, weight, bias, mean, rstd, plus, through
+    const bool has_w = s[2].defined(), has_b = s[3].defined();
+    const bool has_plus = ctx->saved_data["plus"].toBool(), has_through = ctx->saved_data["through"].toBool();
+    const size_t at_plus = 4 + has_w + has_b, at_through = at_plus + has_plus;
+    const bool want_dy = ctx->needs_input_grad(0);
+    const bool want_x = has_through ? ctx->needs_input_grad(at_through) : ctx->needs_input_grad(1);
+    const bool want_w = has_w && ctx->needs_input_grad(2), want_b = has_b && ctx->needs_input_grad(2 + has_w);
+    if (has_plus && ctx->needs_input_grad(at_plus)) out[11] = grads[0];
+    if (!want_dy && !want_x && !want_w && !want_b) return out;
     BackwardGuard guard;
     auto [gx, gdy, gw, gb] =
         op.call(opt(grads[0]), opt(grads[1]), opt(grads[2]), s[0], s[1], opt(s[2]), opt(s[3]), s[4], s[5],
                 ctx->saved_data["eps"].toDouble(), ctx->saved_data["act"].toInt(), want_x, want_dy, want_w, want_b);
     if (want_dy) out[0] = gdy;
-    if (want_x) out[1] = gx;
+    if (want_x) out[has_through ? 12 : 1] = gx;
     if (want_w) out[2] = gw;
     if (want_b) out[3] = gb;
     return out;
@@ -225,37 +242,46 @@ struct LayerNormBackwardFn : public torch::autograd::Function<LayerNormBackwardF
 std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& dy, const Tensor& x, const optional<Tensor>& w,
                                                                 const optional<Tensor>& b, const Tensor& mean,
                                                                 const Tensor& rstd, double eps, int64_t act, bool want_x,
-                                                                bool want_w, bool want_b) {
-  if (differentiates({dy, x, some(w), some(b)})) {
-    auto r = LayerNormBackwardFn::apply(dy, x, w, b, mean, rstd, eps, act, want_x, want_w, want_b);
+                                                                bool want_w, bool want_b, const optional<Tensor>& plus,
+                                                                const optional<Tensor>& through) {
+  if (differentiates({dy, x, some(w), some(b), some(plus), some(through)})) {
+    auto r = LayerNormBackwardFn::apply(dy, x, w, b, mean, rstd, eps, act, want_x, want_w, want_b, plus, through);
     return {r[0], r[1], r[2]};
   }
   at::AutoDispatchBelowADInplaceOrView guard;
-  return layer_norm_backward_op().call(dy, x, w, b, mean, rstd, eps, act, want_x, want_w, want_b);
+  return layer_norm_backward_op().call(dy, x, w, b, mean, rstd, eps, act, want_x, want_w, want_b, plus, through);
 }
 
+// A force loss sends two gradients to x, one through y and one through the backward's own backward.  The second comes to this
+// function's node as the gradient of `through`, an output of x's shape that holds nothing, and the kernel that makes the first
+// adds it (`plus`): a pass over x less than autograd's addition takes.
 struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   static variable_list forward(AutogradContext* ctx, Tensor x, optional<Tensor> w, optional<Tensor> b, double eps,
                                int64_t act) {
     at::AutoDispatchBelowADInplaceOrView guard;
     auto [y, mean, rstd] = layer_norm_op().call(x, w, b, eps, act, true);
-    ctx->save_for_backward({x, some(w), some(b), mean, rstd});
+    Tensor through = at::empty_strided_symint(x.sym_sizes(), {0, 0}, x.options());
+    ctx->save_for_backward({x, some(w), some(b), mean, rstd, through});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["act"] = act;
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({mean, rstd});
-    return {y, mean, rstd};
+    return {y, mean, rstd, through};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(5);
-    if (!grads[0].defined()) return out;
-    auto s = ctx->get_saved_variables();
     const bool want_x = ctx->needs_input_grad(0);
+    if (!grads[0].defined()) {
+      if (want_x) out[0] = grads[3];
+      return out;
+    }
+    auto s = ctx->get_saved_variables();
     const bool want_w = s[1].defined() && ctx->needs_input_grad(1);
     const bool want_b = s[2].defined() && ctx->needs_input_grad(s[1].defined() ? 2 : 1);    // counts the tensors there are
-    auto [dx, dw, db] = layer_norm_backward_op().call(grads[0], s[0], opt(s[1]), opt(s[2]), s[3], s[4],
-                                                      ctx->saved_data["eps"].toDouble(), ctx->saved_data["act"].toInt(),
-                                                      want_x, want_w, want_b);
+    auto [dx, dw, db] = layer_norm_backward_op().call(
+        grads[0], s[0], opt(s[1]), opt(s[2]), s[3], s[4], ctx->saved_data["eps"].toDouble(), ctx->saved_data["act"].toInt(),
+        want_x, want_w, want_b, want_x ? opt(grads[3]) : std::nullopt,
+        want_x && at::GradMode::is_enabled() ? opt(s[5]) : std::nullopt);
     if (want_x) out[0] = dx;
     if (want_w) out[1] = dw;
     if (want_b) out[2] = db;
@@ -587,7 +613,8 @@ TORCH_LIBRARY_FRAGMENT(fsctep, m) {
   m.def("layer_norm(Tensor x, Tensor? weight, Tensor? bias, float eps, int activation, bool keep)"
         " -> (Tensor y, Tensor mean, Tensor rstd)");
   m.def("layer_norm_backward(Tensor dy, Tensor x, Tensor? weight, Tensor? bias, Tensor mean, Tensor rstd, float eps,"
-        " int activation, bool want_x, bool want_weight, bool want_bias) -> (Tensor dx, Tensor dweight, Tensor dbias)");
+        " int activation, bool want_x, bool want_weight, bool want_bias, Tensor? plus=None, Tensor? through=None)"
+        " -> (Tensor dx, Tensor dweight, Tensor dbias)");
   m.def("layer_norm_backward_twice(Tensor? v, Tensor? v_weight, Tensor? v_bias, Tensor dy, Tensor x, Tensor? weight,"
         " Tensor? bias, Tensor mean, Tensor rstd, float eps, int activation, bool want_x, bool want_dy, bool want_weight,"
         " bool want_bias) -> (Tensor grad_x, Tensor grad_dy, Tensor grad_weight, Tensor grad_bias)");

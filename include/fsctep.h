@@ -603,7 +603,8 @@ int fsc_expert_mlp_q8(const FscExpertDims* dims, int64_t x_stride, const int8_t*
  * MainNet (models/mlp.py:8-66) in the training step.  dtype of x, y, dy, dx, v, grad_x, grad_dy: FSC_F32 or FSC_BF16;
  * weight, bias and what belongs to them FSC_F32 or the rows' type (weight null: 1, bias null: 0).  Outputs are contiguous.
  * mean [rows] (64 bits) and rstd [rows] are kept for the gradients (both null: not kept).
- * Backward: dx (null: not wanted), dweight and dbias (each null: not wanted; either needs the workspace).
+ * Backward: dx (null: not wanted) with plus [rows][width] added (null: nothing; another share of x's gradient), dweight and
+ * dbias (each null: not wanted; either needs the workspace).
  * Backward of the backward: from cotangents v of dx, v_weight of dweight, v_bias of dbias (each null: 0) the gradients of
  * x, dy, weight and bias (each null: not wanted).  Sums over rows are in a fixed order. */
 #define FSC_ACT_NONE 0
@@ -613,9 +614,9 @@ int fsc_layer_norm_forward(int64_t rows, int32_t width, int32_t dtype, int32_t w
                            double* mean, float* rstd, hipStream_t stream);
 int fsc_layer_norm_workspace(int64_t rows, int32_t width, int64_t* floats);
 int fsc_layer_norm_backward(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
-                            int64_t x_stride, int64_t dy_stride, const void* x, const void* weight, const void* bias,
-                            float eps, const double* mean, const float* rstd, const void* dy, void* dx, void* dweight,
-                            void* dbias, float* workspace, hipStream_t stream);
+                            int64_t x_stride, int64_t dy_stride, int64_t plus_stride, const void* x, const void* weight,
+                            const void* bias, float eps, const double* mean, const float* rstd, const void* dy,
+                            const void* plus, void* dx, void* dweight, void* dbias, float* workspace, hipStream_t stream);
 int fsc_layer_norm_backward_twice(int64_t rows, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t activation,
                                   int64_t x_stride, int64_t dy_stride, int64_t v_stride, const void* x,
                                   const void* weight, const void* bias, float eps, const double* mean,

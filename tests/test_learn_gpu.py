@@ -170,6 +170,53 @@ def test_silu_at_large_arguments():
     close(got["y"], want["y"], O.norm_sizes(eps=EPS, silu=True, **a)["y"], 100, "y")
 
 
+@pytest.mark.parametrize("rows,width", [(40, 20), (33, 128), (9, 331), (300, 640), (7, 1600), (3, 3000)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_both_gradients_of_a_force_loss(rows, width, dtype):
+    """A loss of the rows' output and of their gradient: what reaches x by the two ways is the sum of the two, and either way
+    alone is there without the other; weight and bias that need no gradient change nothing."""
+    a = norm_inputs(rows, width, dtype, dtype)
+    g = gen(rows)
+    ey = randn(g, rows, width, dtype=dtype)
+
+    def grads(ends, needs):
+        x, dy = a["x"].detach().requires_grad_(True), a["dy"].detach().requires_grad_(True)
+        w, b = (a[k].detach().requires_grad_(needs) for k in ("w", "b"))
+        y = L.layer_norm(x, w, b, EPS, "silu")
+        dx, = torch.autograd.grad(y, x, dy, create_graph=True)
+        pick = {"dx": (dx, a["v"]), "y": (y, ey)}
+        outs = [pick[e] for e in ends]
+        ins = [x, w, b] if needs else [x]
+        return torch.autograd.grad([o for o, _ in outs], ins, [c for _, c in outs])
+
+    one, two, both = grads(["dx"], True), grads(["y"], True), grads(["dx", "y"], True)
+    size = O.norm_sizes(a["x"], a["w"], a["b"], EPS, True, a["dy"], a["v"])
+    other = O.norm_sizes(a["x"], a["w"], a["b"], EPS, True, ey, a["v"])
+    for k, (p, q, s) in enumerate(zip(one, two, both)):
+        # each part and their sum are rounded to the type, x's sum once: half a step of each of the three
+        step = 2.0 ** -8 if dtype == BF16 else U
+        terms = (p.double().abs() + q.double().abs() + s.double().abs()) * step
+        name = ("gx", "gw", "gb")[k], ("dx", "dw", "db")[k]
+        assert ((p.double() + q.double() - s.double()).abs() <= terms + 4 * U * (size[name[0]] + other[name[1]])).all(), name
+    for ends in (["dx"], ["y"], ["dx", "y"]):
+        assert torch.equal(grads(ends, False)[0], grads(ends, True)[0])
+
+
+def test_gradients_of_weight_and_bias_alone():
+    """Rows that need no gradient."""
+    a = norm_inputs(50, 200, F32, F32)
+    w, b, dy = (a[k].detach().requires_grad_(True) for k in ("w", "b", "dy"))
+    y = L.layer_norm(a["x"], w, b, EPS, "silu")
+    dw, db = torch.autograd.grad(y, (w, b), dy, create_graph=True)
+    got = torch.autograd.grad((dw, db, y), (w, b, dy), (a["vw"], a["vb"], a["v"]), allow_unused=True)
+    w6, b6, dy6 = (a[k].detach().double().requires_grad_(True) for k in ("w", "b", "dy"))
+    y6 = O.layer_norm(a["x"].double(), w6, b6, EPS, True)
+    dw6, db6 = torch.autograd.grad(y6, (w6, b6), dy6, create_graph=True)
+    want = torch.autograd.grad((dw6, db6, y6), (w6, b6, dy6), (a["vw"].double(), a["vb"].double(), a["v"].double()))
+    for p, q in zip(got, want):
+        assert float((p.double() - q).abs().max()) <= 200 * U * max(1.0, float(q.abs().max()))
+
+
 def test_no_rows():
     x, w, b = torch.zeros(0, 70, device=DEV), torch.ones(70, device=DEV), torch.zeros(70, device=DEV)
     got = norm_call(x, w, b, True, x, x, w, b)
