@@ -357,7 +357,8 @@ __global__ __launch_bounds__(NT) void values_kernel(int64_t n, const uint8_t* __
 
 inline int64_t blocks_of(int64_t n, int share) { return (n + share - 1) / share; }
 
-// Calls f(table, its blocks, its first tensor) for runs of at most MOST tensors whose blocks a grid can have.
+// Calls f(table, its blocks, its first tensor) for runs of at most MOST tensors whose blocks a grid can have (check_tensors: each
+// tensor's by itself fits one).
 template <typename F>
 int by_tables(int32_t count, const FscAdamTensor* t, int share, F&& f) {
   constexpr int64_t GRID = 1ll << 23;          // blocks of 256 threads: fewer than 2^32 threads
@@ -368,7 +369,6 @@ int by_tables(int32_t count, const FscAdamTensor* t, int share, F&& f) {
     for (; i < count && tab.count < MOST; ++i) {
       const FscAdamTensor& s = t[i];
       const int64_t b = blocks_of(s.n, share);
-      FSC_CHECK_ARG(b <= GRID, "adamw: a tensor has more than 2^34 values");
       if (blocks + b > GRID) break;
       const int k = tab.count++;
       tab.first[k] = (int32_t)blocks;
@@ -386,6 +386,7 @@ int check_tensors(int32_t count, const FscAdamTensor* t, const char* what) {
   FSC_CHECK_ARG(count >= 0 && (count == 0 || t), std::string(what) + ": no tensors");
   for (int32_t i = 0; i < count; ++i) {
     FSC_CHECK_ARG(t[i].n >= 0 && (t[i].n == 0 || t[i].g), std::string(what) + ": a gradient is null");
+    FSC_CHECK_ARG(t[i].n <= (int64_t)SHARE << 23, std::string(what) + ": a tensor has more than 2^34 values");
     FSC_CHECK_ARG(t[i].dtype == FSC_F32 || t[i].dtype == FSC_BF16, std::string(what) + ": tensors are float32 or bfloat16");
   }
   return 0;

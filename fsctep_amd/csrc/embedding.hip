@@ -669,6 +669,7 @@ int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int3
   if (table_rows == 0) return 0;
   FSC_CHECK_ARG(dtable && (rows == 0 || (dy && index)), "embedding_backward: null array");
   FSC_CHECK_ARG(dy_stride >= 0, "embedding_backward: negative row stride");
+  FSC_CHECK_ARG(rows * (int64_t)width <= 1ll << 41, "embedding_backward: dy has more than 2^41 values");   // grids of 32 bits
   const Args a{rows, dy_stride, table_rows, width, scale, dy, index, dtable};
   FSC_CHECK_ARG(rows <= FEW || workspace, "embedding_backward: null workspace");
   FSC_EMBED_TYPES((launch_backward<T, I>(a, (char*)workspace, stream)));

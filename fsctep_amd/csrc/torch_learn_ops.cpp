@@ -496,7 +496,8 @@ void adamw_check(at::TensorList params, at::TensorList grads, at::TensorList m, 
   }
   bool half = false;
   for (const Tensor& p : params) half |= p.scalar_type() == at::kBFloat16;
-  TORCH_CHECK(!half || masters.size() == params.size(), op, ": bfloat16 parameters need their float32 copies (masters)");
+  TORCH_CHECK(masters.size() == params.size() || (masters.empty() && !half), op,
+              ": bfloat16 parameters need their float32 copies (masters), as many as parameters");
   for (size_t i = 0; i < params.size() && half; ++i)
     TORCH_CHECK(params[i].scalar_type() == at::kFloat ||
                     (masters[i].scalar_type() == at::kFloat && masters[i].sizes() == params[i].sizes() &&

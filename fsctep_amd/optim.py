@@ -112,9 +112,14 @@ class AdamW(torch.optim.Optimizer):
         self.max_norm, self.state_bits, self.grad_norm = max_norm, int(state_bits), None
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay))
 
+    def __getstate__(self):
+        return super().__getstate__() | {"max_norm": self.max_norm, "state_bits": self.state_bits, "grad_norm": None}
+
     def _state(self, p):
         s = self.state[p]
         if not s:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("AdamW: take a step before one is captured (a replay would start the states anew)")
             s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
             if self.state_bits == 32:
                 for name in ("exp_avg", "exp_avg_sq"):
@@ -157,6 +162,8 @@ class AdamW(torch.optim.Optimizer):
         for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
             number.update(zip(mine["params"], theirs["params"]))
         for p, s in self.state.items():
+            if p not in number:
+                continue
             for name, value in held[number[p]].items():
                 if name == "step":
                     s[name] = torch.as_tensor(value, dtype=torch.float32).to(p.device).reshape(()).clone()
@@ -175,6 +182,8 @@ def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy
     ``ictd.energy_forces`` are the same evaluation without the step): energies (G,) of the structures and forces F = -dE/dpos
     (N, 3), loss = energy_weight mean (E - energy)^2 + force_weight mean (F - forces)^2 (training/trainer.py:1292-1297),
     its gradients, and the optimiser's step.  Returns (loss, E, F), detached; nothing waits for the GPU."""
+    if not model.training:
+        raise ValueError("train_step: the model is not in train() mode")
     optimizer.zero_grad(set_to_none=True)
     pos = pos.detach().requires_grad_(True)
     if external_tensor is None:
@@ -188,7 +197,7 @@ def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy
     loss = (energy_weight * (total - energy).square().mean()
             + force_weight * (gradient + forces).square().mean())
     # of the parameters alone: the positions are not trained
-    params = [p for group in optimizer.param_groups for p in group["params"]]
+    params = [p for group in optimizer.param_groups for p in group["params"] if p.requires_grad]
     for p, g in zip(params, torch.autograd.grad(loss, params, allow_unused=True)):
         p.grad = g
     optimizer.step()

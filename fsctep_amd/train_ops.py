@@ -257,7 +257,8 @@ def readout_energy(net, weighted_sum, x):
     from .sparse import MainNet
     norms = [net.input_norm, *net.layer_norms] if type(net) is MainNet else []
     if (not norms or not all(_plain_norm(ln) for ln in norms) or net._forward_hooks or net._forward_pre_hooks
-            or net._backward_hooks or net._backward_pre_hooks or torch.is_autocast_enabled()):
+            or net._backward_hooks or net._backward_pre_hooks or nn.modules.module._has_any_global_hook()
+            or torch.is_autocast_enabled()):
         return weighted_sum(net(x))
     y = _norm(net.input_norm, x)
     for lin, ln in zip(net.layers, net.layer_norms):

@@ -650,6 +650,51 @@ def test_autograd_sees_the_step():
         y.backward()
 
 
+def test_a_first_step_is_not_captured():
+    """A replay would make the states anew each time."""
+    p = torch.nn.Parameter(torch.randn(50, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt = optim.AdamW([p])
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="take a step before"):
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=DEV)
+            opt.step()
+    opt.step()
+    assert float(opt.state[p]["step"]) == 1
+
+
+def test_tensors_past_32_bits():
+    """More than 2^31 values in one tensor of a step, and in the rows of a norm."""
+    n = 2 ** 31 + 300
+    p, g, m, v = (torch.full((n,), c, device=DEV) for c in (1.0, 0.5, 0.0, 0.0))
+    step = torch.zeros((), device=DEV)
+    norm = optim.adamw_step([p], [g], [m], [v], [step], lr=0.25, weight_decay=0.0, max_norm=1e9)
+    assert abs(float(norm) - 0.5 * math.sqrt(n)) <= 2 * U * 0.5 * math.sqrt(n)
+    # the first step's size is lr g / (|g| + eps)
+    for t, c in ((p, 0.75), (m, 0.05), (v, 0.25e-3)):
+        lo, hi = t.aminmax()
+        assert abs(float(lo) - c) <= 16 * U * c and float(lo) == float(hi)
+    del p, g, m, v
+    rows, width = 2 ** 21 + 5, 1040
+    x = torch.zeros(rows, width, dtype=BF16, device=DEV)
+    x[:] = randn(gen(14), 1, width, dtype=BF16)
+    x[-1] = randn(gen(15), width, dtype=BF16)
+    w = torch.ones(width, dtype=BF16, device=DEV)
+    y, mean, rstd = torch.ops.fsctep.layer_norm(x, w, None, EPS, 0, True)
+    small = x[-3:].contiguous()
+    y3, mean3, rstd3 = torch.ops.fsctep.layer_norm(small, w, None, EPS, 0, True)
+    assert torch.equal(y[-3:], y3) and torch.equal(mean[-3:], mean3) and torch.equal(y[0], y[rows // 2])
+    dx, _, _ = torch.ops.fsctep.layer_norm_backward(x, x, w, None, mean, rstd, EPS, 0, True, False, False)
+    d3, _, _ = torch.ops.fsctep.layer_norm_backward(small, small, w, None, mean3, rstd3, EPS, 0, True, False, False)
+    assert torch.equal(dx[-3:], d3)
+    del y
+    gx, gdy, _, _ = torch.ops.fsctep.layer_norm_backward_twice(x, None, None, x, x, w, None, mean, rstd, EPS, 0, True, True, False, False)
+    g3, h3, _, _ = torch.ops.fsctep.layer_norm_backward_twice(small, None, None, small, small, w, None, mean3, rstd3, EPS, 0, True,
+                                                              True, False, False)
+    assert torch.equal(gx[-3:], g3) and torch.equal(gdy[-3:], h3)
+
+
 # ------------------------------------------------------------------ streams and graphs
 def test_another_stream():
     a = norm_inputs(300, 640, F32, F32)

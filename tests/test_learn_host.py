@@ -104,7 +104,7 @@ def step_args(n=300, dtype=torch.float32):
     (dict(steps=[meta(2)]), "step counts"), (dict(steps=[meta((), dtype=torch.int64)]), "step counts"),
     (dict(params=[meta(20, 15).t()], grads=[meta(15, 20)], exp_avgs=[meta(15, 20)], exp_avg_sqs=[meta(15, 20)]), "not contiguous"),
     (dict(lr=torch.zeros((), device="meta", dtype=torch.float64)), "single float32"),
-    (step_args(dtype=torch.bfloat16), "masters"), (step_args(dtype=torch.bfloat16) | dict(masters=[meta(299)]), "master 0")])
+    (dict(masters=[meta(300), meta(300)]), "as many as parameters"), (step_args(dtype=torch.bfloat16), "masters"), (step_args(dtype=torch.bfloat16) | dict(masters=[meta(299)]), "master 0")])
 def test_step_arguments(change, msg):
     # meta tensors have no GPU kernel's refusal of devices before these checks
     a = step_args() | change
@@ -137,6 +137,55 @@ def test_third_derivatives_of_the_norm_are_refused():
     gx, = torch.autograd.grad(dx.sum(), x, create_graph=True)
     with pytest.raises(RuntimeError, match="not implemented|does not require grad"):
         torch.autograd.grad(gx.sum(), x)
+
+
+def test_optimiser_is_copied_with_its_settings():
+    import copy
+    p = torch.zeros(3, requires_grad=True)
+    opt = copy.deepcopy(optim.AdamW([p], lr=0.5, max_norm=2.0, state_bits=8))
+    assert opt.max_norm == 2.0 and opt.state_bits == 8 and opt.param_groups[0]["lr"] == 0.5 and opt.grad_norm is None
+
+
+def test_train_step_wants_a_model_in_training():
+    with pytest.raises(ValueError, match="train"):
+        optim.train_step(torch.nn.Linear(2, 2).eval(), None, None, None, None, None, None, None)
+
+
+class Adam(ctypes.Structure):
+    _fields_ = [("n", ctypes.c_int64), ("dtype", ctypes.c_int32), ("pad", ctypes.c_int32)] + \
+        [(k, ctypes.c_void_p) for k in ("p", "g", "m", "v", "m_scale", "v_scale", "master", "step")]
+
+
+class Settings(ctypes.Structure):
+    _fields_ = [(k, ctypes.c_double) for k in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + \
+        [("lr_tensor", ctypes.c_void_p), ("norm", ctypes.c_void_p), ("bits", ctypes.c_int32), ("pad", ctypes.c_int32)]
+
+
+def test_c_abi_of_the_step_refuses_without_a_gpu():
+    """No pointer here is one: every call has to end in a check."""
+    lib, one = _lib.load(), 1 << 20
+    ok = dict(n=300, dtype=0, p=one, g=one, m=one, v=one, step=one)
+    rule = dict(lr=1e-3, beta1=0.9, beta2=0.99, eps=1e-8, weight_decay=0.0, max_norm=0.0, bits=32)
+    for tensor, settings, msg in (
+            (ok | dict(g=None), rule, b"gradient is null"), (ok | dict(p=None), rule, b"parameter or a state"),
+            (ok | dict(v=None), rule, b"parameter or a state"), (ok | dict(step=None), rule, b"step count"),
+            (ok | dict(dtype=1), rule, b"float32 copy"), (ok | dict(dtype=2), rule, b"float32 or bfloat16"),
+            (ok | dict(n=-1), rule, b"gradient is null"), (ok | dict(n=(1 << 34) + 1), rule, b"2^34"),
+            (ok, rule | dict(bits=16), b"32 or 8 bits"), (ok, rule | dict(bits=8), b"scale is null"),
+            (ok, rule | dict(beta1=1.0), b"betas"), (ok, rule | dict(beta2=float("nan")), b"betas"),
+            (ok, rule | dict(eps=-1.0), b"negative"), (ok, rule | dict(norm=one), b"max_norm")):
+        t, s = Adam(**tensor), Settings(**settings)
+        assert lib.fsc_adamw_step(1, ctypes.byref(t), ctypes.byref(s), ctypes.c_void_p(one), None) == 1
+        assert msg in lib.fsc_last_error(), (msg, lib.fsc_last_error())
+    t, s = Adam(**ok), Settings(**rule)
+    assert lib.fsc_adamw_step(1, ctypes.byref(t), ctypes.byref(s), None, None) == 1
+    assert lib.fsc_adamw_step(1, ctypes.byref(t), None, ctypes.c_void_p(one), None) == 1
+    assert lib.fsc_grad_norm(1, ctypes.byref(t), None, None, None) == 1
+    a, b = ctypes.c_int64(), ctypes.c_int64()
+    assert lib.fsc_adamw_workspace(1, ctypes.byref(t), ctypes.byref(a), ctypes.byref(b)) == 0 and a.value > 0 and b.value == 8
+    assert lib.fsc_embedding_backward((1 << 31) - 1, 1 << 20, 5, 0, 32, 0, ctypes.c_void_p(one), ctypes.c_void_p(one), 1.0,
+                                      ctypes.c_void_p(one), ctypes.c_void_p(one), None) == 1
+    assert b"2^41" in lib.fsc_last_error()
 
 
 def test_c_abi_refuses_without_a_gpu():
