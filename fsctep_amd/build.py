@@ -15,6 +15,7 @@ import glob
 import os
 import subprocess
 import sys
+from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
@@ -25,10 +26,10 @@ CORE_RUN_SRC = os.path.join(ROOT, "tests", "cpp", "core_run.cpp")
 CORE_RUN = os.path.join(ROOT, "tests", "cpp", "core_run")
 
 HIP_FLAGS = [
-    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-shared",
+    "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC",
     # packed fp32 (v_pk_*_f32) code generation disabled for every kernel
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
-    "-Wno-unused-command-line-argument", "-Wl,-soname,libfsctep_hip.so",
+    "-Wno-unused-command-line-argument",
 ]
 
 
@@ -55,7 +56,10 @@ def build(verbose: bool = False) -> str:
     hipcc = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
     inc = ["-I", os.path.join(ROOT, "include"), "-I", CSRC]
     tmp = LIB + ".tmp"
-    hip_cmd = [hipcc, *HIP_FLAGS, *inc, *sources(), "-o", tmp]
+    hip_srcs = sources()
+    hip_objs = [os.path.join(CSRC, os.path.basename(src) + ".o.tmp") for src in hip_srcs]
+    hip_ccs = [[hipcc, *HIP_FLAGS, *inc, "-c", src, "-o", obj] for src, obj in zip(hip_srcs, hip_objs)]
+    hip_link = [hipcc, *HIP_FLAGS, "-shared", "-Wl,-soname,libfsctep_hip.so", *hip_objs, "-o", tmp]
     tinc, tlib = _torch_dirs()
     torch_srcs = ["torch_ops.cpp", "torch_bucket_ops.cpp", "torch_expert_ops.cpp", "torch_learn_ops.cpp"]
     objs = [os.path.join(PKG, src.replace(".cpp", ".o.tmp")) for src in torch_srcs]
@@ -69,14 +73,22 @@ def build(verbose: bool = False) -> str:
                CORE_RUN_SRC, "-o", crun_tmp,
                "-L", tlib, "-Wl,--no-as-needed", "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip",
                f"-Wl,-rpath,{tlib}", "-L", "/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib", "-ldl"]
+    jobs = [*zip(hip_ccs, map(os.path.basename, hip_srcs)), *zip(torch_ccs, torch_srcs), (core_cc, "tests/cpp/core_run")]
     if verbose:
-        print(" ".join(hip_cmd), "\n", "\n ".join(" ".join(c) for c in torch_ccs), "\n", " ".join(core_cc),
-              flush=True)
-    procs = [subprocess.Popen(c, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
-             for c in (hip_cmd, *torch_ccs, core_cc)]
-    notes = [_check(None, procs[0], "libfsctep_hip.so")]
-    notes += [_check(None, pr, src) for pr, src in zip(procs[1:-1], torch_srcs)]
-    notes.append(_check(None, procs[-1], "tests/cpp/core_run"))
+        print("\n".join(" ".join(c) for c in (*(c for c, _ in jobs), hip_link)), flush=True)
+
+    def compile_one(job):
+        proc = subprocess.Popen(job[0], stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True)
+        return _check(None, proc, job[1])
+
+    # the sources with the most kernels first: they take the longest
+    jobs.sort(key=lambda job: -os.path.getsize(next(a for a in job[0] if a.endswith((".hip", ".cpp")))))
+    with ThreadPoolExecutor(min(8, os.cpu_count() or 1)) as pool:
+        notes = list(pool.map(compile_one, jobs))
+    notes.append(_check(None, subprocess.Popen(hip_link, stdout=subprocess.PIPE, stderr=subprocess.PIPE, text=True),
+                        "libfsctep_hip.so"))
+    for obj in hip_objs:
+        os.remove(obj)
     os.replace(crun_tmp, CORE_RUN)
     os.replace(tmp, LIB)
     ttmp = TORCH_LIB + ".tmp"
