@@ -95,9 +95,11 @@ __global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint3
 }
 
 // ---------------------------------------------------------------- gradient, few tokens
-// Up to FEW tokens: a block owns a row of the table and a vector a lane of its columns, its four waves look through a
-// quarter of the tokens each, 64 at a time, and add the rows they find; one launch, no sort.
-constexpr int FEW = 1024;
+// A block owns a row of the table and a vector a lane of its columns, its four waves look through a quarter of the tokens
+// each, 64 at a time, and add the rows they find; one launch, no sort.  Up to 1,024 tokens (64 columns of 5,000 rows: 5.4 us, by
+// the sort 31 us; all of one token 19 and 29 us), 256 where the table is small (192 columns of 9 rows, 1,024 tokens: 5.3 and
+// 7.9 us, all of one 19.3 and 7.6 us).
+inline int64_t few(int64_t table_rows);
 template <typename T, typename I, bool FULL>
 __global__ __launch_bounds__(NT) void few_kernel(Args a) {
   constexpr int N = Vec<T>::N, AHEAD = 4;
@@ -145,7 +147,10 @@ __global__ __launch_bounds__(NT) void few_kernel(Args a) {
 // ---------------------------------------------------------------- gradient, small tables
 // Up to SMALL table rows: no sort.  Every group of lanes adds the rows it streams through, in order and AHEAD on their way, to its
 // own copy of 256 columns of the table in LDS; a block's copies are added to a partial table, and those by small_join_kernel.
-constexpr int SMALL = 32;
+// More rows leave too few copies for the chip (520,000 x 192 by copies and by the sort: 9 rows 81 and 116 us, 24 rows 105 and
+// 111 us, 32 rows 123 and 110 us).
+constexpr int SMALL = 24;
+inline int64_t few(int64_t table_rows) { return table_rows <= SMALL ? 256 : 1024; }
 inline int small_waves(int64_t table_rows) { return table_rows <= 16 ? 4 : 2; }       // at most 64 KB of copies a block
 struct Stream {
   int lanes;                             // of a row's columns: four values each, 256 at most for the group
@@ -219,7 +224,8 @@ __global__ __launch_bounds__(1024) void small_join_kernel(Args a, const float* _
 // The tokens' numbers sorted by token (a stable radix sort, 8 bits a pass, tokens outside the table last), so that
 // sums are over runs of the sorted list.  A pass: counts by digit and block, each digit's counts scanned over the blocks, and
 // the places: a digit's first place (all smaller digits' totals), the blocks before, the waves before, the lanes before.
-// A block takes PER tokens a thread: 16 where that leaves a block for every CU, 4 otherwise.
+// A block takes PER tokens a thread: 16 where that leaves a block for every CU, 4 otherwise (the whole gradient of 64 columns
+// of 100 rows: 100,000 tokens 35 and 26 us, 2,000,000 tokens 160 and 170 us).
 constexpr int DIGITS = 256;
 inline int per_thread(int64_t rows) { return rows >= (int64_t)256 * 16 * NT ? 16 : 4; }
 
@@ -498,7 +504,6 @@ __global__ __launch_bounds__(JT) void join_kernel(Args a, Sums s) {
 }
 
 // Workspace of the gradient: the sorted tokens and their numbers, twice, the counts, and the partial rows.
-constexpr int64_t WAVES = 16384;         // of the sums
 struct Layout {
   int passes, share, lanes, columns;
   int64_t blocks, shares, key[2], pos[2], counts, totals, part, bytes;
@@ -515,9 +520,9 @@ Layout layout_of(int64_t rows, int width, int64_t table_rows, int size) {
   l.passes = 1;
   while (l.passes < 4 && (table_rows >> (8 * l.passes))) ++l.passes;
   l.blocks = (rows + NT * per_thread(rows) - 1) / (NT * per_thread(rows));
-  // enough shares to fill the chip with waves, not so many that a token's partial rows take long to join
-  const int64_t waves = rows * l.columns * l.lanes / 64;
-  l.share = (int)std::min<int64_t>(1024, std::max<int64_t>({32, waves / WAVES, rows / 8192}));
+  // shares of 32 tokens, more where there would be more than 8,192 shares, whose partial rows take long to join (65,536 x 331 in
+  // bf16 by 16, 32, 64 tokens: 58, 54, 57 us)
+  l.share = (int)std::min<int64_t>(1024, std::max<int64_t>(32, rows / 8192));
   l.shares = (rows + l.share - 1) / l.share;
   int64_t at = 0;
   auto take = [&](int64_t n) {
@@ -568,7 +573,7 @@ void launch_lookup(const Args& a, hipStream_t st) {
 template <typename T, typename I>
 void launch_backward(const Args& a, char* ws, hipStream_t st) {
   constexpr int N = Vec<T>::N;
-  if (a.rows <= FEW) {
+  if (a.rows <= few(a.table_rows)) {
     const dim3 grid((unsigned)std::min<int64_t>(a.table_rows, 1 << 16), (a.width + 64 * N - 1) / (64 * N));
     FSC_EMBED_FULL(a.width >= N, (few_kernel<T, I, FULL><<<grid, NT, 0, st>>>(a)));
     return;
@@ -587,8 +592,9 @@ void launch_backward(const Args& a, char* ws, hipStream_t st) {
     key[i] = (int32_t*)(ws + l.key[i]);
     pos[i] = (int32_t*)(ws + l.pos[i]);
   }
-  // few table rows: a block a row joins them, and writes the zeros; many: a block a share, zeros written first
-  const bool by_token = a.table_rows <= l.shares;
+  // few table rows: a block a row joins them, and writes the zeros; many: a block a share, zeros written first (65,536 x 331 in
+  // bf16, 2,048 shares: 100 rows 36 and 37 us, 1,000 rows 54 and 51 us, 30,000 rows 188 and 65 us)
+  const bool by_token = a.table_rows <= l.shares / 4;
   Source<I> src{(const I*)a.index, nullptr, nullptr, a.rows, a.table_rows};
   for (int p = 0; p < l.passes; ++p) {
     const int64_t values = p == 0 && !by_token ? a.table_rows * a.width : 0;
@@ -653,7 +659,7 @@ int fsc_embedding_workspace(int64_t rows, int32_t width, int64_t table_rows, int
   FSC_CHECK_ARG(bytes != nullptr, "embedding: null output");
   if (int rc = fsc::embed::check_sizes(rows, width, table_rows, FSC_F32, 32)) return rc;
   // the layout depends on the type: room for either
-  if (rows <= fsc::embed::FEW || table_rows == 0) *bytes = 0;
+  if (rows <= fsc::embed::few(table_rows) || table_rows == 0) *bytes = 0;
   else if (table_rows <= fsc::embed::SMALL) *bytes = fsc::embed::small_layout(rows, width, table_rows).bytes;
   else *bytes = std::max(fsc::embed::layout_of(rows, width, table_rows, 4).bytes,
                           fsc::embed::layout_of(rows, width, table_rows, 2).bytes);
@@ -671,7 +677,7 @@ int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int3
   FSC_CHECK_ARG(dy_stride >= 0, "embedding_backward: negative row stride");
   FSC_CHECK_ARG(rows * (int64_t)width <= 1ll << 41, "embedding_backward: dy has more than 2^41 values");   // grids of 32 bits
   const Args a{rows, dy_stride, table_rows, width, scale, dy, index, dtable};
-  FSC_CHECK_ARG(rows <= FEW || workspace, "embedding_backward: null workspace");
+  FSC_CHECK_ARG(rows <= few(table_rows) || workspace, "embedding_backward: null workspace");
   FSC_EMBED_TYPES((launch_backward<T, I>(a, (char*)workspace, stream)));
   return check_launch("embedding_backward") ? 2 : 0;
 }

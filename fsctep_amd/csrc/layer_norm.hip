@@ -462,12 +462,39 @@ __device__ __forceinline__ F normalised(const Args& a, const Row<T, L, CH>& at, 
 }
 
 // Adds a lane's sums of the weight's and the bias' gradients over the wave's rows and the block's waves: a partial row
-// for the block, or the gradients themselves where there is one block.
+// for the block, or the gradients themselves where there is one block.  buf: [2][width] unless a row takes the block's lanes, where
+// every column is one thread's own.
 template <typename T, typename W, int L, int CH, int V>
 __device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at, float (&gw)[CH][V], float (&gb)[CH][V],
                                          float* buf) {
-  const int wave = threadIdx.x >> 6;
-  if constexpr (L < 64)
+  float* part = a.part + (int64_t)blockIdx.x * 2 * a.width;
+  auto put = [&](int i, float w, float b) {
+    if (gridDim.x > 1) {
+      part[i] = w;
+      part[a.width + i] = b;
+    } else {
+      if (a.dw) ((W*)a.dw)[i] = from_f<W>(w);
+      if (a.db) ((W*)a.db)[i] = from_f<W>(b);
+    }
+  };
+  if constexpr (L == NT) {
+#pragma unroll
+    for (int c = 0; c < CH; ++c) {
+      const int i = at.base(c), skip = at.skip(c);
+      if (skip == 0 && gridDim.x > 1) {
+#pragma unroll
+        for (int h = 0; h < V; h += 4) {
+          *reinterpret_cast<Vec<float>*>(part + i + h) = Vec<float>{gw[c][h], gw[c][h + 1], gw[c][h + 2], gw[c][h + 3]};
+          *reinterpret_cast<Vec<float>*>(part + a.width + i + h) = Vec<float>{gb[c][h], gb[c][h + 1], gb[c][h + 2], gb[c][h + 3]};
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+          if (j >= skip) put(i + j, gw[c][j], gb[c][j]);
+      }
+    }
+  } else {
+    const int wave = threadIdx.x >> 6;
 #pragma unroll
     for (int off = L; off < 64; off <<= 1)
 #pragma unroll
@@ -477,38 +504,30 @@ __device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at,
           gw[c][j] += __shfl_xor(gw[c][j], off, 64);
           gb[c][j] += __shfl_xor(gb[c][j], off, 64);
         }
-  // a row of the block's lanes: every column is one thread's own
 #pragma unroll 1
-  for (int k = 0; k < (L == NT ? 1 : NW); ++k) {
-    if (L == NT || (wave == k && (threadIdx.x & 63) < L)) {
+    for (int k = 0; k < NW; ++k) {
+      if (wave == k && (threadIdx.x & 63) < L) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c)
+        for (int c = 0; c < CH; ++c)
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-          if (j >= at.skip(c)) {
-            const int i = at.base(c) + j;
-            buf[i] = k ? buf[i] + gw[c][j] : gw[c][j];
-            buf[a.width + i] = k ? buf[a.width + i] + gb[c][j] : gb[c][j];
-          }
+          for (int j = 0; j < V; ++j)
+            if (j >= at.skip(c)) {
+              const int i = at.base(c) + j;
+              buf[i] = k ? buf[i] + gw[c][j] : gw[c][j];
+              buf[a.width + i] = k ? buf[a.width + i] + gb[c][j] : gb[c][j];
+            }
+      }
+      __syncthreads();
     }
-    __syncthreads();
+    for (int i = threadIdx.x; i < a.width; i += NT) put(i, buf[i], buf[a.width + i]);
   }
-  if (gridDim.x == 1) {
-    for (int i = threadIdx.x; i < a.width; i += NT) {
-      if (a.dw) ((W*)a.dw)[i] = from_f<W>(buf[i]);
-      if (a.db) ((W*)a.db)[i] = from_f<W>(buf[a.width + i]);
-    }
-    return;
-  }
-  float* part = a.part + (int64_t)blockIdx.x * 2 * a.width;
-  for (int i = threadIdx.x; i < 2 * a.width; i += NT) part[i] = buf[i];
 }
 
 template <typename T, typename W, bool SILU, typename F, int L, int CH>
 __global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
   using R = Row<T, L, CH>;
   constexpr int V = R::V, ROWS = NT / L;
-  __shared__ float buf[2 * L * CH * V];
+  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
   __shared__ F red[L == NT ? 2 * 5 * NW : 1];
   RowAdd<L, F> row_add(red);
   const R at(a.width);
@@ -567,7 +586,7 @@ template <typename T, typename W, bool SILU, typename F, int L, int CH>
 __global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
   using R = Row<T, L, CH>;
   constexpr int V = R::V, ROWS = NT / L;
-  __shared__ float buf[2 * L * CH * V];
+  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
   __shared__ F red[L == NT ? 2 * 5 * NW : 1];
   RowAdd<L, F> row_add(red);
   const R at(a.width);
@@ -697,15 +716,18 @@ bool by_shape(int width, F&& f) {
   FSC_LN_SHAPE(64, 3)
   FSC_LN_SHAPE(256, 1)
   FSC_LN_SHAPE(256, 2)
+  FSC_LN_SHAPE(256, 4)
 #undef FSC_LN_SHAPE
   return false;
 }
 
-// Blocks of the two backward passes on rows of L lanes: four rows in turn at least, so that few rows take one block, which needs
-// no partial rows (32 x 128, both passes: 2 launches in place of 4); at most 1,024.
+// Blocks of the two backward passes on rows of L lanes.  Two rounds of rows are left to one block, which needs no partial rows
+// (32 x 128: 7.5 us, by two blocks 8.9 us; 64 x 128: 9.6 us by one, 9.0 us by four).  At most 512, 1,024 where a row takes a
+// block (100,000 x 640 in bf16 by 512 and 1,024: 80 and 90 us; 10,000 x 1,600: 47 and 44 us).
 inline int back_blocks(int64_t rows, int L) {
   const int64_t at_once = NT / L;
-  return (int)std::max<int64_t>(1, std::min<int64_t>(rows <= 4 * at_once ? 1 : (rows + at_once - 1) / at_once, 1024));
+  if (rows <= 2 * at_once) return 1;
+  return (int)std::min<int64_t>((rows + at_once - 1) / at_once, L == NT ? 1024 : 512);
 }
 
 template <typename T, typename W, bool SILU>

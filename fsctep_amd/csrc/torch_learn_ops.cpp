@@ -5,8 +5,8 @@
 
 #include <c10/core/DeviceGuard.h>
 
+#include <algorithm>
 #include <cmath>
-#include <unordered_set>
 
 #include "torch_args.h"
 
@@ -507,14 +507,14 @@ void adamw_check(at::TensorList params, at::TensorList grads, at::TensorList m, 
     TORCH_CHECK(!t.defined() || (t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == params[0].device()), op,
                 ": norm and lr are single float32 values on the parameters' device");
   // what is written twice in one step would depend on the order
-  std::unordered_set<const void*> seen;
-  for (const at::TensorList list : {params, m, v, m_scales, v_scales, steps})
-    for (const Tensor& t : list)
-      TORCH_CHECK(t.is_meta() || t.numel() == 0 || seen.insert(t.const_data_ptr()).second, op, ": a tensor is given twice");
-  for (size_t i = 0; i < masters.size(); ++i)
-    TORCH_CHECK(params[i].is_meta() || params[i].scalar_type() == at::kFloat || params[i].numel() == 0 ||
-                    seen.insert(masters[i].const_data_ptr()).second,
-                op, ": a tensor is given twice");
+  std::vector<const void*> seen;
+  seen.reserve(7 * params.size());
+  for (const at::TensorList list : {params, m, v, m_scales, v_scales, steps, half ? masters : at::TensorList()})
+    for (size_t i = 0; i < list.size(); ++i)
+      if (!list[i].is_meta() && list[i].numel() && (list.data() != masters.data() || params[i].scalar_type() == at::kBFloat16))
+        seen.push_back(list[i].const_data_ptr());
+  std::sort(seen.begin(), seen.end());
+  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), op, ": a tensor is given twice");
 }
 
 void adamw_any(at::TensorList params, at::TensorList grads, at::TensorList m, at::TensorList m_scales, at::TensorList v,
