@@ -306,6 +306,10 @@ int32_t check_index(const Tensor& index, const char* op) {
               index.scalar_type());
   return index.scalar_type() == at::kInt ? 32 : 64;
 }
+// the C entry's width has 32 bits
+void check_width(const c10::SymInt& width, const char* op) {
+  TORCH_CHECK(width <= (1 << 20), op, ": the width must be at most 2^20, got ", width);
+}
 void check_scale(double scale, const char* op) {
   TORCH_CHECK(std::isfinite((float)scale), op, ": scale must be finite, got ", scale);
 }
@@ -315,6 +319,7 @@ Tensor embedding(const Tensor& table_, const Tensor& index_, double scale) {
   TORCH_CHECK(table_.dim() == 2, "embedding: table must be (rows, width), got ", table_.dim(), " dimensions");
   const int32_t dt = code_of(table_.scalar_type(), "table"), bits = check_index(index_, "embedding");
   check_scale(scale, "embedding");
+  check_width(table_.sym_size(1), "embedding");
   const c10::OptionalDeviceGuard device(table_.device());
   const Tensor table = rows2d(table_, "table"), index = index_.contiguous();
   Tensor out = at::empty({index.size(0), table.size(1)}, table.options());
@@ -330,6 +335,7 @@ Tensor embedding_meta(const Tensor& table, const Tensor& index, double scale) {
   code_of(table.scalar_type(), "table");
   check_index(index, "embedding");
   check_scale(scale, "embedding");
+  check_width(table.sym_size(1), "embedding");
   return at::empty_symint({index.sym_size(0), table.sym_size(1)}, table.options());
 }
 
@@ -341,6 +347,7 @@ Tensor embedding_backward(const Tensor& dy_, const Tensor& index_, c10::SymInt t
   const int64_t table_rows = table_rows_.expect_int();
   TORCH_CHECK(table_rows >= 0, op, ": negative table rows");
   check_scale(scale, op);
+  check_width(dy_.sym_size(1), op);
   const c10::OptionalDeviceGuard device(dy_.device());
   const Tensor dy = rows2d(dy_, "dy"), index = index_.contiguous();
   Tensor out = at::empty({table_rows, dy.size(1)}, dy.options());
@@ -359,6 +366,7 @@ Tensor embedding_backward_meta(const Tensor& dy, const Tensor& index, c10::SymIn
   code_of(dy.scalar_type(), "dy");
   check_index(index, "embedding_backward");
   check_scale(scale, "embedding_backward");
+  check_width(dy.sym_size(1), "embedding_backward");
   return at::empty_symint({table_rows, dy.sym_size(1)}, dy.options());
 }
 
@@ -506,15 +514,27 @@ void adamw_check(at::TensorList params, at::TensorList grads, at::TensorList m, 
   for (const Tensor& t : {some(norm), some(lr_tensor)})
     TORCH_CHECK(!t.defined() || (t.numel() == 1 && t.scalar_type() == at::kFloat && t.device() == params[0].device()), op,
                 ": norm and lr are single float32 values on the parameters' device");
-  // what is written twice in one step would depend on the order
-  std::vector<const void*> seen;
-  seen.reserve(7 * params.size());
-  for (const at::TensorList list : {params, m, v, m_scales, v_scales, steps, half ? masters : at::TensorList()})
-    for (size_t i = 0; i < list.size(); ++i)
-      if (!list[i].is_meta() && list[i].numel() && (list.data() != masters.data() || params[i].scalar_type() == at::kBFloat16))
-        seen.push_back(list[i].const_data_ptr());
-  std::sort(seen.begin(), seen.end());
-  TORCH_CHECK(std::adjacent_find(seen.begin(), seen.end()) == seen.end(), op, ": a tensor is given twice");
+  // a value that two of them hold would depend on the order in which it is written (and gradients on what was written before)
+  struct Range { const char *from, *to; bool written; };
+  std::vector<Range> ranges;
+  ranges.reserve(8 * params.size());
+  const auto add = [&](const Tensor& x, bool written) {
+    if (x.is_meta() || !x.numel()) return;
+    const char* from = (const char*)x.const_data_ptr();
+    ranges.push_back({from, from + x.nbytes(), written});
+  };
+  for (const at::TensorList list : {params, m, v, m_scales, v_scales, steps})
+    for (const Tensor& x : list) add(x, true);
+  for (size_t i = 0; i < params.size() && half; ++i)
+    if (params[i].scalar_type() == at::kBFloat16) add(masters[i], true);
+  for (const Tensor& x : g) add(x, false);
+  std::sort(ranges.begin(), ranges.end(), [](const Range& a, const Range& b) { return a.from < b.from; });
+  const char *end = nullptr, *written_end = nullptr;     // of the ranges so far
+  for (const Range& r : ranges) {
+    TORCH_CHECK(r.from >= (r.written ? end : written_end), op, ": a tensor is given twice, or two tensors overlap");
+    end = std::max(end, r.to);
+    if (r.written) written_end = std::max(written_end, r.to);
+  }
 }
 
 void adamw_any(at::TensorList params, at::TensorList grads, at::TensorList m, at::TensorList m_scales, at::TensorList v,

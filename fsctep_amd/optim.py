@@ -7,7 +7,7 @@
 
 The formulas are torch.optim.AdamW's (the reference's trainer, training/trainer.py), states of 32 bits have its names,
 so that its checkpoints load.  Parameters are float32, or bfloat16 with a float32 copy ("master") in the state that
-is stepped and rounded.  Step counts live on the GPU and nothing waits for it, so a step can be captured into a graph
+is stepped and rounded (who writes other values into such a parameter writes them into its copy as well).  Step counts live on the GPU and nothing waits for it, so a step can be captured into a graph
 (``lr`` as a float32 tensor then changes between replays).  The ops are registered in C++
 (``csrc/torch_learn_ops.cpp``, kernels ``csrc/adamw.hip``).
 
@@ -154,15 +154,21 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """Also a checkpoint of ``torch.optim.AdamW`` (states in 32 bits).  States keep their own types, which the base
-        class would cast to the parameter's."""
-        super().load_state_dict(state_dict)
+        """Also a checkpoint of ``torch.optim.AdamW`` without its variants (states in 32 bits).  States keep their own types,
+        which the base class would cast to the parameter's."""
         held = state_dict["state"]
+        want = {"exp_avg", "exp_avg_sq"} if self.state_bits == 32 else {"exp_avg", "exp_avg_scale", "root", "root_scale"}
+        if not all(want <= set(s) for s in held.values() if s):
+            raise ValueError(f"the checkpoint's states do not have {self.state_bits} bits")
+        for name in ("amsgrad", "maximize"):
+            if any(g.get(name) for g in state_dict["param_groups"]):
+                raise ValueError(f"the checkpoint is of an optimiser with {name}, which this one does not have")
+        super().load_state_dict(state_dict)
         number = {}
         for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
             number.update(zip(mine["params"], theirs["params"]))
         for p, s in self.state.items():
-            if p not in number:
+            if p not in number or not s:
                 continue
             for name, value in held[number[p]].items():
                 if name == "step":
@@ -171,9 +177,6 @@ class AdamW(torch.optim.Optimizer):
                     s[name] = value.detach().to(p.device).clone(memory_format=torch.contiguous_format)
             if p.dtype == torch.bfloat16 and "master" not in s:
                 s["master"] = p.detach().float()
-            want = {"exp_avg_sq"} if self.state_bits == 32 else {"root", "root_scale", "exp_avg_scale"}
-            if not want <= set(s):
-                raise ValueError(f"the checkpoint's states do not have {self.state_bits} bits")
 
 
 def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy_weight: float = 1.0,
@@ -184,6 +187,12 @@ def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy
     its gradients, and the optimiser's step.  Returns (loss, E, F), detached; nothing waits for the GPU."""
     if not model.training:
         raise ValueError("train_step: the model is not in train() mode")
+    if tuple(energy.shape) != (cell.shape[0],) or forces.shape != pos.shape:
+        raise ValueError(f"train_step: energy must be ({cell.shape[0]},) and forces {tuple(pos.shape)}, "
+                         f"got {tuple(energy.shape)} and {tuple(forces.shape)}")
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        # torch's sums over many blocks clear memory by nodes that a replay does not repeat reliably
+        raise RuntimeError("train_step is not captured into a graph; the optimiser's step by itself can be")
     optimizer.zero_grad(set_to_none=True)
     pos = pos.detach().requires_grad_(True)
     if external_tensor is None:

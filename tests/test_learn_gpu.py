@@ -319,6 +319,16 @@ def test_embedding(rows, width, table, kind, index_type, dtype):
                  randn(g, rows, width, dtype=dtype))
 
 
+@pytest.mark.parametrize("table", [1, 23, 24, 25, 100, 255, 256, 257, 520, 65535, 65536, 65537])
+@pytest.mark.parametrize("rows", [255, 256, 257, 1023, 1024, 1025, 2049, 33000])
+def test_embedding_at_the_rules_borders(rows, table):
+    """Where another kernel takes over: by tokens, table rows, digits of the sort, shares."""
+    g = gen(rows * table)
+    for dtype, width in ((F32, 36), (BF16, 75)):
+        lookup_check(randn(g, table, width, dtype=dtype), tokens(g, rows, table, torch.int32, "tail"), 1.0,
+                     randn(g, rows, width, dtype=dtype))
+
+
 def test_embedding_of_any_shape_and_scale():
     g = gen(1)
     t = randn(g, 20, 24)
@@ -573,6 +583,32 @@ def test_the_same_tensor_twice_is_refused():
                     bad[k][1] = bad[k][0].clone()
         with pytest.raises(RuntimeError, match="twice"):
             optim.adamw_step(**bad)
+
+
+@pytest.mark.parametrize("first,second", [("params", "params"), ("params", "grads"), ("exp_avgs", "exp_avg_sqs"), ("params", "exp_avgs"),
+                                          ("steps", "params")])
+def test_overlapping_tensors_are_refused(first, second):
+    """Two views of one array that share a value; the same views one value further apart are taken."""
+    def step(apart):
+        flat = torch.zeros(1000, device="cuda")
+        a = {k: [torch.zeros(100, device="cuda") for _ in range(2)] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs")}
+        a["steps"] = [torch.zeros((), device="cuda") for _ in range(2)]
+        n = a[first][0].numel()
+        a[first][0] = flat[:n].view(a[first][0].shape)
+        a[second][1] = flat[n - 1 + apart:n - 1 + apart + a[second][1].numel()].view(a[second][1].shape)
+        optim.adamw_step(*(a[k] for k in ("params", "grads", "exp_avgs", "exp_avg_sqs", "steps")))
+
+    step(1)
+    with pytest.raises(RuntimeError, match="overlap"):
+        step(0)
+
+
+def test_parameters_may_share_a_gradient():
+    p = [torch.full((300,), 2.0, device="cuda") for _ in range(2)]
+    g = torch.linspace(-1.0, 1.0, 300, device="cuda")
+    z = lambda: [torch.zeros(300, device="cuda") for _ in range(2)]
+    optim.adamw_step(p, [g, g], z(), z(), [torch.zeros((), device="cuda") for _ in range(2)])
+    assert torch.equal(p[0], p[1]) and not torch.equal(p[0], torch.full_like(p[0], 2.0))
 
 
 def test_nan_gradients_pass_into_the_parameters():

@@ -225,3 +225,56 @@ def test_8_bit_rounding_keeps_the_mean():
             total += O.decode(*O.encode(x, step, root), root)
         spread = x * 2.0 ** -(4 if root else 3) / 2 / np.sqrt(4000)
         assert (np.abs(total / 4000 - x) <= 6 * spread + 1e-7 * x).all()
+
+
+@pytest.mark.parametrize("shape", [(2 ** 20 + 1,), (2 ** 31 + 5,), (2 ** 32 + 8,)])
+def test_lookups_of_wider_rows_are_refused(shape):
+    """Also where the width's lower 32 bits by themselves are a width."""
+    with pytest.raises(RuntimeError, match="at most 2\\^20"):
+        L.embedding(meta(1, *shape), meta(3, dtype=torch.int64))
+    with pytest.raises(RuntimeError, match="at most 2\\^20"):
+        torch.ops.fsctep.embedding_backward(meta(3, *shape), meta(3, dtype=torch.int64), 2, 1.0)
+
+
+def test_step_of_a_trunk_checks_what_it_is_compared_with():
+    """A column of energies would be compared with every structure's, one row of forces with every atom's."""
+    class Trunk(torch.nn.Module):
+        def forward_graph(self, *args, **kwargs):
+            raise AssertionError("run before the check")
+
+    pos, batch, cell, e = torch.zeros(5, 3), torch.zeros(5, dtype=torch.int64), torch.zeros(2, 3, 3), torch.zeros(2)
+    w = torch.zeros(3, requires_grad=True)
+    opt = optim.AdamW([w])
+    for energy, forces in ((e[:, None], pos), (e[:1], pos), (e[0], pos), (e, pos[:1]), (e, pos.t()), (e, pos[0])):
+        with pytest.raises(ValueError, match="energy must be"):
+            optim.train_step(Trunk().train(), opt, pos, batch, cell, None, energy, forces)
+
+
+@pytest.mark.parametrize("variant", ["amsgrad", "maximize"])
+def test_checkpoints_of_other_optimisers_are_refused(variant):
+    p, q = torch.zeros(3, requires_grad=True), torch.zeros(3, requires_grad=True)
+    theirs, mine = torch.optim.AdamW([p], lr=0.5, **{variant: True}), optim.AdamW([q], lr=0.25)
+    p.grad = torch.ones(3)
+    theirs.step()
+    with pytest.raises(ValueError, match=variant):
+        mine.load_state_dict(theirs.state_dict())
+    assert mine.param_groups[0]["lr"] == 0.25 and not mine.state
+
+
+def test_checkpoints_of_other_states_leave_the_optimiser_as_it_was():
+    p, q = torch.zeros(300, requires_grad=True), torch.zeros(300, requires_grad=True)
+    theirs, mine = torch.optim.AdamW([p], lr=0.5), optim.AdamW([q], lr=0.25, state_bits=8)
+    p.grad = torch.ones(300)
+    theirs.step()
+    with pytest.raises(ValueError, match="8 bits"):
+        mine.load_state_dict(theirs.state_dict())
+    assert mine.param_groups[0]["lr"] == 0.25 and not mine.state
+
+
+def test_step_of_a_trunk_is_not_captured(monkeypatch):
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: True)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+    pos, batch, cell = torch.zeros(5, 3), torch.zeros(5, dtype=torch.int64), torch.zeros(2, 3, 3)
+    opt = optim.AdamW([torch.zeros(3, requires_grad=True)])
+    with pytest.raises(RuntimeError, match="captured"):
+        optim.train_step(torch.nn.Linear(2, 2), opt, pos, batch, cell, None, torch.zeros(2), pos)
