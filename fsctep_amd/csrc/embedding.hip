@@ -227,11 +227,14 @@ __global__ __launch_bounds__(1024) void small_join_kernel(Args a, const float* _
 
 // ---------------------------------------------------------------- gradient, many tokens: sort
 // The tokens' numbers sorted by token (a stable radix sort, 8 bits a pass, tokens outside the table last), so that
-// sums are over runs of the sorted list.  A pass has counts by digit and block, each digit's counts scanned over the blocks, and
+// sums are over runs of the sorted list.  A pass has counts by digit and block, each digit's counts added up over the blocks, and
 // the places: a digit's first place (all smaller digits' totals), the blocks before, the waves before, the lanes before.  Bound
-// by its three launches (65,536 tokens: 15 us a pass).  A block takes PER tokens a thread: 16 where that leaves a block for every CU,
+// by its launches (65,536 tokens: 15 us a pass).  A block takes PER tokens a thread: 16 where that leaves a block for every CU,
 // 4 otherwise (the whole gradient of 64 columns of 100 rows: 100,000 tokens 35 and 26 us, 2,000,000 tokens 160 and 170 us).
-constexpr int DIGITS = 256;
+// Up to FEW_BLOCKS blocks each block of the places adds the counts itself, one launch less (BY_DIGIT false: counts [block][digit];
+// by themselves and by a scan: 2,000 tokens of 5,000 rows x 331 30.6 and 34.5 us, 32,768 of 5,000 x 64 34.3 and 37.0 us, 65,536 of
+// 30,011 x 331 in bf16 53.1 and 53.4 us); more are scanned (counts [digit][block]; 130,000 of 5,000 x 64 52.1 and 49.7 us).
+constexpr int DIGITS = 256, FEW_BLOCKS = 64;
 inline int per_thread(int64_t rows) { return rows >= (int64_t)256 * 16 * NT ? 16 : 4; }
 
 // key of token i for the sort, from the index (first pass) or the pass before
@@ -249,7 +252,7 @@ struct Source {
 };
 
 // Blocks from `blocks` on fill the table's gradient with zeros (rows that no token names).
-template <int PER, typename I, typename T>
+template <int PER, bool BY_DIGIT, typename I, typename T>
 __global__ __launch_bounds__(NT) void count_kernel(Source<I> src, int shift, int blocks, int32_t* __restrict__ counts,
                                                    T* __restrict__ table, int64_t values) {
   if ((int)blockIdx.x >= blocks) {
@@ -271,7 +274,7 @@ __global__ __launch_bounds__(NT) void count_kernel(Source<I> src, int shift, int
     if (i < src.rows) atomicAdd(&cnt[src.key_of(i) >> shift & (DIGITS - 1)], 1);   // counts: any order
   }
   __syncthreads();
-  counts[(int64_t)threadIdx.x * blocks + blockIdx.x] = cnt[threadIdx.x];
+  counts[BY_DIGIT ? (int64_t)threadIdx.x * blocks + blockIdx.x : (int64_t)blockIdx.x * DIGITS + threadIdx.x] = cnt[threadIdx.x];
 }
 
 __device__ __forceinline__ int wave_scan(int v, int lane) {       // inclusive
@@ -308,7 +311,7 @@ __device__ __forceinline__ uint64_t peers(int digit, bool ok) {
   return m;
 }
 
-template <int PER, typename I>
+template <int PER, bool BY_DIGIT, typename I>
 __global__ __launch_bounds__(NT) void place_kernel(Source<I> src, int shift, int blocks, const int32_t* __restrict__ counts,
                                                    const int32_t* __restrict__ totals, int32_t* __restrict__ key,
                                                    int32_t* __restrict__ pos) {
@@ -317,11 +320,28 @@ __global__ __launch_bounds__(NT) void place_kernel(Source<I> src, int shift, int
 #pragma unroll
   for (int w = 0; w < NT / 64; ++w) cnt[w][d] = 0;
   // the digit's first place
-  const int total = totals[d];
+  int total = 0, blocks_before = 0;
+  if (BY_DIGIT) {
+    total = totals[d];
+    blocks_before = counts[(int64_t)d * blocks + blockIdx.x];
+  } else {
+#pragma unroll
+    for (int b0 = 0; b0 < FEW_BLOCKS; b0 += 16) {
+      if (b0 >= blocks) break;
+      int v[16];
+#pragma unroll
+      for (int b = 0; b < 16; ++b) v[b] = counts[std::min(b0 + b, blocks - 1) * DIGITS + d];
+#pragma unroll
+      for (int b = 0; b < 16; ++b) {
+        total += b0 + b < blocks ? v[b] : 0;
+        blocks_before += b0 + b < (int)blockIdx.x ? v[b] : 0;
+      }
+    }
+  }
   const int run = wave_scan(total, lane);
   if (lane == 63) sums[wave] = run;
   __syncthreads();
-  int base = run - total + counts[(int64_t)d * blocks + blockIdx.x];
+  int base = run - total + blocks_before;
   for (int w = 0; w < wave; ++w) base += sums[w];
   const int64_t w0 = ((int64_t)blockIdx.x * NT + wave * 64) * PER;
   int32_t k[PER];
@@ -605,14 +625,18 @@ void launch_backward(const Args& a, char* ws, hipStream_t st) {
   for (int p = 0; p < l.passes; ++p) {
     const int64_t values = p == 0 && !by_token ? a.table_rows * a.width : 0;
     const unsigned fill = (unsigned)std::min<int64_t>((values + NT * N - 1) / (NT * N), 2048);
-    auto sort = [&](auto per) {
+    auto sort = [&](auto per, auto by_digit) {
       constexpr int PER = decltype(per)::value;
-      count_kernel<PER, I, T><<<(unsigned)l.blocks + fill, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, (T*)a.out, values);
-      scan_kernel<<<DIGITS, 64, 0, st>>>((int)l.blocks, counts, totals);
-      place_kernel<PER, I><<<(unsigned)l.blocks, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, totals, key[p & 1], pos[p & 1]);
+      constexpr bool BY_DIGIT = decltype(by_digit)::value;
+      count_kernel<PER, BY_DIGIT, I, T><<<(unsigned)l.blocks + fill, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, (T*)a.out,
+                                                                                  values);
+      if (BY_DIGIT) scan_kernel<<<DIGITS, 64, 0, st>>>((int)l.blocks, counts, totals);
+      place_kernel<PER, BY_DIGIT, I><<<(unsigned)l.blocks, NT, 0, st>>>(src, 8 * p, (int)l.blocks, counts, totals, key[p & 1],
+                                                                        pos[p & 1]);
     };
-    if (per_thread(a.rows) == 16) sort(std::integral_constant<int, 16>{});
-    else sort(std::integral_constant<int, 4>{});
+    if (l.blocks <= FEW_BLOCKS) sort(std::integral_constant<int, 4>{}, std::false_type{});
+    else if (per_thread(a.rows) == 4) sort(std::integral_constant<int, 4>{}, std::true_type{});
+    else sort(std::integral_constant<int, 16>{}, std::true_type{});
     src.key = key[p & 1];
     src.pos = pos[p & 1];
   }

@@ -202,6 +202,41 @@ def test_both_gradients_of_a_force_loss(rows, width, dtype):
         assert torch.equal(grads(ends, False)[0], grads(ends, True)[0])
 
 
+def test_any_part_of_both_gradients():
+    """Every choice of the ends of a force loss and of the leaves asked for, against 64 bits; a weight or bias that needs no
+    gradient, or is not there."""
+    a = norm_inputs(37, 150, F32, F32)
+    g = gen(5)
+    ey, ew = randn(g, 37, 150), randn(g, 150)
+
+    def grads(norm, t, ends, first, ask, frozen):
+        leaf = {k: v.detach().requires_grad_(k not in frozen) for k, v in t.items() if k in ("x", "w", "b", "dy") and "no " + k not in frozen}
+        y = norm(leaf["x"], leaf.get("w"), leaf.get("b"))
+        d = dict(zip(first, torch.autograd.grad(y, [leaf[k] for k in first], leaf["dy"], create_graph=True)))
+        out = {"y": (y, t["ey"])} | {"d" + k: (d[k], t["c" + k]) for k in first}
+        pairs = [out[e] for e in ends if e in out]
+        return torch.autograd.grad([p for p, _ in pairs], [leaf[k] for k in ask], [c for _, c in pairs], allow_unused=True)
+
+    t = {"x": a["x"], "w": a["w"], "b": a["b"], "dy": a["dy"], "ey": ey, "cx": a["v"], "cw": ew, "cb": a["vb"]}
+    wide = {k: v.double() for k, v in t.items()}
+    mine = lambda x, w, b: L.layer_norm(x, w, b, EPS, "silu")  # noqa: E731
+    plain = lambda x, w, b: O.layer_norm(x, w, b, EPS, True)  # noqa: E731
+    for frozen in ((), ("w",), ("b",), ("no w",), ("no b",), ("no w", "no b"), ("x",)):
+        have = [k for k in ("x", "w", "b") if k not in frozen and "no " + k not in frozen]
+        for first in ([k for k in have if k == "x"], have, have[-1:]):
+            for ends in (["y"], ["d" + k for k in first], ["y"] + ["d" + k for k in first]):
+                for ask in (have, have[:1], have[-1:], have + ["dy"]):
+                    if not first:
+                        continue
+                    got, want = grads(mine, t, ends, first, ask, frozen), grads(plain, wide, ends, first, ask, frozen)
+                    for k, p, q in zip(ask, got, want):
+                        what = (frozen, first, ends, ask, k)
+                        p = torch.zeros_like(t[k]) if p is None else p
+                        q = torch.zeros_like(wide[k]) if q is None else q
+                        # terms of order 1, 10 at most after the weights: sums of 150 and 37 of them
+                        assert float((p.double() - q).abs().max()) <= 400 * U * 10 * max(1.0, float(q.abs().max())), what
+
+
 def test_gradients_of_weight_and_bias_alone():
     """Rows that need no gradient."""
     a = norm_inputs(50, 200, F32, F32)
