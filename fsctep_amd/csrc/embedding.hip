@@ -100,18 +100,21 @@ __global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint3
 }
 
 // ---------------------------------------------------------------- gradient, few tokens
-// A block owns a row of the table and a vector a lane of its columns, its four waves look through a quarter of the tokens
-// each, 64 at a time, and add the rows they find; one launch, no sort.  Up to 1,024 tokens (64 columns of 5,000 rows: 5.4 us, by
-// the sort 31 us; all of one token 19 and 29 us), 256 where the table is small (192 columns of 9 rows, 1,024 tokens: 5.3 and
-// 7.9 us, all of one 19.3 and 7.6 us).
-inline int64_t few(int64_t table_rows);
-template <typename T, typename I, bool FULL>
-__global__ __launch_bounds__(NT) void few_kernel(Args a) {
-  constexpr int N = Vec<T>::N, AHEAD = 4;
-  __shared__ float red[NT / 64][64 * N];
+// A block owns a row of the table and a vector a lane of its columns, its waves look through a share of the tokens each, 64 at a
+// time, and add the rows they find, AHEAD on their way; one launch, no sort.  Eight waves a block where the chip holds all blocks at
+// once, four where it does not (1,024 tokens by four and eight: 64 columns of 100 rows, all of one token, 17.7 and 11.0 us; 640
+// columns of 5,000 rows 13.7 and 19.1 us).  For up to 2,048 tokens and 2^23 pairs of token and row to look at (by it and by the
+// sort: 2,048 tokens, 640 columns of 100 rows 5.8 and 21.0 us, all of one token 28.7 and 18.7 us; 1,024 of 5,000 rows 13.7 and 29.4
+// us; 256 of 30,000 rows x 331 24.6 and 33.5 us, 1,024 40.2 and 35.6 us), 512 where the table is small (192 columns of 9 rows, all
+// of one token: 512 tokens 6.3 and 7.6 us, 1,024 tokens 11.1 and 7.9 us).
+inline bool few(int64_t rows, int64_t table_rows);
+template <int WAVES, typename T, typename I, bool FULL>
+__global__ __launch_bounds__(64 * WAVES) void few_kernel(Args a) {
+  constexpr int N = Vec<T>::N, AHEAD = 8;
+  __shared__ float red[WAVES][64 * N];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int n = FULL ? N : a.width, first = (blockIdx.y * 64 + lane) * N, col = std::min(first, a.width - n);
-  const int per = (int)((a.rows + 255) / 256) * 64;
+  const int per = (int)((a.rows + 64 * WAVES - 1) / (64 * WAVES)) * 64;
   const int i0 = std::min<int>(a.rows, wave * per), i1 = std::min<int>(a.rows, i0 + per);
   for (int64_t v = blockIdx.x; v < a.table_rows; v += gridDim.x) {
     float s[N];
@@ -141,8 +144,11 @@ __global__ __launch_bounds__(NT) void few_kernel(Args a) {
     __syncthreads();
     if (wave == 0 && first < a.width) {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        s[j] = a.scale * ((red[0][lane * N + j] + red[1][lane * N + j]) + (red[2][lane * N + j] + red[3][lane * N + j]));
+      for (int j = 0; j < N; ++j) {
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w) s[j] += red[w][lane * N + j];
+        s[j] *= a.scale;
+      }
       store_some<FULL, N>((T*)a.out + v * a.width + col, n, s);
     }
     __syncthreads();
@@ -155,7 +161,9 @@ __global__ __launch_bounds__(NT) void few_kernel(Args a) {
 // More rows leave too few copies for the chip (520,000 x 192 by copies and by the sort: 9 rows 81 and 116 us, 24 rows 105 and
 // 111 us, 32 rows 123 and 110 us).
 constexpr int SMALL = 24;
-inline int64_t few(int64_t table_rows) { return table_rows <= SMALL ? 256 : 1024; }
+inline bool few(int64_t rows, int64_t table_rows) {
+  return table_rows <= SMALL ? rows <= 512 : rows <= 2048 && rows * table_rows <= 1 << 23;
+}
 inline int small_waves(int64_t table_rows) { return table_rows <= 16 ? 4 : 2; }       // at most 64 KB of copies a block
 struct Stream {
   int lanes;                             // of a row's columns: four values each, 256 at most for the group
@@ -599,9 +607,10 @@ void launch_lookup(const Args& a, hipStream_t st) {
 template <typename T, typename I>
 void launch_backward(const Args& a, char* ws, hipStream_t st) {
   constexpr int N = Vec<T>::N;
-  if (a.rows <= few(a.table_rows)) {
+  if (few(a.rows, a.table_rows)) {
     const dim3 grid((unsigned)std::min<int64_t>(a.table_rows, 1 << 16), (a.width + 64 * N - 1) / (64 * N));
-    FSC_EMBED_FULL(a.width >= N, (few_kernel<T, I, FULL><<<grid, NT, 0, st>>>(a)));
+    if ((int64_t)grid.x * grid.y <= 2048) FSC_EMBED_FULL(a.width >= N, (few_kernel<8, T, I, FULL><<<grid, 512, 0, st>>>(a)))
+    else FSC_EMBED_FULL(a.width >= N, (few_kernel<4, T, I, FULL><<<grid, 256, 0, st>>>(a)))
     return;
   }
   if (a.table_rows <= SMALL) {
@@ -689,7 +698,7 @@ int fsc_embedding_workspace(int64_t rows, int32_t width, int64_t table_rows, int
   FSC_CHECK_ARG(bytes != nullptr, "embedding: null output");
   if (int rc = fsc::embed::check_sizes(rows, width, table_rows, FSC_F32, 32)) return rc;
   // the layout depends on the type: room for either
-  if (rows <= fsc::embed::few(table_rows) || table_rows == 0) *bytes = 0;
+  if (fsc::embed::few(rows, table_rows) || table_rows == 0) *bytes = 0;
   else if (table_rows <= fsc::embed::SMALL) *bytes = fsc::embed::small_layout(rows, width, table_rows).bytes;
   else *bytes = std::max(fsc::embed::layout_of(rows, width, table_rows, 4).bytes,
                           fsc::embed::layout_of(rows, width, table_rows, 2).bytes);
@@ -707,7 +716,7 @@ int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int3
   FSC_CHECK_ARG(dy_stride >= 0, "embedding_backward: negative row stride");
   FSC_CHECK_ARG(rows * (int64_t)width <= 1ll << 41, "embedding_backward: dy has more than 2^41 values");   // grids of 32 bits
   const Args a{rows, dy_stride, table_rows, width, scale, dy, index, dtable};
-  FSC_CHECK_ARG(rows <= few(table_rows) || workspace, "embedding_backward: null workspace");
+  FSC_CHECK_ARG(few(rows, table_rows) || workspace, "embedding_backward: null workspace");
   FSC_EMBED_TYPES((launch_backward<T, I>(a, (char*)workspace, stream)));
   return check_launch("embedding_backward") ? 2 : 0;
 }

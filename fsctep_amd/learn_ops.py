@@ -37,5 +37,7 @@ def embedding(table, index, scale: float = 1.0):
     """``scale * table[index]``, (\\*index.shape, width), of a (rows, width) table, float32 or bfloat16, for an index of
     any shape, int32 or int64; zeros, without a gradient, where the index lies outside the table (-1: padding).  The
     table's gradient sums the rows of each token in 32 bits and in a fixed order."""
+    if index.dim() == 1:
+        return torch.ops.fsctep.embedding(table, index, float(scale))
     rows = torch.ops.fsctep.embedding(table, index.reshape(-1), float(scale))
-    return rows.view(*index.shape, rows.shape[1]) if index.dim() != 1 else rows
+    return rows.view(*index.shape, rows.shape[1])

@@ -364,6 +364,17 @@ def test_embedding_at_the_rules_borders(rows, table):
                      randn(g, rows, width, dtype=dtype))
 
 
+@pytest.mark.parametrize("kind", ["tail", "one", "outside"])
+@pytest.mark.parametrize("rows,table", [(512, 9), (513, 9), (512, 24), (513, 24), (2048, 25), (2049, 25), (511, 2048), (65, 2049), (2048, 4096),
+                                        (2048, 4097), (1024, 8193), (256, 32768), (256, 32769), (1, 70000), (7, 66000)])
+def test_embedding_of_few_tokens(rows, table, kind):
+    """Where one launch takes over from the sort, by tokens and by table rows, and where a block has fewer waves."""
+    g = gen(rows + table)
+    for dtype, width in ((F32, 36), (BF16, 75), (F32, 3)):
+        lookup_check(randn(g, table, width, dtype=dtype), tokens(g, rows, table, torch.int64, kind), 0.5,
+                     randn(g, rows, width, dtype=dtype))
+
+
 def test_embedding_of_any_shape_and_scale():
     g = gen(1)
     t = randn(g, 20, 24)
