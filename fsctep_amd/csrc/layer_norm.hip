@@ -15,7 +15,7 @@
 //
 // Measured alone (large copies and fills on this card: 5.2 and 6.8 TB/s): 10,000 x 1,600 fp32 forward 20.6 us (128 MB, 6.2 TB/s),
 // backward 37 us (192 MB, 5.2 TB/s) with 5 us for the sums, twice 60 us (320 MB, 5.3 TB/s); 100,000 x 640 bf16 57 us (256 MB, 4.5 TB/s)
-// and 74 us (384 MB, 5.2 TB/s); 10,000 x 3,200 fp32 47, 82 and 138 us; 4,000 x 8,192 fp32 by wide_kernel 103, 346 and 450 us.
+// and 74 us (384 MB, 5.2 TB/s); 10,000 x 3,200 fp32 47, 82 and 138 us; 4,000 x 8,192 fp32 49, 84 and 136 us (131 MB an array).
 #include <algorithm>
 
 #include "common.h"
@@ -263,6 +263,9 @@ struct alignas(sizeof(T)) Vec {          // at any address a value may lie at
   T t[N];
 };
 
+// threads of a block whose rows take L lanes
+constexpr int threads_of(int L) { return L > NT ? L : NT; }
+
 template <typename T, int L, int CH>
 struct Row {
   static constexpr int V = Vec<T>::N;
@@ -348,7 +351,8 @@ __device__ __forceinline__ double dpp(double v) {
 // turns: who still reads the one has not passed the barrier before the next but one sum.
 template <int L, typename F>
 struct RowAdd {
-  F* red;                                // [2][5][NW] where a row takes the block
+  static constexpr int WAVES = L / 64;
+  F* red;                                // [2][5][WAVES] where a row takes the block
   int turn = 0;
   __device__ __forceinline__ explicit RowAdd(F* r) : red(r) {}
   template <int N>
@@ -365,15 +369,20 @@ struct RowAdd {
     for (int off = 16; off < (L < 64 ? L : 64); off <<= 1)
 #pragma unroll
       for (int i = 0; i < N; ++i) v[i] += __shfl_xor(v[i], off, 64);
-    if constexpr (L == NT) {
-      F* at = red + turn * 5 * NW;
+    if constexpr (L >= NT) {
+      F* at = red + turn * 5 * WAVES;
       turn ^= 1;
       if ((threadIdx.x & 63) == 0)
 #pragma unroll
-        for (int i = 0; i < N; ++i) at[i * NW + (threadIdx.x >> 6)] = v[i];
+        for (int i = 0; i < N; ++i) at[i * WAVES + (threadIdx.x >> 6)] = v[i];
       __syncthreads();
 #pragma unroll
-      for (int i = 0; i < N; ++i) v[i] = (at[i * NW] + at[i * NW + 1]) + (at[i * NW + 2] + at[i * NW + 3]);
+      for (int i = 0; i < N; ++i) {
+        v[i] = F(0);
+#pragma unroll
+        for (int k = 0; k < WAVES; k += 4)
+          v[i] += (at[i * WAVES + k] + at[i * WAVES + k + 1]) + (at[i * WAVES + k + 2] + at[i * WAVES + k + 3]);
+      }
     }
   }
 };
@@ -385,14 +394,14 @@ __device__ __forceinline__ void parts_of(double mean, float& hi, float& lo) {
 }
 
 template <typename T, typename W, bool SILU, int L, int CH>
-__global__ __launch_bounds__(NT) void row_kernel(Args a) {
+__global__ __launch_bounds__(threads_of(L)) void row_kernel(Args a) {
   using R = Row<T, L, CH>;
   constexpr int V = R::V;
-  __shared__ double red64[L == NT ? 2 * 5 * NW : 1];
-  __shared__ float red32[L == NT ? 2 * 5 * NW : 1];
+  __shared__ double red64[L >= NT ? 2 * 5 * L / 64 : 1];
+  __shared__ float red32[L >= NT ? 2 * 5 * L / 64 : 1];
   RowAdd<L, double> add64(red64);
   RowAdd<L, float> add32(red32);
-  const int64_t row = ((int64_t)blockIdx.x * NT + threadIdx.x) / L;
+  const int64_t row = ((int64_t)blockIdx.x * threads_of(L) + threadIdx.x) / L;
   if (row >= a.rows) return;
   const R at(a.width);
   float x[CH][V], w[CH][V], b[CH][V];
@@ -484,7 +493,7 @@ __device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at,
       if (a.db) ((W*)a.db)[i] = from_f<W>(b);
     }
   };
-  if constexpr (L == NT) {
+  if constexpr (L >= NT) {
 #pragma unroll
     for (int c = 0; c < CH; ++c) {
       const int i = at.base(c), skip = at.skip(c);
@@ -531,11 +540,11 @@ __device__ __forceinline__ void put_part(const Args& a, const Row<T, L, CH>& at,
 }
 
 template <typename T, typename W, bool SILU, typename F, int L, int CH>
-__global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
+__global__ __launch_bounds__(threads_of(L)) void row_back_kernel(Args a) {
   using R = Row<T, L, CH>;
-  constexpr int V = R::V, ROWS = NT / L;
-  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
-  __shared__ F red[L == NT ? 2 * 5 * NW : 1];
+  constexpr int V = R::V, ROWS = threads_of(L) / L;
+  __shared__ float buf[L >= NT ? 1 : 2 * L * CH * V];
+  __shared__ F red[L >= NT ? 2 * 5 * L / 64 : 1];
   RowAdd<L, F> row_add(red);
   const R at(a.width);
   float w[CH][V], b[CH][V], gw[CH][V] = {}, gb[CH][V] = {};
@@ -590,11 +599,11 @@ __global__ __launch_bounds__(NT) void row_back_kernel(Args a) {
 }
 
 template <typename T, typename W, bool SILU, typename F, int L, int CH>
-__global__ __launch_bounds__(NT) void row_twice_kernel(Args a) {
+__global__ __launch_bounds__(threads_of(L)) void row_twice_kernel(Args a) {
   using R = Row<T, L, CH>;
-  constexpr int V = R::V, ROWS = NT / L;
-  __shared__ float buf[L == NT ? 1 : 2 * L * CH * V];
-  __shared__ F red[L == NT ? 2 * 5 * NW : 1];
+  constexpr int V = R::V, ROWS = threads_of(L) / L;
+  __shared__ float buf[L >= NT ? 1 : 2 * L * CH * V];
+  __shared__ F red[L >= NT ? 2 * 5 * L / 64 : 1];
   RowAdd<L, F> row_add(red);
   const R at(a.width);
   float w[CH][V], b[CH][V], gw[CH][V] = {}, gb[CH][V] = {};
@@ -698,7 +707,9 @@ __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ par
 
 // Calls f(L, CH) for the fewest vectors of L lanes that hold a row; false where none do (a row shorter than a vector, or too
 // wide).  FORWARD shapes may have the registers of five vectors of 16 bits a lane, the backward passes three (100,000 x 640 in
-// bf16 backward, five vectors of 16 lanes: 130 us, three of 32: 88 us), the second one three of either type.
+// bf16 backward, five vectors of 16 lanes: 130 us, three of 32: 88 us), the second one three of either type.  Rows of 4,097 to 8,192
+// float32 values take 512 lanes (4,000 x 8,192 by 512 lanes, 1,024 lanes of two vectors and wide_kernel: forward 49, 50 and 105 us,
+// backward 84, 86 and 344 us, twice 136, 269 and 439 us; the same vectors of bfloat16 have no room for the second pass).
 enum Pass { FORWARD, BACK, TWICE };
 template <typename T, Pass P, typename F>
 bool by_shape(int width, F&& f) {
@@ -725,22 +736,25 @@ bool by_shape(int width, F&& f) {
   FSC_LN_SHAPE(256, 1)
   FSC_LN_SHAPE(256, 2)
   FSC_LN_SHAPE(256, 4)
+  if constexpr (V == 4) {
+    FSC_LN_SHAPE(512, 4)
+  }
 #undef FSC_LN_SHAPE
   return false;
 }
 
 // Blocks of the two backward passes on rows of L lanes.  Two rounds of rows are left to one block, which needs no partial rows
 // (32 x 128: 7.5 us, by two blocks 8.9 us; 64 x 128: 9.6 us by one, 9.0 us by four).  At most 512, 1,024 where a row takes a
-// block (100,000 x 640 in bf16 by 512 and 1,024: 80 and 90 us; 10,000 x 1,600: 47 and 44 us).
+// block's four waves (100,000 x 640 in bf16 by 512 and 1,024: 80 and 90 us; 10,000 x 1,600: 47 and 44 us).
 inline int back_blocks(int64_t rows, int L) {
-  const int64_t at_once = NT / L;
+  const int64_t at_once = threads_of(L) / L;
   if (rows <= 2 * at_once) return 1;
   return (int)std::min<int64_t>((rows + at_once - 1) / at_once, L == NT ? 1024 : 512);
 }
 
 template <typename T, typename W, bool SILU>
 void launch_forward(const Args& all, hipStream_t st) {
-  constexpr int64_t MOST = 1ll << 23;    // rows of a launch: a grid has fewer than 2^32 threads
+  constexpr int64_t MOST = 1ll << 22;    // rows of a launch: a grid has fewer than 2^32 threads
   for (int64_t r0 = 0; r0 < all.rows; r0 += MOST) {
     Args a = all;
     a.rows = std::min(all.rows - r0, MOST);
@@ -752,7 +766,7 @@ void launch_forward(const Args& all, hipStream_t st) {
     }
     if (!by_shape<T, FORWARD>(a.width, [&](auto L, auto CH) {
           constexpr int l = decltype(L)::value, ch = decltype(CH)::value;
-          row_kernel<T, W, SILU, l, ch><<<(unsigned)((a.rows * l + NT - 1) / NT), NT, 0, st>>>(a);
+          row_kernel<T, W, SILU, l, ch><<<(unsigned)((a.rows * l + threads_of(l) - 1) / threads_of(l)), threads_of(l), 0, st>>>(a);
         }))
       wide_kernel<T, W, SILU><<<(unsigned)a.rows, NT, 0, st>>>(a);
   }
@@ -772,8 +786,8 @@ void launch_backward(const Args& a, hipStream_t st) {
       }
     }
     if constexpr (l * ch > 16 || sizeof(T) == 2) {
-      if constexpr (P == TWICE) row_twice_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
-      else row_back_kernel<T, W, SILU, float, l, ch><<<blocks, NT, 0, st>>>(a);
+      if constexpr (P == TWICE) row_twice_kernel<T, W, SILU, float, l, ch><<<blocks, threads_of(l), 0, st>>>(a);
+      else row_back_kernel<T, W, SILU, float, l, ch><<<blocks, threads_of(l), 0, st>>>(a);
     }
   });
   if (!done) {

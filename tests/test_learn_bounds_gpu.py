@@ -49,7 +49,8 @@ def code(dtype):
 @pytest.mark.parametrize("off", [0, 1])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("rows,width", [(1, 1), (3, 3), (2, 7), (5, 9), (17, 64), (33, 65), (4, 128), (130, 331), (70, 384), (9, 640),
-                                        (21, 770), (5, 1024), (3, 1600), (2, 2049), (1025, 96), (0, 50)])
+                                        (21, 770), (5, 1024), (3, 1600), (2, 2049), (1025, 96), (0, 50), (3, 4097), (2, 5003), (1026, 4100),
+                                        (2, 8192), (1, 8193)])
 def test_layer_norm_writes_its_outputs_alone(rows, width, dtype, off):
     a = norm_inputs(max(rows, 1), width, dtype, dtype)
     a = {k: (t[:rows] if t.dim() == 2 else t) for k, t in a.items()}

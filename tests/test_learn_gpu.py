@@ -101,6 +101,12 @@ def test_narrow_rows(rows, width, dtype, silu):
         assert ((t.double() - want[name]).abs() <= tol).all(), name
 
 
+@pytest.mark.parametrize("rows,width", [(1, 4097), (3, 4100), (5, 5001), (40, 6144), (2, 8191), (600, 8192), (3, 8193), (2, 12001)])
+@pytest.mark.parametrize("dtype,silu", [(F32, False), (F32, True), (BF16, True)])
+def test_wide_rows(rows, width, dtype, silu):
+    norm_check(silu=silu, **norm_inputs(rows, width, dtype, F32))
+
+
 @pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True)])
 @pytest.mark.parametrize("silu", [False, True])
 def test_layer_norm_without_weight_or_bias(weight, bias, silu):
