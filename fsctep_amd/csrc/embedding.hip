@@ -8,7 +8,7 @@
 // Bound by memory: rows x width values written forward, read backward.  Measured (a fill of 400 MB takes 59 us, torch's sum of it
 // 106 us): 520,000 x 192 fp32 into 9 rows 58 us forward (6.9 TB/s; 95 us in a pass with its gradient, which reads what is not yet
 // written back) and 81 us backward (4.9 TB/s), into 100 rows by the sort 111 us (3.6 TB/s), into 1,000 rows 137 us; 8,125 x
-// 12,288 into 16 rows 59 and 79 us; 65,536 x 331 bf16 into 30,011 rows 13 and 54 us, 29 us of those the sort; 32 x 16 a launch each.
+// 12,288 into 16 rows 59 and 79 us; 65,536 x 331 bf16 into 30,011 rows 13 and 53 us, 28 us of those the sort; 32 x 16 a launch each.
 #include <algorithm>
 
 #include "common.h"
@@ -237,7 +237,7 @@ __global__ __launch_bounds__(1024) void small_join_kernel(Args a, const float* _
 // The tokens' numbers sorted by token (a stable radix sort, 8 bits a pass, tokens outside the table last), so that
 // sums are over runs of the sorted list.  A pass has counts by digit and block, each digit's counts added up over the blocks, and
 // the places: a digit's first place (all smaller digits' totals), the blocks before, the waves before, the lanes before.  Bound
-// by its launches (65,536 tokens: 15 us a pass).  A block takes PER tokens a thread: 16 where that leaves a block for every CU,
+// by its launches (65,536 tokens: 14 us a pass).  A block takes PER tokens a thread: 16 where that leaves a block for every CU,
 // 4 otherwise (the whole gradient of 64 columns of 100 rows: 100,000 tokens 35 and 26 us, 2,000,000 tokens 160 and 170 us).
 // Up to FEW_BLOCKS blocks each block of the places adds the counts itself, one launch less (BY_DIGIT false: counts [block][digit];
 // by themselves and by a scan: 2,000 tokens of 5,000 rows x 331 30.6 and 34.5 us, 32,768 of 5,000 x 64 34.3 and 37.0 us, 65,536 of
