@@ -99,6 +99,19 @@ def root_values(codes, scale):
     return torch.ops.fsctep.adamw_values(codes, scale, True)
 
 
+def _check_rule(group):
+    """Refuses a checkpoint's group whose settings are not of AdamW without its variants."""
+    for name in ("amsgrad", "maximize"):
+        if group.get(name):
+            raise ValueError(f"the checkpoint is of an optimiser with {name}, which this one does not have")
+    missing = {"lr", "betas", "eps", "weight_decay"} - set(group)
+    # torch's Adam and AdamW always say amsgrad; NAdam and RAdam, whose states have the same names, never do
+    if missing or "momentum_decay" in group or ("maximize" in group and "amsgrad" not in group):
+        raise ValueError(f"the checkpoint is of another optimiser: its settings are {sorted(set(group) - {'params'})}")
+    if group.get("decoupled_weight_decay") is False and group["weight_decay"] != 0:
+        raise ValueError("the checkpoint is of an optimiser whose weight_decay is not decoupled from the gradient (Adam)")
+
+
 class AdamW(torch.optim.Optimizer):
     """``torch.optim.AdamW`` without its variants, on the GPU, for float32 and bfloat16 parameters (contiguous).
     ``max_norm`` clips by the norm of all groups' gradients together (``grad_norm`` holds the last one's; a norm that is
@@ -160,9 +173,12 @@ class AdamW(torch.optim.Optimizer):
         want = {"exp_avg", "exp_avg_sq"} if self.state_bits == 32 else {"exp_avg", "exp_avg_scale", "root", "root_scale"}
         if not all(want <= set(s) for s in held.values() if s):
             raise ValueError(f"the checkpoint's states do not have {self.state_bits} bits")
-        for name in ("amsgrad", "maximize"):
-            if any(g.get(name) for g in state_dict["param_groups"]):
-                raise ValueError(f"the checkpoint is of an optimiser with {name}, which this one does not have")
+        for g in state_dict["param_groups"]:
+            _check_rule(g)
+        for s in held.values():
+            if s and set(s) - want - {"step", "master"}:
+                raise ValueError(f"the checkpoint is of another optimiser: it has states "
+                                 f"{sorted(set(s) - want - {'step', 'master'})}")
         super().load_state_dict(state_dict)
         number = {}
         for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
