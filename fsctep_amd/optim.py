@@ -166,9 +166,25 @@ class AdamW(torch.optim.Optimizer):
                  masters=[s.get("master", p) for s, p in zip(states, ps)], norm=self.grad_norm)
         return loss
 
+    def _loaded(self, p, held):
+        """A parameter's state from a checkpoint's, in this optimiser's types (torch's moments have their parameter's)."""
+        codes, values, scales = (torch.uint8, p.shape), (torch.float32, p.shape), (torch.float32, (math.ceil(p.numel() / GROUP),))
+        kinds = dict(step=(torch.float32, ()), exp_avg=values if self.state_bits == 32 else codes, exp_avg_sq=values, root=codes,
+                     exp_avg_scale=scales, root_scale=scales, master=values)
+        out = {}
+        for name, value in held.items():
+            dtype, shape = kinds[name]
+            value = torch.as_tensor(value)
+            if value.numel() != math.prod(shape) or (value.dtype == torch.uint8) != (dtype == torch.uint8):
+                raise ValueError(f"the checkpoint's {name} is {tuple(value.shape)} of {value.dtype}, its parameter {tuple(p.shape)}")
+            out[name] = value.detach().to(p.device, dtype, copy=True).reshape(shape).contiguous()
+        if p.dtype == torch.bfloat16 and "master" not in out:
+            out["master"] = p.detach().float()
+        return out
+
     def load_state_dict(self, state_dict):
         """Also a checkpoint of ``torch.optim.AdamW`` without its variants (states in 32 bits).  States keep their own types,
-        which the base class would cast to the parameter's."""
+        which the base class would cast to the parameter's.  What is refused is refused before anything changes."""
         held = state_dict["state"]
         want = {"exp_avg", "exp_avg_sq"} if self.state_bits == 32 else {"exp_avg", "exp_avg_scale", "root", "root_scale"}
         if not all(want <= set(s) for s in held.values() if s):
@@ -179,20 +195,13 @@ class AdamW(torch.optim.Optimizer):
             if s and set(s) - want - {"step", "master"}:
                 raise ValueError(f"the checkpoint is of another optimiser: it has states "
                                  f"{sorted(set(s) - want - {'step', 'master'})}")
-        super().load_state_dict(state_dict)
-        number = {}
+            if s and "step" not in s:
+                raise ValueError("the checkpoint has a state without its step count")
+        ready = {}
         for mine, theirs in zip(self.param_groups, state_dict["param_groups"]):
-            number.update(zip(mine["params"], theirs["params"]))
-        for p, s in self.state.items():
-            if p not in number or not s:
-                continue
-            for name, value in held[number[p]].items():
-                if name == "step":
-                    s[name] = torch.as_tensor(value, dtype=torch.float32).to(p.device).reshape(()).clone()
-                elif isinstance(value, torch.Tensor):
-                    s[name] = value.detach().to(p.device).clone(memory_format=torch.contiguous_format)
-            if p.dtype == torch.bfloat16 and "master" not in s:
-                s["master"] = p.detach().float()
+            ready.update((p, self._loaded(p, held[i])) for p, i in zip(mine["params"], theirs["params"]) if held.get(i))
+        super().load_state_dict(state_dict)
+        self.state.update(ready)
 
 
 def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy_weight: float = 1.0,

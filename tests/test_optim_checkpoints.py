@@ -70,3 +70,55 @@ def test_a_checkpoint_of_a_scheduled_run_is_taken():
     opt = mine()
     opt.load_state_dict(theirs.state_dict())
     assert opt.param_groups[0]["lr"] == theirs.param_groups[0]["lr"]
+
+
+def test_moments_of_16_bits_are_loaded_in_32():
+    """torch.optim.AdamW holds the moments of a bfloat16 parameter in bfloat16."""
+    p = torch.linspace(-1, 1, 300).bfloat16().requires_grad_(True)
+    theirs, opt = stepped(torch.optim.AdamW, p, lr=0.5), mine(torch.bfloat16)
+    opt.load_state_dict(theirs.state_dict())
+    (a,), (b,) = theirs.state.values(), opt.state.values()
+    for name in ("exp_avg", "exp_avg_sq"):
+        assert a[name].dtype == torch.bfloat16 and b[name].dtype == torch.float32 and torch.equal(a[name].float(), b[name])
+
+
+def state_of_8_bits(n=300):
+    return dict(step=torch.ones(()), exp_avg=torch.zeros(n, dtype=torch.uint8), exp_avg_scale=torch.ones(2),
+                root=torch.zeros(n, dtype=torch.uint8), root_scale=torch.ones(2))
+
+
+@pytest.mark.parametrize("bits,change,match", [
+    (32, dict(exp_avg=torch.zeros(299)), "exp_avg is"), (32, dict(exp_avg_sq=torch.zeros(300, 2)), "exp_avg_sq is"),
+    (32, dict(step=torch.zeros(2)), "step is"), (32, dict(master=torch.zeros(3)), "master is"),
+    (32, dict(exp_avg=torch.zeros(300, dtype=torch.uint8)), "exp_avg is"), (32, dict(step=None), "step count"),
+    (8, dict(exp_avg=torch.zeros(300)), "exp_avg is"), (8, dict(root=torch.zeros(301, dtype=torch.uint8)), "root is"),
+    (8, dict(root_scale=torch.ones(3)), "root_scale is"), (8, dict(exp_avg_scale=torch.ones(2, dtype=torch.uint8)), "scale is"),
+    (8, dict(step=None), "step count")])
+def test_states_of_other_sizes_and_types_are_refused(bits, change, match):
+    """Before the optimiser's own states go."""
+    held = stepped(torch.optim.AdamW, lr=0.5).state_dict()
+    if bits == 8:
+        held["state"][0] = state_of_8_bits()
+    held["state"][0] = {k: v for k, v in (held["state"][0] | change).items() if v is not None}
+    refused(mine(state_bits=bits), held, match)
+
+
+def test_states_of_8_bits_are_loaded_apart_from_the_checkpoint():
+    held = mine(state_bits=8).state_dict()
+    held["state"][0] = state_of_8_bits()
+    opt = mine(state_bits=8)
+    opt.load_state_dict(held)
+    (s,) = opt.state.values()
+    for name, t in held["state"][0].items():
+        assert torch.equal(s[name], t) and s[name].dtype == t.dtype and s[name].data_ptr() != t.data_ptr()
+
+
+def test_states_of_any_order_are_loaded_contiguous():
+    p = torch.zeros(20, 30, requires_grad=True)
+    held = stepped(torch.optim.AdamW, torch.ones(20, 30, requires_grad=True), lr=0.5).state_dict()
+    turned = torch.randn(30, 20).t()
+    held["state"][0]["exp_avg"], held["state"][0]["step"] = turned, 7
+    opt = optim.AdamW([p])
+    opt.load_state_dict(held)
+    assert torch.equal(opt.state[p]["exp_avg"], turned) and opt.state[p]["exp_avg"].is_contiguous()
+    assert opt.state[p]["step"].shape == () and float(opt.state[p]["step"]) == 7
