@@ -130,9 +130,10 @@ class AdamW(torch.optim.Optimizer):
 
     def _state(self, p):
         s = self.state[p]
+        copied = p.dtype == torch.bfloat16
+        if (not s or (copied and "master" not in s)) and torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("AdamW: take a step before one is captured (a replay would start the states anew)")
         if not s:
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("AdamW: take a step before one is captured (a replay would start the states anew)")
             s["step"] = torch.zeros((), dtype=torch.float32, device=p.device)
             if self.state_bits == 32:
                 for name in ("exp_avg", "exp_avg_sq"):
@@ -141,8 +142,8 @@ class AdamW(torch.optim.Optimizer):
                 for name in ("exp_avg", "root"):
                     s[name] = torch.zeros(p.shape, dtype=torch.uint8, device=p.device)
                     s[name + "_scale"] = torch.zeros(math.ceil(p.numel() / GROUP), dtype=torch.float32, device=p.device)
-            if p.dtype == torch.bfloat16:
-                s["master"] = p.detach().float()
+        if copied and "master" not in s:     # a checkpoint without copies: of what the parameter holds now
+            s["master"] = p.detach().float()
         return s
 
     @torch.no_grad()
@@ -178,8 +179,8 @@ class AdamW(torch.optim.Optimizer):
             if value.numel() != math.prod(shape) or (value.dtype == torch.uint8) != (dtype == torch.uint8):
                 raise ValueError(f"the checkpoint's {name} is {tuple(value.shape)} of {value.dtype}, its parameter {tuple(p.shape)}")
             out[name] = value.detach().to(p.device, dtype, copy=True).reshape(shape).contiguous()
-        if p.dtype == torch.bfloat16 and "master" not in out:
-            out["master"] = p.detach().float()
+        if p.dtype != torch.bfloat16:
+            out.pop("master", None)          # of a bfloat16 run: no step would keep it up
         return out
 
     def load_state_dict(self, state_dict):

@@ -122,3 +122,19 @@ def test_states_of_any_order_are_loaded_contiguous():
     opt.load_state_dict(held)
     assert torch.equal(opt.state[p]["exp_avg"], turned) and opt.state[p]["exp_avg"].is_contiguous()
     assert opt.state[p]["step"].shape == () and float(opt.state[p]["step"]) == 7
+
+
+def test_a_copy_is_held_for_16_bit_parameters_alone():
+    """A bfloat16 run's copies would stand still beside float32 parameters, and be taken for theirs when those go back."""
+    held = stepped(torch.optim.AdamW, lr=0.5).state_dict()
+    held["state"][0]["master"] = torch.full((300,), 5.0)
+    for dtype, there in ((torch.float32, False), (torch.bfloat16, True)):
+        opt = mine(dtype)
+        opt.load_state_dict(held)
+        (s,) = opt.state.values()
+        assert ("master" in s) == there and ("master" in opt.state_dict()["state"][0]) == there
+    del held["state"][0]["master"]
+    opt = mine(torch.bfloat16)
+    opt.load_state_dict(held)
+    (s,) = opt.state.values()
+    assert "master" not in s           # the parameter's values may still be to come; the first step copies them

@@ -37,3 +37,45 @@ def test_a_step_from_torchs_states_of_16_bits():
     # a step is at most a few lr, its quotient off by as many roundings
     assert ((s["master"].double() - twin.detach()).abs() <= 16 * U * (p.detach().double().abs() + 20 * 1e-2)).all()
     assert torch.equal(q.detach(), s["master"].bfloat16())
+
+
+def test_a_float32_run_between_two_of_16_bits():
+    """The second bfloat16 run goes on from what the float32 run left, not from the first one's copies."""
+    def run(dtype, values, held, lr):
+        p = values.to(dtype).requires_grad_(True)
+        opt = optim.AdamW([p], lr=lr, weight_decay=0.0)
+        if held is not None:
+            opt.load_state_dict(held)
+        for group in opt.param_groups:
+            group["lr"] = lr
+        p.grad = torch.ones_like(p)
+        opt.step()
+        return p.detach(), opt.state_dict()
+
+    start = torch.linspace(-1, 1, 300, device=DEV)
+    a, held = run(torch.bfloat16, start, None, 0.0)
+    b, held = run(torch.float32, a.float() + 1.0, held, 0.0)
+    c, held = run(torch.bfloat16, b, held, 0.0)
+    assert torch.equal(b, a.float() + 1.0) and torch.equal(c, b.bfloat16())
+    assert torch.equal(held["state"][0]["master"], c.float())
+
+
+def test_values_that_come_after_the_states():
+    """A program that loads the optimiser before the model, from a checkpoint without 32-bit copies."""
+    q = torch.ones(300, device=DEV, requires_grad=True)
+    theirs = torch.optim.AdamW([q], lr=0.0, weight_decay=0.0)
+    q.grad = torch.ones_like(q)
+    theirs.step()
+    p = torch.zeros(300, device=DEV, dtype=torch.bfloat16, requires_grad=True)
+    opt = optim.AdamW([p], lr=0.0, weight_decay=0.0)
+    opt.load_state_dict(theirs.state_dict())
+    with torch.no_grad():
+        p.fill_(3.0)
+    p.grad = torch.ones_like(p)
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="take a step before"):
+        with torch.cuda.graph(graph):
+            torch.zeros(1, device=DEV)
+            opt.step()
+    opt.step()
+    assert (p == 3.0).all() and (opt.state[p]["master"] == 3.0).all() and float(opt.state[p]["step"]) == 2
