@@ -203,6 +203,9 @@ class AdamW(torch.optim.Optimizer):
             ready.update((p, self._loaded(p, held[i])) for p, i in zip(mine["params"], theirs["params"]) if held.get(i))
         super().load_state_dict(state_dict)
         self.state.update(ready)
+        for g in self.param_groups:          # a checkpoint read to the host, or one of 64 bits
+            if isinstance(g["lr"], torch.Tensor) and g["params"]:
+                g["lr"] = g["lr"].detach().to(g["params"][0].device, torch.float32)
 
 
 def train_step(model, optimizer, pos, batch, cell, graph, energy, forces, energy_weight: float = 1.0,

@@ -138,3 +138,10 @@ def test_a_copy_is_held_for_16_bit_parameters_alone():
     opt.load_state_dict(held)
     (s,) = opt.state.values()
     assert "master" not in s           # the parameter's values may still be to come; the first step copies them
+
+
+def test_a_learning_rate_of_64_bits_is_loaded_in_32():
+    held = stepped(torch.optim.AdamW, lr=torch.tensor(0.125, dtype=torch.float64), foreach=False).state_dict()
+    opt = mine()
+    opt.load_state_dict(held)
+    assert opt.param_groups[0]["lr"].dtype == torch.float32 and float(opt.param_groups[0]["lr"]) == 0.125

@@ -79,3 +79,19 @@ def test_values_that_come_after_the_states():
             opt.step()
     opt.step()
     assert (p == 3.0).all() and (opt.state[p]["master"] == 3.0).all() and float(opt.state[p]["step"]) == 2
+
+
+def test_a_learning_rate_on_the_gpu_comes_back_from_the_host(tmp_path):
+    """A checkpoint is read with its tensors on the host; the states go where the parameters are, and so does the rate."""
+    p = torch.linspace(-1, 1, 300, device=DEV).requires_grad_(True)
+    opt = optim.AdamW([p], lr=torch.full((), 1e-2, device=DEV))
+    p.grad = torch.ones_like(p)
+    opt.step()
+    torch.save(opt.state_dict(), tmp_path / "opt.pt")
+    q = p.detach().clone().requires_grad_(True)
+    other = optim.AdamW([q], lr=0.5)
+    other.load_state_dict(torch.load(tmp_path / "opt.pt", map_location="cpu", weights_only=True))
+    q.grad = torch.ones_like(q)
+    opt.step()
+    other.step()
+    assert torch.equal(p, q) and other.param_groups[0]["lr"].device == p.device
