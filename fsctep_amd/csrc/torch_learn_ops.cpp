@@ -254,7 +254,8 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_backward_autograd(const Tensor& dy
 
 // A force loss sends two gradients to x, one through y and one through the backward's own backward.  The second comes to this
 // function's node as the gradient of `through`, an output of x's shape that holds nothing, and the kernel that makes the first
-// adds it (`plus`): a pass over x less than autograd's addition takes.
+// adds it (`plus`): a pass over x less than autograd's addition takes.  A run of the node that only passes the second one on
+// reads nothing that the node keeps, and leaves it (release_variables below).
 struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   static variable_list forward(AutogradContext* ctx, Tensor x, optional<Tensor> w, optional<Tensor> b, double eps,
                                int64_t act) {
@@ -264,6 +265,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     ctx->save_for_backward({x, some(w), some(b), mean, rstd, through});
     ctx->saved_data["eps"] = eps;
     ctx->saved_data["act"] = act;
+    ctx->saved_data["passed"] = false;
     ctx->set_materialize_grads(false);
     ctx->mark_non_differentiable({mean, rstd});
     return {y, mean, rstd, through};
@@ -271,6 +273,7 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(5);
     const bool want_x = ctx->needs_input_grad(0);
+    ctx->saved_data["passed"] = !grads[0].defined();
     if (!grads[0].defined()) {
       if (want_x) out[0] = grads[3];
       return out;
@@ -288,6 +291,20 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
     return out;
   }
 };
+
+}  // namespace
+
+// The engine calls this after a node's run unless the graph is to be kept.  x's second gradient alone comes through LayerNormFn's
+// node without using it up: y can still be differentiated, as where the second gradient goes straight to x.
+template <>
+void torch::autograd::CppNode<LayerNormFn>::release_variables() {
+  std::lock_guard<std::mutex> lock(mutex_);
+  if (ctx_.saved_data["passed"].toBool()) return;
+  ctx_.saved_variables_.clear();
+  ctx_.has_freed_buffers_ = true;
+}
+
+namespace {
 
 std::tuple<Tensor, Tensor, Tensor> layer_norm_autograd(const Tensor& x, const optional<Tensor>& w, const optional<Tensor>& b,
                                                        double eps, int64_t act, bool keep) {
