@@ -92,6 +92,7 @@ SIGNATURES = {
     "fsc_layer_norm_backward": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _f32] + [_p] * 9,
     "fsc_layer_norm_backward_twice": [_i64, _i32, _i32, _i32, _i32, _i64, _i64, _i64, _p, _p, _p, _f32] + [_p] * 12,
     "fsc_embedding_forward": [_i64, _i32, _i64, _i32, _i32, _i64, _p, _p, _f32, _p, _p],
+    "fsc_embedding_forward_or": [_i64, _i32, _i64, _i32, _i32, _i64, _p, _p, _f32, _f32, _p, _p],
     "fsc_embedding_workspace": [_i64, _i32, _i64, _pi64],
     "fsc_embedding_backward": [_i64, _i32, _i64, _i32, _i32, _i64, _p, _p, _f32, _p, _p, _p],
     "fsc_adamw_workspace": [_i32, _p, _pi64, _pi64],

@@ -2,7 +2,7 @@
 // gradients by token.  Replaces the indexing of the training step's first convolution and of the expert readout's
 // table of scores, whose gradient was an atomic addition into a handful of rows
 // (models/pure_cartesian_sparse_layers.py:258-259 embeds the species of every atom).
-//   out_i = scale table[index_i], zeros where index_i lies outside the table
+//   out_i = scale table[index_i], a given value (zeros) where index_i lies outside the table
 //   dtable_v = scale sum over i with index_i = v, in 32 bits and an order that the sizes alone give
 //
 // Bound by memory: rows x width values written forward, read backward.  Measured (a fill of 400 MB takes 59 us, torch's sum of it
@@ -34,6 +34,7 @@ struct Args {
   float scale;
   const void *in, *index;
   void* out;
+  float outside;               // forward: what stands where a token has no row
 };
 
 template <typename T>
@@ -86,7 +87,7 @@ __global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint3
   float v[N];
   load_some<FULL, N>((const T*)a.in + (there ? t : 0) * a.stride + col, n, v);
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = there ? a.scale * v[j] : 0.f;
+  for (int j = 0; j < N; ++j) v[j] = there ? a.scale * v[j] : a.outside;
   T* out = (T*)a.out + row * a.width + col;
   if constexpr (FULL) {
     typedef unsigned u4s __attribute__((ext_vector_type(4), aligned(2)));
@@ -679,9 +680,9 @@ int check_sizes(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, 
 
 extern "C" {
 
-int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits,
-                          int64_t table_stride, const void* table, const void* index, float scale, void* out,
-                          hipStream_t stream) {
+int fsc_embedding_forward_or(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits,
+                             int64_t table_stride, const void* table, const void* index, float scale, float outside, void* out,
+                             hipStream_t stream) {
   using namespace fsc;
   using namespace fsc::embed;
   if (int rc = check_sizes(rows, width, table_rows, dtype, index_bits)) return rc;
@@ -689,9 +690,15 @@ int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32
   FSC_CHECK_ARG(index && out && (table || table_rows == 0), "embedding: null array");
   FSC_CHECK_ARG(table_stride >= 0, "embedding: negative row stride");
   // without a table no row is read for its values: any array does
-  const Args a{rows, table_rows ? table_stride : 0, table_rows, width, scale, table_rows ? table : out, index, out};
+  const Args a{rows, table_rows ? table_stride : 0, table_rows, width, scale, table_rows ? table : out, index, out, outside};
   FSC_EMBED_TYPES((launch_lookup<T, I>(a, stream)));
   return check_launch("embedding") ? 2 : 0;
+}
+
+int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits,
+                          int64_t table_stride, const void* table, const void* index, float scale, void* out,
+                          hipStream_t stream) {
+  return fsc_embedding_forward_or(rows, width, table_rows, dtype, index_bits, table_stride, table, index, scale, 0.f, out, stream);
 }
 
 int fsc_embedding_workspace(int64_t rows, int32_t width, int64_t table_rows, int64_t* bytes) {
@@ -715,7 +722,7 @@ int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int3
   FSC_CHECK_ARG(dtable && (rows == 0 || (dy && index)), "embedding_backward: null array");
   FSC_CHECK_ARG(dy_stride >= 0, "embedding_backward: negative row stride");
   FSC_CHECK_ARG(rows * (int64_t)width <= 1ll << 41, "embedding_backward: dy has more than 2^41 values");   // grids of 32 bits
-  const Args a{rows, dy_stride, table_rows, width, scale, dy, index, dtable};
+  const Args a{rows, dy_stride, table_rows, width, scale, dy, index, dtable, 0.f};
   FSC_CHECK_ARG(few(rows, table_rows) || workspace, "embedding_backward: null workspace");
   FSC_EMBED_TYPES((launch_backward<T, I>(a, (char*)workspace, stream)));
   return check_launch("embedding_backward") ? 2 : 0;

@@ -331,7 +331,7 @@ void check_scale(double scale, const char* op) {
   TORCH_CHECK(std::isfinite((float)scale), op, ": scale must be finite, got ", scale);
 }
 
-Tensor embedding(const Tensor& table_, const Tensor& index_, double scale) {
+Tensor embedding(const Tensor& table_, const Tensor& index_, double scale, double outside) {
   require_gpu({table_, index_}, "embedding");
   TORCH_CHECK(table_.dim() == 2, "embedding: table must be (rows, width), got ", table_.dim(), " dimensions");
   const int32_t dt = code_of(table_.scalar_type(), "table"), bits = check_index(index_, "embedding");
@@ -341,13 +341,13 @@ Tensor embedding(const Tensor& table_, const Tensor& index_, double scale) {
   const Tensor table = rows2d(table_, "table"), index = index_.contiguous();
   Tensor out = at::empty({index.size(0), table.size(1)}, table.options());
   if (out.numel() == 0) return out;
-  check(fsc_embedding_forward(index.size(0), (int32_t)table.size(1), table.size(0), dt, bits, stride_of(table), ptr(table),
-                              ptr(index), (float)scale, mptr(out), stream_of(table)),
-        "fsc_embedding_forward");
+  check(fsc_embedding_forward_or(index.size(0), (int32_t)table.size(1), table.size(0), dt, bits, stride_of(table), ptr(table),
+                                 ptr(index), (float)scale, (float)outside, mptr(out), stream_of(table)),
+        "fsc_embedding_forward_or");
   return out;
 }
 
-Tensor embedding_meta(const Tensor& table, const Tensor& index, double scale) {
+Tensor embedding_meta(const Tensor& table, const Tensor& index, double scale, double) {
   TORCH_CHECK(table.dim() == 2, "embedding: table must be (rows, width), got ", table.dim(), " dimensions");
   code_of(table.scalar_type(), "table");
   check_index(index, "embedding");
@@ -388,7 +388,7 @@ Tensor embedding_backward_meta(const Tensor& dy, const Tensor& index, c10::SymIn
 }
 
 auto& embedding_op() {
-  static auto op = op_handle<Tensor(const Tensor&, const Tensor&, double)>("fsctep::embedding");
+  static auto op = op_handle<Tensor(const Tensor&, const Tensor&, double, double)>("fsctep::embedding");
   return op;
 }
 auto& embedding_backward_op() {
@@ -407,7 +407,7 @@ struct EmbeddingBackwardFn : public torch::autograd::Function<EmbeddingBackwardF
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     variable_list out(4);
     if (ctx->needs_input_grad(0))
-      out[0] = embedding_op().call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble());
+      out[0] = embedding_op().call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["scale"].toDouble(), 0.0);
     return out;
   }
 };
@@ -419,15 +419,15 @@ Tensor embedding_backward_autograd(const Tensor& dy, const Tensor& index, c10::S
 }
 
 struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
-  static variable_list forward(AutogradContext* ctx, Tensor table, Tensor index, double scale) {
+  static variable_list forward(AutogradContext* ctx, Tensor table, Tensor index, double scale, double outside) {
     at::AutoDispatchBelowADInplaceOrView guard;
     ctx->save_for_backward({index});
     ctx->saved_data["rows"] = table.sym_size(0);
     ctx->saved_data["scale"] = scale;
-    return {embedding_op().call(table, index, scale)};
+    return {embedding_op().call(table, index, scale, outside)};
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
-    variable_list out(3);
+    variable_list out(4);
     if (ctx->needs_input_grad(0))
       out[0] = embedding_backward_op().call(grads[0], ctx->get_saved_variables()[0], ctx->saved_data["rows"].toSymInt(),
                                             ctx->saved_data["scale"].toDouble());
@@ -435,10 +435,10 @@ struct EmbeddingFn : public torch::autograd::Function<EmbeddingFn> {
   }
 };
 
-Tensor embedding_autograd(const Tensor& table, const Tensor& index, double scale) {
-  if (differentiates({table})) return EmbeddingFn::apply(table, index, scale)[0];
+Tensor embedding_autograd(const Tensor& table, const Tensor& index, double scale, double outside) {
+  if (differentiates({table})) return EmbeddingFn::apply(table, index, scale, outside)[0];
   at::AutoDispatchBelowADInplaceOrView guard;
-  return embedding_op().call(table, index, scale);
+  return embedding_op().call(table, index, scale, outside);
 }
 
 // ============================================================== optimiser
@@ -656,7 +656,7 @@ TORCH_LIBRARY_FRAGMENT(fsctep, m) {
   m.def("layer_norm_backward_twice(Tensor? v, Tensor? v_weight, Tensor? v_bias, Tensor dy, Tensor x, Tensor? weight,"
         " Tensor? bias, Tensor mean, Tensor rstd, float eps, int activation, bool want_x, bool want_dy, bool want_weight,"
         " bool want_bias) -> (Tensor grad_x, Tensor grad_dy, Tensor grad_weight, Tensor grad_bias)");
-  m.def("embedding(Tensor table, Tensor index, float scale) -> Tensor");
+  m.def("embedding(Tensor table, Tensor index, float scale, float outside=0.) -> Tensor");
   m.def("embedding_backward(Tensor dy, Tensor index, SymInt table_rows, float scale) -> Tensor");
   m.def("grad_norm(Tensor[] grads) -> Tensor");
   m.def("adamw_(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avg, Tensor(c!)[] exp_avg_sq, Tensor(d!)[] steps,"

@@ -101,7 +101,7 @@ class Router:
         if self.n_species is None:
             return F.linear(y, layer.gate)
         from . import train_ops as T
-        l = T.lookup(layer.gate, species)
+        l = T.lookup(layer.gate, species, outside=math.nan)
         return l if none is None else l.masked_fill(none, math.nan)
 
     def choose(self, layer, logits):

@@ -8,7 +8,7 @@ and SiLU, models/mlp.py:8-66, and its lookups by species, models/pure_cartesian_
 ``fsctep_amd.optim`` has the optimiser.
 
     layer_norm(x, weight=None, bias=None, eps=1e-5, activation=None) -> y
-    embedding(table, index, scale=1.0) -> rows
+    embedding(table, index, scale=1.0, outside=0.0) -> rows
 
 ``layer_norm`` differentiates twice (rows, weight, bias), ``embedding`` to any order (table); a third derivative of
 ``layer_norm`` and forward-mode derivatives raise.
@@ -33,11 +33,11 @@ def layer_norm(x, weight=None, bias=None, eps: float = 1e-5, activation: str | N
     return torch.ops.fsctep.layer_norm(x, weight, bias, float(eps), ACTIVATIONS[activation], False)[0]
 
 
-def embedding(table, index, scale: float = 1.0):
+def embedding(table, index, scale: float = 1.0, outside: float = 0.0):
     """``scale * table[index]``, (\\*index.shape, width), of a (rows, width) table, float32 or bfloat16, for an index of
-    any shape, int32 or int64; zeros, without a gradient, where the index lies outside the table (-1: padding).  The
+    any shape, int32 or int64; ``outside``, without a gradient, where the index lies outside the table (-1: padding).  The
     table's gradient sums the rows of each token in 32 bits and in a fixed order."""
     if index.dim() == 1:
-        return torch.ops.fsctep.embedding(table, index, float(scale))
-    rows = torch.ops.fsctep.embedding(table, index.reshape(-1), float(scale))
+        return torch.ops.fsctep.embedding(table, index, float(scale), float(outside))
+    rows = torch.ops.fsctep.embedding(table, index.reshape(-1), float(scale), float(outside))
     return rows.view(*index.shape, rows.shape[1])

@@ -36,12 +36,13 @@ def _on_ops(t) -> bool:
 
 
 # ------------------------------------------------------------------ lookups (embedding.hip)
-def lookup(table, index):
-    """``table.index_select(0, index)`` of a table of any shape, its gradient summed by row in a fixed order."""
+def lookup(table, index, outside: float = 0.0):
+    """``table.index_select(0, index)`` of a table of any shape, its gradient summed by row in a fixed order; ``outside``
+    where the ops are given an index outside the table (which index_select refuses)."""
     if not _on_ops(table) or table.numel() == 0 or table.numel() // table.shape[0] > 1 << 20:
         return table.index_select(0, index)
     from . import learn_ops
-    return learn_ops.embedding(table.reshape(table.shape[0], -1), index).view(-1, *table.shape[1:])
+    return learn_ops.embedding(table.reshape(table.shape[0], -1), index, outside=outside).view(-1, *table.shape[1:])
 
 
 # ------------------------------------------------------------------ edge geometry (edge_radial.hip)
