@@ -106,9 +106,12 @@ __global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint3
 // once, four where it does not (1,024 tokens by four and eight: 64 columns of 100 rows, all of one token, 17.7 and 11.0 us; 640
 // columns of 5,000 rows 13.7 and 19.1 us).  For up to 2,048 tokens and 2^23 pairs of token and row to look at (by it and by the
 // sort: 2,048 tokens, 640 columns of 100 rows 5.8 and 21.0 us, all of one token 28.7 and 18.7 us; 1,024 of 5,000 rows 13.7 and 29.4
-// us; 256 of 30,000 rows x 331 24.6 and 33.5 us, 1,024 40.2 and 35.6 us), 512 where the table is small (192 columns of 9 rows, all
-// of one token: 512 tokens 6.3 and 7.6 us, 1,024 tokens 11.1 and 7.9 us).
-inline bool few(int64_t rows, int64_t table_rows);
+// us; 256 of 30,000 rows x 331 24.6 and 33.5 us, 1,024 40.2 and 35.6 us), and 2^25 for those pairs times the blocks of columns,
+// each of which looks through the tokens again (fp32: 1,024 tokens of 1,600 rows x 4,096 29.3 and 35.5 us, 2,048 tokens 47.9 and 37.9 us, of
+// 1,600 rows x 12,288 156 and 70 us, of 4,000 rows 331 and 95 us; bf16: 256 of 30,000 rows x 2,048 54.9 and 55.4 us, 1,024 of 1,600
+// rows x 12,288 48.6 and 45.8 us).  512 tokens where the table is small (192 columns of 9 rows, all of one token: 512 tokens 6.3
+// and 7.6 us, 1,024 tokens 11.1 and 7.9 us; 12,288 columns of 24 rows 6.6 and 27.1 us).
+inline bool few(int64_t rows, int64_t table_rows, int width, int size);
 template <int WAVES, typename T, typename I, bool FULL>
 __global__ __launch_bounds__(64 * WAVES) void few_kernel(Args a) {
   constexpr int N = Vec<T>::N, AHEAD = 8;
@@ -162,8 +165,11 @@ __global__ __launch_bounds__(64 * WAVES) void few_kernel(Args a) {
 // More rows leave too few copies for the chip (520,000 x 192 by copies and by the sort: 9 rows 81 and 116 us, 24 rows 105 and
 // 111 us, 32 rows 123 and 110 us).
 constexpr int SMALL = 24;
-inline bool few(int64_t rows, int64_t table_rows) {
-  return table_rows <= SMALL ? rows <= 512 : rows <= 2048 && rows * table_rows <= 1 << 23;
+inline bool few(int64_t rows, int64_t table_rows, int width, int size) {
+  if (table_rows <= SMALL) return rows <= 512;
+  if (rows > 2048 || rows * table_rows > 1 << 23) return false;
+  const int columns = 64 * (16 / size);                                   // of a block
+  return rows * table_rows * ((width + columns - 1) / columns) <= 1 << 25;
 }
 inline int small_waves(int64_t table_rows) { return table_rows <= 16 ? 4 : 2; }       // at most 64 KB of copies a block
 struct Stream {
@@ -608,7 +614,7 @@ void launch_lookup(const Args& a, hipStream_t st) {
 template <typename T, typename I>
 void launch_backward(const Args& a, char* ws, hipStream_t st) {
   constexpr int N = Vec<T>::N;
-  if (few(a.rows, a.table_rows)) {
+  if (few(a.rows, a.table_rows, a.width, sizeof(T))) {
     const dim3 grid((unsigned)std::min<int64_t>(a.table_rows, 1 << 16), (a.width + 64 * N - 1) / (64 * N));
     if ((int64_t)grid.x * grid.y <= 2048) FSC_EMBED_FULL(a.width >= N, (few_kernel<8, T, I, FULL><<<grid, 512, 0, st>>>(a)))
     else FSC_EMBED_FULL(a.width >= N, (few_kernel<4, T, I, FULL><<<grid, 256, 0, st>>>(a)))
@@ -704,11 +710,13 @@ int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32
 int fsc_embedding_workspace(int64_t rows, int32_t width, int64_t table_rows, int64_t* bytes) {
   FSC_CHECK_ARG(bytes != nullptr, "embedding: null output");
   if (int rc = fsc::embed::check_sizes(rows, width, table_rows, FSC_F32, 32)) return rc;
-  // the layout depends on the type: room for either
-  if (fsc::embed::few(rows, table_rows) || table_rows == 0) *bytes = 0;
-  else if (table_rows <= fsc::embed::SMALL) *bytes = fsc::embed::small_layout(rows, width, table_rows).bytes;
-  else *bytes = std::max(fsc::embed::layout_of(rows, width, table_rows, 4).bytes,
-                          fsc::embed::layout_of(rows, width, table_rows, 2).bytes);
+  *bytes = 0;
+  if (table_rows == 0) return 0;
+  for (int size : {2, 4}) {              // path and layout depend on the type: room for either
+    if (fsc::embed::few(rows, table_rows, width, size)) continue;
+    if (table_rows <= fsc::embed::SMALL) *bytes = std::max(*bytes, fsc::embed::small_layout(rows, width, table_rows).bytes);
+    else *bytes = std::max(*bytes, fsc::embed::layout_of(rows, width, table_rows, size).bytes);
+  }
   return 0;
 }
 
@@ -723,7 +731,7 @@ int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int3
   FSC_CHECK_ARG(dy_stride >= 0, "embedding_backward: negative row stride");
   FSC_CHECK_ARG(rows * (int64_t)width <= 1ll << 41, "embedding_backward: dy has more than 2^41 values");   // grids of 32 bits
   const Args a{rows, dy_stride, table_rows, width, scale, dy, index, dtable, 0.f};
-  FSC_CHECK_ARG(few(rows, table_rows) || workspace, "embedding_backward: null workspace");
+  FSC_CHECK_ARG(few(rows, table_rows, width, dtype == FSC_F32 ? 4 : 2) || workspace, "embedding_backward: null workspace");
   FSC_EMBED_TYPES((launch_backward<T, I>(a, (char*)workspace, stream)));
   return check_launch("embedding_backward") ? 2 : 0;
 }
