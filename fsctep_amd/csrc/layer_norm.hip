@@ -428,7 +428,19 @@ __global__ __launch_bounds__(threads_of(L)) void row_kernel(Args a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) t[0] += x[c][j] * x[c][j];
   add32(t);
-  const float rstd = 1.f / sqrtf(t[0] / a.width + a.eps);
+  const float var = t[0] / a.width + a.eps;
+  float rstd = 1.f / sqrtf(var);
+  if (!(var > 0x1p-110f && var < 0x1p126f)) {
+    // squares past 32 bits' range (deviations from 2^63 on, or below 2^-55 with an eps as small): again in 64 bits.  The whole row
+    // comes here: every lane of it has the same sum.
+    s[0] = 0.0;
+#pragma unroll
+    for (int c = 0; c < CH; ++c)
+#pragma unroll
+      for (int j = 0; j < V; ++j) s[0] += (double)x[c][j] * (double)x[c][j];
+    add64(s);
+    rstd = (float)(1.0 / sqrt(s[0] / a.width + (double)a.eps));
+  }
   T* y = (T*)a.y + row * a.width;
 #pragma unroll
   for (int c = 0; c < CH; ++c) {
