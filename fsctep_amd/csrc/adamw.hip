@@ -99,7 +99,10 @@ __device__ __forceinline__ float decode(uint32_t c, float scale) {
   if (!ROOT && c >= 128u) y = -y;
   return y * scale;
 }
-// over: 1 / the block's largest (0 where the block is zeros); bits: what the rounding adds below the last bit kept
+// over: 1 / the block's largest (0 where the block is zeros); bits: what the rounding adds below the last bit kept.  The mean of
+// the roundings is the value from code 1 on (1.25 2^-16 of the largest, ROOT: 1.125 2^-16).  Below it there is no neighbour at a
+// float's spacing: a root above zero becomes code 1, whose step is smaller than the value's own, others 0 from one
+// spacing below code 1 on.
 template <bool ROOT>
 __device__ __forceinline__ uint32_t encode(float x, float over, uint32_t bits) {
   using K = Code<ROOT>;

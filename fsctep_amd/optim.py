@@ -13,7 +13,9 @@ is stepped and rounded (who writes other values into such a parameter writes the
 
 States in 8 bits (``state_bits=8``): m and sqrt(v) as 8-bit floats with a float32 scale for each 256 values, rounded
 up or down by a hash of the value's number and the step, so that small changes add up over the steps instead of being
-rounded away.  16 bytes a value are moved in place of 28.
+rounded away.  16 bytes a value are moved in place of 28.  The format reaches down to 2e-5 of the largest of the 256: a value
+whose gradients stay below that share of its neighbours' loses its momentum (m becomes 0), and its steps are divided by
+the smallest sqrt(v) there is, which makes them smaller than its own would.
 
     train_step(model, optimizer, pos, batch, cell, graph, energy, forces, ...)       # a trunk's step on energies and forces
     adamw_step(params, grads, exp_avgs, exp_avg_sqs, steps, lr, betas, eps, weight_decay, max_norm, masters, norm)

@@ -647,8 +647,9 @@ int fsc_embedding_backward(int64_t rows, int32_t width, int64_t table_rows, int3
  * bits 32: m and v are float32 [n].  bits 8: m and sqrt(v) are uint8 codes [n] with a float32 scale for each 256 values
  * ([ceil(n / 256)]), the block's largest.  A code is a floating number, for m a sign, 4 exponent and 3 fraction bits, for
  * sqrt(v) 4 and 4, the largest code standing for 1 and code 0 for 0; values are rounded up or down by a hash of their
- * number and the step, so that the mean of the roundings is the value; sqrt(v) above zero has a code above zero, and
- * a block whose largest is below 2^-100 is zeros.
+ * number and the step, so that the mean of the roundings is the value, from code 1 on: for m 1.25 2^-16 of the block's largest, for
+ * sqrt(v) 1.125 2^-16.  Below it sqrt(v) above zero becomes code 1 (never 0, so that no step grows by it), and m is rounded
+ * towards zero: between 1.125 2^-16 and code 1 to either, below always to 0.  A block whose largest is below 2^-100 is zeros.
  * lr_tensor (a float32 on the GPU, null: lr) takes the place of lr.  workspace: fsc_adamw_workspace bytes.
  * fsc_grad_norm: norm = sqrt of the sum of all gradients' squares (64-bit sums), a float32 on the GPU.
  * fsc_adamw_values: the values that codes stand for (root 0: m's, 1: sqrt(v)'s). */
