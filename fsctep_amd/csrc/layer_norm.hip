@@ -13,9 +13,11 @@
 // Bound by memory: forward 2 arrays of the rows' size, backward 3 (4 with plus), twice 5.  A row is read once and kept in registers
 // between its passes; rows shorter than a vector and rows past the registers take a block that reads them again (wide_kernel).
 //
-// Measured alone (large copies and fills on this card: 5.2 and 6.8 TB/s): 10,000 x 1,600 fp32 forward 20.6 us (128 MB, 6.2 TB/s),
-// backward 37 us (192 MB, 5.2 TB/s) with 5 us for the sums, twice 60 us (320 MB, 5.3 TB/s); 100,000 x 640 bf16 57 us (256 MB, 4.5 TB/s)
-// and 74 us (384 MB, 5.2 TB/s); 10,000 x 3,200 fp32 47, 82 and 138 us; 4,000 x 8,192 fp32 49, 84 and 136 us (131 MB an array).
+// Measured alone, without an activation (large copies and fills on this card: 5.2 and 6.8 TB/s): 10,000 x 1,600 fp32 forward 20.7 us
+// (128 MB, 6.2 TB/s), backward 38 us (192 MB, 5.0 TB/s) with 5 us for the sums, twice 59 us (320 MB, 5.5 TB/s); 100,000 x 640 bf16 50 us
+// (256 MB, 5.1 TB/s), 76 us (384 MB, 5.1 TB/s) and 227 us; 10,000 x 3,200 fp32 46, 80 and 135 us; 4,000 x 8,192 fp32 49, 84 and 135 us (131
+// MB an array).  With SiLU 29, 45 and 75 us; 70, 135 and 318 us; 54, 95 and 232 us; 54, 95 and 212 us: its second pass is bound by
+// registers, 512 x 4 in fp32 keeps 188 bytes a lane in scratch there and 256 x 4 in bf16 128.
 #include <algorithm>
 
 #include "common.h"
@@ -255,8 +257,9 @@ __global__ __launch_bounds__(NT) void wide_twice_kernel(Args a) {
 // width no vector divides is read from the row's end back, and its lane takes the values from `skip` on as its own; lanes
 // past the end own none.  Values that are not a lane's own are zeros in every sum.
 //
-// Bound by the vector units as much as by memory (a wave's instruction takes four cycles): shapes leave few lanes
-// idle, sums within 16 lanes are DPP additions, and a value takes about a dozen instructions in each pass.
+// Bound by memory with the vector units behind it, which issue in 42 to 56 % of the cycles at the large cases (a wave's instruction
+// takes four): shapes leave few lanes idle, sums within 16 lanes are DPP additions, and a value takes about a dozen instructions in
+// each pass.
 template <typename T>
 struct alignas(sizeof(T)) Vec {          // at any address a value may lie at
   static constexpr int N = 16 / sizeof(T);
@@ -720,8 +723,9 @@ __global__ __launch_bounds__(1024) void sum_kernel(const float* __restrict__ par
 // Calls f(L, CH) for the fewest vectors of L lanes that hold a row; false where none do (a row shorter than a vector, or too
 // wide).  FORWARD shapes may have the registers of five vectors of 16 bits a lane, the backward passes three (100,000 x 640 in
 // bf16 backward, five vectors of 16 lanes: 130 us, three of 32: 88 us), the second one three of either type.  Rows of 4,097 to 8,192
-// float32 values take 512 lanes (4,000 x 8,192 by 512 lanes, 1,024 lanes of two vectors and wide_kernel: forward 49, 50 and 105 us,
-// backward 84, 86 and 344 us, twice 136, 269 and 439 us; the same vectors of bfloat16 have no room for the second pass).
+// float32 values take 512 lanes (4,000 x 8,192 without an activation by 512 lanes, 1,024 lanes of two vectors and wide_kernel: forward
+// 49, 50 and 105 us, backward 84, 86 and 344 us, twice 136, 269 and 439 us; the same vectors of bfloat16 have no room for the second
+// pass).
 enum Pass { FORWARD, BACK, TWICE };
 template <typename T, Pass P, typename F>
 bool by_shape(int width, F&& f) {

@@ -129,7 +129,7 @@ class ExpertReadout(nn.Module):
     def forward(self, x, species=None, differentiable: bool = False, species_below: int | None = None):
         """(N, width) -> (N, width); ``species``: atomic numbers (N,), below n_species (an atom with another becomes NaN).
         ``differentiable``: twice differentiable (force losses).  ``species_below``: what the caller knows ``species`` to
-        lie under from 0 on, so that they need not be looked at."""
+        lie under from 0 on, so that they need not be looked at (on the GPU an atom that does not becomes NaN as well)."""
         if x.dtype not in ROW_TYPES:
             raise ValueError(f"expert readout: rows are float32 or bfloat16, got {x.dtype}")
         rows = self.router.rows_of(species, species_below)

@@ -1,12 +1,12 @@
-"""AdamW on the GPU: one launch for a model's tensors, the gradients clipped by their common norm on the way, states in
-32 or in 8 bits.
+"""AdamW on the GPU: two launches for each 48 tensors, the gradients clipped by their common norm on the way (one launch
+for each 48 tensors more, and one), states in 32 or in 8 bits.
 
     opt = AdamW(model.parameters(), lr=1e-3, weight_decay=0.01, max_norm=1.0)       # a torch.optim.Optimizer
     loss.backward(); opt.step(); opt.zero_grad()
     opt.grad_norm                                                                    # of the last step, on the GPU
 
 The formulas are torch.optim.AdamW's (the reference's trainer, training/trainer.py), states of 32 bits have its names,
-so that its checkpoints load.  Parameters are float32, or bfloat16 with a float32 copy ("master") in the state that
+so that its checkpoints load (other optimisers' are refused).  Parameters are float32, or bfloat16 with a float32 copy ("master") in the state that
 is stepped and rounded (who writes other values into such a parameter writes them into its copy as well).  Step counts live on the GPU and nothing waits for it, so a step can be captured into a graph
 (``lr`` as a float32 tensor then changes between replays).  The ops are registered in C++
 (``csrc/torch_learn_ops.cpp``, kernels ``csrc/adamw.hip``).
