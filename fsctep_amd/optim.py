@@ -146,6 +146,8 @@ class AdamW(torch.optim.Optimizer):
                     s[name + "_scale"] = torch.zeros(math.ceil(p.numel() / GROUP), dtype=torch.float32, device=p.device)
         if copied and "master" not in s:     # a checkpoint without copies: of what the parameter holds now
             s["master"] = p.detach().float()
+        if not copied:                       # the model went from bfloat16 to float32
+            s.pop("master", None)
         return s
 
     @torch.no_grad()

@@ -95,3 +95,20 @@ def test_a_learning_rate_on_the_gpu_comes_back_from_the_host(tmp_path):
     opt.step()
     other.step()
     assert torch.equal(p, q) and other.param_groups[0]["lr"].device == p.device
+
+
+def test_a_model_that_goes_to_float32_and_back():
+    """The copy of the first bfloat16 steps is not taken back after steps in float32."""
+    p = torch.linspace(-1, 1, 300, device=DEV).bfloat16().requires_grad_(True)
+    opt = optim.AdamW([p], lr=0.0, weight_decay=0.0)
+
+    def step(values):
+        p.data = values
+        p.grad = torch.ones_like(p)
+        opt.step()
+        assert torch.equal(p.detach(), values) and ("master" in opt.state[p]) == (p.dtype == torch.bfloat16)
+
+    step(p.data)
+    step(p.data.float() + 1.0)
+    step((p.data + 1.0).bfloat16())
+    assert float(opt.state[p]["step"]) == 3 and torch.equal(opt.state[p]["master"], p.detach().float())
