@@ -237,10 +237,14 @@ def readout_features(feats, Ws, scales, maps):
 
 
 # ------------------------------------------------------------------ energy head (layer_norm.hip)
+def _as_made(m) -> bool:
+    """Whether a call of the module is its class's forward alone: nothing hooked to it, and no forward of its own in its place."""
+    return not (m._forward_hooks or m._forward_pre_hooks or m._backward_hooks or m._backward_pre_hooks or "forward" in vars(m))
+
+
 def _plain_norm(ln) -> bool:
-    """A LayerNorm over the last dimension as it was made, with nothing hooked to its call."""
-    return (type(ln) is nn.LayerNorm and len(ln.normalized_shape) == 1 and not ln._forward_hooks
-            and not ln._forward_pre_hooks and not ln._backward_hooks and not ln._backward_pre_hooks)
+    """A LayerNorm over the last dimension as it was made."""
+    return type(ln) is nn.LayerNorm and len(ln.normalized_shape) == 1 and _as_made(ln)
 
 
 def _norm(ln, x, activation=None):
@@ -257,9 +261,8 @@ def readout_energy(net, weighted_sum, x):
     their SiLU on the HIP op, the products in torch.  Heads that are not as ``sparse.MainNet`` makes them run as the modules."""
     from .sparse import MainNet
     norms = [net.input_norm, *net.layer_norms] if type(net) is MainNet else []
-    if (not norms or not all(_plain_norm(ln) for ln in norms) or net._forward_hooks or net._forward_pre_hooks
-            or net._backward_hooks or net._backward_pre_hooks or nn.modules.module._has_any_global_hook()
-            or torch.is_autocast_enabled()):
+    if (not norms or not all(_plain_norm(ln) for ln in norms) or not _as_made(net)
+            or nn.modules.module._has_any_global_hook() or torch.is_autocast_enabled()):
         return weighted_sum(net(x))
     y = _norm(net.input_norm, x)
     for lin, ln in zip(net.layers, net.layer_norms):
