@@ -8,7 +8,8 @@
 // Measured (additions over large arrays move 6.1 TB/s here): 43 tensors of 44.5 M fp32 values 214 us (1,246 MB, 5.8 TB/s) and 57 us
 // for the norm (178 MB); 39 M bf16 values with fp32 copies 192 and 28 us (1,101 MB, 5.7 TB/s); 79 M fp32 values with states in 8
 // bits 234 us (1,258 MB, 5.4 TB/s, and vector instructions issued in 98 % of the cycles: 120 M of four cycles each on 1,024 SIMDs of
-// 478,000; states in 32 bits 18 %) and 73 us for the norm (314 MB), their values 65 us for each state (393 MB, 6.0 TB/s); 1.7 M values 10 us.  prepare_kernel and norm_kernel are launches (3 us).
+// 478,000; states in 32 bits 18 %) and 73 us for the norm (314 MB), their values 65 us for each state (393 MB, 6.0 TB/s); 1.7 M
+// values 10 us.  prepare_kernel and norm_kernel are launches (3 us).
 #include <algorithm>
 #include <cstring>
 

@@ -107,9 +107,9 @@ __global__ __launch_bounds__(NT) void lookup_kernel(Args a, int64_t first, uint3
 // columns of 5,000 rows 13.7 and 19.1 us).  For up to 2,048 tokens and 2^23 pairs of token and row to look at (by it and by the
 // sort: 2,048 tokens, 640 columns of 100 rows 5.8 and 21.0 us, all of one token 28.7 and 18.7 us; 1,024 of 5,000 rows 13.7 and 29.4
 // us; 256 of 30,000 rows x 331 24.6 and 33.5 us, 1,024 40.2 and 35.6 us), and 2^25 for those pairs times the blocks of columns,
-// each of which looks through the tokens again (fp32: 1,024 tokens of 1,600 rows x 4,096 29.3 and 35.5 us, 2,048 tokens 47.9 and 37.9 us, of
-// 1,600 rows x 12,288 156 and 70 us, of 4,000 rows 331 and 95 us; bf16: 256 of 30,000 rows x 2,048 54.9 and 55.4 us, 1,024 of 1,600
-// rows x 12,288 48.6 and 45.8 us).  512 tokens where the table is small (192 columns of 9 rows, all of one token: 512 tokens 6.3
+// each of which looks through the tokens again (fp32: 1,024 tokens of 1,600 rows x 4,096 29.3 and 35.5 us, 2,048 tokens 47.9 and
+// 37.9 us, of 1,600 rows x 12,288 156 and 70 us, of 4,000 rows 331 and 95 us; bf16: 256 of 30,000 rows x 2,048 54.9 and 55.4 us,
+// 1,024 of 1,600 rows x 12,288 48.6 and 45.8 us).  512 tokens where the table is small (192 columns of 9 rows, all of one token: 512 tokens 6.3
 // and 7.6 us, 1,024 tokens 11.1 and 7.9 us; 12,288 columns of 24 rows 6.6 and 27.1 us).
 inline bool few(int64_t rows, int64_t table_rows, int width, int size);
 template <int WAVES, typename T, typename I, bool FULL>

@@ -6,10 +6,11 @@ for each 48 tensors more, and one), states in 32 or in 8 bits.
     opt.grad_norm                                                                    # of the last step, on the GPU
 
 The formulas are torch.optim.AdamW's (the reference's trainer, training/trainer.py), states of 32 bits have its names,
-so that its checkpoints load (other optimisers' are refused).  Parameters are float32, or bfloat16 with a float32 copy ("master") in the state that
-is stepped and rounded (who writes other values into such a parameter writes them into its copy as well).  Step counts live on the GPU and nothing waits for it, so a step can be captured into a graph
-(``lr`` as a float32 tensor then changes between replays).  The ops are registered in C++
-(``csrc/torch_learn_ops.cpp``, kernels ``csrc/adamw.hip``).
+so that its checkpoints load (other optimisers' are refused).  Parameters are float32, or bfloat16 with a float32 copy
+("master") in the state that is stepped and rounded (who writes other values into such a parameter writes them into its
+copy as well).  Step counts live on the GPU and nothing waits for it, so a step can be captured into a graph (``lr`` as a
+float32 tensor then changes between replays).  The ops are registered in C++ (``csrc/torch_learn_ops.cpp``, kernels
+``csrc/adamw.hip``).
 
 States in 8 bits (``state_bits=8``): m and sqrt(v) as 8-bit floats with a float32 scale for each 256 values, rounded
 up or down by a hash of the value's number and the step, so that small changes add up over the steps instead of being

@@ -625,8 +625,8 @@ int fsc_layer_norm_backward_twice(int64_t rows, int32_t width, int32_t dtype, in
                                   float* workspace, hipStream_t stream);
 
 /* Lookup: out[i] = scale table[index[i]] for `rows` tokens (index contiguous, int32 or int64 by index_bits), zeros where
- * the index lies outside [0, table_rows) (the second form: `outside` there).  dtype of table and out: FSC_F32 or FSC_BF16; rows of the table at any stride, out
- * [rows][width] contiguous.  Backward: dtable [table_rows][width] (contiguous, every row written) = scale times the sum
+ * the index lies outside [0, table_rows) (the second form: `outside` there).  dtype of table and out: FSC_F32 or FSC_BF16; rows of
+ * the table at any stride, out [rows][width] contiguous.  Backward: dtable [table_rows][width] (contiguous, every row written) = scale times the sum
  * of dy's rows by token, in 32 bits and a fixed order.  The workspace (bytes, 16-byte aligned) is the backward's. */
 int fsc_embedding_forward(int64_t rows, int32_t width, int64_t table_rows, int32_t dtype, int32_t index_bits,
                           int64_t table_stride, const void* table, const void* index, float scale, void* out,
